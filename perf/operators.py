@@ -227,8 +227,8 @@ def workspace(size):
 
 
 def run_own(state):
-    from x0ne_core import Kv8
     g, case = gpu(), state["case"]
+    from x0ne_core import Kv8
     at = {k: v.data_ptr() for k, v in state.items() if isinstance(v, torch.Tensor)}
     kv = Kv8(codes=at["codes"], scales=at["scales"], page_table=at["table"], pool=state["pool"], kv_heads=case["kv_heads"],
              seqs=case["seqs"], seq_pages=pages_of(case))
