@@ -199,6 +199,65 @@ uint64_t x0ne_split_state_bytes(uint32_t q_heads, uint32_t splits);
 x0ne_status x0ne_gpu_time_attention(x0ne_gpu* g, uint32_t q_heads, uint32_t kv_heads, uint32_t ctx, uint32_t splits,
                                     uint32_t iters, uint64_t seed, double* us, uint32_t* planes_out);
 
+/* ---- the 8-bit paged K/V cache: no counterpart in the reference, whose cache is bf16 ----
+   A row of 128 values is held as e4m3 codes of x 2^-e and one scale byte e + 127, e the smallest
+   exponent from -117 on with 448 2^e >= the largest finite |x|; what is not finite is held as NaN.
+   A position and kv head takes 258 bytes for its key and value instead of 512. Device addresses:
+   codes [pool][kv_heads][4096]: 16 positions' keys [16][128], then their values dim-major [128][16];
+   scales [pool][kv_heads][32]: the keys' scale bytes, then the values'; both 16-byte aligned.
+   page_table [seqs][seq_pages] u32: the physical page of 16 positions of each sequence. An entry of
+   pool or more names no page: its positions are not written, read back as zeros, and hold no keys.
+   1 to 1024 kv heads, up to 65535 sequences, seq_pages 1 to 2^24 - 1, else X0NE_ERR_FORMAT, as for a
+   required address that is 0 or not aligned as stated. A call without rows or sequences does
+   nothing. The calls run on the Gpu's stream, allocate nothing, and may be captured into a graph. */
+typedef struct {
+    uint64_t codes, scales, page_table;
+    uint32_t pool, kv_heads, seqs, seq_pages;
+} x0ne_kv8;
+
+/* Writes rows of any mix of sequences: qkv [rows][(q_heads + 2 kv_heads) 128] bf16, row r at position
+   row_pos[r] of sequence row_seq[r] (u32 each; the rows name distinct positions). RMSNorm of each
+   head of q and k (weights q_norm, k_norm, 128 bf16) and rotate-half RoPE from rope_cs, the f64 (cos,
+   sin) table of `positions` positions (x0ne_rope_table_f64): q_out [rows][q_heads 128] bf16 has the
+   bits of x0ne_qk_norm_rope_kv_write_rows_bf16, the cache holds the codes of its k and v rows. A row
+   whose sequence is not below seqs, or whose position has no table entry or no page-table entry, is
+   padding: nothing of it is written. bounds (0: none): [pool][kv_heads][2][128] bf16, of every page
+   whose last position is among the rows the smallest and the largest key value of each dim over its
+   16 positions (NaN where a key is), for x0ne_gpu_kv8_select. qkv, q_norm, k_norm, rope_cs, q_out and
+   bounds are 16-byte aligned; q_heads 1 to 16384, rows below 2^24. */
+x0ne_status x0ne_gpu_kv8_write(x0ne_gpu* g, const x0ne_kv8* c, uint64_t qkv, uint64_t rows, uint32_t q_heads,
+                               uint64_t q_norm, uint64_t k_norm, float eps, uint64_t rope_cs, uint32_t positions,
+                               uint64_t row_seq, uint64_t row_pos, uint64_t q_out, uint64_t bounds);
+/* Reads it back as bf16 pages (exact): sequence s's positions below lens[s] (u32; at most its pages')
+   into the K plane [out_pool][kv_heads][16][128] and the V plane [out_pool][kv_heads][128][16] at the
+   pages that out_table [seqs][seq_pages] names, the layout that the bf16 kernels of this library take
+   (x0ne_attention_prefill_g*_bf16, x0ne_gpu_attention_split). Positions of a sequence's last page at
+   or past its length are zero; pages past it, and entries of out_pool or more, are left alone. */
+x0ne_status x0ne_gpu_kv8_read(x0ne_gpu* g, const x0ne_kv8* c, uint64_t lens, uint64_t k, uint64_t v, uint64_t out_table,
+                              uint32_t out_pool);
+/* Bytes of the workspace of x0ne_gpu_kv8_attention and _select for this cache (0 where they refuse
+   it): 256-byte aligned, zeroed once before its first call and left ready for the next one by each.
+   Calls that share it must not overlap (those of one Gpu, and its graphs, run one after the other). */
+uint64_t x0ne_kv8_work_bytes(const x0ne_kv8* c, uint32_t q_heads);
+/* Decode attention of one query per sequence: out [seqs][q_heads 128] bf16 = softmax(scale q k) v over
+   the keys below lens[s] (u32; at most its pages'), q [seqs][q_heads 128] bf16 from the same layout,
+   q head h reading kv head h / (q_heads / kv_heads), 1 to 16 q heads per kv head. Scores, softmax and
+   sums in f32. A sequence without keys gives zeros. page_list (0, with budget 0: every page):
+   [seqs][kv_heads][budget] u32, the logical pages that the queries of a kv head attend: the first
+   min(budget, pages of the sequence) entries, each page once, entries past the sequence's pages
+   skipped. A row's bits depend on the sequence itself and the seqs, seq_pages and heads of the call,
+   not on the other sequences. */
+x0ne_status x0ne_gpu_kv8_attention(x0ne_gpu* g, const x0ne_kv8* c, uint64_t q, uint32_t q_heads, uint64_t lens,
+                                   uint64_t page_list, uint32_t budget, uint64_t out, float scale, uint64_t work,
+                                   uint64_t work_bytes);
+/* The pages worth attending: for each sequence and kv head its last page and the budget - 1 others of
+   the largest score, the most that q k can be for any key within the page's bounds (the largest over
+   the kv head's queries; f64), ties to the lower page, a NaN score above all, a page that is not there
+   below all. page_list [seqs][kv_heads][budget] u32: ascending, 0xFFFFFFFF behind the last. Every
+   page of a sequence but its last must have its bounds (x0ne_gpu_kv8_write). */
+x0ne_status x0ne_gpu_kv8_select(x0ne_gpu* g, const x0ne_kv8* c, uint64_t bounds, uint64_t q, uint32_t q_heads,
+                                uint64_t lens, uint32_t budget, uint64_t page_list, uint64_t work, uint64_t work_bytes);
+
 /* Graph capture (gpu.rs:1170-1238): every launch between begin and end is recorded, then
    replayed by x0ne_gpu_launch_graph on the Gpu that captured it (another Gpu is refused with
    X0NE_ERR_GPU, gpu.rs:1225-1230). */

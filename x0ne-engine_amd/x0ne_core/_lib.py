@@ -81,6 +81,12 @@ class GemvFusedC(C.Structure):
                [(n, C.c_uint32) for n in ("prologue", "epilogue", "f64_sums")]
 
 
+class Kv8C(C.Structure):
+    """x0ne_kv8: an 8-bit paged K/V cache."""
+    _fields_ = [(n, C.c_uint64) for n in ("codes", "scales", "page_table")] + \
+               [(n, C.c_uint32) for n in ("pool", "kv_heads", "seqs", "seq_pages")]
+
+
 class EngineOptionsC(C.Structure):
     _fields_ = [("max_ctx", C.c_uint64), ("page_seed", C.c_uint64), ("sums", C.c_uint32),
                 ("prefill_chunk", C.c_uint32), ("max_batch", C.c_uint32), ("reserved", C.c_uint32)]
@@ -119,6 +125,11 @@ SIGNATURES = {
                                           U32, U32, U32, F32], ST),
     "x0ne_split_state_bytes": ([U32, U32], U64),
     "x0ne_gpu_time_attention": ([P, U32, U32, U32, U32, U32, U64, C.POINTER(F64), C.POINTER(U32)], ST),
+    "x0ne_gpu_kv8_write": ([P, C.POINTER(Kv8C), U64, U64, U32, U64, U64, F32, U64, U32, U64, U64, U64, U64], ST),
+    "x0ne_gpu_kv8_read": ([P, C.POINTER(Kv8C), U64, U64, U64, U64, U32], ST),
+    "x0ne_kv8_work_bytes": ([C.POINTER(Kv8C), U32], U64),
+    "x0ne_gpu_kv8_attention": ([P, C.POINTER(Kv8C), U64, U32, U64, U64, U32, U64, F32, U64, U64], ST),
+    "x0ne_gpu_kv8_select": ([P, C.POINTER(Kv8C), U64, U64, U32, U64, U32, U64, U64, U64], ST),
     "x0ne_gpu_capture_begin": ([P], ST),
     "x0ne_gpu_capture_end": ([P, C.POINTER(P)], ST),
     "x0ne_gpu_launch_graph": ([P, P], ST),

@@ -15,7 +15,7 @@ import numpy as np
 
 from ._lib import FormatError, GpuError
 from .arena import Arena, Class
-from .gpu import Arg, Gpu, SplitPlan, split_state_bytes
+from .gpu import Arg, Gpu, Kv8, SplitPlan, split_state_bytes
 
 HEAD_DIM = 128
 PAGE = 16
@@ -64,6 +64,23 @@ class QkvOut:
     k_row: np.ndarray
     v_row: np.ndarray
     rest_untouched: bool
+
+
+@dataclass
+class Kv8Pages:
+    """An 8-bit paged K/V cache on the host: codes [pool][kv_heads][4096] and scales [pool][kv_heads][32] (uint8),
+    table [seqs][seq_pages] (uint32), as x0ne_kv8 lays them out."""
+    codes: np.ndarray
+    scales: np.ndarray
+    table: np.ndarray
+
+    @property
+    def pool(self):
+        return self.codes.shape[0]
+
+    @property
+    def kv_heads(self):
+        return self.codes.shape[1]
 
 
 def inv_freq(head_dim: int, theta: float) -> np.ndarray:
@@ -1030,3 +1047,88 @@ class Kernels:
         if v >= logits.size:
             raise GpuError("argmax: no finite maximum (NaN row)")
         return v
+
+    # -- the 8-bit paged K/V cache (kv8.hip) --
+    SENTINEL = 0xA5A5  # bf16 pattern of outputs that a call may leave alone
+
+    def _kv8(self, pages: Kv8Pages, extra: dict):
+        """An arena with the cache and the arrays of `extra`: (arena, Kv8, slice of each name)."""
+        a = self._arena()
+        arrays = {"codes": pages.codes, "scales": pages.scales, "table": np.asarray(pages.table, np.uint32), **extra}
+        arrays = {k: np.ascontiguousarray(v) for k, v in arrays.items()}
+        s = {k: a.alloc(k, max(v.nbytes, 16), Class.CLIENT_DATA) for k, v in arrays.items()}
+        self._freeze(a)
+        for k, v in arrays.items():
+            if v.nbytes:
+                a.write(s[k], 0, v)
+        seqs, seq_pages = pages.table.shape
+        return a, Kv8(a.ptr(s["codes"]), a.ptr(s["scales"]), a.ptr(s["table"]), pages.pool, pages.kv_heads, seqs,
+                      seq_pages), s
+
+    def kv8_write(self, pages: Kv8Pages, qkv, q_heads: int, q_norm, k_norm, theta: float, eps: float, positions: int,
+                  row_seq, row_pos, bounds=None):
+        """x0ne_gpu_kv8_write of qkv's rows ([rows][(q_heads + 2 kv_heads) 128] bf16 bits): (q_out with SENTINEL
+        where nothing was written, the cache after, the bounds after)."""
+        qkv = np.asarray(qkv, np.uint16)
+        rows = qkv.shape[0]
+        extra = {"qkv": qkv, "q_norm": np.asarray(q_norm, np.uint16), "k_norm": np.asarray(k_norm, np.uint16),
+                 "inv": inv_freq(HEAD_DIM, theta), "cs": np.zeros(positions * HEAD_DIM, np.float64),
+                 "row_seq": np.asarray(row_seq, np.uint32), "row_pos": np.asarray(row_pos, np.uint32),
+                 "q_out": np.full((rows, q_heads * HEAD_DIM), self.SENTINEL, np.uint16)}
+        if bounds is not None:
+            extra["bounds"] = np.asarray(bounds, np.uint16)
+        a, kv, s = self._kv8(pages, extra)
+        self._rope_table(a.ptr(s["inv"]), a.ptr(s["cs"]), positions, HEAD_DIM)
+        self.gpu.kv8_write(kv, a.ptr(s["qkv"]), rows, q_heads, a.ptr(s["q_norm"]), a.ptr(s["k_norm"]), eps, a.ptr(s["cs"]),
+                           positions, a.ptr(s["row_seq"]), a.ptr(s["row_pos"]), a.ptr(s["q_out"]),
+                           a.ptr(s["bounds"]) if bounds is not None else 0)
+        self.gpu.sync()
+        after = Kv8Pages(a.read_array(s["codes"], 0, pages.codes.size, np.uint8).reshape(pages.codes.shape),
+                         a.read_array(s["scales"], 0, pages.scales.size, np.uint8).reshape(pages.scales.shape), pages.table)
+        return (a.read_array(s["q_out"], 0, rows * q_heads * HEAD_DIM, np.uint16).reshape(rows, q_heads, HEAD_DIM), after,
+                None if bounds is None else
+                a.read_array(s["bounds"], 0, extra["bounds"].size, np.uint16).reshape(extra["bounds"].shape))
+
+    def kv8_read(self, pages: Kv8Pages, lens, out_table, out_pool: int):
+        """x0ne_gpu_kv8_read: K [out_pool][kv_heads][16][128] and V [out_pool][kv_heads][128][16] bf16 bits, SENTINEL
+        where nothing was written."""
+        n = out_pool * pages.kv_heads * PAGE * HEAD_DIM
+        extra = {"lens": np.asarray(lens, np.uint32), "out_table": np.asarray(out_table, np.uint32),
+                 "k": np.full(n, self.SENTINEL, np.uint16), "v": np.full(n, self.SENTINEL, np.uint16)}
+        a, kv, s = self._kv8(pages, extra)
+        self.gpu.kv8_read(kv, a.ptr(s["lens"]), a.ptr(s["k"]), a.ptr(s["v"]), a.ptr(s["out_table"]), out_pool)
+        self.gpu.sync()
+        return (a.read_array(s["k"], 0, n, np.uint16).reshape(out_pool, pages.kv_heads, PAGE, HEAD_DIM),
+                a.read_array(s["v"], 0, n, np.uint16).reshape(out_pool, pages.kv_heads, HEAD_DIM, PAGE))
+
+    def kv8_attention(self, pages: Kv8Pages, q, q_heads: int, lens, page_list=None, scale: float | None = None,
+                      calls: int = 1) -> np.ndarray:
+        """x0ne_gpu_kv8_attention, `calls` times over one workspace: out [seqs][q_heads][128] bf16 bits of the last."""
+        seqs = pages.table.shape[0]
+        n = seqs * q_heads * HEAD_DIM
+        size = self.gpu.kv8_work_bytes(Kv8(16, 16, 16, pages.pool, pages.kv_heads, *pages.table.shape), q_heads)
+        extra = {"q": np.asarray(q, np.uint16), "lens": np.asarray(lens, np.uint32), "work": np.zeros(size, np.uint8),
+                 "out": np.full(n, self.SENTINEL, np.uint16)}
+        if page_list is not None:
+            extra["list"] = np.asarray(page_list, np.uint32)
+        a, kv, s = self._kv8(pages, extra)
+        for _ in range(calls):
+            self.gpu.kv8_attention(kv, a.ptr(s["q"]), q_heads, a.ptr(s["lens"]), a.ptr(s["out"]),
+                                   attn_scale(HEAD_DIM) if scale is None else scale, a.ptr(s["work"]), size,
+                                   *((a.ptr(s["list"]), page_list.shape[-1]) if page_list is not None else ()))
+        self.gpu.sync()
+        return a.read_array(s["out"], 0, n, np.uint16).reshape(seqs, q_heads, HEAD_DIM)
+
+    def kv8_select(self, pages: Kv8Pages, bounds, q, q_heads: int, lens, budget: int, calls: int = 1) -> np.ndarray:
+        """x0ne_gpu_kv8_select, `calls` times over one workspace: the page list [seqs][kv_heads][budget] (uint32)."""
+        seqs = pages.table.shape[0]
+        n = seqs * pages.kv_heads * budget
+        size = self.gpu.kv8_work_bytes(Kv8(16, 16, 16, pages.pool, pages.kv_heads, *pages.table.shape), q_heads)
+        extra = {"q": np.asarray(q, np.uint16), "lens": np.asarray(lens, np.uint32), "work": np.zeros(size, np.uint8),
+                 "bounds": np.asarray(bounds, np.uint16), "list": np.full(n, 0xA5A5A5A5, np.uint32)}
+        a, kv, s = self._kv8(pages, extra)
+        for _ in range(calls):
+            self.gpu.kv8_select(kv, a.ptr(s["bounds"]), a.ptr(s["q"]), q_heads, a.ptr(s["lens"]), budget, a.ptr(s["list"]),
+                                a.ptr(s["work"]), size)
+        self.gpu.sync()
+        return a.read_array(s["list"], 0, n, np.uint32).reshape(seqs, pages.kv_heads, budget)
