@@ -136,58 +136,271 @@ __global__ void __launch_bounds__(256)
     }
 }
 
-// Decode attention, one wavefront per (sequence, q head): 64 keys at a time, a lane per key for the
-// scores, then lane i dims i and i + 64 of the weighted values, with the running maximum and sum.
-__global__ void __launch_bounds__(64)
-    kv8_attention_kernel(Table t, const uint8_t* __restrict__ codes, const uint8_t* __restrict__ scales,
-                         const bf16_t* __restrict__ q, const uint32_t* __restrict__ lens,
-                         const uint32_t* __restrict__ list, uint32_t budget, bf16_t* __restrict__ out, uint32_t q_heads,
-                         float scale) {
-    __shared__ float qs[KV8_HEAD], ps[64], vscale[64];
-    __shared__ size_t rec_of[64];
-    const uint32_t h = blockIdx.x, s = blockIdx.y, i = threadIdx.x, kh = h / (q_heads / t.kv_heads);
-    const uint32_t keys = kv8_keys(lens[s], t.seq_pages), pages = (keys + KV8_PAGE - 1) / KV8_PAGE;
-    const uint32_t n = list ? min(budget, pages) : pages;
-    const bf16_t* qr = q + ((size_t)s * q_heads + h) * KV8_HEAD;
-    qs[i] = bf2f(qr[i]);
-    qs[i + 64] = bf2f(qr[i + 64]);
-    float m = -INFINITY, l = 0.f, o0 = 0.f, o1 = 0.f;
-    for (uint32_t p0 = 0; p0 < n; p0 += 4) {
-        const uint32_t at = p0 + i / 16, slot = i % 16;
-        const uint32_t logical = at >= n ? KV8_NONE : list ? list[((size_t)s * t.kv_heads + kh) * budget + at] : at;
-        const uint32_t page = logical < pages ? t.page(s, logical) : KV8_NONE;
-        const bool live = page != KV8_NONE && logical * KV8_PAGE + slot < keys;
-        const size_t rec = kv8_record(live ? page : 0, t.kv_heads, kh);
-        const size_t sc = kv8_scale(live ? page : 0, t.kv_heads, kh);
-        float score = -INFINITY;
-        __syncthreads();
-        if (live) {
-            float sum = 0.f;
-            for (uint32_t d = 0; d < KV8_HEAD; ++d) sum = fmaf(kv8_value(codes[rec + slot * KV8_HEAD + d], scales[sc + slot]), qs[d], sum);
-            score = sum * scale;
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+
+__device__ __forceinline__ f32x4 mfma(u32x4 a, u32x4 b, f32x4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+}
+__device__ __forceinline__ uint32_t pack(float lo, float hi) {
+    return __builtin_bit_cast(uint32_t, bf16x2{(__bf16)lo, (__bf16)hi});
+}
+// Eight codes as bf16, times the power of two `scale`: exact.
+__device__ __forceinline__ u32x4 decode(uint32_t lo, uint32_t hi, float scale) {
+    u32x4 r;
+    r[0] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, scale, false));
+    r[1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, scale, true));
+    r[2] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, scale, false));
+    r[3] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, scale, true));
+    return r;
+}
+
+// Partial states go between blocks through agent-scope accesses, coherent across the XCDs' caches.
+__device__ __forceinline__ void put2(float* p, float a, float b) {
+    __hip_atomic_store((uint64_t*)p, (uint64_t)__float_as_uint(b) << 32 | __float_as_uint(a), __ATOMIC_RELAXED,
+                       __HIP_MEMORY_SCOPE_AGENT);
+}
+__device__ __forceinline__ float2 get2(const float* p) {
+    const uint64_t v = __hip_atomic_load((const uint64_t*)p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    return make_float2(__uint_as_float((uint32_t)v), __uint_as_float((uint32_t)(v >> 32)));
+}
+// 2^(m - top), 0 for a state without a key.
+__device__ __forceinline__ float factor(float m, float top) {
+    return __builtin_amdgcn_exp2f(m - (top == -INFINITY ? 0.f : top));
+}
+
+constexpr uint32_t ATTEND_WAVES = 4, TILE_PAGES = 4;
+constexpr uint32_t MAX_SLICES = 64;
+constexpr uint32_t STATE = KV8_HEAD + 4;  // floats of a partial state: m, l, two unused, o
+constexpr uint32_t MAX_GROUP = 16;
+
+struct Attend {
+    Table t;
+    const uint8_t *codes, *scales;
+    const bf16_t* q;
+    const uint32_t *lens, *list;
+    bf16_t* out;
+    float* state;
+    uint32_t* counter;
+    uint32_t budget, q_heads, group, slices;
+    float scale2;  // the scale times log2 e: a weight is one exp2
+};
+
+// Decode attention. A block of 4 wavefronts takes a slice of one sequence's tiles for the q heads of one kv head,
+// wavefront w the slice's tiles w, w + 4, ...; a tile is 4 pages. The products are S^T = K Q^T and O^T = V^T P^T on
+// the matrix cores (16 x 16 x 32, bf16 with f32 sums), the group's heads the 16 columns: lane (n = lane % 16, g =
+// lane / 16) holds column n, so the softmax of a head is lane-local but for the four lanes n, n + 16, n + 32, n + 48.
+// Codes become bf16 in one conversion, keys times their scale (exact); a value's scale goes into its weight (exact).
+//  - Product m's row r = 4 g' + i is key 4 m + i of the tile's page g': its 16 outputs per lane are then the 16 keys of
+//    page g, and with the value of dim 16 c + n at those keys as row n of product c (one 16-byte load: V is dim-major)
+//    the weights are an operand as they lie, without a move between lanes.
+//  - Dims of a product's k step j are 32 g + 8 j ..: a lane's keys come as two 16-byte loads.
+//  - Weights enter as bf16 hi + lo (2^-17 of the weight): one bf16 would add as much error as the output's rounding.
+// The running maximum and sum are f32. A slice's state (m, l, o) is joined by the last block of its (sequence, kv head)
+// to count itself, slices in order; a sequence of one slice is written at once. Keys past the length, entries behind a
+// list and pages that are not there weigh 0, their values are taken as 0.
+__global__ void __launch_bounds__(64 * ATTEND_WAVES) kv8_attention_kernel(const Attend a) {
+    __shared__ float wm[ATTEND_WAVES][MAX_GROUP], wl[ATTEND_WAVES][MAX_GROUP];
+    __shared__ float wo[ATTEND_WAVES][MAX_GROUP][KV8_HEAD + 4];
+    __shared__ uint32_t last;
+    const uint32_t kh = blockIdx.x, y = blockIdx.y, s = blockIdx.z;
+    const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), n = lane & 15, g = lane >> 4;
+    const uint32_t keys = kv8_keys(a.lens[s], a.t.seq_pages), pages = (keys + KV8_PAGE - 1) / KV8_PAGE;
+    const uint32_t np = a.list ? min(a.budget, pages) : pages, tiles = (np + TILE_PAGES - 1) / TILE_PAGES;
+    bf16_t* out = a.out + ((size_t)s * a.q_heads + kh * a.group) * KV8_HEAD;
+    if (tiles == 0) {
+        if (y == 0)
+            for (uint32_t e = threadIdx.x; e < a.group * KV8_HEAD / 8; e += 256) reinterpret_cast<uint4*>(out)[e] = make_uint4(0, 0, 0, 0);
+        return;
+    }
+    const uint32_t rounds = (tiles + ATTEND_WAVES - 1) / ATTEND_WAVES;
+    const uint32_t per = ATTEND_WAVES * ((rounds + a.slices - 1) / a.slices), active = (tiles + per - 1) / per;
+    if (y >= active) return;
+    const uint32_t t_end = min(tiles, (y + 1) * per);
+
+    // The page of the tile at index 4 t + j, with how many of its keys count.
+    const uint32_t* list = a.list ? a.list + ((size_t)s * a.t.kv_heads + kh) * a.budget : nullptr;
+    struct Place {
+        uint32_t page, valid;
+    };
+    auto logical_of = [&](uint32_t t, uint32_t j) -> uint32_t {
+        const uint32_t at = TILE_PAGES * t + j;
+        return t >= t_end || at >= np ? KV8_NONE : list ? list[at] : at;
+    };
+    auto place = [&](uint32_t logical) -> Place {
+        const uint32_t page = logical < pages ? a.t.page(s, logical) : KV8_NONE;
+        return page == KV8_NONE ? Place{0u, 0u} : Place{page, (uint32_t)min(keys - logical * KV8_PAGE, KV8_PAGE)};
+    };
+    u32x4 k[4][2], v[8], ks, vs;
+    auto load_k = [&](uint32_t page) {
+        const uint8_t* p = a.codes + kv8_record(page, a.t.kv_heads, kh) + (n & 3) * KV8_HEAD + 32 * g;
+#pragma unroll
+        for (int m = 0; m < 4; ++m) {
+            k[m][0] = *reinterpret_cast<const u32x4*>(p + m * 4 * KV8_HEAD);
+            k[m][1] = *reinterpret_cast<const u32x4*>(p + m * 4 * KV8_HEAD + 16);
         }
-        vscale[i] = live ? __uint_as_float((uint32_t)scales[sc + KV8_PAGE + slot] << 23) : 0.f;
-        rec_of[i] = rec + KV8_PART + slot;
-        float top = wave_max(score);
-        top = fmaxf(m, top);
-        const float ref = top == -INFINITY ? 0.f : top;
-        const float p = expf(score - ref), alpha = expf(m - ref);
-        m = top;
-        l = l * alpha + wave_sum(p);
-        ps[i] = live ? p : -1.f;
-        __syncthreads();
-        o0 *= alpha;
-        o1 *= alpha;
-        for (uint32_t k = 0; k < 64; ++k) {
-            if (ps[k] < 0.f) continue;
-            const float w = ps[k] * vscale[k];
-            o0 = fmaf(w, kv8_value(codes[rec_of[k] + i * KV8_PAGE], 127), o0);
-            o1 = fmaf(w, kv8_value(codes[rec_of[k] + (i + 64) * KV8_PAGE], 127), o1);
+        ks = *reinterpret_cast<const u32x4*>(a.scales + kv8_scale(page, a.t.kv_heads, kh));
+    };
+    auto load_v = [&](uint32_t page) {
+        const uint8_t* p = a.codes + kv8_record(page, a.t.kv_heads, kh) + KV8_PART + n * KV8_PAGE;
+#pragma unroll
+        for (int c = 0; c < 8; ++c) v[c] = *reinterpret_cast<const u32x4*>(p + c * 16 * KV8_PAGE);
+        vs = *reinterpret_cast<const u32x4*>(a.scales + kv8_scale(page, a.t.kv_heads, kh) + KV8_PAGE);
+    };
+    const uint32_t t0 = y * per + wave, step = ATTEND_WAVES;
+    Place pk = place(logical_of(t0, n >> 2)), pv = place(logical_of(t0, g));
+    u32x4 qb[4];
+    if (t0 < t_end) {
+        load_k(pk.page);
+        load_v(pv.page);
+    }
+    const bf16_t* qr = a.q + ((size_t)s * a.q_heads + kh * a.group + min(n, a.group - 1)) * KV8_HEAD + 32 * g;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        qb[j] = reinterpret_cast<const u32x4*>(qr)[j];
+        if (n >= a.group) qb[j] = u32x4{0, 0, 0, 0};
+    }
+    Place pk1 = place(logical_of(t0 + step, n >> 2)), pv1 = place(logical_of(t0 + step, g));
+    uint32_t lk2 = logical_of(t0 + 2 * step, n >> 2), lv2 = logical_of(t0 + 2 * step, g);
+
+    float m_run = -INFINITY, lsum = 0.f;
+    f32x4 o[8];
+#pragma unroll
+    for (int c = 0; c < 8; ++c) o[c] = f32x4{0.f, 0.f, 0.f, 0.f};
+    for (uint32_t t = t0; t < t_end; t += step) {
+        float sc[4][4];
+#pragma unroll
+        for (int m = 0; m < 4; ++m) {
+            const float scale = __uint_as_float(((ks[m] >> (8 * (n & 3))) & 0xFFu) << 23);
+            f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int j = 0; j < 4; ++j) acc = mfma(decode(k[m][j >> 1][2 * (j & 1)], k[m][j >> 1][2 * (j & 1) + 1], scale), qb[j], acc);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) sc[m][i] = acc[i] * a.scale2;
+        }
+        if (t + step < t_end) load_k(pk1.page);
+        const bool whole = __all(pv.valid == KV8_PAGE);
+        uint32_t keep[4];
+        if (!whole) {
+#pragma unroll
+            for (int m = 0; m < 4; ++m) {
+                const int left = (int)pv.valid - 4 * m;
+                keep[m] = left >= 4 ? 0xFFFFFFFFu : left <= 0 ? 0u : (1u << (8 * left)) - 1u;
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    if (i >= left) sc[m][i] = -INFINITY;
+                vs[m] &= keep[m];
+            }
+        }
+        float mx = -INFINITY;
+#pragma unroll
+        for (int m = 0; m < 4; ++m)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) mx = fmaxf(mx, sc[m][i]);
+        mx = fmaxf(m_run, rows_max(mx));
+        if (__any(mx > m_run)) {
+            const float alpha = factor(m_run, mx);
+            lsum *= alpha;
+#pragma unroll
+            for (int c = 0; c < 8; ++c) o[c] *= alpha;
+            m_run = mx;
+        }
+        const float ref = m_run == -INFINITY ? 0.f : m_run;
+        u32x4 hi[2], lo[2];
+#pragma unroll
+        for (int m = 0; m < 4; ++m) {
+            float w[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const float p = __builtin_amdgcn_exp2f(sc[m][i] - ref);
+                lsum += p;
+                w[i] = p * __uint_as_float(((vs[m] >> (8 * i)) & 0xFFu) << 23);
+            }
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                const uint32_t h = pack(w[2 * i], w[2 * i + 1]);
+                hi[m >> 1][2 * (m & 1) + i] = h;
+                lo[m >> 1][2 * (m & 1) + i] = pack(w[2 * i] - bf_lo(h), w[2 * i + 1] - bf_hi(h));
+            }
+        }
+#pragma unroll
+        for (int c = 0; c < 8; ++c) {
+            if (!whole) v[c] &= u32x4{keep[0], keep[1], keep[2], keep[3]};
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+                const u32x4 x = decode(v[c][2 * j], v[c][2 * j + 1], 1.f);
+                o[c] = mfma(x, hi[j], o[c]);
+                o[c] = mfma(x, lo[j], o[c]);
+            }
+        }
+        pk = pk1;
+        pv = pv1;
+        pk1 = place(lk2);
+        pv1 = place(lv2);
+        lk2 = logical_of(t + 3 * step, n >> 2);
+        lv2 = logical_of(t + 3 * step, g);
+        if (t + step < t_end) load_v(pv.page);
+    }
+    lsum = rows_sum(lsum);
+
+    // The block's four states.
+    if (n < a.group) {
+        if (g == 0) {
+            wm[wave][n] = m_run;
+            wl[wave][n] = lsum;
+        }
+#pragma unroll
+        for (int c = 0; c < 8; ++c) *reinterpret_cast<f32x4*>(&wo[wave][n][16 * c + 4 * g]) = o[c];
+    }
+    __syncthreads();
+    for (uint32_t e = threadIdx.x; e < a.group * (KV8_HEAD / 4); e += 256) {
+        const uint32_t h = e / (KV8_HEAD / 4), d = 4 * (e % (KV8_HEAD / 4));
+        float top = wm[0][h], l = 0.f;
+        f32x4 x = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (uint32_t w = 1; w < ATTEND_WAVES; ++w) top = fmaxf(top, wm[w][h]);
+#pragma unroll
+        for (uint32_t w = 0; w < ATTEND_WAVES; ++w) {
+            const float f = factor(wm[w][h], top);
+            l += f * wl[w][h];
+            x += f * *reinterpret_cast<const f32x4*>(&wo[w][h][d]);
+        }
+        if (active == 1) {
+            const float r = l == 0.f ? 0.f : 1.f / l;
+            *reinterpret_cast<uint2*>(out + h * KV8_HEAD + d) = make_uint2(pack(x[0] * r, x[1] * r), pack(x[2] * r, x[3] * r));
+        } else {
+            float* st = a.state + (((size_t)s * a.q_heads + kh * a.group + h) * a.slices + y) * STATE;
+            put2(st + 4 + d, x[0], x[1]);
+            put2(st + 6 + d, x[2], x[3]);
+            if (d == 0) put2(st, top, l);
         }
     }
-    bf16_t* d = out + ((size_t)s * q_heads + h) * KV8_HEAD;
-    d[i] = f2bf(l == 0.f ? 0.f : o0 / l);
-    d[i + 64] = f2bf(l == 0.f ? 0.f : o1 / l);
+    if (active == 1) return;
+    // The states acknowledged, then the count: the block that completes it joins the slices.
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __syncthreads();
+    uint32_t* counter = a.counter + (size_t)s * a.t.kv_heads + kh;
+    if (threadIdx.x == 0) last = __hip_atomic_fetch_add(counter, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == active - 1;
+    __syncthreads();
+    if (!last) return;
+    for (uint32_t e = threadIdx.x; e < a.group * (KV8_HEAD / 4); e += 256) {
+        const uint32_t h = e / (KV8_HEAD / 4), d = 4 * (e % (KV8_HEAD / 4));
+        const float* st = a.state + ((size_t)s * a.q_heads + kh * a.group + h) * a.slices * STATE;
+        float top = -INFINITY, l = 0.f;
+        f32x4 x = {0.f, 0.f, 0.f, 0.f};
+        for (uint32_t z = 0; z < active; ++z) top = fmaxf(top, get2(st + z * STATE).x);
+        for (uint32_t z = 0; z < active; ++z) {
+            const float2 ml = get2(st + z * STATE), x0 = get2(st + z * STATE + 4 + d), x1 = get2(st + z * STATE + 6 + d);
+            const float f = factor(ml.x, top);
+            l += f * ml.y;
+            x += f * f32x4{x0.x, x0.y, x1.x, x1.y};
+        }
+        const float r = l == 0.f ? 0.f : 1.f / l;
+        *reinterpret_cast<uint2*>(out + h * KV8_HEAD + d) = make_uint2(pack(x[0] * r, x[1] * r), pack(x[2] * r, x[3] * r));
+    }
+    if (threadIdx.x == 0) __hip_atomic_store(counter, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);  // for the next call
 }
 
 // The order of scores as whole numbers: larger scores larger, NaN above all.
@@ -333,9 +546,20 @@ extern "C" x0ne_status x0ne_gpu_kv8_read(x0ne_gpu* g, const x0ne_kv8* c, uint64_
     return X0NE_OK;
 }
 
+// Slices of a sequence's tiles: enough that the pairs of sequence and kv head fill 256 CUs with two blocks each.
+static uint32_t slices_of(const x0ne_kv8* c) {
+    const uint64_t pairs = std::max<uint64_t>(1, (uint64_t)c->seqs * c->kv_heads);
+    return (uint32_t)std::min<uint64_t>(MAX_SLICES, std::max<uint64_t>(16, 512 / pairs));
+}
+
+// The workspace: a counter per (sequence, kv head), then the states of attention or the scores of selection.
+static uint64_t counter_bytes(const x0ne_kv8* c) { return ((uint64_t)c->seqs * c->kv_heads * 4 + 255) / 256 * 256; }
+
 extern "C" uint64_t x0ne_kv8_work_bytes(const x0ne_kv8* c, uint32_t q_heads) {
-    if (!c || check_cache("kv8 workspace", c) != X0NE_OK || check_heads("kv8 workspace", c, q_heads) != X0NE_OK) return 0;
-    return std::max<uint64_t>(256, (uint64_t)c->seqs * c->kv_heads * c->seq_pages * 8);
+    if (check_cache("kv8 workspace", c) != X0NE_OK || check_heads("kv8 workspace", c, q_heads) != X0NE_OK) return 0;
+    const uint64_t states = (uint64_t)c->seqs * q_heads * slices_of(c) * STATE * 4;
+    const uint64_t scores = (uint64_t)c->seqs * c->kv_heads * c->seq_pages * 8;
+    return std::max<uint64_t>(256, counter_bytes(c) + std::max(states, scores));
 }
 
 extern "C" x0ne_status x0ne_gpu_kv8_attention(x0ne_gpu* g, const x0ne_kv8* c, uint64_t q, uint32_t q_heads, uint64_t lens,
@@ -353,9 +577,22 @@ extern "C" x0ne_status x0ne_gpu_kv8_attention(x0ne_gpu* g, const x0ne_kv8* c, ui
     if (c->seqs == 0) return X0NE_OK;
     const OnDevice on(g->device);
     g->counts.launches++;
-    hipLaunchKernelGGL(kv8_attention_kernel, dim3(q_heads, c->seqs), dim3(64), 0, g->stream, table_of(c),
-                       (const uint8_t*)c->codes, (const uint8_t*)c->scales, (const bf16_t*)q, (const uint32_t*)lens,
-                       (const uint32_t*)page_list, budget, (bf16_t*)out, q_heads, scale);
+    Attend a = {};
+    a.t = table_of(c);
+    a.codes = (const uint8_t*)c->codes;
+    a.scales = (const uint8_t*)c->scales;
+    a.q = (const bf16_t*)q;
+    a.lens = (const uint32_t*)lens;
+    a.list = (const uint32_t*)page_list;
+    a.out = (bf16_t*)out;
+    a.counter = (uint32_t*)work;
+    a.state = (float*)(work + counter_bytes(c));
+    a.budget = budget;
+    a.q_heads = q_heads;
+    a.group = q_heads / c->kv_heads;
+    a.slices = slices_of(c);
+    a.scale2 = scale * 1.44269504088896340736f;
+    hipLaunchKernelGGL(kv8_attention_kernel, dim3(c->kv_heads, a.slices, c->seqs), dim3(64 * ATTEND_WAVES), 0, g->stream, a);
     X0NE_HIP(hipGetLastError(), what);
     return X0NE_OK;
 }
@@ -377,7 +614,7 @@ extern "C" x0ne_status x0ne_gpu_kv8_select(x0ne_gpu* g, const x0ne_kv8* c, uint6
     g->counts.launches++;
     hipLaunchKernelGGL(kv8_select_kernel, dim3(c->kv_heads, c->seqs), dim3(256), 0, g->stream, table_of(c),
                        (const bf16_t*)bounds, (const bf16_t*)q, (const uint32_t*)lens, budget, (uint32_t*)page_list,
-                       (uint64_t*)work, q_heads);
+                       (uint64_t*)(work + counter_bytes(c)), q_heads);
     X0NE_HIP(hipGetLastError(), what);
     return X0NE_OK;
 }
