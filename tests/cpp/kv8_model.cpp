@@ -1,10 +1,12 @@
 // The 8-bit cache's own rules (csrc/kv8.h, included, not copied) on the host: the scale exponent of every
 // magnitude against its definition, page lookup with entries that are not there, offsets past 4 GiB, lengths
-// past the table. Exit status 0: all hold.
+// past the table, the selection's ranges. Exit status 0: all hold.
+#include <algorithm>
 #include <cmath>
 #include <cstdio>
 #include <cstdlib>
 #include <cstring>
+#include <vector>
 
 #include "kv8.h"
 
@@ -36,5 +38,46 @@ int main() {
     CHECK(kv8_record(0xFFFFFFFEu, 1024, 1023) == (0xFFFFFFFEull * 1024 + 1023) * 4096, "64-bit records");
     CHECK(kv8_scale(1u << 31, 8, 3) == ((1ull << 34) + 3) * 32 && kv8_bound(1u << 31, 8, 3) == ((1ull << 34) + 3) * 256, "64-bit offsets");
     CHECK(kv8_keys(0, 4) == 0 && kv8_keys(64, 4) == 64 && kv8_keys(65, 4) == 64 && kv8_keys(0xFFFFFFFFu, (1u << 24) - 1) == 16 * ((1u << 24) - 1), "lengths");
+    // The selection's passes over keys at both ends of 64 bits, equal ones among them: as a sort takes them.
+    uint64_t seed = 1;
+    auto random = [&] { return seed = seed * 6364136223846793005ull + 1442695040888963407ull, seed ^ seed >> 29; };
+    for (int round = 0; round < 3000; ++round) {
+        std::vector<uint64_t> keys(2 + random() % 60);
+        for (uint64_t& x : keys) {
+            const uint64_t r = random();
+            x = r % 7 == 0 ? ~0ull : r % 7 == 1 ? 0 : r % 7 == 2 ? ~0ull - random() % 5 : r % 7 == 3 ? random() % 3 : random() >> random() % 64;
+        }
+        const uint32_t take = 1 + random() % (keys.size() - 1);
+        uint64_t lo = *std::min_element(keys.begin(), keys.end()), hi = *std::max_element(keys.begin(), keys.end());
+        uint32_t need = take;
+        bool ties = true;
+        for (int pass = 0; pass < KV8_PASSES && lo != hi; ++pass) {
+            const int shift = kv8_shift(lo, hi);
+            std::vector<uint32_t> bin(2048, 0);
+            for (uint64_t x : keys)
+                if (x >= lo && x <= hi) {
+                    CHECK((x - lo) >> shift < 2048, "bin of %llx", (unsigned long long)x);
+                    ++bin[(x - lo) >> shift];
+                }
+            uint32_t above = 0;
+            int b = 2047;
+            while (above + bin[b] < need) above += bin[b--];
+            need -= above;
+            kv8_narrow(lo, hi, shift, (uint32_t)b);
+            CHECK(lo <= hi, "range %llx .. %llx", (unsigned long long)lo, (unsigned long long)hi);
+            if (bin[b] == need) {
+                ties = false;
+                break;
+            }
+        }
+        CHECK(!ties || lo == hi, "%d passes end at one key", KV8_PASSES);
+        std::vector<uint64_t> got, want = keys;
+        for (uint64_t x : keys)
+            if (ties ? x > lo || (x == lo && need && need--) : x >= lo) got.push_back(x);
+        std::sort(want.rbegin(), want.rend());
+        want.resize(take);
+        std::sort(got.rbegin(), got.rend());
+        CHECK(got == want, "%zu of %u keys", got.size(), take);
+    }
     std::puts("ok");
 }

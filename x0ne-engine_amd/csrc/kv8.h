@@ -61,3 +61,17 @@ KV8_BOTH int kv8_exponent(uint32_t magnitude) {
     const int e = (int)(magnitude >> 7) - 127 - ((magnitude & 0x7Fu) <= 0x60u ? 8 : 7);
     return e < KV8_LOWEST ? KV8_LOWEST : e;
 }
+
+// Radix selection of 64-bit keys over the range lo .. hi (lo < hi) that holds the undecided ones: its keys fall into
+// 2048 bins, (key - lo) >> shift; then one bin's range takes its place. The range loses 11 bits each time, so KV8_PASSES
+// of them end at a single key. The bin's end is not computed where it would pass hi (it can pass 2^64 there).
+constexpr int KV8_PASSES = 6;
+KV8_BOTH int kv8_shift(uint64_t lo, uint64_t hi) {
+    const int bits = 64 - __builtin_clzll(hi - lo);
+    return bits > 11 ? bits - 11 : 0;
+}
+KV8_BOTH void kv8_narrow(uint64_t& lo, uint64_t& hi, int shift, uint32_t bin) {
+    const uint64_t span = (1ull << shift) - 1;
+    lo += (uint64_t)bin << shift;
+    if (hi - lo > span) hi = lo + span;
+}

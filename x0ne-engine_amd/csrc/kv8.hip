@@ -184,279 +184,617 @@ struct Attend {
     bf16_t* out;
     float* state;
     uint32_t* counter;
-    uint32_t budget, q_heads, group, slices;
+    uint32_t budget, q_heads, group, slices, rounds;
     float scale2;  // the scale times log2 e: a weight is one exp2
 };
 
-// Decode attention. A block of 4 wavefronts takes a slice of one sequence's tiles for the q heads of one kv head,
-// wavefront w the slice's tiles w, w + 4, ...; a tile is 4 pages. The products are S^T = K Q^T and O^T = V^T P^T on
-// the matrix cores (16 x 16 x 32, bf16 with f32 sums), the group's heads the 16 columns: lane (n = lane % 16, g =
-// lane / 16) holds column n, so the softmax of a head is lane-local but for the four lanes n, n + 16, n + 32, n + 48.
-// Codes become bf16 in one conversion, keys times their scale (exact); a value's scale goes into its weight (exact).
+struct Shared {
+    float wm[ATTEND_WAVES][MAX_GROUP], wl[ATTEND_WAVES][MAX_GROUP];
+    float wo[ATTEND_WAVES][MAX_GROUP][KV8_HEAD + 4];
+    float m[MAX_GROUP][MAX_SLICES], l[MAX_GROUP][MAX_SLICES];  // the join's: each slice's maximum (then factor) and sum
+    uint32_t last;
+};
+
+// The slices' states of a group's heads joined, in slice order within each part: a thread has four dims of one head
+// and, for a group of at most 4 heads, every second, fourth .. slice (the parts meet in LDS). All of a thread's
+// loads of up to JOIN_AHEAD slices are requested before the maxima are known, so they cost one round trip.
+constexpr uint32_t JOIN_AHEAD = 8;
+__device__ __forceinline__ void join(const Attend& a, const float* __restrict__ st, bf16_t* __restrict__ out,
+                                     uint32_t active, Shared& sh) {
+    const uint32_t t = threadIdx.x, quads = a.group * (KV8_HEAD / 4);
+    const uint32_t parts = quads <= 64 ? 4 : quads <= 128 ? 2 : 1;
+    const uint32_t part = t / (256 / parts), first = t % (256 / parts);
+    auto request = [&](uint32_t e, uint32_t z0, f32x4 (&x)[JOIN_AHEAD]) {
+        const float* p = st + (size_t)(e / (KV8_HEAD / 4)) * a.slices * STATE + 4 + 4 * (e % (KV8_HEAD / 4));
+#pragma unroll
+        for (uint32_t i = 0; i < JOIN_AHEAD; ++i) {
+            const uint32_t z = z0 + i * parts;
+            if (z < active && e < quads) {
+                const float2 u = get2(p + z * STATE), v = get2(p + z * STATE + 2);
+                x[i] = f32x4{u.x, u.y, v.x, v.y};
+            }
+        }
+    };
+    f32x4 ahead[JOIN_AHEAD];
+    request(first, part, ahead);
+    for (uint32_t i = t; i < a.group * active; i += 256) {
+        const uint32_t h = i / active, z = i % active;
+        const float2 ml = get2(st + ((size_t)h * a.slices + z) * STATE);
+        sh.m[h][z] = ml.x;
+        sh.l[h][z] = ml.y;
+    }
+    lds_barrier();
+    // Each head's factors and sum by one wavefront, a lane per slice.
+    for (uint32_t h = t / 64; h < a.group; h += 4) {
+        const uint32_t z = t % 64;
+        const float m = z < active ? sh.m[h][z] : -INFINITY, f = factor(m, wave_max(m));
+        if (z < active) sh.m[h][z] = f;
+        const float l = wave_sum(z < active ? f * sh.l[h][z] : 0.f);
+        if (z == 0) sh.wl[0][h] = l;
+    }
+    lds_barrier();
+    auto sum = [&](uint32_t e) -> f32x4 {
+        const uint32_t h = e / (KV8_HEAD / 4);
+        f32x4 x = {0.f, 0.f, 0.f, 0.f};
+        for (uint32_t z0 = part; z0 < active; z0 += JOIN_AHEAD * parts) {
+            if (e != first || z0 != part) request(e, z0, ahead);
+#pragma unroll
+            for (uint32_t i = 0; i < JOIN_AHEAD; ++i)
+                if (z0 + i * parts < active) x += sh.m[h][z0 + i * parts] * ahead[i];
+        }
+        return x;
+    };
+    auto store = [&](uint32_t e, f32x4 x) {
+        const uint32_t h = e / (KV8_HEAD / 4);
+        const float l = sh.wl[0][h], r = l == 0.f ? 0.f : 1.f / l;
+        *reinterpret_cast<uint2*>(out + 4 * e) = make_uint2(pack(x[0] * r, x[1] * r), pack(x[2] * r, x[3] * r));
+    };
+    if (parts == 1) {
+        for (uint32_t e = first; e < quads; e += 256) store(e, sum(e));  // twice for more than 8 heads
+        return;
+    }
+    float* mine = &sh.wo[0][0][0] + 4 * t;
+    f32x4 x = {0.f, 0.f, 0.f, 0.f};
+    if (first < quads) x = sum(first);
+    *reinterpret_cast<f32x4*>(mine) = x;
+    lds_barrier();
+    if (part || first >= quads) return;
+    for (uint32_t w = 1; w < parts; ++w) x += *reinterpret_cast<const f32x4*>(mine + 4 * w * (256 / parts));
+    store(first, x);
+}
+
+// The slices of sequences: a sequence's tiles are cut into `active` slices of `per` tiles, by its own length and
+// the call's `slices` and `rounds` only. A block walks every gridDim.y-th slice of its kv head and its 64 sequences:
+// lane l of each wavefront holds sequence l's length and the slices up to and with it.
+struct Item {
+    uint32_t s, y, keys, pages, np, per, active, t0, t_end;  // sequence and slice; this wavefront's tiles t0, t0 + 4 ..
+    __device__ __forceinline__ bool any() const { return t0 < t_end; }
+};
+
+// Decode attention. A block of 4 wavefronts takes slices of the sequences' tiles for the q heads of one kv head, one
+// after the other, wavefront w a slice's tiles w, w + 4, ...; a tile is 4 pages. The products are S^T = K Q^T and
+// O^T = V^T P^T on the matrix cores (16 x 16 x 32, bf16 with f32 sums), the group's heads the 16 columns: lane
+// (n = lane % 16, g = lane / 16) holds column n, so the softmax of a head is lane-local but for the four lanes n,
+// n + 16, n + 32, n + 48. Codes become bf16 in one conversion, keys times their scale (exact); a value's scale goes
+// into its weight (exact).
 //  - Product m's row r = 4 g' + i is key 4 m + i of the tile's page g': its 16 outputs per lane are then the 16 keys of
 //    page g, and with the value of dim 16 c + n at those keys as row n of product c (one 16-byte load: V is dim-major)
 //    the weights are an operand as they lie, without a move between lanes.
 //  - Dims of a product's k step j are 32 g + 8 j ..: a lane's keys come as two 16-byte loads.
 //  - Weights enter as bf16 hi + lo (2^-17 of the weight): one bf16 would add as much error as the output's rounding.
-// The running maximum and sum are f32. A slice's state (m, l, o) is joined by the last block of its (sequence, kv head)
-// to count itself, slices in order; a sequence of one slice is written at once. Keys past the length, entries behind a
-// list and pages that are not there weigh 0, their values are taken as 0.
-__global__ void __launch_bounds__(64 * ATTEND_WAVES) kv8_attention_kernel(const Attend a) {
-    __shared__ float wm[ATTEND_WAVES][MAX_GROUP], wl[ATTEND_WAVES][MAX_GROUP];
-    __shared__ float wo[ATTEND_WAVES][MAX_GROUP][KV8_HEAD + 4];
-    __shared__ uint32_t last;
-    const uint32_t kh = blockIdx.x, y = blockIdx.y, s = blockIdx.z;
+// The next tile's keys are requested behind the scores, its values behind the value products; the next slice's first
+// tile and queries likewise, so the memory is busy while a slice's states are joined. The running maximum and sum are
+// f32. A slice's state (m, l, o) is joined by the last block of its (sequence, kv head) to count itself, slices in
+// order; a sequence of one slice is written at once. Keys past the length, entries behind a list and pages that are
+// not there weigh 0, their values are taken as 0.
+__global__ void __launch_bounds__(64 * ATTEND_WAVES, 2) kv8_attention_kernel(const Attend a) {
+    __shared__ Shared sh;
+    const uint32_t kh = blockIdx.x, s0 = blockIdx.z * 64, step = ATTEND_WAVES;
     const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), n = lane & 15, g = lane >> 4;
-    const uint32_t keys = kv8_keys(a.lens[s], a.t.seq_pages), pages = (keys + KV8_PAGE - 1) / KV8_PAGE;
-    const uint32_t np = a.list ? min(a.budget, pages) : pages, tiles = (np + TILE_PAGES - 1) / TILE_PAGES;
-    bf16_t* out = a.out + ((size_t)s * a.q_heads + kh * a.group) * KV8_HEAD;
-    if (tiles == 0) {
-        if (y == 0)
-            for (uint32_t e = threadIdx.x; e < a.group * KV8_HEAD / 8; e += 256) reinterpret_cast<uint4*>(out)[e] = make_uint4(0, 0, 0, 0);
-        return;
+    auto shape = [&](uint32_t keys) -> Item {
+        Item it = {};
+        it.keys = keys;
+        it.pages = (keys + KV8_PAGE - 1) / KV8_PAGE;
+        it.np = a.list ? min(a.budget, it.pages) : it.pages;
+        const uint32_t tiles = (it.np + TILE_PAGES - 1) / TILE_PAGES, rounds = (tiles + ATTEND_WAVES - 1) / ATTEND_WAVES;
+        it.active = max(1u, min(a.slices, (rounds + a.rounds - 1) / a.rounds));
+        it.per = ATTEND_WAVES * max(1u, (rounds + it.active - 1) / it.active);
+        it.active = max(1u, (tiles + it.per - 1) / it.per);
+        it.t_end = tiles;
+        return it;
+    };
+    uint32_t my_keys = s0 + lane < a.t.seqs ? kv8_keys(a.lens[s0 + lane], a.t.seq_pages) : 0u, my_seq = lane;
+    uint32_t mine = s0 + lane < a.t.seqs ? shape(my_keys).active : 0u;
+    auto up_to = [&](uint32_t x) -> uint32_t {
+#pragma unroll
+        for (int d = 1; d < 64; d <<= 1) {
+            const uint32_t below = __shfl_up(x, d, 64);
+            if (lane >= (uint32_t)d) x += below;
+        }
+        return x;
+    };
+    uint32_t upto = up_to(mine);
+    const uint32_t total = __builtin_amdgcn_readlane(upto, 63), blocks = gridDim.y;
+    if (total > blocks) {  // several slices per block: the longest sequences' first
+        uint32_t rank = 0;
+        for (int j = 0; j < 64; ++j) {
+            const uint32_t other = __builtin_amdgcn_readlane(my_keys, j);
+            rank += other > my_keys || (other == my_keys && (uint32_t)j < lane);
+        }
+        my_seq = (uint32_t)__builtin_amdgcn_ds_permute((int)(4 * rank), (int)lane);
+        my_keys = (uint32_t)__builtin_amdgcn_ds_permute((int)(4 * rank), (int)my_keys);
+        upto = up_to((uint32_t)__builtin_amdgcn_ds_permute((int)(4 * rank), (int)mine));
     }
-    const uint32_t rounds = (tiles + ATTEND_WAVES - 1) / ATTEND_WAVES;
-    const uint32_t per = ATTEND_WAVES * ((rounds + a.slices - 1) / a.slices), active = (tiles + per - 1) / per;
-    if (y >= active) return;
-    const uint32_t t_end = min(tiles, (y + 1) * per);
+    // A block's slice of round r, the rounds to and fro over the blocks.
+    auto item = [&](uint32_t r) -> Item {
+        const uint32_t i = r * blocks + (r & 1 ? blocks - 1 - blockIdx.y : blockIdx.y);
+        if (i >= total) return Item{};
+        const uint32_t at = (uint32_t)__popcll(__ballot(upto <= i));
+        Item it = shape(__builtin_amdgcn_readlane(my_keys, at));
+        it.s = s0 + __builtin_amdgcn_readlane(my_seq, at);
+        it.y = i - (__builtin_amdgcn_readlane(upto, at) - it.active);
+        it.t0 = it.y * it.per + wave;
+        it.t_end = min(it.t_end, (it.y + 1) * it.per);
+        return it;
+    };
 
-    // The page of the tile at index 4 t + j, with how many of its keys count.
-    const uint32_t* list = a.list ? a.list + ((size_t)s * a.t.kv_heads + kh) * a.budget : nullptr;
+    // A lane's page of a tile is the one at index 4 t + g: its logical number (from the list two tiles ahead), its
+    // table entry (one tile ahead), and then the physical page with how many of its keys count.
     struct Place {
         uint32_t page, valid;
     };
-    auto logical_of = [&](uint32_t t, uint32_t j) -> uint32_t {
-        const uint32_t at = TILE_PAGES * t + j;
-        return t >= t_end || at >= np ? KV8_NONE : list ? list[at] : at;
+    auto logical_at = [&](const Item& it, uint32_t t) -> uint32_t {
+        const uint32_t at = TILE_PAGES * t + g;
+        if (t >= it.t_end || at >= it.np) return KV8_NONE;
+        return a.list ? a.list[((size_t)it.s * a.t.kv_heads + kh) * a.budget + at] : at;
     };
-    auto place = [&](uint32_t logical) -> Place {
-        const uint32_t page = logical < pages ? a.t.page(s, logical) : KV8_NONE;
-        return page == KV8_NONE ? Place{0u, 0u} : Place{page, (uint32_t)min(keys - logical * KV8_PAGE, KV8_PAGE)};
+    auto entry_of = [&](const Item& it, uint32_t logical) -> uint32_t {
+        return logical < it.pages ? a.t.pages[(size_t)it.s * a.t.seq_pages + logical] : KV8_NONE;
     };
-    u32x4 k[4][2], v[8], ks, vs;
-    auto load_k = [&](uint32_t page) {
-        const uint8_t* p = a.codes + kv8_record(page, a.t.kv_heads, kh) + (n & 3) * KV8_HEAD + 32 * g;
+    auto place = [&](const Item& it, uint32_t logical, uint32_t entry) -> Place {
+        if (entry >= a.t.pool) return Place{0u, 0u};
+        return Place{entry, (uint32_t)min(it.keys - logical * KV8_PAGE, KV8_PAGE)};
+    };
+    u32x4 k[4][2], v[8], ks, vs, qb[4];
+    auto key_at = [&](uint32_t page) -> const uint8_t* {
+        return a.codes + kv8_record(page, a.t.kv_heads, kh) + (n & 3) * KV8_HEAD + 32 * g;
+    };
+    auto key_scales = [&](uint32_t page) { return reinterpret_cast<const u32x4*>(a.scales + kv8_scale(page, a.t.kv_heads, kh)); };
+    auto value_at = [&](uint32_t page) -> const uint8_t* {
+        return a.codes + kv8_record(page, a.t.kv_heads, kh) + KV8_PART + n * KV8_PAGE;
+    };
+    // The lanes of row n of a key product take page n / 4, the page of the lanes 16 (n / 4) ...
+    auto key_page = [&](uint32_t page) -> uint32_t { return __shfl(page, 16 * (n >> 2), 64); };
+    auto load_k = [&](const uint8_t* p, int m) {
+        k[m][0] = *reinterpret_cast<const u32x4*>(p + m * 4 * KV8_HEAD);
+        k[m][1] = *reinterpret_cast<const u32x4*>(p + m * 4 * KV8_HEAD + 16);
+    };
+    auto load_v = [&](const uint8_t* p, int c) { v[c] = *reinterpret_cast<const u32x4*>(p + c * 16 * KV8_PAGE); };
+    // Columns past the group repeat its last head: their results are not used.
+    auto load_q = [&](const Item& it) {
+        const bf16_t* p = a.q + ((size_t)it.s * a.q_heads + kh * a.group + min(n, a.group - 1)) * KV8_HEAD + 32 * g;
 #pragma unroll
-        for (int m = 0; m < 4; ++m) {
-            k[m][0] = *reinterpret_cast<const u32x4*>(p + m * 4 * KV8_HEAD);
-            k[m][1] = *reinterpret_cast<const u32x4*>(p + m * 4 * KV8_HEAD + 16);
-        }
-        ks = *reinterpret_cast<const u32x4*>(a.scales + kv8_scale(page, a.t.kv_heads, kh));
+        for (int j = 0; j < 4; ++j) qb[j] = reinterpret_cast<const u32x4*>(p)[j];
     };
-    auto load_v = [&](uint32_t page) {
-        const uint8_t* p = a.codes + kv8_record(page, a.t.kv_heads, kh) + KV8_PART + n * KV8_PAGE;
+    auto load_first = [&](const Item& it, const Place& at) {
+        const uint32_t page = key_page(at.page);
+        const uint8_t *kp = key_at(page), *vp = value_at(at.page);
+        ks = *key_scales(page);
 #pragma unroll
-        for (int c = 0; c < 8; ++c) v[c] = *reinterpret_cast<const u32x4*>(p + c * 16 * KV8_PAGE);
-        vs = *reinterpret_cast<const u32x4*>(a.scales + kv8_scale(page, a.t.kv_heads, kh) + KV8_PAGE);
+        for (int m = 0; m < 4; ++m) load_k(kp, m);
+        vs = key_scales(at.page)[1];
+#pragma unroll
+        for (int c = 0; c < 8; ++c) load_v(vp, c);
+        load_q(it);
     };
-    const uint32_t t0 = y * per + wave, step = ATTEND_WAVES;
-    Place pk = place(logical_of(t0, n >> 2)), pv = place(logical_of(t0, g));
-    u32x4 qb[4];
-    if (t0 < t_end) {
-        load_k(pk.page);
-        load_v(pv.page);
-    }
-    const bf16_t* qr = a.q + ((size_t)s * a.q_heads + kh * a.group + min(n, a.group - 1)) * KV8_HEAD + 32 * g;
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-        qb[j] = reinterpret_cast<const u32x4*>(qr)[j];
-        if (n >= a.group) qb[j] = u32x4{0, 0, 0, 0};
-    }
-    Place pk1 = place(logical_of(t0 + step, n >> 2)), pv1 = place(logical_of(t0 + step, g));
-    uint32_t lk2 = logical_of(t0 + 2 * step, n >> 2), lv2 = logical_of(t0 + 2 * step, g);
 
-    float m_run = -INFINITY, lsum = 0.f;
-    f32x4 o[8];
+    Item it = item(0);
+    if (!it.active) return;
+    // A slice whose states are written but not counted: its sequence and how many slices that has. The block that
+    // counts the last one joins them.
+    struct Waiting {
+        uint32_t s, active;
+    };
+    auto counter_of = [&](const Waiting& w) { return a.counter + (size_t)w.s * a.t.kv_heads + kh; };
+    auto finish = [&](const Waiting& w) {
+        if (threadIdx.x == 0) __hip_atomic_store(counter_of(w), 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);  // for the next call
+        const size_t head = (size_t)w.s * a.q_heads + kh * a.group;
+        join(a, a.state + head * a.slices * STATE, a.out + head * KV8_HEAD, w.active, sh);
+    };
+    uint32_t l0 = logical_at(it, it.t0), l1 = logical_at(it, it.t0 + step), l2 = logical_at(it, it.t0 + 2 * step);
+    uint32_t e0 = entry_of(it, l0), e1 = entry_of(it, l1);
+    Place here = place(it, l0, e0);
+    if (it.any()) load_first(it, here);
+    Waiting waiting = {};
+    for (uint32_t r = 1;; ++r) {
+        const Item next = item(r);
+        const uint32_t n0 = logical_at(next, next.t0), n1 = logical_at(next, next.t0 + step), n2 = logical_at(next, next.t0 + 2 * step);
+        const uint32_t f0 = entry_of(next, n0), f1 = entry_of(next, n1);
+        float m_run = -INFINITY, lsum = 0.f;
+        f32x4 o[8];
 #pragma unroll
-    for (int c = 0; c < 8; ++c) o[c] = f32x4{0.f, 0.f, 0.f, 0.f};
-    for (uint32_t t = t0; t < t_end; t += step) {
-        float sc[4][4];
-#pragma unroll
-        for (int m = 0; m < 4; ++m) {
-            const float scale = __uint_as_float(((ks[m] >> (8 * (n & 3))) & 0xFFu) << 23);
-            f32x4 acc = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-            for (int j = 0; j < 4; ++j) acc = mfma(decode(k[m][j >> 1][2 * (j & 1)], k[m][j >> 1][2 * (j & 1) + 1], scale), qb[j], acc);
-#pragma unroll
-            for (int i = 0; i < 4; ++i) sc[m][i] = acc[i] * a.scale2;
-        }
-        if (t + step < t_end) load_k(pk1.page);
-        const bool whole = __all(pv.valid == KV8_PAGE);
-        uint32_t keep[4];
-        if (!whole) {
+        for (int c = 0; c < 8; ++c) o[c] = f32x4{0.f, 0.f, 0.f, 0.f};
+        for (uint32_t t = it.t0; t < it.t_end; t += step) {
+            const uint32_t e2 = entry_of(it, l2), l3 = logical_at(it, t + 3 * step);
+            // The tile behind this one: of this slice, the first of the next, or (behind the last) page 0, without use.
+            const bool more = t + step < it.t_end;
+            const Place then = more ? place(it, l1, e1) : place(next, n0, f0);
+            const uint32_t then_page = key_page(then.page);
+            const uint8_t *kp = key_at(then_page), *vp = value_at(then.page);
+            float sc[4][4];
 #pragma unroll
             for (int m = 0; m < 4; ++m) {
-                const int left = (int)pv.valid - 4 * m;
-                keep[m] = left >= 4 ? 0xFFFFFFFFu : left <= 0 ? 0u : (1u << (8 * left)) - 1u;
+                const float scale = __uint_as_float(((ks[m] >> (8 * (n & 3))) & 0xFFu) << 23);
+                f32x4 acc = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-                for (int i = 0; i < 4; ++i)
-                    if (i >= left) sc[m][i] = -INFINITY;
-                vs[m] &= keep[m];
+                for (int j = 0; j < 4; ++j) acc = mfma(decode(k[m][j >> 1][2 * (j & 1)], k[m][j >> 1][2 * (j & 1) + 1], scale), qb[j], acc);
+                load_k(kp, m);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) sc[m][e] = acc[e] * a.scale2;
             }
-        }
-        float mx = -INFINITY;
+            ks = *key_scales(then_page);
+            if (!more && next.any()) load_q(next);
+            const bool whole = __all(here.valid == KV8_PAGE);
+            uint32_t keep[4];
+            if (!whole) {
 #pragma unroll
-        for (int m = 0; m < 4; ++m)
+                for (int m = 0; m < 4; ++m) {
+                    const int left = (int)here.valid - 4 * m;
+                    keep[m] = left >= 4 ? 0xFFFFFFFFu : left <= 0 ? 0u : (1u << (8 * left)) - 1u;
 #pragma unroll
-            for (int i = 0; i < 4; ++i) mx = fmaxf(mx, sc[m][i]);
-        mx = fmaxf(m_run, rows_max(mx));
-        if (__any(mx > m_run)) {
-            const float alpha = factor(m_run, mx);
-            lsum *= alpha;
+                    for (int e = 0; e < 4; ++e)
+                        if (e >= left) sc[m][e] = -INFINITY;
+                    vs[m] &= keep[m];
 #pragma unroll
-            for (int c = 0; c < 8; ++c) o[c] *= alpha;
-            m_run = mx;
-        }
-        const float ref = m_run == -INFINITY ? 0.f : m_run;
-        u32x4 hi[2], lo[2];
-#pragma unroll
-        for (int m = 0; m < 4; ++m) {
-            float w[4];
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const float p = __builtin_amdgcn_exp2f(sc[m][i] - ref);
-                lsum += p;
-                w[i] = p * __uint_as_float(((vs[m] >> (8 * i)) & 0xFFu) << 23);
+                    for (int c = 0; c < 8; ++c) v[c][m] &= keep[m];
+                }
             }
+            float mx = -INFINITY;
 #pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                const uint32_t h = pack(w[2 * i], w[2 * i + 1]);
-                hi[m >> 1][2 * (m & 1) + i] = h;
-                lo[m >> 1][2 * (m & 1) + i] = pack(w[2 * i] - bf_lo(h), w[2 * i + 1] - bf_hi(h));
+            for (int m = 0; m < 4; ++m)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) mx = fmaxf(mx, sc[m][e]);
+            mx = fmaxf(m_run, rows_max(mx));
+            if (__any(mx > m_run)) {
+                const float alpha = factor(m_run, mx);
+                lsum *= alpha;
+#pragma unroll
+                for (int c = 0; c < 8; ++c) o[c] *= alpha;
+                m_run = mx;
             }
-        }
+            const float ref = m_run == -INFINITY ? 0.f : m_run;
+            u32x4 hi[2], lo[2];
 #pragma unroll
-        for (int c = 0; c < 8; ++c) {
-            if (!whole) v[c] &= u32x4{keep[0], keep[1], keep[2], keep[3]};
+            for (int m = 0; m < 4; ++m) {
+                float w[4];
 #pragma unroll
-            for (int j = 0; j < 2; ++j) {
-                const u32x4 x = decode(v[c][2 * j], v[c][2 * j + 1], 1.f);
-                o[c] = mfma(x, hi[j], o[c]);
-                o[c] = mfma(x, lo[j], o[c]);
+                for (int e = 0; e < 4; ++e) {
+                    const float p = __builtin_amdgcn_exp2f(sc[m][e] - ref);
+                    lsum += p;
+                    w[e] = p * __uint_as_float(((vs[m] >> (8 * e)) & 0xFFu) << 23);
+                }
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    const uint32_t h = pack(w[2 * e], w[2 * e + 1]);
+                    hi[m >> 1][2 * (m & 1) + e] = h;
+                    lo[m >> 1][2 * (m & 1) + e] = pack(w[2 * e] - bf_lo(h), w[2 * e + 1] - bf_hi(h));
+                }
             }
+            vs = key_scales(then.page)[1];
+#pragma unroll
+            for (int c = 0; c < 8; ++c) {
+#pragma unroll
+                for (int j = 0; j < 2; ++j) {
+                    const u32x4 x = decode(v[c][2 * j], v[c][2 * j + 1], 1.f);
+                    o[c] = mfma(x, hi[j], o[c]);
+                    o[c] = mfma(x, lo[j], o[c]);
+                }
+                load_v(vp, c);
+            }
+            here = then;
+            l1 = l2;
+            e1 = e2;
+            l2 = l3;
         }
-        pk = pk1;
-        pv = pv1;
-        pk1 = place(lk2);
-        pv1 = place(lv2);
-        lk2 = logical_of(t + 3 * step, n >> 2);
-        lv2 = logical_of(t + 3 * step, g);
-        if (t + step < t_end) load_v(pv.page);
-    }
-    lsum = rows_sum(lsum);
+        if (!it.any() && next.any()) {
+            here = place(next, n0, f0);
+            load_first(next, here);
+        }
+        lsum = rows_sum(lsum);
 
-    // The block's four states.
-    if (n < a.group) {
-        if (g == 0) {
-            wm[wave][n] = m_run;
-            wl[wave][n] = lsum;
-        }
+        // The block's four states meet; then the output, or the slice's state. The states of the slice before are
+        // counted here: this wavefront's stores of them are older than the loads of at least one tile.
+        if (n < a.group) {
+            if (g == 0) {
+                sh.wm[wave][n] = m_run;
+                sh.wl[wave][n] = lsum;
+            }
 #pragma unroll
-        for (int c = 0; c < 8; ++c) *reinterpret_cast<f32x4*>(&wo[wave][n][16 * c + 4 * g]) = o[c];
+            for (int c = 0; c < 8; ++c) *reinterpret_cast<f32x4*>(&sh.wo[wave][n][16 * c + 4 * g]) = o[c];
+        }
+        if (waiting.active) {
+            if (it.any() && next.any())
+                asm volatile("s_waitcnt vmcnt(16)" ::: "memory");
+            else
+                asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        }
+        lds_barrier();
+        uint32_t before = 0;
+        if (waiting.active && threadIdx.x == 0)
+            before = __hip_atomic_fetch_add(counter_of(waiting), 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        bf16_t* out = a.out + ((size_t)it.s * a.q_heads + kh * a.group) * KV8_HEAD;
+        float* state = a.state + ((size_t)it.s * a.q_heads + kh * a.group) * a.slices * STATE;
+        for (uint32_t e = threadIdx.x; e < a.group * (KV8_HEAD / 4); e += 64 * ATTEND_WAVES) {
+            const uint32_t h = e / (KV8_HEAD / 4), d = 4 * (e % (KV8_HEAD / 4));
+            float top = sh.wm[0][h], l = 0.f;
+            f32x4 x = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (uint32_t w = 1; w < ATTEND_WAVES; ++w) top = fmaxf(top, sh.wm[w][h]);
+#pragma unroll
+            for (uint32_t w = 0; w < ATTEND_WAVES; ++w) {
+                const float f = factor(sh.wm[w][h], top);
+                l += f * sh.wl[w][h];
+                x += f * *reinterpret_cast<const f32x4*>(&sh.wo[w][h][d]);
+            }
+            if (it.active == 1) {
+                const float r = l == 0.f ? 0.f : 1.f / l;
+                *reinterpret_cast<uint2*>(out + h * KV8_HEAD + d) = make_uint2(pack(x[0] * r, x[1] * r), pack(x[2] * r, x[3] * r));
+            } else {
+                float* st = state + ((size_t)h * a.slices + it.y) * STATE;
+                put2(st + 4 + d, x[0], x[1]);
+                put2(st + 6 + d, x[2], x[3]);
+                if (d == 0) put2(st, top, l);
+            }
+        }
+        if (waiting.active) {
+            if (threadIdx.x == 0) sh.last = before == waiting.active - 1;
+            lds_barrier();
+            if (sh.last) finish(waiting);
+        }
+        waiting = it.active > 1 ? Waiting{it.s, it.active} : Waiting{};
+        if (!next.active) break;
+        lds_barrier();  // the states in LDS are read
+        it = next;
+        l1 = n1;
+        e1 = f1;
+        l2 = n2;
     }
-    __syncthreads();
-    for (uint32_t e = threadIdx.x; e < a.group * (KV8_HEAD / 4); e += 256) {
-        const uint32_t h = e / (KV8_HEAD / 4), d = 4 * (e % (KV8_HEAD / 4));
-        float top = wm[0][h], l = 0.f;
-        f32x4 x = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (uint32_t w = 1; w < ATTEND_WAVES; ++w) top = fmaxf(top, wm[w][h]);
-#pragma unroll
-        for (uint32_t w = 0; w < ATTEND_WAVES; ++w) {
-            const float f = factor(wm[w][h], top);
-            l += f * wl[w][h];
-            x += f * *reinterpret_cast<const f32x4*>(&wo[w][h][d]);
-        }
-        if (active == 1) {
-            const float r = l == 0.f ? 0.f : 1.f / l;
-            *reinterpret_cast<uint2*>(out + h * KV8_HEAD + d) = make_uint2(pack(x[0] * r, x[1] * r), pack(x[2] * r, x[3] * r));
-        } else {
-            float* st = a.state + (((size_t)s * a.q_heads + kh * a.group + h) * a.slices + y) * STATE;
-            put2(st + 4 + d, x[0], x[1]);
-            put2(st + 6 + d, x[2], x[3]);
-            if (d == 0) put2(st, top, l);
-        }
-    }
-    if (active == 1) return;
-    // The states acknowledged, then the count: the block that completes it joins the slices.
+    if (!waiting.active) return;
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    __syncthreads();
-    uint32_t* counter = a.counter + (size_t)s * a.t.kv_heads + kh;
-    if (threadIdx.x == 0) last = __hip_atomic_fetch_add(counter, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == active - 1;
-    __syncthreads();
-    if (!last) return;
-    for (uint32_t e = threadIdx.x; e < a.group * (KV8_HEAD / 4); e += 256) {
-        const uint32_t h = e / (KV8_HEAD / 4), d = 4 * (e % (KV8_HEAD / 4));
-        const float* st = a.state + ((size_t)s * a.q_heads + kh * a.group + h) * a.slices * STATE;
-        float top = -INFINITY, l = 0.f;
-        f32x4 x = {0.f, 0.f, 0.f, 0.f};
-        for (uint32_t z = 0; z < active; ++z) top = fmaxf(top, get2(st + z * STATE).x);
-        for (uint32_t z = 0; z < active; ++z) {
-            const float2 ml = get2(st + z * STATE), x0 = get2(st + z * STATE + 4 + d), x1 = get2(st + z * STATE + 6 + d);
-            const float f = factor(ml.x, top);
-            l += f * ml.y;
-            x += f * f32x4{x0.x, x0.y, x1.x, x1.y};
-        }
-        const float r = l == 0.f ? 0.f : 1.f / l;
-        *reinterpret_cast<uint2*>(out + h * KV8_HEAD + d) = make_uint2(pack(x[0] * r, x[1] * r), pack(x[2] * r, x[3] * r));
-    }
-    if (threadIdx.x == 0) __hip_atomic_store(counter, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);  // for the next call
+    lds_barrier();
+    if (threadIdx.x == 0)
+        sh.last = __hip_atomic_fetch_add(counter_of(waiting), 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == waiting.active - 1;
+    lds_barrier();
+    if (sh.last) finish(waiting);
 }
 
-// The order of scores as whole numbers: larger scores larger, NaN above all.
+// The order of scores as whole numbers: larger scores larger, zeros of either sign equal, NaN above all, 0 below all
+// (for a page that is not there).
 __device__ __forceinline__ uint64_t score_key(double x) {
-    if (x != x) return ~1ull;
+    if (x != x) return ~0ull;
     const uint64_t b = (uint64_t)__double_as_longlong(x + 0.0);
     return b >> 63 ? ~b : b | 0x8000000000000000ull;
 }
 
-// The pages of (sequence, kv head): scores in f64, then each page's rank by counting the better ones. The
-// last page comes before all others; a page that is not there comes behind them.
+constexpr uint32_t SELECT_PAGES = 64;     // pages that a block scores, 16 per wavefront
+constexpr uint32_t SELECT_KEYS = 16;      // keys that a thread holds while a block selects: 4096 pages at once
+constexpr uint32_t SELECT_BINS = 2048;
+
+struct SelectShared {
+    union {
+        double q[MAX_GROUP][KV8_HEAD];
+        uint32_t bin[SELECT_BINS];
+    };
+    uint64_t low[4], high[4];
+    uint32_t part[4], count[SELECT_KEYS * 4], equal[SELECT_KEYS * 4];
+    uint32_t found, above, inside, last;
+};
+
+__device__ __forceinline__ uint32_t wave_up_to(uint32_t x) {
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+        const uint32_t below = __shfl_up(x, d, 64);
+        if ((threadIdx.x & 63) >= (uint32_t)d) x += below;
+    }
+    return x;
+}
+
+// The `take` largest of n keys (0 < take < n; ties to the lower index), their indices ascending in `to`. Radix
+// selection over the range of the keys that are still undecided, 11 bits at a time: the range is that of the keys and
+// not of all numbers, so scores of one sign and size are told apart in a pass or two. A thread holds keys t, t + 256,
+// ...; more than 4096 are read again in each pass.
+__device__ void select_keys(const uint64_t* __restrict__ keys, uint32_t n, uint32_t take, uint32_t* __restrict__ to,
+                            SelectShared& sh) {
+    constexpr uint32_t AT_ONCE = SELECT_KEYS * 256;
+    const uint32_t t = threadIdx.x, lane = t & 63, wave = t >> 6;
+    uint64_t key[SELECT_KEYS];
+    auto load = [&](uint32_t first) {
+#pragma unroll
+        for (uint32_t j = 0; j < SELECT_KEYS; ++j) {
+            const uint32_t at = first + 256 * j + t;
+            if (at < n) key[j] = __hip_atomic_load(keys + at, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        }
+    };
+    auto each = [&](auto&& f) {  // f(index, key) of every key
+        for (uint32_t first = 0; first < n; first += AT_ONCE) {
+            if (n > AT_ONCE) load(first);
+#pragma unroll
+            for (uint32_t j = 0; j < SELECT_KEYS; ++j)
+                if (first + 256 * j + t < n) f(first + 256 * j + t, key[j]);
+        }
+    };
+    if (n <= AT_ONCE) load(0);
+    uint64_t lo = ~0ull, hi = 0;
+    each([&](uint32_t, uint64_t x) {
+        lo = min(lo, x);
+        hi = max(hi, x);
+    });
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+        lo = min(lo, (uint64_t)__shfl_xor((unsigned long long)lo, d, 64));
+        hi = max(hi, (uint64_t)__shfl_xor((unsigned long long)hi, d, 64));
+    }
+    if (lane == 0) {
+        sh.low[wave] = lo;
+        sh.high[wave] = hi;
+    }
+    __syncthreads();
+    for (int w = 0; w < 4; ++w) {
+        lo = min(lo, sh.low[w]);
+        hi = max(hi, sh.high[w]);
+    }
+    uint32_t need = take;  // of the keys from lo to hi; those above are taken
+    bool ties = true;      // all keys from lo to hi are equal: the first `need` of them
+    for (int pass = 0; pass < KV8_PASSES && lo != hi; ++pass) {
+        const int shift = kv8_shift(lo, hi);
+        for (uint32_t j = t; j < SELECT_BINS; j += 256) sh.bin[j] = 0;
+        __syncthreads();
+        each([&](uint32_t, uint64_t x) {
+            if (x >= lo && x <= hi) atomicAdd(&sh.bin[(uint32_t)((x - lo) >> shift)], 1u);
+        });
+        __syncthreads();
+        // Bins from the top, 8 to a thread: the one in which the count reaches `need`.
+        uint32_t mine = 0;
+#pragma unroll
+        for (uint32_t j = 0; j < 8; ++j) mine += sh.bin[SELECT_BINS - 1 - 8 * t - j];
+        const uint32_t upto = wave_up_to(mine);
+        if (lane == 63) sh.part[wave] = upto;
+        __syncthreads();
+        uint32_t above = upto - mine;
+        for (uint32_t w = 0; w < wave; ++w) above += sh.part[w];
+        if (above < need && above + mine >= need) {
+            uint32_t b = SELECT_BINS - 1 - 8 * t;
+            while (above + sh.bin[b] < need) above += sh.bin[b--];
+            sh.found = b;
+            sh.above = above;
+            sh.inside = sh.bin[b];
+        }
+        __syncthreads();
+        need -= sh.above;
+        kv8_narrow(lo, hi, shift, sh.found);
+        if (sh.inside == need) {
+            ties = false;
+            break;
+        }
+        __syncthreads();  // found, above and inside are read
+    }
+    // Indices in order: per row of 256 keys and wavefront the number taken, then its place.
+    uint32_t placed = 0, equals = 0;
+    for (uint32_t first = 0; first < n; first += AT_ONCE) {
+        if (n > AT_ONCE) load(first);
+        uint32_t equal_before[SELECT_KEYS];
+        __syncthreads();
+        if (ties) {
+#pragma unroll
+            for (uint32_t j = 0; j < SELECT_KEYS; ++j) {
+                const uint64_t m = __ballot(first + 256 * j + t < n && key[j] == lo);
+                equal_before[j] = (uint32_t)__popcll(m & ((1ull << lane) - 1));
+                if (lane == 0) sh.equal[4 * j + wave] = (uint32_t)__popcll(m);
+            }
+            __syncthreads();
+            const uint32_t upto = wave_up_to(sh.equal[lane]);
+#pragma unroll
+            for (uint32_t j = 0; j < SELECT_KEYS; ++j)
+                equal_before[j] += equals + __shfl(upto, 4 * j + wave, 64) - sh.equal[4 * j + wave];
+            equals += __shfl(upto, 63, 64);
+        }
+        uint64_t taken[SELECT_KEYS];
+#pragma unroll
+        for (uint32_t j = 0; j < SELECT_KEYS; ++j) {
+            const bool in = first + 256 * j + t < n;
+            taken[j] = __ballot(in && (ties ? key[j] > lo || (key[j] == lo && equal_before[j] < need) : key[j] >= lo));
+            if (lane == 0) sh.count[4 * j + wave] = (uint32_t)__popcll(taken[j]);
+        }
+        __syncthreads();
+        const uint32_t upto = wave_up_to(sh.count[lane]);
+#pragma unroll
+        for (uint32_t j = 0; j < SELECT_KEYS; ++j) {
+            const uint32_t at = placed + __shfl(upto, 4 * j + wave, 64) - sh.count[4 * j + wave];
+            if (taken[j] >> lane & 1) to[at + (uint32_t)__popcll(taken[j] & ((1ull << lane) - 1))] = first + 256 * j + t;
+        }
+        placed += __shfl(upto, 63, 64);
+    }
+}
+
+// The pages of (sequence, kv head). A block scores 64 pages, a wavefront 16 of them: 16 lanes have 8 dims each of a
+// page's bounds (two 16-byte loads), four pages are in flight; products and sums in f64, so that equal pages score
+// equal and near ones in their order (a score's bytes, 512 per page, take longer than its 128 multiply-adds per head).
+// The last block of its (sequence, kv head) to count itself selects. The last page stands outside: it is always kept.
 __global__ void __launch_bounds__(256)
     kv8_select_kernel(Table t, const bf16_t* __restrict__ bounds, const bf16_t* __restrict__ q,
                       const uint32_t* __restrict__ lens, uint32_t budget, uint32_t* __restrict__ list,
-                      uint64_t* __restrict__ keys_of, uint32_t q_heads) {
-    __shared__ uint32_t flags[256];
-    const uint32_t kh = blockIdx.x, s = blockIdx.y, i = threadIdx.x, group = q_heads / t.kv_heads;
+                      uint64_t* __restrict__ keys_of, uint32_t* __restrict__ counter_of, uint32_t q_heads) {
+    __shared__ SelectShared sh;
+    const uint32_t kh = blockIdx.x, s = blockIdx.z, i = threadIdx.x, group = q_heads / t.kv_heads;
+    const uint32_t lane = i & 63, wave = i >> 6, n = lane & 15, g = lane >> 4;
     const uint32_t pages = (kv8_keys(lens[s], t.seq_pages) + KV8_PAGE - 1) / KV8_PAGE;
-    uint64_t* key = keys_of + ((size_t)s * t.kv_heads + kh) * t.seq_pages;
-    uint32_t* to = list + ((size_t)s * t.kv_heads + kh) * budget;
-    for (uint32_t p = i; p < pages; p += 256) {
-        const uint32_t page = t.page(s, p);
-        uint64_t best = 0;
-        if (page != KV8_NONE) {
-            const bf16_t* b = bounds + kv8_bound(page, t.kv_heads, kh);
-            for (uint32_t g = 0; g < group; ++g) {
-                const bf16_t* qr = q + ((size_t)s * q_heads + kh * group + g) * KV8_HEAD;
-                double sum = 0.0;
-                for (uint32_t d = 0; d < KV8_HEAD; ++d) {
-                    const float x = bf2f(qr[d]);
-                    sum = fma((double)x, (double)bf2f(b[x < 0.f ? d : KV8_HEAD + d]), sum);
-                }
-                best = max(best, score_key(sum));
-            }
-        }
-        key[p] = p == pages - 1 ? ~0ull : best;
+    const size_t pair = (size_t)s * t.kv_heads + kh;
+    uint32_t* to = list + pair * budget;
+    if (pages <= budget || budget == 1) {
+        if (blockIdx.y == 0)
+            for (uint32_t j = i; j < budget; j += 256) to[j] = j >= pages ? KV8_NONE : budget == 1 ? pages - 1 : j;
+        return;
+    }
+    const uint32_t scored = pages - 1, first = blockIdx.y * SELECT_PAGES;
+    if (first >= scored) return;
+    uint32_t entry[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        const uint32_t p = first + 16 * wave + 4 * j + g;
+        entry[j] = p < scored ? t.pages[(size_t)s * t.seq_pages + p] : KV8_NONE;
+    }
+    for (uint32_t e = i; e < group * KV8_HEAD; e += 256)
+        sh.q[0][e] = (double)bf2f(q[((size_t)s * q_heads + kh * group) * KV8_HEAD + e]);
+    u32x4 lo[4], hi[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        const u32x4* b = reinterpret_cast<const u32x4*>(bounds + kv8_bound(entry[j] < t.pool ? entry[j] : 0u, t.kv_heads, kh)) + n;
+        lo[j] = b[0];
+        hi[j] = b[KV8_HEAD / 8];
     }
     __syncthreads();
-    uint32_t taken = 0;
-    for (uint32_t p0 = 0; p0 < pages; p0 += 256) {
-        const uint32_t p = p0 + i;
-        uint32_t rank = 0;
-        if (p < pages)
-            for (uint32_t o = 0; o < pages; ++o) rank += key[o] > key[p] || (key[o] == key[p] && o < p);
-        flags[i] = p < pages && rank < budget;
-        __syncthreads();
-        uint32_t before = 0, all = 0;
-        for (uint32_t j = 0; j < 256; ++j) {
-            before += j < i ? flags[j] : 0;
-            all += flags[j];
+    uint64_t best[4] = {0, 0, 0, 0};
+    for (uint32_t h = 0; h < group; ++h) {
+        double x[8];
+#pragma unroll
+        for (int d = 0; d < 8; ++d) x[d] = sh.q[h][8 * n + d];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            double sum = 0.0;
+#pragma unroll
+            for (int d = 0; d < 8; ++d) {
+                const uint32_t w = x[d] < 0.0 ? lo[j][d / 2] : hi[j][d / 2];
+                sum = fma(x[d], (double)(d & 1 ? bf_hi(w) : bf_lo(w)), sum);
+            }
+            sum += dpp_d<0x124>(sum);
+            sum += dpp_d<0x128>(sum);
+            sum += dpp_d<0x4E>(sum);
+            sum += dpp_d<0xB1>(sum);
+            best[j] = max(best[j], score_key(sum));
         }
-        if (flags[i]) to[taken + before] = p;
-        taken += all;
-        __syncthreads();
     }
-    for (uint32_t j = taken + i; j < budget; j += 256) to[j] = KV8_NONE;
+    uint64_t* key = keys_of + pair * t.seq_pages;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        const uint32_t p = first + 16 * wave + 4 * j + g;
+        if (n == 0 && p < scored)
+            __hip_atomic_store(key + p, entry[j] < t.pool ? best[j] : 0ull, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    }
+    // The keys acknowledged, then the count: the block that completes it selects.
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __syncthreads();
+    uint32_t* counter = counter_of + pair;
+    if (i == 0) {
+        const uint32_t before = __hip_atomic_fetch_add(counter, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        sh.last = before == (scored - 1) / SELECT_PAGES;
+    }
+    __syncthreads();
+    if (!sh.last) return;
+    if (i == 0) {
+        __hip_atomic_store(counter, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);  // for the next call
+        to[budget - 1] = pages - 1;
+    }
+    select_keys(key, scored, budget - 1, to, sh);
 }
 
 // ---- host ----
@@ -546,10 +884,28 @@ extern "C" x0ne_status x0ne_gpu_kv8_read(x0ne_gpu* g, const x0ne_kv8* c, uint64_
     return X0NE_OK;
 }
 
-// Slices of a sequence's tiles: enough that the pairs of sequence and kv head fill 256 CUs with two blocks each.
-static uint32_t slices_of(const x0ne_kv8* c) {
-    const uint64_t pairs = std::max<uint64_t>(1, (uint64_t)c->seqs * c->kv_heads);
-    return (uint32_t)std::min<uint64_t>(MAX_SLICES, std::max<uint64_t>(16, 512 / pairs));
+// How sequences are cut: at most `slices` slices of at least `rounds` rounds of 4 tiles (a tile per wavefront), over
+// `blocks` blocks for each kv head and 64 sequences.
+//  - Few pairs of sequence and kv head (us, 32768 keys, 8 pairs): slices for one block on each of 256 CUs; two on each
+//    bring more states to join than overlap gains (16 / 32 / 64 slices 27.2 / 21.7 / 26.8).
+//  - Many: two blocks per CU walk the slices, longest first. A slice of one round costs about four rounds (its
+//    lookups, states and count are not hidden), so slices are two thirds of what a block has to do if every sequence
+//    fills its table, one or two per block (64 sequences of up to 6000 keys, 1 / 4 / 8 / 16 / 24 rounds: 134 / 101 / 92 /
+//    84 / 95; 16 of up to 8192, 1 / 3 / 5 / 8: 48 / 42 / 35 / 41), up to 16, and fewer for fewer pairs, whose lengths
+//    may be far below their tables'.
+struct Cut {
+    uint32_t slices, rounds, blocks;
+};
+static Cut cut_of(const x0ne_kv8* c, uint32_t budget = 0) {
+    const uint64_t pairs = std::max<uint64_t>(1, (uint64_t)c->seqs * c->kv_heads), parts = (c->seqs + 63) / 64;
+    Cut cut;
+    cut.slices = (uint32_t)std::min<uint64_t>(MAX_SLICES, std::max<uint64_t>(16, 256 / pairs));
+    cut.blocks = (uint32_t)std::max<uint64_t>(1, 512 / std::max<uint64_t>(1, parts * c->kv_heads));
+    const uint32_t most = budget ? std::min(budget, c->seq_pages) : c->seq_pages;  // pages a sequence attends
+    const uint64_t fullest = (uint64_t)((most + 15) / 16) * std::min(c->seqs, 64u);
+    cut.rounds = (uint32_t)std::max<uint64_t>(1, std::min(std::min<uint64_t>(16, pairs / 24), 2 * fullest / (3 * cut.blocks)));
+    cut.blocks = std::max(1u, std::min(cut.blocks, cut.slices * std::min(c->seqs, 64u)));
+    return cut;
 }
 
 // The workspace: a counter per (sequence, kv head), then the states of attention or the scores of selection.
@@ -557,7 +913,7 @@ static uint64_t counter_bytes(const x0ne_kv8* c) { return ((uint64_t)c->seqs * c
 
 extern "C" uint64_t x0ne_kv8_work_bytes(const x0ne_kv8* c, uint32_t q_heads) {
     if (check_cache("kv8 workspace", c) != X0NE_OK || check_heads("kv8 workspace", c, q_heads) != X0NE_OK) return 0;
-    const uint64_t states = (uint64_t)c->seqs * q_heads * slices_of(c) * STATE * 4;
+    const uint64_t states = (uint64_t)c->seqs * q_heads * cut_of(c).slices * STATE * 4;
     const uint64_t scores = (uint64_t)c->seqs * c->kv_heads * c->seq_pages * 8;
     return std::max<uint64_t>(256, counter_bytes(c) + std::max(states, scores));
 }
@@ -590,9 +946,12 @@ extern "C" x0ne_status x0ne_gpu_kv8_attention(x0ne_gpu* g, const x0ne_kv8* c, ui
     a.budget = budget;
     a.q_heads = q_heads;
     a.group = q_heads / c->kv_heads;
-    a.slices = slices_of(c);
+    const Cut cut = cut_of(c, budget);
+    a.slices = cut.slices;
+    a.rounds = cut.rounds;
     a.scale2 = scale * 1.44269504088896340736f;
-    hipLaunchKernelGGL(kv8_attention_kernel, dim3(c->kv_heads, a.slices, c->seqs), dim3(64 * ATTEND_WAVES), 0, g->stream, a);
+    hipLaunchKernelGGL(kv8_attention_kernel, dim3(c->kv_heads, cut.blocks, (c->seqs + 63) / 64), dim3(64 * ATTEND_WAVES), 0,
+                       g->stream, a);
     X0NE_HIP(hipGetLastError(), what);
     return X0NE_OK;
 }
@@ -612,9 +971,11 @@ extern "C" x0ne_status x0ne_gpu_kv8_select(x0ne_gpu* g, const x0ne_kv8* c, uint6
     if (c->seqs == 0) return X0NE_OK;
     const OnDevice on(g->device);
     g->counts.launches++;
-    hipLaunchKernelGGL(kv8_select_kernel, dim3(c->kv_heads, c->seqs), dim3(256), 0, g->stream, table_of(c),
+    const uint32_t chunks = (c->seq_pages + SELECT_PAGES - 1) / SELECT_PAGES;
+    if (chunks > 65535) return bad(what, std::to_string(c->seq_pages) + " pages of a sequence (up to 65535 x 64)");
+    hipLaunchKernelGGL(kv8_select_kernel, dim3(c->kv_heads, chunks, c->seqs), dim3(256), 0, g->stream, table_of(c),
                        (const bf16_t*)bounds, (const bf16_t*)q, (const uint32_t*)lens, budget, (uint32_t*)page_list,
-                       (uint64_t*)(work + counter_bytes(c)), q_heads);
+                       (uint64_t*)(work + counter_bytes(c)), (uint32_t*)work, q_heads);
     X0NE_HIP(hipGetLastError(), what);
     return X0NE_OK;
 }
