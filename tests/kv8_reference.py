@@ -128,7 +128,7 @@ def bounds_of(c, page):
     """[kv_heads][2][128] bf16 bits of a complete page."""
     k, _ = page_values(c, page)
     with np.errstate(invalid="ignore"):
-        b = np.stack([k.min(1), k.max(1)], 1)  # numpy's min and max pass a NaN on
+        b = np.stack([k.min(1), k.max(1)], 1) + 0.0  # numpy's min and max pass a NaN on; zeros are +0
     return np.where(np.isnan(b), 0x7FC0, bits(np.where(np.isnan(b), 0.0, b)).reshape(b.shape)).astype(np.uint16)
 
 

@@ -12,7 +12,7 @@
 //        [128][16] (the 16 positions of one dim contiguous: the operand order of P V)
 // scales [pool][kv_heads][32]: the 16 keys' scale bytes, then the 16 values'
 // bounds [pool][kv_heads][2][128] bf16: the smallest and the largest value of each dim over the 16
-//        keys of a complete page (exact: the values are bf16; NaN where a key holds one)
+//        keys of a complete page (exact: the values are bf16; zeros are +0; NaN where a key holds one)
 #pragma once
 #include <stddef.h>
 #include <stdint.h>

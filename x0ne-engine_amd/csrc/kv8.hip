@@ -26,127 +26,220 @@ __device__ __forceinline__ float kv8_value(uint32_t code, uint32_t scale) {
 
 __device__ __forceinline__ bool finite(float x) { return (__float_as_uint(x) & 0x7F800000u) != 0x7F800000u; }
 
-// The scale exponent and the two codes of a lane's values a and b of a row that lies in the 64 lanes.
-__device__ __forceinline__ uint32_t quantise_pair(float a, float b, int& e) {
-    const float top = wave_max(fmaxf(finite(a) ? fabsf(a) : 0.f, finite(b) ? fabsf(b) : 0.f));
-    e = kv8_exponent(__float_as_uint(top) >> 16);
-    const float down = __uint_as_float((uint32_t)(127 - e) << 23);
-    // The conversion's own NaN has either sign: 0x7F stands for all that is not finite.
-    const uint32_t w = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(a * down, b * down, 0, false);
-    return (finite(a) ? w & 0xFFu : 0x7Fu) | (finite(b) ? w & 0xFF00u : 0x7F00u);
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+
+__device__ __forceinline__ uint32_t pack(float lo, float hi) {
+    return __builtin_bit_cast(uint32_t, bf16x2{(__bf16)lo, (__bf16)hi});
+}
+__device__ __forceinline__ float half_of(const u32x4& x, int e) { return e & 1 ? bf_hi(x[e / 2]) : bf_lo(x[e / 2]); }
+
+// f32 and f64 values moved within a row of 16 lanes by DPP (CTRL 0xB1, 0x4E: xor 1 and 2; 0x141: lane 7 - i of each
+// half row; 0x128: 8 lanes round).
+template <int CTRL>
+__device__ __forceinline__ float dpp_f(float v) {
+    return __uint_as_float((uint32_t)__builtin_amdgcn_update_dpp(0, (int)__float_as_uint(v), CTRL, 0xF, 0xF, false));
+}
+__device__ __forceinline__ float row_max(float v) {
+    v = fmaxf(v, dpp_f<0xB1>(v));
+    v = fmaxf(v, dpp_f<0x4E>(v));
+    v = fmaxf(v, dpp_f<0x141>(v));
+    return fmaxf(v, dpp_f<0x128>(v));
 }
 
-// RMSNorm of each head of q and k, rotate-half RoPE from the table, q to q_out as bf16, k and v
-// quantised into their page: the arithmetic of x0ne_qk_norm_rope_kv_write_rows_bf16, so q_out has its
-// bits and the codes are those of its k row. One wavefront per (row, head of q and k), lane i the pair
-// (i, i + 64). A row of no sequence, or past the sequence's pages or the rope table, writes nothing.
+// The codes of a lane's 8 values of a row that lies in 16 lanes, and the row's scale byte.
+__device__ __forceinline__ u32x2 quantise(const float (&x)[8], uint32_t& scale) {
+    float top = 0.f;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) top = fmaxf(top, finite(x[j]) ? fabsf(x[j]) : 0.f);
+    const int e = kv8_exponent(__float_as_uint(row_max(top)) >> 16);
+    scale = (uint32_t)(e + 127);
+    const float down = __uint_as_float((uint32_t)(127 - e) << 23);
+    u32x2 w;
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+        int c = __builtin_amdgcn_cvt_pk_fp8_f32(x[4 * j] * down, x[4 * j + 1] * down, 0, false);
+        w[j] = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(x[4 * j + 2] * down, x[4 * j + 3] * down, c, true);
+    }
+    // The conversion's own NaN has either sign: 0x7F stands for all that is not finite.
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+        if (!finite(x[j])) w[j / 4] = (w[j / 4] & ~(0xFFu << 8 * (j % 4))) | 0x7Fu << 8 * (j % 4);
+    return w;
+}
+
+constexpr uint32_t WRITE_ROWS = 16;  // rows of a block, one to 16 lanes
+constexpr uint32_t WRITE_VALUES = 4;  // kv heads whose values a block takes
+
+// RMSNorm of each head of q and k, rotate-half RoPE from the table, q to q_out as bf16, k and v quantised into their
+// page: the arithmetic of x0ne_qk_norm_rope_kv_write_rows_bf16, its sum of squares added in the same tree, so q_out has
+// its bits and the codes are those of its k row. A block takes 16 rows; 16 lanes have one row, lane n dims 8 n .. + 7 (16
+// bytes), so a dim and its pair 64 dims on are 8 lanes apart (a DPP move). blockIdx.y: HEADS heads of q and k, whose
+// loads are all requested at once, whose cos and sin are read once and whose f64 square roots and divisions are one
+// (lane h computes head h's); or, behind those, the values of WRITE_VALUES kv heads, turned dim-major in LDS: where the
+// block's rows are one whole page, as in a prompt, that is stored as such, else byte by byte. A row of no sequence, or
+// past the sequence's pages or the rope table, writes nothing.
+template <int HEADS>
 __global__ void __launch_bounds__(256)
     kv8_write_kernel(Table t, uint8_t* __restrict__ codes, uint8_t* __restrict__ scales, const bf16_t* __restrict__ qkv,
                      const bf16_t* __restrict__ q_norm, const bf16_t* __restrict__ k_norm, const double* __restrict__ cs,
                      const uint32_t* __restrict__ row_seq, const uint32_t* __restrict__ row_pos,
-                     bf16_t* __restrict__ q_out, uint32_t q_heads, uint32_t positions, float eps) {
-    constexpr uint32_t HD = KV8_HEAD, HALF = HD / 2;
-    const uint32_t head = blockIdx.y * 4 + (threadIdx.x >> 6), row = blockIdx.x, i = threadIdx.x & 63;
-    if (head >= q_heads + t.kv_heads) return;
-    const uint32_t seq = row_seq[row], pos = row_pos[row];
-    if (seq >= t.seqs || pos >= positions || pos / KV8_PAGE >= t.seq_pages) return;
-    const bool is_q = head < q_heads;
-    const uint32_t kh = is_q ? 0 : head - q_heads;
-    const bf16_t* line = qkv + (size_t)row * (q_heads + 2 * t.kv_heads) * HD;
-    const bf16_t *src = line + (size_t)head * HD, *nw = is_q ? q_norm : k_norm;
-    const double2 c = reinterpret_cast<const double2*>(cs)[(size_t)pos * HALF + i];
-    const float a = bf2f(src[i]), b = bf2f(src[i + HALF]);
-    const double ss = wave_sum_d((double)a * (double)a + (double)b * (double)b);
-    const double scale = 1.0 / sqrt(ss / (double)HD + (double)eps);
-    const double na = (double)a * scale * (double)bf2f(nw[i]), nb = (double)b * scale * (double)bf2f(nw[i + HALF]);
-    const bf16_t ra = f2bf((float)(na * c.x - nb * c.y)), rb = f2bf((float)(nb * c.x + na * c.y));
-    if (is_q) {
-        bf16_t* d = q_out + ((size_t)row * q_heads + head) * HD;
-        d[i] = ra;
-        d[i + HALF] = rb;
+                     bf16_t* __restrict__ q_out, uint32_t rows, uint32_t q_heads, uint32_t positions, float eps) {
+    constexpr uint32_t HD = KV8_HEAD;
+    __shared__ uint32_t turned[WRITE_VALUES][KV8_PART / 4];
+    __shared__ uint32_t page_of[WRITE_ROWS], slot_of[WRITE_ROWS];
+    const uint32_t n = threadIdx.x & 15, r = threadIdx.x >> 4, row = blockIdx.x * WRITE_ROWS + r, at = min(row, rows - 1);
+    const uint32_t seq = row_seq[at], pos = row_pos[at], slot = pos % KV8_PAGE;
+    const bool live = row < rows && seq < t.seqs && pos < positions && pos / KV8_PAGE < t.seq_pages;
+    const uint32_t page = live ? t.page(seq, pos / KV8_PAGE) : KV8_NONE;
+    const uint32_t heads = q_heads + t.kv_heads, parts = (heads + HEADS - 1) / HEADS;
+    const bf16_t* line = qkv + (size_t)at * (heads + t.kv_heads) * HD + 8 * n;
+    if (blockIdx.y < parts) {
+        const uint32_t h0 = blockIdx.y * HEADS;
+        u32x4 x[HEADS];
+#pragma unroll
+        for (int i = 0; i < HEADS; ++i) x[i] = *reinterpret_cast<const u32x4*>(line + (size_t)min(h0 + i, heads - 1) * HD);
+        const double2* c = reinterpret_cast<const double2*>(cs) + (size_t)(live ? pos : 0) * (HD / 2) + 8 * (n & 7);
+        double co[8], si[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            const double2 v = c[j];
+            co[j] = v.x;
+            si[j] = n < 8 ? -v.y : v.y;
+        }
+        const u32x4 wq = *reinterpret_cast<const u32x4*>(q_norm + 8 * n), wk = *reinterpret_cast<const u32x4*>(k_norm + 8 * n);
+        double square = 0.0;
+#pragma unroll
+        for (int i = 0; i < HEADS; ++i) {
+            double s[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const double v = (double)half_of(x[i], j);
+                s[j] = v * v;
+            }
+#pragma unroll
+            for (int j = 0; j < 8; ++j) s[j] += dpp_d<0x128>(s[j]);
+            double sum = ((s[0] + s[1]) + (s[2] + s[3])) + ((s[4] + s[5]) + (s[6] + s[7]));
+            sum += dpp_d<0xB1>(sum);
+            sum += dpp_d<0x4E>(sum);
+            sum += dpp_d<0x141>(sum);
+            if (n == (uint32_t)i) square = sum;
+        }
+        const double root = 1.0 / sqrt(square / (double)HD + (double)eps);
+#pragma unroll
+        for (int i = 0; i < HEADS; ++i) {
+            const uint32_t head = h0 + i;
+            if (head >= heads) break;
+            const bool is_q = head < q_heads;
+            const double scale = __shfl(root, (threadIdx.x & 48) + i, 64);
+            double own[8];
+            float out[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) own[j] = (double)half_of(x[i], j) * scale * (double)half_of(is_q ? wq : wk, j);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) out[j] = (float)(own[j] * co[j] + dpp_d<0x128>(own[j]) * si[j]);
+            const u32x4 b = {pack(out[0], out[1]), pack(out[2], out[3]), pack(out[4], out[5]), pack(out[6], out[7])};
+            if (is_q) {
+                if (live) *reinterpret_cast<u32x4*>(q_out + ((size_t)row * q_heads + head) * HD + 8 * n) = b;
+                continue;
+            }
+            float v[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) v[j] = half_of(b, j);
+            uint32_t byte;
+            const u32x2 w = quantise(v, byte);
+            if (page == KV8_NONE) continue;
+            *reinterpret_cast<u32x2*>(codes + kv8_record(page, t.kv_heads, head - q_heads) + slot * HD + 8 * n) = w;
+            if (n == 0) scales[kv8_scale(page, t.kv_heads, head - q_heads) + slot] = (uint8_t)byte;
+        }
         return;
     }
-    const uint32_t page = t.page(seq, pos / KV8_PAGE), slot = pos % KV8_PAGE;
-    if (page == KV8_NONE) return;
-    uint8_t *rec = codes + kv8_record(page, t.kv_heads, kh), *sc = scales + kv8_scale(page, t.kv_heads, kh);
-    int e;
-    uint32_t w = quantise_pair(bf2f(ra), bf2f(rb), e);
-    rec[slot * HD + i] = (uint8_t)w;
-    rec[slot * HD + i + HALF] = (uint8_t)(w >> 8);
-    if (i == 0) sc[slot] = (uint8_t)(e + 127);
-    const bf16_t* vs = line + (size_t)(q_heads + t.kv_heads + kh) * HD;
-    w = quantise_pair(bf2f(vs[i]), bf2f(vs[i + HALF]), e);
-    rec[KV8_PART + i * KV8_PAGE + slot] = (uint8_t)w;
-    rec[KV8_PART + (i + HALF) * KV8_PAGE + slot] = (uint8_t)(w >> 8);
-    if (i == 0) sc[KV8_PAGE + slot] = (uint8_t)(e + 127);
-}
-
-// The bounds of the pages that the rows complete (slot 15), from the codes; a wavefront per (row, kv
-// head), lane i dims 2i and 2i + 1.
-__global__ void __launch_bounds__(256)
-    kv8_bounds_kernel(Table t, const uint8_t* __restrict__ codes, const uint8_t* __restrict__ scales,
-                      const uint32_t* __restrict__ row_seq, const uint32_t* __restrict__ row_pos, uint32_t positions,
-                      bf16_t* __restrict__ bounds) {
-    const uint32_t kh = blockIdx.y * 4 + (threadIdx.x >> 6), row = blockIdx.x, i = threadIdx.x & 63;
-    if (kh >= t.kv_heads) return;
-    const uint32_t pos = row_pos[row];
-    if (pos % KV8_PAGE != KV8_PAGE - 1 || pos >= positions) return;
-    const uint32_t page = t.page(row_seq[row], pos / KV8_PAGE);
-    if (page == KV8_NONE) return;
-    const uint8_t *rec = codes + kv8_record(page, t.kv_heads, kh), *sc = scales + kv8_scale(page, t.kv_heads, kh);
-    float lo[2] = {INFINITY, INFINITY}, hi[2] = {-INFINITY, -INFINITY};
-    bool nan[2] = {false, false};
-    for (uint32_t s = 0; s < KV8_PAGE; ++s) {
-        const uint32_t w = *reinterpret_cast<const uint16_t*>(rec + s * KV8_HEAD + 2 * i);
-        for (int j = 0; j < 2; ++j) {
-            const float v = kv8_value(j ? w >> 8 : w, sc[s]);
-            nan[j] |= v != v;
-            lo[j] = fminf(lo[j], v);
-            hi[j] = fmaxf(hi[j], v);
+    const uint32_t k0 = (blockIdx.y - parts) * WRITE_VALUES;
+    u32x4 x[WRITE_VALUES];
+#pragma unroll
+    for (uint32_t i = 0; i < WRITE_VALUES; ++i) x[i] = *reinterpret_cast<const u32x4*>(line + (size_t)(heads + min(k0 + i, t.kv_heads - 1)) * HD);
+    if (n == 0) {
+        page_of[r] = page;
+        slot_of[r] = slot;
+    }
+#pragma unroll
+    for (uint32_t i = 0; i < WRITE_VALUES; ++i) {
+        float v[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[j] = half_of(x[i], j);
+        uint32_t byte;
+        const u32x2 w = quantise(v, byte);
+        uint8_t* to = reinterpret_cast<uint8_t*>(turned[i]) + 8 * n * WRITE_ROWS + r;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) to[j * WRITE_ROWS] = (uint8_t)(w[j / 4] >> 8 * (j % 4));
+        if (n == 0 && page != KV8_NONE && k0 + i < t.kv_heads)
+            scales[kv8_scale(page, t.kv_heads, k0 + i) + KV8_PAGE + slot] = (uint8_t)byte;
+    }
+    __syncthreads();
+    const bool whole = __all(page_of[n] == page_of[0] && page_of[0] != KV8_NONE && slot_of[n] == n);
+#pragma unroll
+    for (uint32_t i = 0; i < WRITE_VALUES; ++i) {
+        if (k0 + i >= t.kv_heads) break;
+        if (whole) {
+            uint8_t* to = codes + kv8_record(page_of[0], t.kv_heads, k0 + i) + KV8_PART;
+            reinterpret_cast<u32x2*>(to)[threadIdx.x] = reinterpret_cast<const u32x2*>(turned[i])[threadIdx.x];
+        } else if (page_of[n] != KV8_NONE) {
+            uint8_t* to = codes + kv8_record(page_of[n], t.kv_heads, k0 + i) + KV8_PART + slot_of[n];
+            for (uint32_t d = r; d < HD; d += 16) to[d * KV8_PAGE] = reinterpret_cast<const uint8_t*>(turned[i])[d * WRITE_ROWS + n];
         }
     }
-    const float q = __uint_as_float(0x7FC00000u);
-    bf16_t* d = bounds + kv8_bound(page, t.kv_heads, kh);
-    for (int j = 0; j < 2; ++j) {
-        d[2 * i + j] = f2bf(nan[j] ? q : lo[j]);
-        d[KV8_HEAD + 2 * i + j] = f2bf(nan[j] ? q : hi[j]);
-    }
 }
 
-// Positions below a sequence's length as bf16, page by page: the codes' order is the bf16 pages' order, so
-// a wavefront streams one page of one head. Slots past the length are zero; a page that is not there reads
-// as zeros, an output page outside its pool is not written.
+// The bounds of the pages that the rows complete (slot 15), from the codes. A wavefront per 16 rows and kv head: lane
+// (n, g) has dims 8 n .. + 7 of keys 4 g .. + 3 of such a page.
 __global__ void __launch_bounds__(256)
-    kv8_read_kernel(Table t, const uint8_t* __restrict__ codes, const uint8_t* __restrict__ scales,
-                    const uint32_t* __restrict__ lens, bf16_t* __restrict__ k_out, bf16_t* __restrict__ v_out,
-                    const uint32_t* __restrict__ out_table, uint32_t out_pool) {
-    const uint32_t p = blockIdx.x, s = blockIdx.z, i = threadIdx.x & 63, kh = blockIdx.y * 4 + (threadIdx.x >> 6);
-    const uint32_t keys = kv8_keys(lens[s], t.seq_pages);
-    if (kh >= t.kv_heads || p * KV8_PAGE >= keys) return;
-    const uint32_t to = kv8_page(out_table, t.seqs, t.seq_pages, out_pool, s, p);
-    if (to == KV8_NONE) return;
-    const uint32_t page = t.page(s, p), valid = page == KV8_NONE ? 0u : min(keys - p * KV8_PAGE, KV8_PAGE);
-    const uint8_t *rec = codes + kv8_record(page == KV8_NONE ? 0 : page, t.kv_heads, kh),
-                  *sc = scales + kv8_scale(page == KV8_NONE ? 0 : page, t.kv_heads, kh);
-    bf16_t *kd = k_out + ((size_t)to * t.kv_heads + kh) * KV8_PART, *vd = v_out + ((size_t)to * t.kv_heads + kh) * KV8_PART;
-    for (uint32_t j = i; j < KV8_PART; j += 64) {
-        const uint32_t ks = j / KV8_HEAD, vs = j % KV8_PAGE;
-        kd[j] = ks < valid ? f2bf(kv8_value(rec[j], sc[ks])) : 0;
-        vd[j] = vs < valid ? f2bf(kv8_value(rec[KV8_PART + j], sc[KV8_PAGE + vs])) : 0;
+    kv8_bounds_kernel(Table t, const uint8_t* __restrict__ codes, const uint8_t* __restrict__ scales,
+                      const uint32_t* __restrict__ row_seq, const uint32_t* __restrict__ row_pos, uint32_t rows,
+                      uint32_t positions, bf16_t* __restrict__ bounds) {
+    const uint32_t lane = threadIdx.x & 63, n = lane & 15, g = lane >> 4, kh = blockIdx.y * 4 + (threadIdx.x >> 6);
+    if (kh >= t.kv_heads) return;
+    const uint32_t row = blockIdx.x * WRITE_ROWS + n;
+    const uint32_t pos = row < rows ? row_pos[row] : 0u;
+    const uint32_t mine = pos % KV8_PAGE == KV8_PAGE - 1 && pos < positions ? t.page(row_seq[row], pos / KV8_PAGE) : KV8_NONE;
+    for (uint64_t left = __ballot(mine != KV8_NONE) & 0xFFFFu; left; left &= left - 1) {
+        const uint32_t page = __builtin_amdgcn_readlane(mine, (uint32_t)__builtin_ctzll(left));
+        const uint8_t* rec = codes + kv8_record(page, t.kv_heads, kh) + 4 * g * KV8_HEAD + 8 * n;
+        u32x2 w[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) w[i] = *reinterpret_cast<const u32x2*>(rec + i * KV8_HEAD);
+        const uint32_t bytes = *reinterpret_cast<const uint32_t*>(scales + kv8_scale(page, t.kv_heads, kh) + 4 * g);
+        float lo[8], hi[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            lo[j] = INFINITY;
+            hi[j] = -INFINITY;
+            uint32_t nan = 0;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const float v = kv8_value(w[i][j / 4] >> 8 * (j % 4) & 0xFFu, bytes >> 8 * i & 0xFFu);
+                nan |= v != v;
+                lo[j] = fminf(lo[j], v);
+                hi[j] = fmaxf(hi[j], v);
+            }
+            lo[j] = -rows_max(-lo[j]) + 0.f;  // a zero of either sign is +0
+            hi[j] = rows_max(hi[j]) + 0.f;
+            nan |= __shfl_xor(nan, 16, 64);
+            nan |= __shfl_xor(nan, 32, 64);
+            if (nan) lo[j] = hi[j] = __uint_as_float(0x7FC00000u);
+        }
+        if (g < 2) {
+            float b[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) b[j] = g ? hi[j] : lo[j];
+            *reinterpret_cast<u32x4*>(bounds + kv8_bound(page, t.kv_heads, kh) + g * KV8_HEAD + 8 * n) =
+                u32x4{pack(b[0], b[1]), pack(b[2], b[3]), pack(b[4], b[5]), pack(b[6], b[7])};
+        }
     }
 }
 
-typedef float f32x4 __attribute__((ext_vector_type(4)));
-typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
-typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
-typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
-
-__device__ __forceinline__ f32x4 mfma(u32x4 a, u32x4 b, f32x4 c) {
-    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
-}
-__device__ __forceinline__ uint32_t pack(float lo, float hi) {
-    return __builtin_bit_cast(uint32_t, bf16x2{(__bf16)lo, (__bf16)hi});
-}
 // Eight codes as bf16, times the power of two `scale`: exact.
 __device__ __forceinline__ u32x4 decode(uint32_t lo, uint32_t hi, float scale) {
     u32x4 r;
@@ -157,6 +250,60 @@ __device__ __forceinline__ u32x4 decode(uint32_t lo, uint32_t hi, float scale) {
     return r;
 }
 
+// Positions below a sequence's length as bf16: the codes' order is the bf16 pages' order, so a wavefront streams one
+// page of one head, 8 codes per lane and load and 16 bytes per lane and store. Slots past the length are zero; a page
+// that is not there reads as zeros, an output page outside its pool is not written.
+__global__ void __launch_bounds__(256)
+    kv8_read_kernel(Table t, const uint8_t* __restrict__ codes, const uint8_t* __restrict__ scales,
+                    const uint32_t* __restrict__ lens, bf16_t* __restrict__ k_out, bf16_t* __restrict__ v_out,
+                    const uint32_t* __restrict__ out_table, uint32_t out_pool) {
+    const uint32_t s = blockIdx.y, i = threadIdx.x & 63;
+    const uint32_t keys = kv8_keys(lens[s], t.seq_pages);
+    const uint64_t records = (uint64_t)((keys + KV8_PAGE - 1) / KV8_PAGE) * t.kv_heads;
+    for (uint64_t id = (uint64_t)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6); id < records; id += (uint64_t)gridDim.x * 4) {
+        const uint32_t p = (uint32_t)(id / t.kv_heads), kh = (uint32_t)(id % t.kv_heads);
+        const uint32_t to = kv8_page(out_table, t.seqs, t.seq_pages, out_pool, s, p), page = t.page(s, p);
+        if (to == KV8_NONE) continue;
+        const uint32_t valid = page == KV8_NONE ? 0u : min(keys - p * KV8_PAGE, KV8_PAGE), from = page == KV8_NONE ? 0u : page;
+        const u32x2* rec = reinterpret_cast<const u32x2*>(codes + kv8_record(from, t.kv_heads, kh)) + i;
+        const uint8_t* sc = scales + kv8_scale(from, t.kv_heads, kh);
+        u32x2 k[4], v[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) k[j] = rec[64 * j];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) v[j] = rec[KV8_PART / 8 + 64 * j];
+        // Keys 4 j + i / 16; the values of positions 8 (i % 2) .. + 7.
+        const u32x4 ks = *reinterpret_cast<const u32x4*>(sc);
+        const u32x2 vs = *reinterpret_cast<const u32x2*>(sc + KV8_PAGE + 8 * (i & 1));
+        u32x4 *kd = reinterpret_cast<u32x4*>(k_out + ((size_t)to * t.kv_heads + kh) * KV8_PART) + i,
+              *vd = reinterpret_cast<u32x4*>(v_out + ((size_t)to * t.kv_heads + kh) * KV8_PART) + i;
+        float power[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) power[e] = __uint_as_float((vs[e / 4] >> 8 * (e % 4) & 0xFFu) << 23);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            u32x4 x = decode(k[j][0], k[j][1], __uint_as_float((ks[j] >> 8 * (i >> 4) & 0xFFu) << 23));
+            if (4 * j + (i >> 4) >= valid) x = u32x4{0, 0, 0, 0};
+            kd[64 * j] = x;
+        }
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            float f[8];
+#pragma unroll
+            for (int e = 0; e < 8; e += 2) {
+                const auto two = (e & 2) ? __builtin_amdgcn_cvt_pk_f32_fp8((int)v[j][e / 4], true)
+                                         : __builtin_amdgcn_cvt_pk_f32_fp8((int)v[j][e / 4], false);
+                f[e] = 8 * (i & 1) + e < valid ? two[0] * power[e] : 0.f;
+                f[e + 1] = 8 * (i & 1) + e + 1 < valid ? two[1] * power[e + 1] : 0.f;
+            }
+            vd[64 * j] = u32x4{pack(f[0], f[1]), pack(f[2], f[3]), pack(f[4], f[5]), pack(f[6], f[7])};
+        }
+    }
+}
+
+__device__ __forceinline__ f32x4 mfma(u32x4 a, u32x4 b, f32x4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+}
 // Partial states go between blocks through agent-scope accesses, coherent across the XCDs' caches.
 __device__ __forceinline__ void put2(float* p, float a, float b) {
     __hip_atomic_store((uint64_t*)p, (uint64_t)__float_as_uint(b) << 32 | __float_as_uint(a), __ATOMIC_RELAXED,
@@ -850,19 +997,24 @@ extern "C" x0ne_status x0ne_gpu_kv8_write(x0ne_gpu* g, const x0ne_kv8* c, uint64
         k_norm % 16 || rope_cs % 16 || row_seq % 4 || row_pos % 4 || q_out % 16 || bounds % 16)
         return bad(what, "qkv, q_norm, k_norm, rope_cs and q_out (16-byte aligned), row_seq and row_pos are required");
     if (!g) return fail(X0NE_ERR_GPU, "no device");
-    if (rows == 0 || c->seqs == 0) return X0NE_OK;
+    if (rows == 0 || c->seqs == 0 || positions == 0) return X0NE_OK;
     const OnDevice on(g->device);
     const Table t = table_of(c);
     g->counts.launches += bounds ? 2 : 1;
-    hipLaunchKernelGGL(kv8_write_kernel, dim3((uint32_t)rows, (q_heads + c->kv_heads + 3) / 4), dim3(256), 0, g->stream, t,
-                       (uint8_t*)c->codes, (uint8_t*)c->scales, (const bf16_t*)qkv, (const bf16_t*)q_norm,
-                       (const bf16_t*)k_norm, (const double*)rope_cs, (const uint32_t*)row_seq, (const uint32_t*)row_pos,
-                       (bf16_t*)q_out, q_heads, positions, eps);
+    // 8 heads to a block read cos and sin, and take square roots, least often; where that leaves CUs idle, 2.
+    const uint32_t tiles = ((uint32_t)rows + WRITE_ROWS - 1) / WRITE_ROWS, heads = q_heads + c->kv_heads;
+    const uint32_t values = (c->kv_heads + WRITE_VALUES - 1) / WRITE_VALUES;
+    const bool many = (uint64_t)tiles * (heads / 8) >= 256;
+    const dim3 grid(tiles, (many ? (heads + 7) / 8 : (heads + 1) / 2) + values);
+    hipLaunchKernelGGL(many ? kv8_write_kernel<8> : kv8_write_kernel<2>, grid, dim3(256), 0, g->stream, t, (uint8_t*)c->codes,
+                       (uint8_t*)c->scales, (const bf16_t*)qkv, (const bf16_t*)q_norm, (const bf16_t*)k_norm,
+                       (const double*)rope_cs, (const uint32_t*)row_seq, (const uint32_t*)row_pos, (bf16_t*)q_out,
+                       (uint32_t)rows, q_heads, positions, eps);
     X0NE_HIP(hipGetLastError(), what);
     if (!bounds) return X0NE_OK;
-    hipLaunchKernelGGL(kv8_bounds_kernel, dim3((uint32_t)rows, (c->kv_heads + 3) / 4), dim3(256), 0, g->stream, t,
+    hipLaunchKernelGGL(kv8_bounds_kernel, dim3(tiles, (c->kv_heads + 3) / 4), dim3(256), 0, g->stream, t,
                        (const uint8_t*)c->codes, (const uint8_t*)c->scales, (const uint32_t*)row_seq,
-                       (const uint32_t*)row_pos, positions, (bf16_t*)bounds);
+                       (const uint32_t*)row_pos, (uint32_t)rows, positions, (bf16_t*)bounds);
     X0NE_HIP(hipGetLastError(), "kv8 bounds");
     return X0NE_OK;
 }
@@ -877,7 +1029,8 @@ extern "C" x0ne_status x0ne_gpu_kv8_read(x0ne_gpu* g, const x0ne_kv8* c, uint64_
     if (c->seqs == 0) return X0NE_OK;
     const OnDevice on(g->device);
     g->counts.launches++;
-    hipLaunchKernelGGL(kv8_read_kernel, dim3(c->seq_pages, (c->kv_heads + 3) / 4, c->seqs), dim3(256), 0, g->stream,
+    const uint64_t blocks = std::min<uint64_t>(65536, ((uint64_t)c->seq_pages * c->kv_heads + 3) / 4);
+    hipLaunchKernelGGL(kv8_read_kernel, dim3((uint32_t)blocks, c->seqs), dim3(256), 0, g->stream,
                        table_of(c), (const uint8_t*)c->codes, (const uint8_t*)c->scales, (const uint32_t*)lens,
                        (bf16_t*)k, (bf16_t*)v, (const uint32_t*)out_table, out_pool);
     X0NE_HIP(hipGetLastError(), what);
