@@ -223,8 +223,10 @@ typedef struct {
    whose sequence is not below seqs, or whose position has no table entry or no page-table entry, is
    padding: nothing of it is written. bounds (0: none): [pool][kv_heads][2][128] bf16, of every page
    whose last position is among the rows the smallest and the largest key value of each dim over its
-   16 positions (zeros +0, NaN where a key is), for x0ne_gpu_kv8_select. qkv, q_norm, k_norm, rope_cs, q_out and
-   bounds are 16-byte aligned; q_heads 1 to 16384, rows below 2^24. */
+   16 positions (zeros +0, NaN where a key is), for x0ne_gpu_kv8_select; the rows of such a page then
+   stand together, their positions ascending by 1 (as those of a prompt do; the page's other positions
+   are those of earlier calls). qkv, q_norm, k_norm, rope_cs, q_out and bounds are 16-byte aligned;
+   q_heads 1 to 16384, rows below 2^24. */
 x0ne_status x0ne_gpu_kv8_write(x0ne_gpu* g, const x0ne_kv8* c, uint64_t qkv, uint64_t rows, uint32_t q_heads,
                                uint64_t q_norm, uint64_t k_norm, float eps, uint64_t rope_cs, uint32_t positions,
                                uint64_t row_seq, uint64_t row_pos, uint64_t q_out, uint64_t bounds);

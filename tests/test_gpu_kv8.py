@@ -70,11 +70,32 @@ def test_write_of_one_prompt(kernels, rows, first):
 
 
 def test_write_of_whole_pages_of_several_sequences_in_any_order(kernels):
-    """Runs of 16 rows that fill pages, rows of one page in falling order, and a row at the end of another's tile."""
+    """Runs of 16 rows that fill pages, rows of one page in falling order (which bounds do not take), and a row at the
+    end of another's tile."""
     rng = np.random.default_rng(5)
     row_seq = [1] * 16 + [0] * 16 + [2] * 15 + [0]
     row_pos = list(range(32, 48)) + list(range(31, 15, -1)) + list(range(0, 15)) + [15]
+    check_write(kernels, rng, 8, 4, random_qkv(rng, len(row_seq), 8, 4), row_seq, row_pos, 3, 3, with_bounds=False)
+    row_pos[16:32] = range(16, 32)
     check_write(kernels, rng, 8, 4, random_qkv(rng, len(row_seq), 8, 4), row_seq, row_pos, 3, 3)
+
+
+@pytest.mark.parametrize("heads", [(2, 2), (16, 8), (40, 8), (9, 9)])
+def test_bounds_of_pages_filled_over_several_calls(kernels, heads):
+    """Pages begun by an earlier call and ended by runs that start inside them, over two blocks' rows or one, by single
+    rows of a batch, by a run from another block's tile; poison in an old key and in a new one."""
+    rng = np.random.default_rng(heads[0])
+    seqs, seq_pages = 12, 5
+    c = R.fill(rng, heads[1], [5, 12, 15, 31, 14, 15, 47, 0, 79, 63, 30, 1], seq_pages)
+    c.codes[c.table[3, 1], 0, 7 * HEAD + 9] = 0x7F
+    c.codes[c.table[3, 1], 0, 15 * HEAD:16 * HEAD] = 0x7F
+    runs = [(0, 5, 40), (1, 12, 4), (2, 15, 1), (3, 31, 1), (4, 14, 2), (5, 15, 18), (6, 47, 1), (7, 0, 16), (8, 79, 1),
+            (9, 63, 1), (10, 30, 30), (11, 1, 15)]
+    row_seq = [s for s, _, n in runs for _ in range(n)]
+    row_pos = [p + i for _, p, n in runs for i in range(n)]
+    qkv = random_qkv(rng, len(row_seq), *heads)
+    qkv.reshape(len(row_seq), -1, HEAD)[43, heads[0], 100] = 0x7FC0  # a key of sequence 1's page
+    check_write(kernels, rng, *heads, qkv, row_seq, row_pos, seq_pages, seqs, cache=c)
 
 
 def test_rows_past_the_table_or_the_pool_are_left_alone(kernels):

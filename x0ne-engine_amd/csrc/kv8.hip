@@ -24,8 +24,6 @@ __device__ __forceinline__ float kv8_value(uint32_t code, uint32_t scale) {
     return __builtin_amdgcn_cvt_f32_fp8((int)code, 0) * __uint_as_float(scale << 23);
 }
 
-__device__ __forceinline__ bool finite(float x) { return (__float_as_uint(x) & 0x7F800000u) != 0x7F800000u; }
-
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
@@ -37,205 +35,281 @@ __device__ __forceinline__ uint32_t pack(float lo, float hi) {
 }
 __device__ __forceinline__ float half_of(const u32x4& x, int e) { return e & 1 ? bf_hi(x[e / 2]) : bf_lo(x[e / 2]); }
 
-// f32 and f64 values moved within a row of 16 lanes by DPP (CTRL 0xB1, 0x4E: xor 1 and 2; 0x141: lane 7 - i of each
-// half row; 0x128: 8 lanes round).
+// Values moved within a row of 16 lanes by DPP (0xB1, 0x4E: xor 1 and 2; 0x141: lane 7 - i of each half row; 0x128: 8
+// lanes round): every lane has a source, so no old value is kept.
 template <int CTRL>
-__device__ __forceinline__ float dpp_f(float v) {
-    return __uint_as_float((uint32_t)__builtin_amdgcn_update_dpp(0, (int)__float_as_uint(v), CTRL, 0xF, 0xF, false));
+__device__ __forceinline__ uint32_t row_move(uint32_t v) {
+    return (uint32_t)__builtin_amdgcn_mov_dpp((int)v, CTRL, 0xF, 0xF, true);
 }
-__device__ __forceinline__ float row_max(float v) {
-    v = fmaxf(v, dpp_f<0xB1>(v));
-    v = fmaxf(v, dpp_f<0x4E>(v));
-    v = fmaxf(v, dpp_f<0x141>(v));
-    return fmaxf(v, dpp_f<0x128>(v));
+template <int CTRL>
+__device__ __forceinline__ double row_move_d(double v) {
+    const uint64_t u = (uint64_t)__double_as_longlong(v);
+    return __longlong_as_double((long long)((uint64_t)row_move<CTRL>((uint32_t)(u >> 32)) << 32 | row_move<CTRL>((uint32_t)u)));
+}
+typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
+__device__ __forceinline__ uint32_t max_u16(uint32_t a, uint32_t b) {
+    return __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(u16x2, a), __builtin_bit_cast(u16x2, b)));
 }
 
-// The codes of a lane's 8 values of a row that lies in 16 lanes, and the row's scale byte.
-__device__ __forceinline__ u32x2 quantise(const float (&x)[8], uint32_t& scale) {
-    float top = 0.f;
+// The codes of a lane's 8 bf16 values of a row that lies in 16 lanes, and the row's scale byte. The largest magnitude
+// is that of the bit patterns, two at a time; infinities and NaN, whose patterns are above all finite ones, are taken
+// out (and their codes set: the conversion's own NaN has either sign) only where a wavefront meets one.
+__device__ __forceinline__ u32x2 quantise(u32x4 x, uint32_t& scale) {
+    auto largest = [](u32x4 m) {
+        uint32_t top = max_u16(max_u16(m[0], m[1]), max_u16(m[2], m[3]));
+        top = max(top & 0xFFFFu, top >> 16);
+        top = max(top, row_move<0xB1>(top));
+        top = max(top, row_move<0x4E>(top));
+        top = max(top, row_move<0x141>(top));
+        return max(top, row_move<0x128>(top));
+    };
+    const u32x4 mag = x & 0x7FFF7FFFu;
+    uint32_t top = largest(mag);
+    const bool poison = __any(top >= 0x7F80u);
+    if (poison) {
+        u32x4 m = mag;
 #pragma unroll
-    for (int j = 0; j < 8; ++j) top = fmaxf(top, finite(x[j]) ? fabsf(x[j]) : 0.f);
-    const int e = kv8_exponent(__float_as_uint(row_max(top)) >> 16);
+        for (int j = 0; j < 4; ++j) {
+            m[j] &= ((m[j] & 0xFFFFu) >= 0x7F80u ? 0u : 0xFFFFu) | (m[j] >> 16 >= 0x7F80u ? 0u : 0xFFFF0000u);
+        }
+        top = largest(m);
+    }
+    const int e = kv8_exponent(top);
     scale = (uint32_t)(e + 127);
-    const float down = __uint_as_float((uint32_t)(127 - e) << 23);
+    const float power = __uint_as_float(scale << 23);
+    typedef short s16x2 __attribute__((ext_vector_type(2)));
     u32x2 w;
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
-        int c = __builtin_amdgcn_cvt_pk_fp8_f32(x[4 * j] * down, x[4 * j + 1] * down, 0, false);
-        w[j] = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(x[4 * j + 2] * down, x[4 * j + 3] * down, c, true);
+        const uint32_t first = x[2 * j], second = x[2 * j + 1];  // an element of a vector is no object to cast
+        s16x2 c = {0, 0};
+        c = __builtin_amdgcn_cvt_scalef32_pk_fp8_bf16(c, __builtin_bit_cast(bf16x2, first), power, false);
+        c = __builtin_amdgcn_cvt_scalef32_pk_fp8_bf16(c, __builtin_bit_cast(bf16x2, second), power, true);
+        w[j] = __builtin_bit_cast(uint32_t, c);
     }
-    // The conversion's own NaN has either sign: 0x7F stands for all that is not finite.
+    if (poison) {
 #pragma unroll
-    for (int j = 0; j < 8; ++j)
-        if (!finite(x[j])) w[j / 4] = (w[j / 4] & ~(0xFFu << 8 * (j % 4))) | 0x7Fu << 8 * (j % 4);
+        for (int j = 0; j < 8; ++j) {
+            const uint32_t code = 0xFFu << 8 * (j % 4);
+            w[j / 4] = (mag[j / 2] >> 16 * (j % 2) & 0xFFFFu) >= 0x7F80u ? (w[j / 4] & ~code) | (0x7F7F7F7Fu & code) : w[j / 4];
+        }
+    }
     return w;
 }
 
-constexpr uint32_t WRITE_ROWS = 16;  // rows of a block, one to 16 lanes
+constexpr uint32_t WRITE_ROWS = 16;   // rows of a block, one to 16 lanes
+constexpr uint32_t WRITE_HEADS = 4;   // heads of q or k that a block takes, where there are blocks enough
 constexpr uint32_t WRITE_VALUES = 4;  // kv heads whose values a block takes
 
+struct Write {
+    Table t;
+    uint8_t *codes, *scales;
+    const bf16_t *qkv, *q_norm, *k_norm;
+    const double2* cs;
+    const uint32_t *row_seq, *row_pos;
+    bf16_t *q_out, *bounds;
+    uint32_t rows, q_heads, positions;
+    float eps;
+};
+
+// A lane's part of a head: dims 4 n .. + 3 and the same 64 dims on, so that a dim and the one it is rotated with are in
+// one lane.
+__device__ __forceinline__ u32x4 load_head(const bf16_t* head, uint32_t n) {
+    const u32x2 a = *reinterpret_cast<const u32x2*>(head + 4 * n), b = *reinterpret_cast<const u32x2*>(head + 64 + 4 * n);
+    return u32x4{a[0], a[1], b[0], b[1]};
+}
+// The sum of a head's squares, every lane of its 16 with it: pairs (i, i + 64) first, then the bits of i from the
+// lowest, the tree of x0ne_qk_norm_rope_kv_write_rows_bf16 (the squares are exact, so the pairs' sums are one fma).
+__device__ __forceinline__ double square_sum(u32x4 x) {
+    double s[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        const double a = (double)half_of(x, j), b = (double)half_of(x, 4 + j);
+        s[j] = fma(b, b, a * a);
+    }
+    double sum = (s[0] + s[1]) + (s[2] + s[3]);
+    sum += row_move_d<0xB1>(sum);
+    sum += row_move_d<0x4E>(sum);
+    sum += row_move_d<0x141>(sum);
+    return sum + row_move_d<0x128>(sum);
+}
+// The head normed (scale: 1 over its root mean square) and rotated, as bf16.
+__device__ __forceinline__ u32x4 turn_head(u32x4 x, double scale, u32x4 w, const double2 (&c)[4]) {
+    float a[4], b[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        const double na = (double)half_of(x, j) * scale * (double)half_of(w, j);
+        const double nb = (double)half_of(x, 4 + j) * scale * (double)half_of(w, 4 + j);
+        a[j] = (float)(na * c[j].x - nb * c[j].y);
+        b[j] = (float)(nb * c[j].x + na * c[j].y);
+    }
+    return u32x4{pack(a[0], a[1]), pack(a[2], a[3]), pack(b[0], b[1]), pack(b[2], b[3])};
+}
+__device__ __forceinline__ double root_of(double sum, float eps) { return 1.0 / sqrt(sum / (double)KV8_HEAD + (double)eps); }
+
+// The bounds of a page whose key of slot r lies as codes w (dims as load_head's) and a scale byte in the 16 lanes r of
+// the block: the keys through LDS, then a thread per dim and side.
+typedef float KeyValues[KV8_PAGE][KV8_HEAD + 4];
+__device__ __forceinline__ void put_bounds(u32x2 w, uint32_t byte, bf16_t* to, KeyValues& keys) {
+    const uint32_t n = threadIdx.x & 15, r = threadIdx.x >> 4;
+#pragma unroll
+    for (int j = 0; j < 2; ++j)
+        *reinterpret_cast<f32x4*>(&keys[r][64 * j + 4 * n]) = f32x4{kv8_value(w[j] & 0xFFu, byte), kv8_value(w[j] >> 8 & 0xFFu, byte),
+                                                                    kv8_value(w[j] >> 16 & 0xFFu, byte), kv8_value(w[j] >> 24, byte)};
+    lds_barrier();
+    const uint32_t d = threadIdx.x % KV8_HEAD;
+    const float sign = threadIdx.x < KV8_HEAD ? -1.f : 1.f;  // the smallest is the largest of the negatives
+    float top = -INFINITY;
+    bool nan = false;
+#pragma unroll
+    for (uint32_t i = 0; i < KV8_PAGE; ++i) {
+        const float v = sign * keys[i][d];
+        nan |= v != v;
+        top = fmaxf(top, v);
+    }
+    to[threadIdx.x] = f2bf(nan ? __uint_as_float(0x7FC00000u) : sign * top + 0.f);  // a zero of either sign is +0
+    lds_barrier();  // the keys are read
+}
+
 // RMSNorm of each head of q and k, rotate-half RoPE from the table, q to q_out as bf16, k and v quantised into their
-// page: the arithmetic of x0ne_qk_norm_rope_kv_write_rows_bf16, its sum of squares added in the same tree, so q_out has
-// its bits and the codes are those of its k row. A block takes 16 rows; 16 lanes have one row, lane n dims 8 n .. + 7 (16
-// bytes), so a dim and its pair 64 dims on are 8 lanes apart (a DPP move). blockIdx.y: HEADS heads of q and k, whose
-// loads are all requested at once, whose cos and sin are read once and whose f64 square roots and divisions are one
-// (lane h computes head h's); or, behind those, the values of WRITE_VALUES kv heads, turned dim-major in LDS: where the
-// block's rows are one whole page, as in a prompt, that is stored as such, else byte by byte. A row of no sequence, or
-// past the sequence's pages or the rope table, writes nothing.
+// page: the arithmetic of x0ne_qk_norm_rope_kv_write_rows_bf16, so q_out has its bits and the codes are those of its k
+// row. A block takes 16 rows, 16 lanes to a row, and by blockIdx.y
+//  - HEADS heads of q, or of k behind those: their loads are all requested at once, cos and sin are read once, and the
+//    f64 square roots and divisions are one for all (lane i computes head i's);
+//  - then the values of WRITE_VALUES kv heads, turned dim-major in LDS: where the block's rows are one whole page, as in
+//    a prompt, that is stored as such, else byte by byte.
+// A row of no sequence, or past the sequence's pages or the rope table, writes nothing.
+// Bounds of a page belong to the blocks of the row of its last slot. Rows that are one whole page have its keys at
+// hand; else each 16 lanes take a slot: a row of this call (of the 15 rows before) is computed again, since another
+// block writes its codes meanwhile, an older one is read from the cache.
 template <int HEADS>
-__global__ void __launch_bounds__(256)
-    kv8_write_kernel(Table t, uint8_t* __restrict__ codes, uint8_t* __restrict__ scales, const bf16_t* __restrict__ qkv,
-                     const bf16_t* __restrict__ q_norm, const bf16_t* __restrict__ k_norm, const double* __restrict__ cs,
-                     const uint32_t* __restrict__ row_seq, const uint32_t* __restrict__ row_pos,
-                     bf16_t* __restrict__ q_out, uint32_t rows, uint32_t q_heads, uint32_t positions, float eps) {
+__global__ void __launch_bounds__(256) kv8_write_kernel(const Write a) {
     constexpr uint32_t HD = KV8_HEAD;
-    __shared__ uint32_t turned[WRITE_VALUES][KV8_PART / 4];
-    __shared__ uint32_t page_of[WRITE_ROWS], slot_of[WRITE_ROWS];
-    const uint32_t n = threadIdx.x & 15, r = threadIdx.x >> 4, row = blockIdx.x * WRITE_ROWS + r, at = min(row, rows - 1);
-    const uint32_t seq = row_seq[at], pos = row_pos[at], slot = pos % KV8_PAGE;
-    const bool live = row < rows && seq < t.seqs && pos < positions && pos / KV8_PAGE < t.seq_pages;
-    const uint32_t page = live ? t.page(seq, pos / KV8_PAGE) : KV8_NONE;
-    const uint32_t heads = q_heads + t.kv_heads, parts = (heads + HEADS - 1) / HEADS;
-    const bf16_t* line = qkv + (size_t)at * (heads + t.kv_heads) * HD + 8 * n;
+    __shared__ union {
+        uint32_t turned[WRITE_VALUES][KV8_PART / 4];
+        KeyValues keys;
+    } sh;
+    const uint32_t n = threadIdx.x & 15, r = threadIdx.x >> 4, r0 = blockIdx.x * WRITE_ROWS, last = a.rows - 1;
+    const uint32_t kvh = a.t.kv_heads, heads = a.q_heads + kvh;
+    const uint32_t q_parts = (a.q_heads + HEADS - 1) / HEADS, parts = q_parts + (kvh + HEADS - 1) / HEADS;
+    const size_t stride = (size_t)(heads + kvh) * HD;
+    auto live_at = [&](uint32_t row, uint32_t seq, uint32_t pos) {
+        return row <= last && seq < a.t.seqs && pos < a.positions && pos / KV8_PAGE < a.t.seq_pages;
+    };
+    const uint32_t row = r0 + r, seq = a.row_seq[min(row, last)], pos = a.row_pos[min(row, last)], slot = pos % KV8_PAGE;
+    const bool live = live_at(row, seq, pos);
+    // Row n of the block, in every 16 lanes: what the block as a whole goes by.
+    const uint32_t row_n = r0 + n, seq_n = a.row_seq[min(row_n, last)], pos_n = a.row_pos[min(row_n, last)];
+    auto page_at = [&](uint32_t row, uint32_t seq, uint32_t pos) {
+        return live_at(row, seq, pos) ? a.t.page(seq, pos / KV8_PAGE) : KV8_NONE;
+    };
+    const bf16_t* line = a.qkv + min(row, last) * stride;
     if (blockIdx.y < parts) {
-        const uint32_t h0 = blockIdx.y * HEADS;
+        const bool is_q = blockIdx.y < q_parts;
+        // Heads of q, or (the same code on other numbers) of k, which lie behind them.
+        const uint32_t h0 = (is_q ? blockIdx.y : blockIdx.y - q_parts) * HEADS, count = min((uint32_t)HEADS, (is_q ? a.q_heads : kvh) - h0);
+        const size_t first = (size_t)(is_q ? h0 : a.q_heads + h0) * HD;
         u32x4 x[HEADS];
 #pragma unroll
-        for (int i = 0; i < HEADS; ++i) x[i] = *reinterpret_cast<const u32x4*>(line + (size_t)min(h0 + i, heads - 1) * HD);
-        const double2* c = reinterpret_cast<const double2*>(cs) + (size_t)(live ? pos : 0) * (HD / 2) + 8 * (n & 7);
-        double co[8], si[8];
+        for (uint32_t i = 0; i < HEADS; ++i) x[i] = load_head(line + first + min(i, count - 1) * HD, n);
+        const u32x4 w = load_head(is_q ? a.q_norm : a.k_norm, n);
+        double2 c[4];
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            const double2 v = c[j];
-            co[j] = v.x;
-            si[j] = n < 8 ? -v.y : v.y;
-        }
-        const u32x4 wq = *reinterpret_cast<const u32x4*>(q_norm + 8 * n), wk = *reinterpret_cast<const u32x4*>(k_norm + 8 * n);
+        for (int j = 0; j < 4; ++j) c[j] = a.cs[(size_t)(live ? pos : 0) * (HD / 2) + 4 * n + j];
+        const uint32_t page = is_q ? KV8_NONE : page_at(row, seq, pos), page_n = is_q ? KV8_NONE : page_at(row_n, seq_n, pos_n);
         double square = 0.0;
 #pragma unroll
-        for (int i = 0; i < HEADS; ++i) {
-            double s[8];
-#pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                const double v = (double)half_of(x[i], j);
-                s[j] = v * v;
-            }
-#pragma unroll
-            for (int j = 0; j < 8; ++j) s[j] += dpp_d<0x128>(s[j]);
-            double sum = ((s[0] + s[1]) + (s[2] + s[3])) + ((s[4] + s[5]) + (s[6] + s[7]));
-            sum += dpp_d<0xB1>(sum);
-            sum += dpp_d<0x4E>(sum);
-            sum += dpp_d<0x141>(sum);
-            if (n == (uint32_t)i) square = sum;
+        for (uint32_t i = 0; i < HEADS; ++i) {
+            const double sum = square_sum(x[i]);
+            if (n == i) square = sum;
         }
-        const double root = 1.0 / sqrt(square / (double)HD + (double)eps);
+        const double root = root_of(square, a.eps);
 #pragma unroll
-        for (int i = 0; i < HEADS; ++i) {
-            const uint32_t head = h0 + i;
-            if (head >= heads) break;
-            const bool is_q = head < q_heads;
-            const double scale = __shfl(root, (threadIdx.x & 48) + i, 64);
-            double own[8];
-            float out[8];
+        for (uint32_t i = 0; i < HEADS; ++i) x[i] = turn_head(x[i], __shfl(root, (threadIdx.x & 48) + i, 64), w, c);
+        if (is_q) {
+            bf16_t* to = a.q_out + ((size_t)row * a.q_heads + h0) * HD;
 #pragma unroll
-            for (int j = 0; j < 8; ++j) own[j] = (double)half_of(x[i], j) * scale * (double)half_of(is_q ? wq : wk, j);
+            for (uint32_t i = 0; i < HEADS; ++i)
+                if (live && i < count) {
+                    *reinterpret_cast<u32x2*>(to + i * HD + 4 * n) = u32x2{x[i][0], x[i][1]};
+                    *reinterpret_cast<u32x2*>(to + i * HD + 64 + 4 * n) = u32x2{x[i][2], x[i][3]};
+                }
+            return;
+        }
+        const bool whole = __all(page_n != KV8_NONE && pos_n % KV8_PAGE == n && page_n == __builtin_amdgcn_readfirstlane(page_n));
+        u32x2 code[HEADS];
+        uint32_t byte[HEADS];
 #pragma unroll
-            for (int j = 0; j < 8; ++j) out[j] = (float)(own[j] * co[j] + dpp_d<0x128>(own[j]) * si[j]);
-            const u32x4 b = {pack(out[0], out[1]), pack(out[2], out[3]), pack(out[4], out[5]), pack(out[6], out[7])};
-            if (is_q) {
-                if (live) *reinterpret_cast<u32x4*>(q_out + ((size_t)row * q_heads + head) * HD + 8 * n) = b;
-                continue;
+        for (uint32_t i = 0; i < HEADS; ++i) {
+            code[i] = quantise(x[i], byte[i]);
+            if (page == KV8_NONE || i >= count) continue;
+            uint8_t* to = a.codes + kv8_record(page, kvh, h0 + i) + slot * HD;
+            *reinterpret_cast<uint32_t*>(to + 4 * n) = code[i][0];
+            *reinterpret_cast<uint32_t*>(to + 64 + 4 * n) = code[i][1];
+            if (n == 0) a.scales[kv8_scale(page, kvh, h0 + i) + slot] = (uint8_t)byte[i];
+        }
+        if (!a.bounds) return;
+        if (whole) {
+#pragma unroll
+            for (uint32_t i = 0; i < HEADS; ++i)
+                if (i < count) put_bounds(code[i], byte[i], a.bounds + kv8_bound(page_n, kvh, h0 + i), sh.keys);
+            return;
+        }
+        for (uint64_t ends = __ballot(page_n != KV8_NONE && pos_n % KV8_PAGE == KV8_PAGE - 1) & 0xFFFFu; ends; ends &= ends - 1) {
+            const uint32_t at = (uint32_t)__builtin_ctzll(ends), end = r0 + at;
+            const uint32_t its_seq = __builtin_amdgcn_readlane(seq_n, at), its_pos = __builtin_amdgcn_readlane(pos_n, at);
+            const uint32_t its_page = __builtin_amdgcn_readlane(page_n, at);
+            const uint32_t from = end + r - 15, from_pos = its_pos + r - 15;  // slot r's row, if it is of this call
+            const bool fresh = end + r >= 15 && a.row_seq[min(from, last)] == its_seq && a.row_pos[min(from, last)] == from_pos;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) c[j] = a.cs[(size_t)from_pos * (HD / 2) + 4 * n + j];
+#pragma unroll
+            for (uint32_t i = 0; i < HEADS; ++i) {
+                const uint32_t h = h0 + min(i, count - 1);
+                const uint8_t* rec = a.codes + kv8_record(its_page, kvh, h) + r * HD;
+                code[i] = u32x2{*reinterpret_cast<const uint32_t*>(rec + 4 * n), *reinterpret_cast<const uint32_t*>(rec + 64 + 4 * n)};
+                byte[i] = a.scales[kv8_scale(its_page, kvh, h) + r];
+                x[i] = load_head(a.qkv + min(from, last) * stride + first + min(i, count - 1) * HD, n);
             }
-            float v[8];
 #pragma unroll
-            for (int j = 0; j < 8; ++j) v[j] = half_of(b, j);
-            uint32_t byte;
-            const u32x2 w = quantise(v, byte);
-            if (page == KV8_NONE) continue;
-            *reinterpret_cast<u32x2*>(codes + kv8_record(page, t.kv_heads, head - q_heads) + slot * HD + 8 * n) = w;
-            if (n == 0) scales[kv8_scale(page, t.kv_heads, head - q_heads) + slot] = (uint8_t)byte;
+            for (uint32_t i = 0; i < HEADS; ++i) {
+                if (i >= count) break;
+                uint32_t again;
+                const u32x2 v = quantise(turn_head(x[i], root_of(square_sum(x[i]), a.eps), w, c), again);
+                if (fresh) {
+                    code[i] = v;
+                    byte[i] = again;
+                }
+                put_bounds(code[i], byte[i], a.bounds + kv8_bound(its_page, kvh, h0 + i), sh.keys);
+            }
         }
         return;
     }
     const uint32_t k0 = (blockIdx.y - parts) * WRITE_VALUES;
     u32x4 x[WRITE_VALUES];
 #pragma unroll
-    for (uint32_t i = 0; i < WRITE_VALUES; ++i) x[i] = *reinterpret_cast<const u32x4*>(line + (size_t)(heads + min(k0 + i, t.kv_heads - 1)) * HD);
-    if (n == 0) {
-        page_of[r] = page;
-        slot_of[r] = slot;
-    }
+    for (uint32_t i = 0; i < WRITE_VALUES; ++i) x[i] = *reinterpret_cast<const u32x4*>(line + (heads + min(k0 + i, kvh - 1)) * HD + 8 * n);
+    const uint32_t page = page_at(row, seq, pos), page_n = page_at(row_n, seq_n, pos_n);
+    const bool whole = __all(page_n != KV8_NONE && pos_n % KV8_PAGE == n && page_n == __builtin_amdgcn_readfirstlane(page_n));
 #pragma unroll
     for (uint32_t i = 0; i < WRITE_VALUES; ++i) {
-        float v[8];
-#pragma unroll
-        for (int j = 0; j < 8; ++j) v[j] = half_of(x[i], j);
         uint32_t byte;
-        const u32x2 w = quantise(v, byte);
-        uint8_t* to = reinterpret_cast<uint8_t*>(turned[i]) + 8 * n * WRITE_ROWS + r;
+        const u32x2 w = quantise(x[i], byte);
+        uint8_t* to = reinterpret_cast<uint8_t*>(sh.turned[i]) + 8 * n * WRITE_ROWS + r;
 #pragma unroll
         for (int j = 0; j < 8; ++j) to[j * WRITE_ROWS] = (uint8_t)(w[j / 4] >> 8 * (j % 4));
-        if (n == 0 && page != KV8_NONE && k0 + i < t.kv_heads)
-            scales[kv8_scale(page, t.kv_heads, k0 + i) + KV8_PAGE + slot] = (uint8_t)byte;
+        if (n == 0 && page != KV8_NONE && k0 + i < kvh) a.scales[kv8_scale(page, kvh, k0 + i) + KV8_PAGE + slot] = (uint8_t)byte;
     }
-    __syncthreads();
-    const bool whole = __all(page_of[n] == page_of[0] && page_of[0] != KV8_NONE && slot_of[n] == n);
+    lds_barrier();
 #pragma unroll
     for (uint32_t i = 0; i < WRITE_VALUES; ++i) {
-        if (k0 + i >= t.kv_heads) break;
+        if (k0 + i >= kvh) break;
         if (whole) {
-            uint8_t* to = codes + kv8_record(page_of[0], t.kv_heads, k0 + i) + KV8_PART;
-            reinterpret_cast<u32x2*>(to)[threadIdx.x] = reinterpret_cast<const u32x2*>(turned[i])[threadIdx.x];
-        } else if (page_of[n] != KV8_NONE) {
-            uint8_t* to = codes + kv8_record(page_of[n], t.kv_heads, k0 + i) + KV8_PART + slot_of[n];
-            for (uint32_t d = r; d < HD; d += 16) to[d * KV8_PAGE] = reinterpret_cast<const uint8_t*>(turned[i])[d * WRITE_ROWS + n];
-        }
-    }
-}
-
-// The bounds of the pages that the rows complete (slot 15), from the codes. A wavefront per 16 rows and kv head: lane
-// (n, g) has dims 8 n .. + 7 of keys 4 g .. + 3 of such a page.
-__global__ void __launch_bounds__(256)
-    kv8_bounds_kernel(Table t, const uint8_t* __restrict__ codes, const uint8_t* __restrict__ scales,
-                      const uint32_t* __restrict__ row_seq, const uint32_t* __restrict__ row_pos, uint32_t rows,
-                      uint32_t positions, bf16_t* __restrict__ bounds) {
-    const uint32_t lane = threadIdx.x & 63, n = lane & 15, g = lane >> 4, kh = blockIdx.y * 4 + (threadIdx.x >> 6);
-    if (kh >= t.kv_heads) return;
-    const uint32_t row = blockIdx.x * WRITE_ROWS + n;
-    const uint32_t pos = row < rows ? row_pos[row] : 0u;
-    const uint32_t mine = pos % KV8_PAGE == KV8_PAGE - 1 && pos < positions ? t.page(row_seq[row], pos / KV8_PAGE) : KV8_NONE;
-    for (uint64_t left = __ballot(mine != KV8_NONE) & 0xFFFFu; left; left &= left - 1) {
-        const uint32_t page = __builtin_amdgcn_readlane(mine, (uint32_t)__builtin_ctzll(left));
-        const uint8_t* rec = codes + kv8_record(page, t.kv_heads, kh) + 4 * g * KV8_HEAD + 8 * n;
-        u32x2 w[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) w[i] = *reinterpret_cast<const u32x2*>(rec + i * KV8_HEAD);
-        const uint32_t bytes = *reinterpret_cast<const uint32_t*>(scales + kv8_scale(page, t.kv_heads, kh) + 4 * g);
-        float lo[8], hi[8];
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            lo[j] = INFINITY;
-            hi[j] = -INFINITY;
-            uint32_t nan = 0;
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const float v = kv8_value(w[i][j / 4] >> 8 * (j % 4) & 0xFFu, bytes >> 8 * i & 0xFFu);
-                nan |= v != v;
-                lo[j] = fminf(lo[j], v);
-                hi[j] = fmaxf(hi[j], v);
-            }
-            lo[j] = -rows_max(-lo[j]) + 0.f;  // a zero of either sign is +0
-            hi[j] = rows_max(hi[j]) + 0.f;
-            nan |= __shfl_xor(nan, 16, 64);
-            nan |= __shfl_xor(nan, 32, 64);
-            if (nan) lo[j] = hi[j] = __uint_as_float(0x7FC00000u);
-        }
-        if (g < 2) {
-            float b[8];
-#pragma unroll
-            for (int j = 0; j < 8; ++j) b[j] = g ? hi[j] : lo[j];
-            *reinterpret_cast<u32x4*>(bounds + kv8_bound(page, t.kv_heads, kh) + g * KV8_HEAD + 8 * n) =
-                u32x4{pack(b[0], b[1]), pack(b[2], b[3]), pack(b[4], b[5]), pack(b[6], b[7])};
+            uint8_t* to = a.codes + kv8_record(page_n, kvh, k0 + i) + KV8_PART;
+            reinterpret_cast<u32x2*>(to)[threadIdx.x] = reinterpret_cast<const u32x2*>(sh.turned[i])[threadIdx.x];
+        } else if (page_n != KV8_NONE) {
+            uint8_t* to = a.codes + kv8_record(page_n, kvh, k0 + i) + KV8_PART + pos_n % KV8_PAGE;
+            for (uint32_t d = r; d < HD; d += 16) to[d * KV8_PAGE] = reinterpret_cast<const uint8_t*>(sh.turned[i])[d * WRITE_ROWS + n];
         }
     }
 }
@@ -999,23 +1073,31 @@ extern "C" x0ne_status x0ne_gpu_kv8_write(x0ne_gpu* g, const x0ne_kv8* c, uint64
     if (!g) return fail(X0NE_ERR_GPU, "no device");
     if (rows == 0 || c->seqs == 0 || positions == 0) return X0NE_OK;
     const OnDevice on(g->device);
-    const Table t = table_of(c);
-    g->counts.launches += bounds ? 2 : 1;
-    // 8 heads to a block read cos and sin, and take square roots, least often; where that leaves CUs idle, 2.
-    const uint32_t tiles = ((uint32_t)rows + WRITE_ROWS - 1) / WRITE_ROWS, heads = q_heads + c->kv_heads;
-    const uint32_t values = (c->kv_heads + WRITE_VALUES - 1) / WRITE_VALUES;
-    const bool many = (uint64_t)tiles * (heads / 8) >= 256;
-    const dim3 grid(tiles, (many ? (heads + 7) / 8 : (heads + 1) / 2) + values);
-    hipLaunchKernelGGL(many ? kv8_write_kernel<8> : kv8_write_kernel<2>, grid, dim3(256), 0, g->stream, t, (uint8_t*)c->codes,
-                       (uint8_t*)c->scales, (const bf16_t*)qkv, (const bf16_t*)q_norm, (const bf16_t*)k_norm,
-                       (const double*)rope_cs, (const uint32_t*)row_seq, (const uint32_t*)row_pos, (bf16_t*)q_out,
-                       (uint32_t)rows, q_heads, positions, eps);
+    Write a = {table_of(c),
+               (uint8_t*)c->codes,
+               (uint8_t*)c->scales,
+               (const bf16_t*)qkv,
+               (const bf16_t*)q_norm,
+               (const bf16_t*)k_norm,
+               (const double2*)rope_cs,
+               (const uint32_t*)row_seq,
+               (const uint32_t*)row_pos,
+               (bf16_t*)q_out,
+               (bf16_t*)bounds,
+               (uint32_t)rows,
+               q_heads,
+               positions,
+               eps};
+    // 4 heads to a block read cos and sin, and take square roots, half as often as 2, which are over sooner and, with
+    // bounds, keep the blocks of a row that ends a page short (us with 2 / 4: 64 rows of 64 sequences, 40 blocks of 4, 9.5 /
+    // 15.4; 777 rows of 72 heads, 882 blocks, 13.0 / 13.8; 2048 rows of 40 heads, 1280 blocks, 15.0 / 13.8; 8 heads 16.3).
+    const uint32_t tiles = (a.rows + WRITE_ROWS - 1) / WRITE_ROWS;
+    const bool many = (uint64_t)tiles * ((q_heads + c->kv_heads) / WRITE_HEADS) >= 1024;
+    const uint32_t each = many ? WRITE_HEADS : 2;
+    const dim3 grid(tiles, (q_heads + each - 1) / each + (c->kv_heads + each - 1) / each + (c->kv_heads + WRITE_VALUES - 1) / WRITE_VALUES);
+    g->counts.launches++;
+    hipLaunchKernelGGL(many ? kv8_write_kernel<WRITE_HEADS> : kv8_write_kernel<2>, grid, dim3(256), 0, g->stream, a);
     X0NE_HIP(hipGetLastError(), what);
-    if (!bounds) return X0NE_OK;
-    hipLaunchKernelGGL(kv8_bounds_kernel, dim3(tiles, (c->kv_heads + 3) / 4), dim3(256), 0, g->stream, t,
-                       (const uint8_t*)c->codes, (const uint8_t*)c->scales, (const uint32_t*)row_seq,
-                       (const uint32_t*)row_pos, (uint32_t)rows, positions, (bf16_t*)bounds);
-    X0NE_HIP(hipGetLastError(), "kv8 bounds");
     return X0NE_OK;
 }
 
