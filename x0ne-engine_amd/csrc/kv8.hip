@@ -42,9 +42,21 @@ __device__ __forceinline__ uint32_t row_move(uint32_t v) {
     return (uint32_t)__builtin_amdgcn_mov_dpp((int)v, CTRL, 0xF, 0xF, true);
 }
 template <int CTRL>
+__device__ __forceinline__ uint64_t row_move_u(uint64_t v) {
+    return (uint64_t)row_move<CTRL>((uint32_t)(v >> 32)) << 32 | row_move<CTRL>((uint32_t)v);
+}
+template <int CTRL>
 __device__ __forceinline__ double row_move_d(double v) {
-    const uint64_t u = (uint64_t)__double_as_longlong(v);
-    return __longlong_as_double((long long)((uint64_t)row_move<CTRL>((uint32_t)(u >> 32)) << 32 | row_move<CTRL>((uint32_t)u)));
+    return __longlong_as_double((long long)row_move_u<CTRL>((uint64_t)__double_as_longlong(v)));
+}
+// The sums of lanes 0 .. i, by DPP: within the rows of 16, then lane 15 of rows 0 and 2, then lane 31.
+__device__ __forceinline__ uint32_t wave_up_to(uint32_t x) {
+    x += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x111, 0xF, 0xF, false);
+    x += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x112, 0xF, 0xF, false);
+    x += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x114, 0xF, 0xF, false);
+    x += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x118, 0xF, 0xF, false);
+    x += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x142, 0xA, 0xF, false);
+    return x + (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x143, 0xC, 0xF, false);
 }
 typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
 __device__ __forceinline__ uint32_t max_u16(uint32_t a, uint32_t b) {
@@ -526,15 +538,7 @@ __global__ void __launch_bounds__(64 * ATTEND_WAVES, 2) kv8_attention_kernel(con
     };
     uint32_t my_keys = s0 + lane < a.t.seqs ? kv8_keys(a.lens[s0 + lane], a.t.seq_pages) : 0u, my_seq = lane;
     uint32_t mine = s0 + lane < a.t.seqs ? shape(my_keys).active : 0u;
-    auto up_to = [&](uint32_t x) -> uint32_t {
-#pragma unroll
-        for (int d = 1; d < 64; d <<= 1) {
-            const uint32_t below = __shfl_up(x, d, 64);
-            if (lane >= (uint32_t)d) x += below;
-        }
-        return x;
-    };
-    uint32_t upto = up_to(mine);
+    uint32_t upto = wave_up_to(mine);
     const uint32_t total = __builtin_amdgcn_readlane(upto, 63), blocks = gridDim.y;
     if (total > blocks) {  // several slices per block: the longest sequences' first
         uint32_t rank = 0;
@@ -544,7 +548,7 @@ __global__ void __launch_bounds__(64 * ATTEND_WAVES, 2) kv8_attention_kernel(con
         }
         my_seq = (uint32_t)__builtin_amdgcn_ds_permute((int)(4 * rank), (int)lane);
         my_keys = (uint32_t)__builtin_amdgcn_ds_permute((int)(4 * rank), (int)my_keys);
-        upto = up_to((uint32_t)__builtin_amdgcn_ds_permute((int)(4 * rank), (int)mine));
+        upto = wave_up_to((uint32_t)__builtin_amdgcn_ds_permute((int)(4 * rank), (int)mine));
     }
     // A block's slice of round r, the rounds to and fro over the blocks.
     auto item = [&](uint32_t r) -> Item {
@@ -806,19 +810,10 @@ struct SelectShared {
         double q[MAX_GROUP][KV8_HEAD];
         uint32_t bin[SELECT_BINS];
     };
-    uint64_t low[4], high[4];
+    uint64_t low[16], high[16];  // of each row of lanes
     uint32_t part[4], count[SELECT_KEYS * 4], equal[SELECT_KEYS * 4];
     uint32_t found, above, inside, last;
 };
-
-__device__ __forceinline__ uint32_t wave_up_to(uint32_t x) {
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-        const uint32_t below = __shfl_up(x, d, 64);
-        if ((threadIdx.x & 63) >= (uint32_t)d) x += below;
-    }
-    return x;
-}
 
 // The `take` largest of n keys (0 < take < n; ties to the lower index), their indices ascending in `to`. Radix
 // selection over the range of the keys that are still undecided, 11 bits at a time: the range is that of the keys and
@@ -850,17 +845,21 @@ __device__ void select_keys(const uint64_t* __restrict__ keys, uint32_t n, uint3
         lo = min(lo, x);
         hi = max(hi, x);
     });
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-        lo = min(lo, (uint64_t)__shfl_xor((unsigned long long)lo, d, 64));
-        hi = max(hi, (uint64_t)__shfl_xor((unsigned long long)hi, d, 64));
-    }
-    if (lane == 0) {
-        sh.low[wave] = lo;
-        sh.high[wave] = hi;
+    lo = min(lo, row_move_u<0xB1>(lo));
+    hi = max(hi, row_move_u<0xB1>(hi));
+    lo = min(lo, row_move_u<0x4E>(lo));
+    hi = max(hi, row_move_u<0x4E>(hi));
+    lo = min(lo, row_move_u<0x141>(lo));
+    hi = max(hi, row_move_u<0x141>(hi));
+    lo = min(lo, row_move_u<0x128>(lo));
+    hi = max(hi, row_move_u<0x128>(hi));
+    if ((lane & 15) == 0) {
+        sh.low[t >> 4] = lo;
+        sh.high[t >> 4] = hi;
     }
     __syncthreads();
-    for (int w = 0; w < 4; ++w) {
+#pragma unroll
+    for (int w = 0; w < 16; ++w) {
         lo = min(lo, sh.low[w]);
         hi = max(hi, sh.high[w]);
     }
@@ -948,21 +947,16 @@ __global__ void __launch_bounds__(256)
     __shared__ SelectShared sh;
     const uint32_t kh = blockIdx.x, s = blockIdx.z, i = threadIdx.x, group = q_heads / t.kv_heads;
     const uint32_t lane = i & 63, wave = i >> 6, n = lane & 15, g = lane >> 4;
-    const uint32_t pages = (kv8_keys(lens[s], t.seq_pages) + KV8_PAGE - 1) / KV8_PAGE;
     const size_t pair = (size_t)s * t.kv_heads + kh;
     uint32_t* to = list + pair * budget;
-    if (pages <= budget || budget == 1) {
-        if (blockIdx.y == 0)
-            for (uint32_t j = i; j < budget; j += 256) to[j] = j >= pages ? KV8_NONE : budget == 1 ? pages - 1 : j;
-        return;
-    }
-    const uint32_t scored = pages - 1, first = blockIdx.y * SELECT_PAGES;
-    if (first >= scored) return;
+    // What is needed of memory is requested at once: the length, the queries, the table's entries, whatever the length.
+    const uint32_t first = blockIdx.y * SELECT_PAGES;
+    const uint32_t pages = (kv8_keys(lens[s], t.seq_pages) + KV8_PAGE - 1) / KV8_PAGE;
     uint32_t entry[4];
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
         const uint32_t p = first + 16 * wave + 4 * j + g;
-        entry[j] = p < scored ? t.pages[(size_t)s * t.seq_pages + p] : KV8_NONE;
+        entry[j] = t.pages[(size_t)s * t.seq_pages + min(p, t.seq_pages - 1)];
     }
     for (uint32_t e = i; e < group * KV8_HEAD; e += 256)
         sh.q[0][e] = (double)bf2f(q[((size_t)s * q_heads + kh * group) * KV8_HEAD + e]);
@@ -973,34 +967,43 @@ __global__ void __launch_bounds__(256)
         lo[j] = b[0];
         hi[j] = b[KV8_HEAD / 8];
     }
+    if (pages <= budget || budget == 1) {
+        if (blockIdx.y == 0)
+            for (uint32_t j = i; j < budget; j += 256) to[j] = j >= pages ? KV8_NONE : budget == 1 ? pages - 1 : j;
+        return;
+    }
+    const uint32_t scored = pages - 1;
+    if (first >= scored) return;
     __syncthreads();
-    uint64_t best[4] = {0, 0, 0, 0};
+    // Four pages' sums over 16 lanes, transposed: at the first two steps a lane keeps two, then one of its sums and adds
+    // its partner's of those, so lane n ends with page j = 2 (n / 8) + (n / 4) % 2's, each added in the same tree.
+    const bool up8 = n & 8, up4 = n & 4;
+    uint64_t best = 0;
     for (uint32_t h = 0; h < group; ++h) {
-        double x[8];
+        double x[8], sum[4];
 #pragma unroll
         for (int d = 0; d < 8; ++d) x[d] = sh.q[h][8 * n + d];
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-            double sum = 0.0;
+            sum[j] = 0.0;
 #pragma unroll
             for (int d = 0; d < 8; ++d) {
                 const uint32_t w = x[d] < 0.0 ? lo[j][d / 2] : hi[j][d / 2];
-                sum = fma(x[d], (double)(d & 1 ? bf_hi(w) : bf_lo(w)), sum);
+                sum[j] = fma(x[d], (double)(d & 1 ? bf_hi(w) : bf_lo(w)), sum[j]);
             }
-            sum += dpp_d<0x124>(sum);
-            sum += dpp_d<0x128>(sum);
-            sum += dpp_d<0x4E>(sum);
-            sum += dpp_d<0xB1>(sum);
-            best[j] = max(best[j], score_key(sum));
         }
+#pragma unroll
+        for (int j = 0; j < 2; ++j) sum[j] = (up8 ? sum[j + 2] : sum[j]) + row_move_d<0x128>(up8 ? sum[j] : sum[j + 2]);
+        double one = (up4 ? sum[1] : sum[0]) + row_move_d<0x141>(up4 ? sum[0] : sum[1]);
+        one += row_move_d<0x4E>(one);
+        one += row_move_d<0xB1>(one);
+        best = max(best, score_key(one));
     }
     uint64_t* key = keys_of + pair * t.seq_pages;
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-        const uint32_t p = first + 16 * wave + 4 * j + g;
-        if (n == 0 && p < scored)
-            __hip_atomic_store(key + p, entry[j] < t.pool ? best[j] : 0ull, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    }
+    const uint32_t mine = up8 ? up4 ? entry[3] : entry[2] : up4 ? entry[1] : entry[0];
+    const uint32_t p = first + 16 * wave + 4 * (n >> 2) + g;
+    if ((n & 3) == 0 && p < scored)
+        __hip_atomic_store(key + p, mine < t.pool ? best : 0ull, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     // The keys acknowledged, then the count: the block that completes it selects.
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     __syncthreads();
