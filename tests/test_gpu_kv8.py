@@ -271,6 +271,66 @@ def test_attention_of_ragged_batches(kernels, seqs, longest):
     assert (kernels.kv8_attention(c, q, 8, lens, calls=2) == out).all()
 
 
+def widened(c, seq_pages):
+    """The same cache under a table of seq_pages entries, those past the sequences' naming no page."""
+    table = np.full((c.table.shape[0], seq_pages), NONE, np.uint32)
+    table[:, :c.table.shape[1]] = c.table
+    return type(c)(c.codes, c.scales, table)
+
+
+@pytest.mark.parametrize("q_heads,kv_heads,lens", [(8, 8, [2000]), (24, 8, [0, 700, 33, 1, 512, 4000]), (5, 1, [9000]),
+                                                   (16, 1, [16, 3333, 0]), (14, 2, [1000] * 9 + [17]), (32, 4, [6001, 5, 90])])
+def test_attention_under_tables_far_wider_than_the_sequences(kernels, q_heads, kv_heads, lens):
+    """Tables that hold millions of positions: blocks of 8 wavefronts and the cuts that go with them, at every group
+    that joins in another number of parts; lists of pages under the same tables."""
+    rng = np.random.default_rng(q_heads)
+    c = R.fill(rng, kv_heads, lens, max(lens) // PAGE + 1)
+    q = random_q(rng, len(lens), q_heads)
+    for width in (c.table.shape[1], 20000, 200000):
+        wide = widened(c, width)
+        out = kernels.kv8_attention(wide, q, q_heads, lens, calls=2)
+        check_attention(c, q, q_heads, lens, out)
+    pages = np.full((len(lens), kv_heads, 4096), NONE, np.uint32)
+    for s, n in enumerate(lens):
+        for h in range(kv_heads):
+            pick = np.sort(rng.permutation(-(-n // PAGE))[:200])
+            pages[s, h, :len(pick)] = pick
+    out = kernels.kv8_attention(widened(c, 20000), q, q_heads, lens, page_list=pages)
+    check_attention(c, q, q_heads, lens, out, page_list=pages)
+
+
+@pytest.mark.parametrize("seqs,kv_heads", [(70, 8), (130, 2), (65, 1), (300, 1)])
+def test_attention_of_more_than_64_sequences(kernels, seqs, kv_heads):
+    """Batches in several parts of 64, sequences of all lengths, empty ones among them, each block with several."""
+    rng = np.random.default_rng(seqs)
+    lens = [int(x) for x in rng.integers(0, 200, seqs)]
+    lens[::7] = [0] * len(lens[::7])
+    lens[-1], lens[63], lens[64] = 333, 1, 600
+    c = R.fill(rng, kv_heads, lens, 40)
+    q = random_q(rng, seqs, 3 * kv_heads)
+    out = kernels.kv8_attention(c, q, 3 * kv_heads, lens, calls=2)
+    check_attention(c, q, 3 * kv_heads, lens, out)
+
+
+def test_a_sequence_has_its_bits_in_any_batch(kernels):
+    """The same sequence beside others of any lengths, at another place of the batch: the same bits."""
+    rng = np.random.default_rng(21)
+    lens = [3000, 17, 2000, 900, 0, 4000, 64, 3000]
+    c = R.fill(rng, 2, lens, 260)
+    q = random_q(rng, 8, 8)
+    first = kernels.kv8_attention(c, q, 8, lens)
+    order = rng.permutation(8)
+    moved = type(c)(c.codes, c.scales, c.table[order])
+    again = kernels.kv8_attention(moved, q[order], 8, [lens[i] for i in order])
+    assert (again == first[order]).all()
+    alone = list(lens)
+    for i in range(8):
+        if i not in (0, 3):
+            alone[i] = 0
+    other = kernels.kv8_attention(c, q, 8, alone)
+    assert (other[[0, 3]] == first[[0, 3]]).all()
+
+
 def test_attention_of_sharp_and_flat_scores(kernels):
     """Scores far apart (one key takes all), a scale of 0 (the mean of the values), and a negative scale."""
     rng = np.random.default_rng(13)

@@ -58,6 +58,18 @@ __device__ __forceinline__ uint32_t wave_up_to(uint32_t x) {
     x += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x142, 0xA, 0xF, false);
     return x + (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x143, 0xC, 0xF, false);
 }
+__device__ __forceinline__ float row_max(float v) {
+    v = fmaxf(v, __uint_as_float(row_move<0xB1>(__float_as_uint(v))));
+    v = fmaxf(v, __uint_as_float(row_move<0x4E>(__float_as_uint(v))));
+    v = fmaxf(v, __uint_as_float(row_move<0x141>(__float_as_uint(v))));
+    return fmaxf(v, __uint_as_float(row_move<0x128>(__float_as_uint(v))));
+}
+__device__ __forceinline__ float row_sum(float v) {
+    v += __uint_as_float(row_move<0xB1>(__float_as_uint(v)));
+    v += __uint_as_float(row_move<0x4E>(__float_as_uint(v)));
+    v += __uint_as_float(row_move<0x141>(__float_as_uint(v)));
+    return v + __uint_as_float(row_move<0x128>(__float_as_uint(v)));
+}
 typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
 __device__ __forceinline__ uint32_t max_u16(uint32_t a, uint32_t b) {
     return __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(u16x2, a), __builtin_bit_cast(u16x2, b)));
@@ -404,7 +416,7 @@ __device__ __forceinline__ float factor(float m, float top) {
     return __builtin_amdgcn_exp2f(m - (top == -INFINITY ? 0.f : top));
 }
 
-constexpr uint32_t ATTEND_WAVES = 4, TILE_PAGES = 4;
+constexpr uint32_t TILE_PAGES = 4;
 constexpr uint32_t MAX_SLICES = 64;
 constexpr uint32_t STATE = KV8_HEAD + 4;  // floats of a partial state: m, l, two unused, o
 constexpr uint32_t MAX_GROUP = 16;
@@ -421,9 +433,10 @@ struct Attend {
     float scale2;  // the scale times log2 e: a weight is one exp2
 };
 
+template <uint32_t WAVES>
 struct Shared {
-    float wm[ATTEND_WAVES][MAX_GROUP], wl[ATTEND_WAVES][MAX_GROUP];
-    float wo[ATTEND_WAVES][MAX_GROUP][KV8_HEAD + 4];
+    float wm[WAVES][MAX_GROUP], wl[WAVES][MAX_GROUP];
+    float wo[WAVES][MAX_GROUP][KV8_HEAD + 4];
     float m[MAX_GROUP][MAX_SLICES], l[MAX_GROUP][MAX_SLICES];  // the join's: each slice's maximum (then factor) and sum
     uint32_t last;
 };
@@ -432,11 +445,13 @@ struct Shared {
 // and, for a group of at most 4 heads, every second, fourth .. slice (the parts meet in LDS). All of a thread's
 // loads of up to JOIN_AHEAD slices are requested before the maxima are known, so they cost one round trip.
 constexpr uint32_t JOIN_AHEAD = 8;
+template <uint32_t WAVES>
 __device__ __forceinline__ void join(const Attend& a, const float* __restrict__ st, bf16_t* __restrict__ out,
-                                     uint32_t active, Shared& sh) {
+                                     uint32_t active, Shared<WAVES>& sh) {
+    constexpr uint32_t THREADS = 64 * WAVES;
     const uint32_t t = threadIdx.x, quads = a.group * (KV8_HEAD / 4);
-    const uint32_t parts = quads <= 64 ? 4 : quads <= 128 ? 2 : 1;
-    const uint32_t part = t / (256 / parts), first = t % (256 / parts);
+    const uint32_t parts = quads <= THREADS / 4 ? 4 : quads <= THREADS / 2 ? 2 : 1;
+    const uint32_t part = t / (THREADS / parts), first = t % (THREADS / parts);
     auto request = [&](uint32_t e, uint32_t z0, f32x4 (&x)[JOIN_AHEAD]) {
         const float* p = st + (size_t)(e / (KV8_HEAD / 4)) * a.slices * STATE + 4 + 4 * (e % (KV8_HEAD / 4));
 #pragma unroll
@@ -450,7 +465,7 @@ __device__ __forceinline__ void join(const Attend& a, const float* __restrict__ 
     };
     f32x4 ahead[JOIN_AHEAD];
     request(first, part, ahead);
-    for (uint32_t i = t; i < a.group * active; i += 256) {
+    for (uint32_t i = t; i < a.group * active; i += THREADS) {
         const uint32_t h = i / active, z = i % active;
         const float2 ml = get2(st + ((size_t)h * a.slices + z) * STATE);
         sh.m[h][z] = ml.x;
@@ -458,11 +473,11 @@ __device__ __forceinline__ void join(const Attend& a, const float* __restrict__ 
     }
     lds_barrier();
     // Each head's factors and sum by one wavefront, a lane per slice.
-    for (uint32_t h = t / 64; h < a.group; h += 4) {
+    for (uint32_t h = t / 64; h < a.group; h += WAVES) {
         const uint32_t z = t % 64;
-        const float m = z < active ? sh.m[h][z] : -INFINITY, f = factor(m, wave_max(m));
+        const float m = z < active ? sh.m[h][z] : -INFINITY, f = factor(m, rows_max(row_max(m)));
         if (z < active) sh.m[h][z] = f;
-        const float l = wave_sum(z < active ? f * sh.l[h][z] : 0.f);
+        const float l = rows_sum(row_sum(z < active ? f * sh.l[h][z] : 0.f));
         if (z == 0) sh.wl[0][h] = l;
     }
     lds_barrier();
@@ -483,7 +498,7 @@ __device__ __forceinline__ void join(const Attend& a, const float* __restrict__ 
         *reinterpret_cast<uint2*>(out + 4 * e) = make_uint2(pack(x[0] * r, x[1] * r), pack(x[2] * r, x[3] * r));
     };
     if (parts == 1) {
-        for (uint32_t e = first; e < quads; e += 256) store(e, sum(e));  // twice for more than 8 heads
+        for (uint32_t e = first; e < quads; e += THREADS) store(e, sum(e));  // twice for more than 8 heads
         return;
     }
     float* mine = &sh.wo[0][0][0] + 4 * t;
@@ -492,20 +507,20 @@ __device__ __forceinline__ void join(const Attend& a, const float* __restrict__ 
     *reinterpret_cast<f32x4*>(mine) = x;
     lds_barrier();
     if (part || first >= quads) return;
-    for (uint32_t w = 1; w < parts; ++w) x += *reinterpret_cast<const f32x4*>(mine + 4 * w * (256 / parts));
+    for (uint32_t w = 1; w < parts; ++w) x += *reinterpret_cast<const f32x4*>(mine + 4 * w * (THREADS / parts));
     store(first, x);
 }
 
-// The slices of sequences: a sequence's tiles are cut into `active` slices of `per` tiles, by its own length and
-// the call's `slices` and `rounds` only. A block walks every gridDim.y-th slice of its kv head and its 64 sequences:
-// lane l of each wavefront holds sequence l's length and the slices up to and with it.
+// A slice of a sequence: its tiles are cut into `active` slices of `per` tiles, by its own length and the call's `slices`
+// and `rounds` only. A block walks slices of its kv head and its 64 sequences: lane l of each wavefront holds a sequence's
+// length and the slices up to and with it.
 struct Item {
-    uint32_t s, y, keys, pages, np, per, active, t0, t_end;  // sequence and slice; this wavefront's tiles t0, t0 + 4 ..
+    uint32_t s, y, keys, pages, np, per, active, t0, t_end;  // sequence and slice; this wavefront's tiles t0, t0 + WAVES ..
     __device__ __forceinline__ bool any() const { return t0 < t_end; }
 };
 
-// Decode attention. A block of 4 wavefronts takes slices of the sequences' tiles for the q heads of one kv head, one
-// after the other, wavefront w a slice's tiles w, w + 4, ...; a tile is 4 pages. The products are S^T = K Q^T and
+// Decode attention. A block takes slices of the sequences' tiles for the q heads of one kv head, one after the other,
+// its wavefront w of WAVES a slice's tiles w, w + WAVES, ...; a tile is 4 pages. The products are S^T = K Q^T and
 // O^T = V^T P^T on the matrix cores (16 x 16 x 32, bf16 with f32 sums), the group's heads the 16 columns: lane
 // (n = lane % 16, g = lane / 16) holds column n, so the softmax of a head is lane-local but for the four lanes n,
 // n + 16, n + 32, n + 48. Codes become bf16 in one conversion, keys times their scale (exact); a value's scale goes
@@ -520,18 +535,20 @@ struct Item {
 // f32. A slice's state (m, l, o) is joined by the last block of its (sequence, kv head) to count itself, slices in
 // order; a sequence of one slice is written at once. Keys past the length, entries behind a list and pages that are
 // not there weigh 0, their values are taken as 0.
-__global__ void __launch_bounds__(64 * ATTEND_WAVES, 2) kv8_attention_kernel(const Attend a) {
-    __shared__ Shared sh;
-    const uint32_t kh = blockIdx.x, s0 = blockIdx.z * 64, step = ATTEND_WAVES;
+template <uint32_t WAVES>
+__global__ void __launch_bounds__(64 * WAVES, 2) kv8_attention_kernel(const Attend a) {
+    constexpr uint32_t THREADS = 64 * WAVES;
+    __shared__ Shared<WAVES> sh;
+    const uint32_t kh = blockIdx.x, s0 = blockIdx.z * 64, step = WAVES;
     const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), n = lane & 15, g = lane >> 4;
     auto shape = [&](uint32_t keys) -> Item {
         Item it = {};
         it.keys = keys;
         it.pages = (keys + KV8_PAGE - 1) / KV8_PAGE;
         it.np = a.list ? min(a.budget, it.pages) : it.pages;
-        const uint32_t tiles = (it.np + TILE_PAGES - 1) / TILE_PAGES, rounds = (tiles + ATTEND_WAVES - 1) / ATTEND_WAVES;
+        const uint32_t tiles = (it.np + TILE_PAGES - 1) / TILE_PAGES, rounds = (tiles + WAVES - 1) / WAVES;
         it.active = max(1u, min(a.slices, (rounds + a.rounds - 1) / a.rounds));
-        it.per = ATTEND_WAVES * max(1u, (rounds + it.active - 1) / it.active);
+        it.per = WAVES * max(1u, (rounds + it.active - 1) / it.active);
         it.active = max(1u, (tiles + it.per - 1) / it.per);
         it.t_end = tiles;
         return it;
@@ -727,7 +744,7 @@ __global__ void __launch_bounds__(64 * ATTEND_WAVES, 2) kv8_attention_kernel(con
         }
         lsum = rows_sum(lsum);
 
-        // The block's four states meet; then the output, or the slice's state. The states of the slice before are
+        // The block's states meet; then the output, or the slice's state. The states of the slice before are
         // counted here: this wavefront's stores of them are older than the loads of at least one tile.
         if (n < a.group) {
             if (g == 0) {
@@ -749,14 +766,14 @@ __global__ void __launch_bounds__(64 * ATTEND_WAVES, 2) kv8_attention_kernel(con
             before = __hip_atomic_fetch_add(counter_of(waiting), 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
         bf16_t* out = a.out + ((size_t)it.s * a.q_heads + kh * a.group) * KV8_HEAD;
         float* state = a.state + ((size_t)it.s * a.q_heads + kh * a.group) * a.slices * STATE;
-        for (uint32_t e = threadIdx.x; e < a.group * (KV8_HEAD / 4); e += 64 * ATTEND_WAVES) {
+        for (uint32_t e = threadIdx.x; e < a.group * (KV8_HEAD / 4); e += THREADS) {
             const uint32_t h = e / (KV8_HEAD / 4), d = 4 * (e % (KV8_HEAD / 4));
             float top = sh.wm[0][h], l = 0.f;
             f32x4 x = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-            for (uint32_t w = 1; w < ATTEND_WAVES; ++w) top = fmaxf(top, sh.wm[w][h]);
+            for (uint32_t w = 1; w < WAVES; ++w) top = fmaxf(top, sh.wm[w][h]);
 #pragma unroll
-            for (uint32_t w = 0; w < ATTEND_WAVES; ++w) {
+            for (uint32_t w = 0; w < WAVES; ++w) {
                 const float f = factor(sh.wm[w][h], top);
                 l += f * sh.wl[w][h];
                 x += f * *reinterpret_cast<const f32x4*>(&sh.wo[w][h][d]);
@@ -1122,25 +1139,28 @@ extern "C" x0ne_status x0ne_gpu_kv8_read(x0ne_gpu* g, const x0ne_kv8* c, uint64_
     return X0NE_OK;
 }
 
-// How sequences are cut: at most `slices` slices of at least `rounds` rounds of 4 tiles (a tile per wavefront), over
-// `blocks` blocks for each kv head and 64 sequences.
-//  - Few pairs of sequence and kv head (us, 32768 keys, 8 pairs): slices for one block on each of 256 CUs; two on each
-//    bring more states to join than overlap gains (16 / 32 / 64 slices 27.2 / 21.7 / 26.8).
-//  - Many: two blocks per CU walk the slices, longest first. A slice of one round costs about four rounds (its
-//    lookups, states and count are not hidden), so slices are two thirds of what a block has to do if every sequence
-//    fills its table, one or two per block (64 sequences of up to 6000 keys, 1 / 4 / 8 / 16 / 24 rounds: 134 / 101 / 92 /
-//    84 / 95; 16 of up to 8192, 1 / 3 / 5 / 8: 48 / 42 / 35 / 41), up to 16, and fewer for fewer pairs, whose lengths
-//    may be far below their tables'.
+// How sequences are cut: at most `slices` slices of at least `rounds` rounds (a tile for each of a block's `waves`
+// wavefronts), over `blocks` blocks for each kv head and 64 sequences.
+//  - Few pairs of sequence and kv head: slices for one block on each of 256 CUs; more bring more states to join than
+//    overlap gains (us, 32768 keys, 8 pairs, blocks of 4, 16 / 32 / 64 slices: 27.2 / 21.7 / 26.8).
+//  - Many: blocks that fill the card walk the slices, longest first. A slice of one round costs about four (its lookups,
+//    states and count are not hidden), so slices are two thirds of what a block has to do if every sequence fills its
+//    table (64 sequences of up to 6000 keys, blocks of 8, 2 / 4 / 8 / 12 rounds: 108 / 95 / 87 / 77; 16 of up to 8192,
+//    2 / 4 / 6 / 8: 48 / 45 / 36 / 40), up to 16, and fewer for fewer pairs, whose lengths may be far below their tables'.
+//  - Blocks of 8 wavefronts, one on a CU, join fewer states than two of 4 and start fewer slices (us with 4 / 8: 32768
+//    keys 21.1 / 19.2, 64 sequences 83 / 77, 16 sequences 35 / 36); where the pages, all attended, are less than two
+//    rounds of 8 for each CU, 4 (128 pages for each of 8 pairs 9 / 11).
 struct Cut {
-    uint32_t slices, rounds, blocks;
+    uint32_t waves, slices, rounds, blocks;
 };
 static Cut cut_of(const x0ne_kv8* c, uint32_t budget = 0) {
     const uint64_t pairs = std::max<uint64_t>(1, (uint64_t)c->seqs * c->kv_heads), parts = (c->seqs + 63) / 64;
-    Cut cut;
-    cut.slices = (uint32_t)std::min<uint64_t>(MAX_SLICES, std::max<uint64_t>(16, 256 / pairs));
-    cut.blocks = (uint32_t)std::max<uint64_t>(1, 512 / std::max<uint64_t>(1, parts * c->kv_heads));
     const uint32_t most = budget ? std::min(budget, c->seq_pages) : c->seq_pages;  // pages a sequence attends
-    const uint64_t fullest = (uint64_t)((most + 15) / 16) * std::min(c->seqs, 64u);
+    Cut cut;
+    cut.waves = pairs * ((most + 31) / 32) >= 512 ? 8 : 4;
+    cut.slices = (uint32_t)std::min<uint64_t>(MAX_SLICES, std::max<uint64_t>(16, 256 / pairs));
+    cut.blocks = (uint32_t)std::max<uint64_t>(1, 2048 / cut.waves / std::max<uint64_t>(1, parts * c->kv_heads));
+    const uint64_t fullest = (uint64_t)((most + 4 * cut.waves - 1) / (4 * cut.waves)) * std::min(c->seqs, 64u);
     cut.rounds = (uint32_t)std::max<uint64_t>(1, std::min(std::min<uint64_t>(16, pairs / 24), 2 * fullest / (3 * cut.blocks)));
     cut.blocks = std::max(1u, std::min(cut.blocks, cut.slices * std::min(c->seqs, 64u)));
     return cut;
@@ -1188,8 +1208,8 @@ extern "C" x0ne_status x0ne_gpu_kv8_attention(x0ne_gpu* g, const x0ne_kv8* c, ui
     a.slices = cut.slices;
     a.rounds = cut.rounds;
     a.scale2 = scale * 1.44269504088896340736f;
-    hipLaunchKernelGGL(kv8_attention_kernel, dim3(c->kv_heads, cut.blocks, (c->seqs + 63) / 64), dim3(64 * ATTEND_WAVES), 0,
-                       g->stream, a);
+    hipLaunchKernelGGL(cut.waves == 8 ? kv8_attention_kernel<8> : kv8_attention_kernel<4>,
+                       dim3(c->kv_heads, cut.blocks, (c->seqs + 63) / 64), dim3(64 * cut.waves), 0, g->stream, a);
     X0NE_HIP(hipGetLastError(), what);
     return X0NE_OK;
 }
