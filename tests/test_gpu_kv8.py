@@ -473,6 +473,34 @@ def test_selection_among_ties_missing_pages_and_nan(kernels):
     assert (got == R.select(c, b, vals(q), lens, 20)).all()
 
 
+@pytest.mark.parametrize("pages,seqs", [(4098, 1), (9001, 2), (257, 3), (258, 3), (65, 2), (66, 2)])
+def test_selection_of_any_number_of_pages(kernels, pages, seqs):
+    """Pages that one block scores and one more, more than a block's threads hold at once, under tables as wide as they
+    and far wider; scores of few values (ties over all of them), of all signs, of both zeros."""
+    rng = np.random.default_rng(pages)
+    lens = [pages * PAGE - 7] + [(pages - 30 * (s + 1)) * PAGE for s in range(seqs - 1)]
+    c = R.empty(pages + 5, 1, seqs, pages // seqs, rng)
+    c.table = rng.integers(0, c.pool, (seqs, pages)).astype(np.uint32)
+    few = bits(rng.integers(-2, 3, (c.pool, 1, 2, HEAD)) * (rng.random((c.pool, 1, 2, HEAD)) < 0.02)).reshape(-1, 1, 2, HEAD)
+    many = bits(rng.standard_normal((c.pool, 1, 2, HEAD))).reshape(-1, 1, 2, HEAD)
+    for b in (few, many):
+        q = random_q(rng, seqs, 2) if b is many else bits(np.sign(rng.standard_normal((seqs, 2, HEAD)))).reshape(seqs, 2, HEAD)
+        for budget in (2, 33, pages - 40):
+            want = R.select(c, b, vals(q), lens, budget)
+            for width in (pages, 40000):
+                assert (kernels.kv8_select(widened(c, width), b, q, 2, lens, budget, calls=2) == want).all(), (budget, width)
+
+
+@pytest.mark.parametrize("q_heads,kv_heads", [(16, 1), (8, 8), (15, 3)])
+def test_selected_pages_under_wide_tables(kernels, q_heads, kv_heads):
+    rng = np.random.default_rng(q_heads)
+    lens = [0, 1, 300, 1030, 1040, 4112, 6000]
+    c = R.fill(rng, kv_heads, lens, 376, drift=2.0)
+    b, q = R.all_bounds(c), random_q(rng, len(lens), q_heads)
+    for budget in (2, 40):
+        assert (kernels.kv8_select(widened(c, 30000), b, q, q_heads, lens, budget) == R.select(c, b, vals(q), lens, budget)).all()
+
+
 # -- together --
 
 def test_a_conversation_through_the_cache(kernels):

@@ -8,6 +8,9 @@
 #include "kv8.h"
 
 using namespace x0ne;
+#ifndef V_WIDE
+#define V_WIDE 0
+#endif
 
 namespace {
 
@@ -818,8 +821,8 @@ __device__ __forceinline__ uint64_t score_key(double x) {
     return b >> 63 ? ~b : b | 0x8000000000000000ull;
 }
 
-constexpr uint32_t SELECT_PAGES = 64;     // pages that a block scores, 16 per wavefront
-constexpr uint32_t SELECT_KEYS = 16;      // keys that a thread holds while a block selects: 4096 pages at once
+constexpr uint32_t SELECT_THREADS = 256, SELECT_WAVES = SELECT_THREADS / 64;
+constexpr uint32_t SELECT_KEYS = 64 / SELECT_WAVES;  // keys that a thread holds while a block selects: 4096 pages at once
 constexpr uint32_t SELECT_BINS = 2048;
 
 struct SelectShared {
@@ -827,38 +830,44 @@ struct SelectShared {
         double q[MAX_GROUP][KV8_HEAD];
         uint32_t bin[SELECT_BINS];
     };
-    uint64_t low[16], high[16];  // of each row of lanes
-    uint32_t part[4], count[SELECT_KEYS * 4], equal[SELECT_KEYS * 4];
+    uint64_t key[SELECT_THREADS / 4];  // of a pair whose pages one block scores
+    uint64_t low[SELECT_WAVES], high[SELECT_WAVES];
+    uint32_t part[SELECT_WAVES], count[SELECT_KEYS * SELECT_WAVES], equal[SELECT_KEYS * SELECT_WAVES];
     uint32_t found, above, inside, last;
 };
 
-// The `take` largest of n keys (0 < take < n; ties to the lower index), their indices ascending in `to`. Radix
-// selection over the range of the keys that are still undecided, 11 bits at a time: the range is that of the keys and
-// not of all numbers, so scores of one sign and size are told apart in a pass or two. A thread holds keys t, t + 256,
-// ...; more than 4096 are read again in each pass.
-__device__ void select_keys(const uint64_t* __restrict__ keys, uint32_t n, uint32_t take, uint32_t* __restrict__ to,
-                            SelectShared& sh) {
-    constexpr uint32_t AT_ONCE = SELECT_KEYS * 256;
+// The `take` largest of the n keys that get(index) gives (0 < take < n; ties to the lower index), their indices ascending
+// in `to`. Radix selection over the range of the keys that are still undecided, 11 bits at a time: the range is that of
+// the keys and not of all numbers, so scores of one sign and size are told apart in a pass or two. A thread holds keys
+// t, t + 256, ...; more than 4096 are read again in each pass.
+template <class Get>
+__device__ __forceinline__ void select_keys(Get&& get, uint32_t n, uint32_t take, uint32_t* __restrict__ to, SelectShared& sh) {
+    constexpr uint32_t AT_ONCE = SELECT_KEYS * SELECT_THREADS, EACH = SELECT_BINS / SELECT_THREADS;
     const uint32_t t = threadIdx.x, lane = t & 63, wave = t >> 6;
     uint64_t key[SELECT_KEYS];
-    auto load = [&](uint32_t first) {
+    auto rows = [&](uint32_t first, auto&& f) {  // f(row, whether this thread has a key of it), of rows that hold one
 #pragma unroll
         for (uint32_t j = 0; j < SELECT_KEYS; ++j) {
-            const uint32_t at = first + 256 * j + t;
-            if (at < n) key[j] = __hip_atomic_load(keys + at, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            if (first + SELECT_THREADS * j >= n) break;
+            f(j, first + SELECT_THREADS * j + t < n);
         }
     };
-    auto each = [&](auto&& f) {  // f(index, key) of every key
+    auto load = [&](uint32_t first) {
+        rows(first, [&](uint32_t j, bool in) {
+            if (in) key[j] = get(first + SELECT_THREADS * j + t);
+        });
+    };
+    auto each = [&](auto&& f) {  // f(key) of every key
         for (uint32_t first = 0; first < n; first += AT_ONCE) {
             if (n > AT_ONCE) load(first);
-#pragma unroll
-            for (uint32_t j = 0; j < SELECT_KEYS; ++j)
-                if (first + 256 * j + t < n) f(first + 256 * j + t, key[j]);
+            rows(first, [&](uint32_t j, bool in) {
+                if (in) f(key[j]);
+            });
         }
     };
     if (n <= AT_ONCE) load(0);
     uint64_t lo = ~0ull, hi = 0;
-    each([&](uint32_t, uint64_t x) {
+    each([&](uint64_t x) {
         lo = min(lo, x);
         hi = max(hi, x);
     });
@@ -870,13 +879,19 @@ __device__ void select_keys(const uint64_t* __restrict__ keys, uint32_t n, uint3
     hi = max(hi, row_move_u<0x141>(hi));
     lo = min(lo, row_move_u<0x128>(lo));
     hi = max(hi, row_move_u<0x128>(hi));
-    if ((lane & 15) == 0) {
-        sh.low[t >> 4] = lo;
-        sh.high[t >> 4] = hi;
+#pragma unroll
+    for (int d = 16; d < 64; d <<= 1) {
+        lo = min(lo, (uint64_t)__shfl_xor((unsigned long long)lo, d, 64));
+        hi = max(hi, (uint64_t)__shfl_xor((unsigned long long)hi, d, 64));
     }
+    if (lane == 0) {
+        sh.low[wave] = lo;
+        sh.high[wave] = hi;
+    }
+    for (uint32_t j = t; j < SELECT_BINS; j += SELECT_THREADS) sh.bin[j] = 0;
     __syncthreads();
 #pragma unroll
-    for (int w = 0; w < 16; ++w) {
+    for (uint32_t w = 0; w < SELECT_WAVES; ++w) {
         lo = min(lo, sh.low[w]);
         hi = max(hi, sh.high[w]);
     }
@@ -884,23 +899,26 @@ __device__ void select_keys(const uint64_t* __restrict__ keys, uint32_t n, uint3
     bool ties = true;      // all keys from lo to hi are equal: the first `need` of them
     for (int pass = 0; pass < KV8_PASSES && lo != hi; ++pass) {
         const int shift = kv8_shift(lo, hi);
-        for (uint32_t j = t; j < SELECT_BINS; j += 256) sh.bin[j] = 0;
-        __syncthreads();
-        each([&](uint32_t, uint64_t x) {
+        if (pass) {
+            for (uint32_t j = t; j < SELECT_BINS; j += SELECT_THREADS) sh.bin[j] = 0;
+            __syncthreads();
+        }
+        each([&](uint64_t x) {
             if (x >= lo && x <= hi) atomicAdd(&sh.bin[(uint32_t)((x - lo) >> shift)], 1u);
         });
         __syncthreads();
-        // Bins from the top, 8 to a thread: the one in which the count reaches `need`.
+        // Bins from the top, EACH to a thread: the one in which the count reaches `need`.
         uint32_t mine = 0;
 #pragma unroll
-        for (uint32_t j = 0; j < 8; ++j) mine += sh.bin[SELECT_BINS - 1 - 8 * t - j];
+        for (uint32_t j = 0; j < EACH; ++j) mine += sh.bin[SELECT_BINS - 1 - EACH * t - j];
         const uint32_t upto = wave_up_to(mine);
         if (lane == 63) sh.part[wave] = upto;
         __syncthreads();
         uint32_t above = upto - mine;
-        for (uint32_t w = 0; w < wave; ++w) above += sh.part[w];
+#pragma unroll
+        for (uint32_t w = 0; w < SELECT_WAVES; ++w) above += w < wave ? sh.part[w] : 0u;
         if (above < need && above + mine >= need) {
-            uint32_t b = SELECT_BINS - 1 - 8 * t;
+            uint32_t b = SELECT_BINS - 1 - EACH * t;
             while (above + sh.bin[b] < need) above += sh.bin[b--];
             sh.found = b;
             sh.above = above;
@@ -920,88 +938,90 @@ __device__ void select_keys(const uint64_t* __restrict__ keys, uint32_t n, uint3
     for (uint32_t first = 0; first < n; first += AT_ONCE) {
         if (n > AT_ONCE) load(first);
         uint32_t equal_before[SELECT_KEYS];
+        const uint64_t below = (1ull << lane) - 1;
+        if (t < SELECT_KEYS * SELECT_WAVES) sh.count[t] = sh.equal[t] = 0;
         __syncthreads();
         if (ties) {
-#pragma unroll
-            for (uint32_t j = 0; j < SELECT_KEYS; ++j) {
-                const uint64_t m = __ballot(first + 256 * j + t < n && key[j] == lo);
-                equal_before[j] = (uint32_t)__popcll(m & ((1ull << lane) - 1));
-                if (lane == 0) sh.equal[4 * j + wave] = (uint32_t)__popcll(m);
-            }
+            rows(first, [&](uint32_t j, bool in) {
+                const uint64_t m = __ballot(in && key[j] == lo);
+                equal_before[j] = (uint32_t)__popcll(m & below);
+                if (lane == 0) sh.equal[SELECT_WAVES * j + wave] = (uint32_t)__popcll(m);
+            });
             __syncthreads();
-            const uint32_t upto = wave_up_to(sh.equal[lane]);
-#pragma unroll
-            for (uint32_t j = 0; j < SELECT_KEYS; ++j)
-                equal_before[j] += equals + __shfl(upto, 4 * j + wave, 64) - sh.equal[4 * j + wave];
-            equals += __shfl(upto, 63, 64);
+            const uint32_t own = sh.equal[lane], upto = wave_up_to(own);
+            rows(first, [&](uint32_t j, bool) { equal_before[j] += equals + __builtin_amdgcn_readlane(upto - own, SELECT_WAVES * j + wave); });
+            equals += __builtin_amdgcn_readlane(upto, 63);
         }
-        uint64_t taken[SELECT_KEYS];
-#pragma unroll
-        for (uint32_t j = 0; j < SELECT_KEYS; ++j) {
-            const bool in = first + 256 * j + t < n;
-            taken[j] = __ballot(in && (ties ? key[j] > lo || (key[j] == lo && equal_before[j] < need) : key[j] >= lo));
-            if (lane == 0) sh.count[4 * j + wave] = (uint32_t)__popcll(taken[j]);
-        }
+        auto taken = [&](uint32_t j, bool in) {
+            return __ballot(in && (ties ? key[j] > lo || (key[j] == lo && equal_before[j] < need) : key[j] >= lo));
+        };
+        rows(first, [&](uint32_t j, bool in) {
+            const uint64_t m = taken(j, in);
+            if (lane == 0) sh.count[SELECT_WAVES * j + wave] = (uint32_t)__popcll(m);
+        });
         __syncthreads();
-        const uint32_t upto = wave_up_to(sh.count[lane]);
-#pragma unroll
-        for (uint32_t j = 0; j < SELECT_KEYS; ++j) {
-            const uint32_t at = placed + __shfl(upto, 4 * j + wave, 64) - sh.count[4 * j + wave];
-            if (taken[j] >> lane & 1) to[at + (uint32_t)__popcll(taken[j] & ((1ull << lane) - 1))] = first + 256 * j + t;
-        }
-        placed += __shfl(upto, 63, 64);
+        const uint32_t own = sh.count[lane], upto = wave_up_to(own);
+        rows(first, [&](uint32_t j, bool in) {
+            const uint64_t m = taken(j, in);
+            const uint32_t at = placed + __builtin_amdgcn_readlane(upto - own, SELECT_WAVES * j + wave);
+            if (m >> lane & 1) to[at + (uint32_t)__popcll(m & below)] = first + SELECT_THREADS * j + t;
+        });
+        placed += __builtin_amdgcn_readlane(upto, 63);
+        __syncthreads();  // the counts are read
     }
 }
 
-// The pages of (sequence, kv head). A block scores 64 pages, a wavefront 16 of them: 16 lanes have 8 dims each of a
-// page's bounds (two 16-byte loads), four pages are in flight; products and sums in f64, so that equal pages score
-// equal and near ones in their order (a score's bytes, 512 per page, take longer than its 128 multiply-adds per head).
-// The last block of its (sequence, kv head) to count itself selects. The last page stands outside: it is always kept.
-__global__ void __launch_bounds__(256)
+// The pages of (sequence, kv head). 16 lanes have 8 dims each of a page's bounds (two 16-byte loads), PAGES pages in
+// flight, so a block scores 64 PAGES of them; products and sums in f64, so that equal pages score equal and near ones in
+// their order. The last block of its (sequence, kv head) to count itself selects; a block that has them all need not
+// count. The last page stands outside: it is always kept.
+template <uint32_t PAGES>
+__global__ void __launch_bounds__(SELECT_THREADS)
     kv8_select_kernel(Table t, const bf16_t* __restrict__ bounds, const bf16_t* __restrict__ q,
                       const uint32_t* __restrict__ lens, uint32_t budget, uint32_t* __restrict__ list,
                       uint64_t* __restrict__ keys_of, uint32_t* __restrict__ counter_of, uint32_t q_heads) {
+    constexpr uint32_t BLOCK = 4 * SELECT_WAVES * PAGES;
     __shared__ SelectShared sh;
     const uint32_t kh = blockIdx.x, s = blockIdx.z, i = threadIdx.x, group = q_heads / t.kv_heads;
-    const uint32_t lane = i & 63, wave = i >> 6, n = lane & 15, g = lane >> 4;
+    const uint32_t lane = i & 63, wave = __builtin_amdgcn_readfirstlane(i >> 6), n = lane & 15, g = lane >> 4;
     const size_t pair = (size_t)s * t.kv_heads + kh;
     uint32_t* to = list + pair * budget;
     // What is needed of memory is requested at once: the length, the queries, the table's entries, whatever the length.
-    const uint32_t first = blockIdx.y * SELECT_PAGES;
+    const uint32_t first = blockIdx.y * BLOCK;
     const uint32_t pages = (kv8_keys(lens[s], t.seq_pages) + KV8_PAGE - 1) / KV8_PAGE;
-    uint32_t entry[4];
+    uint32_t entry[PAGES];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-        const uint32_t p = first + 16 * wave + 4 * j + g;
+    for (uint32_t j = 0; j < PAGES; ++j) {
+        const uint32_t p = first + 4 * PAGES * wave + 4 * j + g;
         entry[j] = t.pages[(size_t)s * t.seq_pages + min(p, t.seq_pages - 1)];
     }
-    for (uint32_t e = i; e < group * KV8_HEAD; e += 256)
+    for (uint32_t e = i; e < group * KV8_HEAD; e += SELECT_THREADS)
         sh.q[0][e] = (double)bf2f(q[((size_t)s * q_heads + kh * group) * KV8_HEAD + e]);
-    u32x4 lo[4], hi[4];
+    u32x4 lo[PAGES], hi[PAGES];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
+    for (uint32_t j = 0; j < PAGES; ++j) {
         const u32x4* b = reinterpret_cast<const u32x4*>(bounds + kv8_bound(entry[j] < t.pool ? entry[j] : 0u, t.kv_heads, kh)) + n;
         lo[j] = b[0];
         hi[j] = b[KV8_HEAD / 8];
     }
     if (pages <= budget || budget == 1) {
         if (blockIdx.y == 0)
-            for (uint32_t j = i; j < budget; j += 256) to[j] = j >= pages ? KV8_NONE : budget == 1 ? pages - 1 : j;
+            for (uint32_t j = i; j < budget; j += SELECT_THREADS) to[j] = j >= pages ? KV8_NONE : budget == 1 ? pages - 1 : j;
         return;
     }
     const uint32_t scored = pages - 1;
     if (first >= scored) return;
     __syncthreads();
     // Four pages' sums over 16 lanes, transposed: at the first two steps a lane keeps two, then one of its sums and adds
-    // its partner's of those, so lane n ends with page j = 2 (n / 8) + (n / 4) % 2's, each added in the same tree.
+    // its partner's of those, so lane n ends with page n / 4's. Each sum is added in the same tree.
     const bool up8 = n & 8, up4 = n & 4;
     uint64_t best = 0;
     for (uint32_t h = 0; h < group; ++h) {
-        double x[8], sum[4];
+        double x[8], sum[PAGES];
 #pragma unroll
         for (int d = 0; d < 8; ++d) x[d] = sh.q[h][8 * n + d];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
+        for (uint32_t j = 0; j < PAGES; ++j) {
             sum[j] = 0.0;
 #pragma unroll
             for (int d = 0; d < 8; ++d) {
@@ -1009,33 +1029,47 @@ __global__ void __launch_bounds__(256)
                 sum[j] = fma(x[d], (double)(d & 1 ? bf_hi(w) : bf_lo(w)), sum[j]);
             }
         }
+        double one = sum[0];
+        if constexpr (PAGES == 4) {
 #pragma unroll
-        for (int j = 0; j < 2; ++j) sum[j] = (up8 ? sum[j + 2] : sum[j]) + row_move_d<0x128>(up8 ? sum[j] : sum[j + 2]);
-        double one = (up4 ? sum[1] : sum[0]) + row_move_d<0x141>(up4 ? sum[0] : sum[1]);
+            for (int j = 0; j < 2; ++j) sum[j] = (up8 ? sum[j + 2] : sum[j]) + row_move_d<0x128>(up8 ? sum[j] : sum[j + 2]);
+            one = (up4 ? sum[1] : sum[0]) + row_move_d<0x141>(up4 ? sum[0] : sum[1]);
+        } else {
+            one += row_move_d<0x128>(one);
+            one += row_move_d<0x141>(one);
+        }
         one += row_move_d<0x4E>(one);
         one += row_move_d<0xB1>(one);
         best = max(best, score_key(one));
     }
     uint64_t* key = keys_of + pair * t.seq_pages;
-    const uint32_t mine = up8 ? up4 ? entry[3] : entry[2] : up4 ? entry[1] : entry[0];
-    const uint32_t p = first + 16 * wave + 4 * (n >> 2) + g;
-    if ((n & 3) == 0 && p < scored)
-        __hip_atomic_store(key + p, mine < t.pool ? best : 0ull, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    // The keys acknowledged, then the count: the block that completes it selects.
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    __syncthreads();
-    uint32_t* counter = counter_of + pair;
-    if (i == 0) {
-        const uint32_t before = __hip_atomic_fetch_add(counter, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-        sh.last = before == (scored - 1) / SELECT_PAGES;
+    uint32_t mine = entry[0];
+    if constexpr (PAGES == 4) mine = up8 ? up4 ? entry[3] : entry[2] : up4 ? entry[1] : entry[0];
+    if (mine >= t.pool) best = 0;
+    const uint32_t at = 4 * PAGES * wave + (PAGES == 4 ? 4 * (n >> 2) : 0u) + g;
+    const bool puts = (n & (PAGES == 4 ? 3 : 15)) == 0 && first + at < scored;
+    if (scored > BLOCK) {
+        if (puts) __hip_atomic_store(key + first + at, best, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        // The keys acknowledged, then the count: the block that completes it selects.
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        __syncthreads();
+        uint32_t* counter = counter_of + pair;
+        if (i == 0) {
+            const uint32_t before = __hip_atomic_fetch_add(counter, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            sh.last = before == (scored - 1) / BLOCK;
+        }
+        __syncthreads();
+        if (!sh.last) return;
+        if (i == 0) __hip_atomic_store(counter, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);  // for the next call
+    } else {
+        if (puts) sh.key[at] = best;
+        __syncthreads();
     }
-    __syncthreads();
-    if (!sh.last) return;
-    if (i == 0) {
-        __hip_atomic_store(counter, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);  // for the next call
-        to[budget - 1] = pages - 1;
-    }
-    select_keys(key, scored, budget - 1, to, sh);
+    if (i == 0) to[budget - 1] = pages - 1;
+    auto key_of = [&](uint32_t x) {
+        return scored > BLOCK ? __hip_atomic_load(key + x, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) : sh.key[x];
+    };
+    select_keys(key_of, scored, budget - 1, to, sh);
 }
 
 // ---- host ----
@@ -1229,11 +1263,13 @@ extern "C" x0ne_status x0ne_gpu_kv8_select(x0ne_gpu* g, const x0ne_kv8* c, uint6
     if (c->seqs == 0) return X0NE_OK;
     const OnDevice on(g->device);
     g->counts.launches++;
-    const uint32_t chunks = (c->seq_pages + SELECT_PAGES - 1) / SELECT_PAGES;
-    if (chunks > 65535) return bad(what, std::to_string(c->seq_pages) + " pages of a sequence (up to 65535 x 64)");
-    hipLaunchKernelGGL(kv8_select_kernel, dim3(c->kv_heads, chunks, c->seqs), dim3(256), 0, g->stream, table_of(c),
-                       (const bf16_t*)bounds, (const bf16_t*)q, (const uint32_t*)lens, budget, (uint32_t*)page_list,
-                       (uint64_t*)(work + counter_bytes(c)), (uint32_t*)work, q_heads);
+    const bool wide = (uint64_t)c->seqs * c->kv_heads * ((c->seq_pages + 63) / 64) > V_WIDE;
+    const uint32_t each = wide ? 16 * SELECT_WAVES : 4 * SELECT_WAVES, blocks = (c->seq_pages + each - 1) / each;
+    if (blocks > 65535) return bad(what, std::to_string(c->seq_pages) + " pages of a sequence (up to 65535 x 64)");
+    hipLaunchKernelGGL(wide ? kv8_select_kernel<4> : kv8_select_kernel<1>, dim3(c->kv_heads, blocks, c->seqs),
+                       dim3(SELECT_THREADS), 0, g->stream, table_of(c), (const bf16_t*)bounds, (const bf16_t*)q,
+                       (const uint32_t*)lens, budget, (uint32_t*)page_list, (uint64_t*)(work + counter_bytes(c)),
+                       (uint32_t*)work, q_heads);
     X0NE_HIP(hipGetLastError(), what);
     return X0NE_OK;
 }
