@@ -171,6 +171,16 @@ def test_read_back(kernels, kv_heads, lens):
     check_read(kernels, c, lens, out_table, k, v)
 
 
+def test_read_under_a_table_far_wider_than_the_sequences(kernels):
+    rng = np.random.default_rng(12)
+    lens = [0, 1000, 17]
+    c = R.fill(rng, 2, lens, 64)
+    out_table = np.full((3, 9000), NONE, np.uint32)
+    out_table[:, :64] = rng.permutation(200)[:192].reshape(3, 64)
+    k, v = kernels.kv8_read(widened(c, 9000), lens, out_table, 200)
+    check_read(kernels, c, lens, out_table, k, v)
+
+
 def check_read(kernels, c, lens, out_table, k, v):
     want_k, want_v = np.full(k.shape, kernels.SENTINEL, np.uint16), np.full(v.shape, kernels.SENTINEL, np.uint16)
     for s, n in enumerate(lens):
@@ -286,7 +296,7 @@ def test_attention_under_tables_far_wider_than_the_sequences(kernels, q_heads, k
     rng = np.random.default_rng(q_heads)
     c = R.fill(rng, kv_heads, lens, max(lens) // PAGE + 1)
     q = random_q(rng, len(lens), q_heads)
-    for width in (c.table.shape[1], 20000, 200000):
+    for width in (c.table.shape[1], 3000, 20000, 200000):
         wide = widened(c, width)
         out = kernels.kv8_attention(wide, q, q_heads, lens, calls=2)
         check_attention(c, q, q_heads, lens, out)

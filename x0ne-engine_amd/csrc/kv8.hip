@@ -341,6 +341,21 @@ __global__ void __launch_bounds__(256) kv8_write_kernel(const Write a) {
     }
 }
 
+// A load or store of what is too much for the Infinity Cache to hold until it is read again (STREAM: not kept there).
+template <bool STREAM, class T>
+__device__ __forceinline__ T take(const T* p) {
+    if constexpr (STREAM) return __builtin_nontemporal_load(p);
+    return *p;
+}
+template <bool STREAM, class T>
+__device__ __forceinline__ void put(T* p, T x) {
+    if constexpr (STREAM)
+        __builtin_nontemporal_store(x, p);
+    else
+        *p = x;
+}
+constexpr uint64_t STREAM_BYTES = 256ull << 20;  // the Infinity Cache
+
 // Eight codes as bf16, times the power of two `scale`: exact.
 __device__ __forceinline__ u32x4 decode(uint32_t lo, uint32_t hi, float scale) {
     u32x4 r;
@@ -354,6 +369,7 @@ __device__ __forceinline__ u32x4 decode(uint32_t lo, uint32_t hi, float scale) {
 // Positions below a sequence's length as bf16: the codes' order is the bf16 pages' order, so a wavefront streams one
 // page of one head, 8 codes per lane and load and 16 bytes per lane and store. Slots past the length are zero; a page
 // that is not there reads as zeros, an output page outside its pool is not written.
+template <bool STREAM>
 __global__ void __launch_bounds__(256)
     kv8_read_kernel(Table t, const uint8_t* __restrict__ codes, const uint8_t* __restrict__ scales,
                     const uint32_t* __restrict__ lens, bf16_t* __restrict__ k_out, bf16_t* __restrict__ v_out,
@@ -370,9 +386,9 @@ __global__ void __launch_bounds__(256)
         const uint8_t* sc = scales + kv8_scale(from, t.kv_heads, kh);
         u32x2 k[4], v[4];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) k[j] = rec[64 * j];
+        for (int j = 0; j < 4; ++j) k[j] = take<STREAM>(rec + 64 * j);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) v[j] = rec[KV8_PART / 8 + 64 * j];
+        for (int j = 0; j < 4; ++j) v[j] = take<STREAM>(rec + KV8_PART / 8 + 64 * j);
         // Keys 4 j + i / 16; the values of positions 8 (i % 2) .. + 7.
         const u32x4 ks = *reinterpret_cast<const u32x4*>(sc);
         const u32x2 vs = *reinterpret_cast<const u32x2*>(sc + KV8_PAGE + 8 * (i & 1));
@@ -385,7 +401,7 @@ __global__ void __launch_bounds__(256)
         for (int j = 0; j < 4; ++j) {
             u32x4 x = decode(k[j][0], k[j][1], __uint_as_float((ks[j] >> 8 * (i >> 4) & 0xFFu) << 23));
             if (4 * j + (i >> 4) >= valid) x = u32x4{0, 0, 0, 0};
-            kd[64 * j] = x;
+            put<STREAM>(kd + 64 * j, x);
         }
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
@@ -397,7 +413,7 @@ __global__ void __launch_bounds__(256)
                 f[e] = 8 * (i & 1) + e < valid ? two[0] * power[e] : 0.f;
                 f[e + 1] = 8 * (i & 1) + e + 1 < valid ? two[1] * power[e + 1] : 0.f;
             }
-            vd[64 * j] = u32x4{pack(f[0], f[1]), pack(f[2], f[3]), pack(f[4], f[5]), pack(f[6], f[7])};
+            put<STREAM>(vd + 64 * j, u32x4{pack(f[0], f[1]), pack(f[2], f[3]), pack(f[4], f[5]), pack(f[6], f[7])});
         }
     }
 }
@@ -538,7 +554,7 @@ struct Item {
 // f32. A slice's state (m, l, o) is joined by the last block of its (sequence, kv head) to count itself, slices in
 // order; a sequence of one slice is written at once. Keys past the length, entries behind a list and pages that are
 // not there weigh 0, their values are taken as 0.
-template <uint32_t WAVES>
+template <uint32_t WAVES, bool STREAM>
 __global__ void __launch_bounds__(64 * WAVES, 2) kv8_attention_kernel(const Attend a) {
     constexpr uint32_t THREADS = 64 * WAVES;
     __shared__ Shared<WAVES> sh;
@@ -611,10 +627,10 @@ __global__ void __launch_bounds__(64 * WAVES, 2) kv8_attention_kernel(const Atte
     // The lanes of row n of a key product take page n / 4, the page of the lanes 16 (n / 4) ...
     auto key_page = [&](uint32_t page) -> uint32_t { return __shfl(page, 16 * (n >> 2), 64); };
     auto load_k = [&](const uint8_t* p, int m) {
-        k[m][0] = *reinterpret_cast<const u32x4*>(p + m * 4 * KV8_HEAD);
-        k[m][1] = *reinterpret_cast<const u32x4*>(p + m * 4 * KV8_HEAD + 16);
+        k[m][0] = take<STREAM>(reinterpret_cast<const u32x4*>(p + m * 4 * KV8_HEAD));
+        k[m][1] = take<STREAM>(reinterpret_cast<const u32x4*>(p + m * 4 * KV8_HEAD + 16));
     };
-    auto load_v = [&](const uint8_t* p, int c) { v[c] = *reinterpret_cast<const u32x4*>(p + c * 16 * KV8_PAGE); };
+    auto load_v = [&](const uint8_t* p, int c) { v[c] = take<STREAM>(reinterpret_cast<const u32x4*>(p + c * 16 * KV8_PAGE)); };
     // Columns past the group repeat its last head: their results are not used.
     auto load_q = [&](const Item& it) {
         const bf16_t* p = a.q + ((size_t)it.s * a.q_heads + kh * a.group + min(n, a.group - 1)) * KV8_HEAD + 32 * g;
@@ -1166,7 +1182,9 @@ extern "C" x0ne_status x0ne_gpu_kv8_read(x0ne_gpu* g, const x0ne_kv8* c, uint64_
     const OnDevice on(g->device);
     g->counts.launches++;
     const uint64_t blocks = std::min<uint64_t>(65536, ((uint64_t)c->seq_pages * c->kv_heads + 3) / 4);
-    hipLaunchKernelGGL(kv8_read_kernel, dim3((uint32_t)blocks, c->seqs), dim3(256), 0, g->stream,
+    // Bypassing the Infinity Cache with more than it holds: 16 sequences of up to 8192 positions 88.5 -> 85.3 us.
+    const bool stream = (uint64_t)c->seqs * c->seq_pages * c->kv_heads * (3 * KV8_RECORD) > STREAM_BYTES;
+    hipLaunchKernelGGL(stream ? kv8_read_kernel<true> : kv8_read_kernel<false>, dim3((uint32_t)blocks, c->seqs), dim3(256), 0, g->stream,
                        table_of(c), (const uint8_t*)c->codes, (const uint8_t*)c->scales, (const uint32_t*)lens,
                        (bf16_t*)k, (bf16_t*)v, (const uint32_t*)out_table, out_pool);
     X0NE_HIP(hipGetLastError(), what);
@@ -1184,14 +1202,18 @@ extern "C" x0ne_status x0ne_gpu_kv8_read(x0ne_gpu* g, const x0ne_kv8* c, uint64_
 //  - Blocks of 8 wavefronts, one on a CU, join fewer states than two of 4 and start fewer slices (us with 4 / 8: 32768
 //    keys 21.1 / 19.2, 64 sequences 83 / 77, 16 sequences 35 / 36); where the pages, all attended, are less than two
 //    rounds of 8 for each CU, 4 (128 pages for each of 8 pairs 9 / 11).
+//  - Loads of more than the Infinity Cache holds bypass it (64 sequences of up to 6000 keys 76.6 -> 72.9 us); 67 MB, read
+//    again before 256 MB of others, come from it (32768 keys 19.2 us with it, 22.3 without).
 struct Cut {
     uint32_t waves, slices, rounds, blocks;
+    bool stream;
 };
 static Cut cut_of(const x0ne_kv8* c, uint32_t budget = 0) {
     const uint64_t pairs = std::max<uint64_t>(1, (uint64_t)c->seqs * c->kv_heads), parts = (c->seqs + 63) / 64;
     const uint32_t most = budget ? std::min(budget, c->seq_pages) : c->seq_pages;  // pages a sequence attends
     Cut cut;
     cut.waves = pairs * ((most + 31) / 32) >= 512 ? 8 : 4;
+    cut.stream = pairs * most * (KV8_RECORD + KV8_SCALES) > STREAM_BYTES;  // 8 wavefronts then
     cut.slices = (uint32_t)std::min<uint64_t>(MAX_SLICES, std::max<uint64_t>(16, 256 / pairs));
     cut.blocks = (uint32_t)std::max<uint64_t>(1, 2048 / cut.waves / std::max<uint64_t>(1, parts * c->kv_heads));
     const uint64_t fullest = (uint64_t)((most + 4 * cut.waves - 1) / (4 * cut.waves)) * std::min(c->seqs, 64u);
@@ -1242,8 +1264,8 @@ extern "C" x0ne_status x0ne_gpu_kv8_attention(x0ne_gpu* g, const x0ne_kv8* c, ui
     a.slices = cut.slices;
     a.rounds = cut.rounds;
     a.scale2 = scale * 1.44269504088896340736f;
-    hipLaunchKernelGGL(cut.waves == 8 ? kv8_attention_kernel<8> : kv8_attention_kernel<4>,
-                       dim3(c->kv_heads, cut.blocks, (c->seqs + 63) / 64), dim3(64 * cut.waves), 0, g->stream, a);
+    const auto kernel = cut.waves == 4 ? kv8_attention_kernel<4, false> : cut.stream ? kv8_attention_kernel<8, true> : kv8_attention_kernel<8, false>;
+    hipLaunchKernelGGL(kernel, dim3(c->kv_heads, cut.blocks, (c->seqs + 63) / 64), dim3(64 * cut.waves), 0, g->stream, a);
     X0NE_HIP(hipGetLastError(), what);
     return X0NE_OK;
 }
