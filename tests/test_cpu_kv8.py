@@ -1,12 +1,14 @@
 """The 8-bit paged K/V cache on the CPU: its host rules (kv8.h) over their whole range, the plain form the GPU tests
 compare with, and every refusal, before any device is touched."""
 import ctypes as C
+import os
+import re
 
 import numpy as np
 import pytest
 
 import kv8_reference as R
-from common import run_cpp
+from common import ROOT, run_cpp
 
 
 def test_the_host_rules(tmp_path):
@@ -80,3 +82,16 @@ def test_the_workspace_size():
     assert f(None, 8) == 0 and f(C.byref(_lib.Kv8C(**ok)), 7) == 0 and f(C.byref(_lib.Kv8C(**{**ok, "pool": 0})), 8) == 0
     big = f(C.byref(_lib.Kv8C(**{**ok, "kv_heads": 1024, "seqs": 65535, "seq_pages": (1 << 24) - 1})), 16384)
     assert 65535 * 1024 * ((1 << 24) - 1) * 8 <= big < 1 << 63
+
+
+def test_the_rust_and_python_structs_are_the_headers():
+    from x0ne_core._lib import Kv8C
+    header = re.sub(r"/\*.*?\*/", "", open(os.path.join(ROOT, "include", "x0ne_core.h")).read(), flags=re.S)
+    body = re.search(r"typedef struct \{([^}]*)\}\s*x0ne_kv8;", header).group(1)
+    fields = [(name.strip(), kind) for kind, names in re.findall(r"(uint\d+_t)\s+([^;]+);", body) for name in names.split(",")]
+    rust = open(os.path.join(ROOT, "x0ne-engine_amd", "rust", "x0ne-core-runtime-mi355x", "src", "sys.rs")).read()
+    m = re.search(r"#\[repr\(C\)\]\s*#\[derive\([^)]*\)\]\s*pub struct x0ne_kv8 \{(.*?)\}", rust, re.S)
+    assert re.findall(r"pub (\w+): (\w+)", m.group(1)) == [(n, {"uint64_t": "u64", "uint32_t": "u32"}[k]) for n, k in fields]
+    assert Kv8C._fields_ == [(n, {"uint64_t": C.c_uint64, "uint32_t": C.c_uint32}[k]) for n, k in fields]
+    for name in re.findall(r"\b(x0ne_\w*kv8_\w+)\s*\(", header):
+        assert f"pub fn {name}(" in rust, name

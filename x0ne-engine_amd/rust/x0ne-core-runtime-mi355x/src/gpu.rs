@@ -1,5 +1,5 @@
 //! The kernel-launch API of x0ne-core/runtime/src/gpu.rs over libx0ne_core.so: `Gpu::{new, launch,
-//! gemm, capture, launch_graph, split_plan, allocate, counts, mem_info, sync}`, `Arg`,
+//! gemm, kv8_*, capture, launch_graph, split_plan, allocate, counts, mem_info, sync}`, `Arg`,
 //! `check_args` and the `launch!` macro, with the reference's names, argument meanings and
 //! errors. The kernels are this library's gfx950 code; its table (x0ne_kernel_name,
 //! x0ne_kernel_params) stands for `x0ne_core_kernels::{KERNEL_NAMES, KERNEL_PARAMS}`, and every
@@ -392,6 +392,72 @@ impl Gpu {
         };
         // SAFETY: a live device handle; the three matrices are the caller's contract.
         check(unsafe { sys::x0ne_gpu_gemv(self.h.0, w, rows as u64, cols as u64, x, n as u64, y, f32_out) })
+    }
+
+    /// QK-norm, RoPE and the quantised K/V write of rows of any mix of sequences
+    /// (`x0ne_gpu_kv8_write`); `bounds` 0 keeps none. No counterpart in the reference.
+    ///
+    /// # Safety
+    ///
+    /// Every address of `c` and of the arguments is device memory of this device of the size that
+    /// `include/x0ne_core.h` states, allocated until the call is done on the stream; the rows name
+    /// distinct positions, with `bounds` those of a page ascending together.
+    #[allow(clippy::too_many_arguments)]
+    pub unsafe fn kv8_write(&self, c: &sys::x0ne_kv8, qkv: u64, rows: usize, q_heads: u32, q_norm: u64, k_norm: u64,
+                            eps: f32, rope_cs: u64, positions: u32, row_seq: u64, row_pos: u64, q_out: u64,
+                            bounds: u64) -> Result<()> {
+        // SAFETY: a live device handle and cache; the addresses are the caller's contract.
+        check(unsafe {
+            sys::x0ne_gpu_kv8_write(self.h.0, c, qkv, rows as u64, q_heads, q_norm, k_norm, eps, rope_cs, positions,
+                                    row_seq, row_pos, q_out, bounds)
+        })
+    }
+
+    /// The cache's positions below `lens` back as bf16 pages (`x0ne_gpu_kv8_read`).
+    ///
+    /// # Safety
+    ///
+    /// As [`Gpu::kv8_write`]; `k` and `v` hold `out_pool` pages.
+    pub unsafe fn kv8_read(&self, c: &sys::x0ne_kv8, lens: u64, k: u64, v: u64, out_table: u64, out_pool: u32)
+                           -> Result<()> {
+        // SAFETY: as kv8_write.
+        check(unsafe { sys::x0ne_gpu_kv8_read(self.h.0, c, lens, k, v, out_table, out_pool) })
+    }
+
+    /// Bytes of the zeroed workspace of `kv8_attention` and `kv8_select`; 0 for a cache they refuse.
+    pub fn kv8_work_bytes(c: &sys::x0ne_kv8, q_heads: u32) -> u64 {
+        // SAFETY: reads the cache's numbers only.
+        unsafe { sys::x0ne_kv8_work_bytes(c, q_heads) }
+    }
+
+    /// Decode attention of one query per sequence (`x0ne_gpu_kv8_attention`), over every page or
+    /// those of `page_list` (0 with a `budget` of 0: every page).
+    ///
+    /// # Safety
+    ///
+    /// As [`Gpu::kv8_write`]; `work` was zeroed before its first call and no other call uses it
+    /// meanwhile.
+    #[allow(clippy::too_many_arguments)]
+    pub unsafe fn kv8_attention(&self, c: &sys::x0ne_kv8, q: u64, q_heads: u32, lens: u64, page_list: u64,
+                                budget: u32, out: u64, scale: f32, work: u64, work_bytes: u64) -> Result<()> {
+        // SAFETY: as kv8_write.
+        check(unsafe {
+            sys::x0ne_gpu_kv8_attention(self.h.0, c, q, q_heads, lens, page_list, budget, out, scale, work, work_bytes)
+        })
+    }
+
+    /// The `budget` pages per sequence and kv head worth attending (`x0ne_gpu_kv8_select`).
+    ///
+    /// # Safety
+    ///
+    /// As [`Gpu::kv8_attention`].
+    #[allow(clippy::too_many_arguments)]
+    pub unsafe fn kv8_select(&self, c: &sys::x0ne_kv8, bounds: u64, q: u64, q_heads: u32, lens: u64, budget: u32,
+                             page_list: u64, work: u64, work_bytes: u64) -> Result<()> {
+        // SAFETY: as kv8_write.
+        check(unsafe {
+            sys::x0ne_gpu_kv8_select(self.h.0, c, bounds, q, q_heads, lens, budget, page_list, work, work_bytes)
+        })
     }
 
     /// Captures every launch `f` issues on the stream into one graph and instantiates it

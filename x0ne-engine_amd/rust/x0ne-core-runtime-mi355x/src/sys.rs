@@ -89,6 +89,18 @@ pub struct x0ne_split_plan {
 }
 
 #[repr(C)]
+#[derive(Clone, Copy, Default, Debug)]
+pub struct x0ne_kv8 {
+    pub codes: u64,
+    pub scales: u64,
+    pub page_table: u64,
+    pub pool: u32,
+    pub kv_heads: u32,
+    pub seqs: u32,
+    pub seq_pages: u32,
+}
+
+#[repr(C)]
 #[derive(Clone, Copy, Default)]
 pub struct x0ne_gemv_fused {
     pub w: u64,
@@ -155,6 +167,17 @@ extern "C" {
     pub fn x0ne_gpu_gemv(g: *mut x0ne_gpu, w: u64, rows: u64, cols: u64, x: u64, n: u64, y: u64, out_f32: c_int)
                          -> c_int;
     pub fn x0ne_gpu_split_plan(g: *const x0ne_gpu, q_heads: u32, kv_heads: u32, out: *mut x0ne_split_plan) -> c_int;
+    pub fn x0ne_gpu_kv8_write(g: *mut x0ne_gpu, c: *const x0ne_kv8, qkv: u64, rows: u64, q_heads: u32, q_norm: u64,
+                              k_norm: u64, eps: f32, rope_cs: u64, positions: u32, row_seq: u64, row_pos: u64,
+                              q_out: u64, bounds: u64) -> c_int;
+    pub fn x0ne_gpu_kv8_read(g: *mut x0ne_gpu, c: *const x0ne_kv8, lens: u64, k: u64, v: u64, out_table: u64,
+                             out_pool: u32) -> c_int;
+    pub fn x0ne_kv8_work_bytes(c: *const x0ne_kv8, q_heads: u32) -> u64;
+    pub fn x0ne_gpu_kv8_attention(g: *mut x0ne_gpu, c: *const x0ne_kv8, q: u64, q_heads: u32, lens: u64,
+                                  page_list: u64, budget: u32, out: u64, scale: f32, work: u64, work_bytes: u64)
+                                  -> c_int;
+    pub fn x0ne_gpu_kv8_select(g: *mut x0ne_gpu, c: *const x0ne_kv8, bounds: u64, q: u64, q_heads: u32, lens: u64,
+                               budget: u32, page_list: u64, work: u64, work_bytes: u64) -> c_int;
     pub fn x0ne_gpu_capture_begin(g: *mut x0ne_gpu) -> c_int;
     pub fn x0ne_gpu_capture_end(g: *mut x0ne_gpu, out: *mut *mut x0ne_graph) -> c_int;
     pub fn x0ne_gpu_launch_graph(g: *mut x0ne_gpu, graph: *const x0ne_graph) -> c_int;
