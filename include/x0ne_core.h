@@ -238,8 +238,9 @@ x0ne_status x0ne_gpu_kv8_write(x0ne_gpu* g, const x0ne_kv8* c, uint64_t qkv, uin
 x0ne_status x0ne_gpu_kv8_read(x0ne_gpu* g, const x0ne_kv8* c, uint64_t lens, uint64_t k, uint64_t v, uint64_t out_table,
                               uint32_t out_pool);
 /* Bytes of the workspace of x0ne_gpu_kv8_attention and _select for this cache (0 where they refuse
-   it): 256-byte aligned, zeroed once before its first call and left ready for the next one by each.
-   Calls that share it must not overlap (those of one Gpu, and its graphs, run one after the other). */
+   it): 256-byte aligned, zeroed once before its first call and left ready for the next one by each,
+   whatever that one's cache. Calls that share it must not overlap (those of one Gpu, and its graphs,
+   run one after the other). */
 uint64_t x0ne_kv8_work_bytes(const x0ne_kv8* c, uint32_t q_heads);
 /* Decode attention of one query per sequence: out [seqs][q_heads 128] bf16 = softmax(scale q k) v over
    the keys below lens[s] (u32; at most its pages'), q [seqs][q_heads 128] bf16 from the same layout,
@@ -256,7 +257,8 @@ x0ne_status x0ne_gpu_kv8_attention(x0ne_gpu* g, const x0ne_kv8* c, uint64_t q, u
    the largest score, the most that q k can be for any key within the page's bounds (the largest over
    the kv head's queries; f64), ties to the lower page, a NaN score above all, a page that is not there
    below all. page_list [seqs][kv_heads][budget] u32: ascending, 0xFFFFFFFF behind the last. Every
-   page of a sequence but its last must have its bounds (x0ne_gpu_kv8_write). */
+   page of a sequence but its last must have its bounds (x0ne_gpu_kv8_write). seq_pages at most
+   65535 x 64. */
 x0ne_status x0ne_gpu_kv8_select(x0ne_gpu* g, const x0ne_kv8* c, uint64_t bounds, uint64_t q, uint32_t q_heads,
                                 uint64_t lens, uint32_t budget, uint64_t page_list, uint64_t work, uint64_t work_bytes);
 

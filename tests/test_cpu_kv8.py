@@ -61,7 +61,7 @@ REFUSED = {
                   dict(page_list=256, budget=1 << 24), dict(work=0), dict(work=128), dict(work_bytes=255)],
     "select": [dict(bounds=0), dict(bounds=264), dict(q=0), dict(q=264), dict(lens=0), dict(lens=258), dict(page_list=0),
                dict(page_list=258), dict(budget=0), dict(budget=1 << 24), dict(q_heads=0), dict(q_heads=7), dict(q_heads=34),
-               dict(work=0), dict(work=128), dict(work_bytes=255)],
+               dict(work=0), dict(work=128), dict(work_bytes=255), dict(seq_pages=65535 * 64 + 1, work_bytes=1 << 60)],
 }
 
 
@@ -95,3 +95,13 @@ def test_the_rust_and_python_structs_are_the_headers():
     assert Kv8C._fields_ == [(n, {"uint64_t": C.c_uint64, "uint32_t": C.c_uint32}[k]) for n, k in fields]
     for name in re.findall(r"\b(x0ne_\w*kv8_\w+)\s*\(", header):
         assert f"pub fn {name}(" in rust, name
+
+
+def test_caches_of_all_shapes_have_their_counters_in_the_same_place():
+    """What a call leaves behind its counters may not lie where a call of another cache counts: the part of the
+    workspace in front of the states (of 132 floats a slice) and scores (8 bytes a page) is the same for all."""
+    from x0ne_core import _lib
+    f = _lib.lib().x0ne_kv8_work_bytes
+    for kv_heads, seqs in [(1, 1), (8, 1), (8, 16), (8, 64), (2, 700), (1024, 64)]:
+        size = [f(C.byref(_lib.Kv8C(16, 16, 16, 8, kv_heads, seqs, pages)), kv_heads) for pages in (1 << 20, 1 << 21)]
+        assert size[0] - (size[1] - size[0]) == 4 * 65536, (kv_heads, seqs, size)

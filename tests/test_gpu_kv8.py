@@ -658,3 +658,73 @@ def test_calls_without_work(kernels):
     k, _ = kernels.kv8_read(none, [], np.zeros((0, 3), np.uint32), 2)
     assert (k == kernels.SENTINEL).all()
     assert kernels.gpu.counts()["launches"] == launches + 1  # the rope table's
+
+
+def test_calls_of_all_sizes_share_a_workspace(kernels):
+    """Selection and attention of one sequence and of batches in turn over one workspace, twice: the numbers of
+    sequences and heads change what lies in it, the results do not."""
+    from x0ne_core import Arena, Kv8
+    from x0ne_core.arena import Class
+    rng = np.random.default_rng(21)
+    g, a, keep, budget = kernels.gpu, Arena(), [], 4
+    shapes = [(8, 16, [4000]), (8, 8, [1500] * 20 + [300]), (1, 2, [2100, 40]), (3, 3, [1300] * 50), (1, 16, [0])]
+    size = 0
+    for kvh, q_heads, lens in shapes:
+        c = R.fill(rng, kvh, [min(n, 1300) for n in lens[:3]], 260)
+        table = np.resize(c.table, (len(lens), 260))  # more sequences of the same pages
+        c = type(c)(c.codes, c.scales, table)
+        q = random_q(rng, len(lens), q_heads)
+        lens = [min(n, 1300) for n in lens]
+        size = max(size, g.kv8_work_bytes(Kv8(16, 16, 16, c.pool, kvh, *table.shape), q_heads))
+        arrays = {"codes": c.codes, "scales": c.scales, "table": table, "q": q, "lens": np.array(lens, np.uint32),
+                  "bounds": R.all_bounds(c)}
+        outs = {"out": q.nbytes, "sparse": q.nbytes, "list": len(lens) * kvh * budget * 4}
+        keep.append((c, q, q_heads, lens, arrays, {k: a.alloc(k, v.nbytes, Class.CLIENT_DATA) for k, v in arrays.items()},
+                     {k: a.alloc(k, n, Class.CLIENT_DATA) for k, n in outs.items()}))
+    work = a.alloc("work", size, Class.CLIENT_DATA)
+    a.freeze(g)
+    a.write(work, 0, np.zeros(size, np.uint8))
+    for turn in range(2):
+        for c, q, q_heads, lens, arrays, s, o in keep:
+            for k, v in arrays.items():
+                a.write(s[k], 0, v)
+            for k in ("out", "sparse"):
+                a.write(o[k], 0, np.full(q.size, kernels.SENTINEL, np.uint16))
+            kv = Kv8(a.ptr(s["codes"]), a.ptr(s["scales"]), a.ptr(s["table"]), c.pool, c.kv_heads, *c.table.shape)
+            g.kv8_select(kv, a.ptr(s["bounds"]), a.ptr(s["q"]), q_heads, a.ptr(s["lens"]), budget, a.ptr(o["list"]), a.ptr(work), size)
+            g.kv8_attention(kv, a.ptr(s["q"]), q_heads, a.ptr(s["lens"]), a.ptr(o["out"]), 0.088, a.ptr(work), size)
+            g.kv8_attention(kv, a.ptr(s["q"]), q_heads, a.ptr(s["lens"]), a.ptr(o["sparse"]), 0.088, a.ptr(work), size,
+                            page_list=a.ptr(o["list"]), budget=budget)
+            g.sync()
+            pages = a.read_array(o["list"], 0, len(lens) * c.kv_heads * budget, np.uint32).reshape(len(lens), c.kv_heads, budget)
+            assert (pages == R.select(c, arrays["bounds"], vals(q), lens, budget)).all(), (turn, len(lens))
+            check_attention(c, q, q_heads, lens, a.read_array(o["out"], 0, q.size, np.uint16), scale=0.088)
+            check_attention(c, q, q_heads, lens, a.read_array(o["sparse"], 0, q.size, np.uint16), page_list=pages, scale=0.088)
+
+
+def test_more_pairs_than_counters(kernels):
+    """1024 kv heads by 130 sequences are three launches (65536 pairs each at most): every sequence's pages and output
+    those of its twin, whose table, queries and length it shares, and the twins' those of the plain form."""
+    rng = np.random.default_rng(22)
+    kvh, seq_pages, budget, n = 1024, 68, 3, 130
+    lens = [1070, 25, 0, 1088]
+    c = R.empty(6, kvh, 4, 1)
+    x = vals(bits(rng.standard_normal((2, 6 * PAGE, kvh, HEAD))))
+    (kc, ks), (vc, vs) = R.quantise(x[0]), R.quantise(x[1])
+    split = lambda b: b.reshape(6, PAGE, kvh, *b.shape[2:])
+    c.codes[:, :, :2048] = split(kc).transpose(0, 2, 1, 3).reshape(6, kvh, 2048)
+    c.codes[:, :, 2048:] = split(vc).transpose(0, 2, 3, 1).reshape(6, kvh, 2048)
+    c.scales[:, :, :PAGE], c.scales[:, :, PAGE:] = split(ks).transpose(0, 2, 1), split(vs).transpose(0, 2, 1)
+    four = rng.integers(0, 6, (4, seq_pages)).astype(np.uint32)
+    q4 = random_q(rng, 4, kvh).reshape(4, kvh, HEAD)
+    of = np.arange(n) % 4
+    c = type(c)(c.codes, c.scales, four[of])
+    launches = kernels.gpu.counts()["launches"]
+    pages = kernels.kv8_select(c, R.all_bounds(c), q4[of], kvh, np.array(lens)[of], budget)
+    out = kernels.kv8_attention(c, q4[of], kvh, np.array(lens)[of])
+    assert kernels.gpu.counts()["launches"] == launches + 6
+    assert (pages == pages[:4][of]).all() and (out == out[:4][of]).all()
+    some = [0, 1, 510, 1023]
+    few = type(c)(c.codes[:, some], c.scales[:, some], four)
+    assert (pages[:4, some] == R.select(few, R.all_bounds(few), vals(q4[:, some]), lens, budget)).all()
+    check_attention(few, q4[:, some], 4, lens, out[:4, some])

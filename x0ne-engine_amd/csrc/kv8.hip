@@ -8,9 +8,6 @@
 #include "kv8.h"
 
 using namespace x0ne;
-#ifndef V_WIDE
-#define V_WIDE 0
-#endif
 
 namespace {
 
@@ -840,13 +837,14 @@ __device__ __forceinline__ uint64_t score_key(double x) {
 constexpr uint32_t SELECT_THREADS = 256, SELECT_WAVES = SELECT_THREADS / 64;
 constexpr uint32_t SELECT_KEYS = 64 / SELECT_WAVES;  // keys that a thread holds while a block selects: 4096 pages at once
 constexpr uint32_t SELECT_BINS = 2048;
+constexpr uint32_t SELECT_PAGES = 4 * 4 * SELECT_WAVES;  // pages that a block scores: 16 lanes have 4
 
 struct SelectShared {
     union {
         double q[MAX_GROUP][KV8_HEAD];
         uint32_t bin[SELECT_BINS];
     };
-    uint64_t key[SELECT_THREADS / 4];  // of a pair whose pages one block scores
+    uint64_t key[SELECT_PAGES];  // of a pair whose pages one block scores
     uint64_t low[SELECT_WAVES], high[SELECT_WAVES];
     uint32_t part[SELECT_WAVES], count[SELECT_KEYS * SELECT_WAVES], equal[SELECT_KEYS * SELECT_WAVES];
     uint32_t found, above, inside, last;
@@ -987,35 +985,34 @@ __device__ __forceinline__ void select_keys(Get&& get, uint32_t n, uint32_t take
     }
 }
 
-// The pages of (sequence, kv head). 16 lanes have 8 dims each of a page's bounds (two 16-byte loads), PAGES pages in
-// flight, so a block scores 64 PAGES of them; products and sums in f64, so that equal pages score equal and near ones in
-// their order. The last block of its (sequence, kv head) to count itself selects; a block that has them all need not
-// count. The last page stands outside: it is always kept.
-template <uint32_t PAGES>
+// The pages of (sequence, kv head). 16 lanes have 8 dims each of a page's bounds (two 16-byte loads) of 4 pages, all in
+// flight at once (us, 2048 pages of 8 pairs: 24.2, with 1 page 33.6: more blocks to count), so a block scores 64 pages;
+// products and sums in f64, so that equal pages score equal and near ones in their order. The last block of its (sequence,
+// kv head) to count itself selects; a block that has them all need not count. The last page stands outside: it is always
+// kept.
 __global__ void __launch_bounds__(SELECT_THREADS)
     kv8_select_kernel(Table t, const bf16_t* __restrict__ bounds, const bf16_t* __restrict__ q,
                       const uint32_t* __restrict__ lens, uint32_t budget, uint32_t* __restrict__ list,
                       uint64_t* __restrict__ keys_of, uint32_t* __restrict__ counter_of, uint32_t q_heads) {
-    constexpr uint32_t BLOCK = 4 * SELECT_WAVES * PAGES;
     __shared__ SelectShared sh;
     const uint32_t kh = blockIdx.x, s = blockIdx.z, i = threadIdx.x, group = q_heads / t.kv_heads;
     const uint32_t lane = i & 63, wave = __builtin_amdgcn_readfirstlane(i >> 6), n = lane & 15, g = lane >> 4;
     const size_t pair = (size_t)s * t.kv_heads + kh;
     uint32_t* to = list + pair * budget;
     // What is needed of memory is requested at once: the length, the queries, the table's entries, whatever the length.
-    const uint32_t first = blockIdx.y * BLOCK;
+    const uint32_t first = blockIdx.y * SELECT_PAGES;
     const uint32_t pages = (kv8_keys(lens[s], t.seq_pages) + KV8_PAGE - 1) / KV8_PAGE;
-    uint32_t entry[PAGES];
+    uint32_t entry[4];
 #pragma unroll
-    for (uint32_t j = 0; j < PAGES; ++j) {
-        const uint32_t p = first + 4 * PAGES * wave + 4 * j + g;
+    for (uint32_t j = 0; j < 4; ++j) {
+        const uint32_t p = first + 16 * wave + 4 * j + g;
         entry[j] = t.pages[(size_t)s * t.seq_pages + min(p, t.seq_pages - 1)];
     }
     for (uint32_t e = i; e < group * KV8_HEAD; e += SELECT_THREADS)
         sh.q[0][e] = (double)bf2f(q[((size_t)s * q_heads + kh * group) * KV8_HEAD + e]);
-    u32x4 lo[PAGES], hi[PAGES];
+    u32x4 lo[4], hi[4];
 #pragma unroll
-    for (uint32_t j = 0; j < PAGES; ++j) {
+    for (uint32_t j = 0; j < 4; ++j) {
         const u32x4* b = reinterpret_cast<const u32x4*>(bounds + kv8_bound(entry[j] < t.pool ? entry[j] : 0u, t.kv_heads, kh)) + n;
         lo[j] = b[0];
         hi[j] = b[KV8_HEAD / 8];
@@ -1033,11 +1030,11 @@ __global__ void __launch_bounds__(SELECT_THREADS)
     const bool up8 = n & 8, up4 = n & 4;
     uint64_t best = 0;
     for (uint32_t h = 0; h < group; ++h) {
-        double x[8], sum[PAGES];
+        double x[8], sum[4];
 #pragma unroll
         for (int d = 0; d < 8; ++d) x[d] = sh.q[h][8 * n + d];
 #pragma unroll
-        for (uint32_t j = 0; j < PAGES; ++j) {
+        for (uint32_t j = 0; j < 4; ++j) {
             sum[j] = 0.0;
 #pragma unroll
             for (int d = 0; d < 8; ++d) {
@@ -1045,26 +1042,19 @@ __global__ void __launch_bounds__(SELECT_THREADS)
                 sum[j] = fma(x[d], (double)(d & 1 ? bf_hi(w) : bf_lo(w)), sum[j]);
             }
         }
-        double one = sum[0];
-        if constexpr (PAGES == 4) {
 #pragma unroll
-            for (int j = 0; j < 2; ++j) sum[j] = (up8 ? sum[j + 2] : sum[j]) + row_move_d<0x128>(up8 ? sum[j] : sum[j + 2]);
-            one = (up4 ? sum[1] : sum[0]) + row_move_d<0x141>(up4 ? sum[0] : sum[1]);
-        } else {
-            one += row_move_d<0x128>(one);
-            one += row_move_d<0x141>(one);
-        }
+        for (int j = 0; j < 2; ++j) sum[j] = (up8 ? sum[j + 2] : sum[j]) + row_move_d<0x128>(up8 ? sum[j] : sum[j + 2]);
+        double one = (up4 ? sum[1] : sum[0]) + row_move_d<0x141>(up4 ? sum[0] : sum[1]);
         one += row_move_d<0x4E>(one);
         one += row_move_d<0xB1>(one);
         best = max(best, score_key(one));
     }
     uint64_t* key = keys_of + pair * t.seq_pages;
-    uint32_t mine = entry[0];
-    if constexpr (PAGES == 4) mine = up8 ? up4 ? entry[3] : entry[2] : up4 ? entry[1] : entry[0];
+    const uint32_t mine = up8 ? up4 ? entry[3] : entry[2] : up4 ? entry[1] : entry[0];
     if (mine >= t.pool) best = 0;
-    const uint32_t at = 4 * PAGES * wave + (PAGES == 4 ? 4 * (n >> 2) : 0u) + g;
-    const bool puts = (n & (PAGES == 4 ? 3 : 15)) == 0 && first + at < scored;
-    if (scored > BLOCK) {
+    const uint32_t at = 16 * wave + 4 * (n >> 2) + g;
+    const bool puts = (n & 3) == 0 && first + at < scored;
+    if (scored > SELECT_PAGES) {
         if (puts) __hip_atomic_store(key + first + at, best, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
         // The keys acknowledged, then the count: the block that completes it selects.
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
@@ -1072,7 +1062,7 @@ __global__ void __launch_bounds__(SELECT_THREADS)
         uint32_t* counter = counter_of + pair;
         if (i == 0) {
             const uint32_t before = __hip_atomic_fetch_add(counter, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-            sh.last = before == (scored - 1) / BLOCK;
+            sh.last = before == (scored - 1) / SELECT_PAGES;
         }
         __syncthreads();
         if (!sh.last) return;
@@ -1083,7 +1073,7 @@ __global__ void __launch_bounds__(SELECT_THREADS)
     }
     if (i == 0) to[budget - 1] = pages - 1;
     auto key_of = [&](uint32_t x) {
-        return scored > BLOCK ? __hip_atomic_load(key + x, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) : sh.key[x];
+        return scored > SELECT_PAGES ? __hip_atomic_load(key + x, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) : sh.key[x];
     };
     select_keys(key_of, scored, budget - 1, to, sh);
 }
@@ -1123,7 +1113,8 @@ x0ne_status check_heads(const char* what, const x0ne_kv8* c, uint32_t q_heads) {
     return X0NE_OK;
 }
 
-Table table_of(const x0ne_kv8* c) {
+
+Table whole_table(const x0ne_kv8* c) {
     return Table{(const uint32_t*)c->page_table, c->seqs, c->seq_pages, c->pool, c->kv_heads};
 }
 
@@ -1143,7 +1134,7 @@ extern "C" x0ne_status x0ne_gpu_kv8_write(x0ne_gpu* g, const x0ne_kv8* c, uint64
     if (!g) return fail(X0NE_ERR_GPU, "no device");
     if (rows == 0 || c->seqs == 0 || positions == 0) return X0NE_OK;
     const OnDevice on(g->device);
-    Write a = {table_of(c),
+    Write a = {whole_table(c),
                (uint8_t*)c->codes,
                (uint8_t*)c->scales,
                (const bf16_t*)qkv,
@@ -1185,7 +1176,7 @@ extern "C" x0ne_status x0ne_gpu_kv8_read(x0ne_gpu* g, const x0ne_kv8* c, uint64_
     // Bypassing the Infinity Cache with more than it holds: 16 sequences of up to 8192 positions 88.5 -> 85.3 us.
     const bool stream = (uint64_t)c->seqs * c->seq_pages * c->kv_heads * (3 * KV8_RECORD) > STREAM_BYTES;
     hipLaunchKernelGGL(stream ? kv8_read_kernel<true> : kv8_read_kernel<false>, dim3((uint32_t)blocks, c->seqs), dim3(256), 0, g->stream,
-                       table_of(c), (const uint8_t*)c->codes, (const uint8_t*)c->scales, (const uint32_t*)lens,
+                       whole_table(c), (const uint8_t*)c->codes, (const uint8_t*)c->scales, (const uint32_t*)lens,
                        (bf16_t*)k, (bf16_t*)v, (const uint32_t*)out_table, out_pool);
     X0NE_HIP(hipGetLastError(), what);
     return X0NE_OK;
@@ -1222,14 +1213,21 @@ static Cut cut_of(const x0ne_kv8* c, uint32_t budget = 0) {
     return cut;
 }
 
-// The workspace: a counter per (sequence, kv head), then the states of attention or the scores of selection.
-static uint64_t counter_bytes(const x0ne_kv8* c) { return ((uint64_t)c->seqs * c->kv_heads * 4 + 255) / 256 * 256; }
+// The workspace: a counter per (sequence, kv head), then the states of attention or the scores of selection. The counters
+// are as many for every cache, so that no call's states lie where another's counters are: caches of any shapes share a
+// workspace. Sequences beyond 65536 pairs are further launches, which come upon the counters left at zero.
+static constexpr uint64_t COUNTERS = 65536, COUNTER_BYTES = 4 * COUNTERS;
+static uint32_t seqs_at_once(const x0ne_kv8* c) { return (uint32_t)(COUNTERS / c->kv_heads) / 64 * 64; }
+static Table table_of(const x0ne_kv8* c, uint64_t first) {  // of a launch's sequences
+    return Table{(const uint32_t*)c->page_table + first * c->seq_pages, (uint32_t)std::min<uint64_t>(c->seqs - first, seqs_at_once(c)),
+                 c->seq_pages, c->pool, c->kv_heads};
+}
 
 extern "C" uint64_t x0ne_kv8_work_bytes(const x0ne_kv8* c, uint32_t q_heads) {
     if (check_cache("kv8 workspace", c) != X0NE_OK || check_heads("kv8 workspace", c, q_heads) != X0NE_OK) return 0;
     const uint64_t states = (uint64_t)c->seqs * q_heads * cut_of(c).slices * STATE * 4;
     const uint64_t scores = (uint64_t)c->seqs * c->kv_heads * c->seq_pages * 8;
-    return std::max<uint64_t>(256, counter_bytes(c) + std::max(states, scores));
+    return COUNTER_BYTES + std::max(states, scores);
 }
 
 extern "C" x0ne_status x0ne_gpu_kv8_attention(x0ne_gpu* g, const x0ne_kv8* c, uint64_t q, uint32_t q_heads, uint64_t lens,
@@ -1246,27 +1244,29 @@ extern "C" x0ne_status x0ne_gpu_kv8_attention(x0ne_gpu* g, const x0ne_kv8* c, ui
     if (!g) return fail(X0NE_ERR_GPU, "no device");
     if (c->seqs == 0) return X0NE_OK;
     const OnDevice on(g->device);
-    g->counts.launches++;
-    Attend a = {};
-    a.t = table_of(c);
-    a.codes = (const uint8_t*)c->codes;
-    a.scales = (const uint8_t*)c->scales;
-    a.q = (const bf16_t*)q;
-    a.lens = (const uint32_t*)lens;
-    a.list = (const uint32_t*)page_list;
-    a.out = (bf16_t*)out;
-    a.counter = (uint32_t*)work;
-    a.state = (float*)(work + counter_bytes(c));
-    a.budget = budget;
-    a.q_heads = q_heads;
-    a.group = q_heads / c->kv_heads;
     const Cut cut = cut_of(c, budget);
-    a.slices = cut.slices;
-    a.rounds = cut.rounds;
-    a.scale2 = scale * 1.44269504088896340736f;
     const auto kernel = cut.waves == 4 ? kv8_attention_kernel<4, false> : cut.stream ? kv8_attention_kernel<8, true> : kv8_attention_kernel<8, false>;
-    hipLaunchKernelGGL(kernel, dim3(c->kv_heads, cut.blocks, (c->seqs + 63) / 64), dim3(64 * cut.waves), 0, g->stream, a);
-    X0NE_HIP(hipGetLastError(), what);
+    for (uint64_t s = 0; s < c->seqs; s += seqs_at_once(c)) {
+        Attend a = {};
+        a.t = table_of(c, s);
+        a.codes = (const uint8_t*)c->codes;
+        a.scales = (const uint8_t*)c->scales;
+        a.q = (const bf16_t*)q + s * q_heads * KV8_HEAD;
+        a.lens = (const uint32_t*)lens + s;
+        a.list = page_list ? (const uint32_t*)page_list + s * c->kv_heads * budget : nullptr;
+        a.out = (bf16_t*)out + s * q_heads * KV8_HEAD;
+        a.counter = (uint32_t*)work;
+        a.state = (float*)(work + COUNTER_BYTES);
+        a.budget = budget;
+        a.q_heads = q_heads;
+        a.group = q_heads / c->kv_heads;
+        a.slices = cut.slices;
+        a.rounds = cut.rounds;
+        a.scale2 = scale * 1.44269504088896340736f;
+        g->counts.launches++;
+        hipLaunchKernelGGL(kernel, dim3(c->kv_heads, cut.blocks, (a.t.seqs + 63) / 64), dim3(64 * cut.waves), 0, g->stream, a);
+        X0NE_HIP(hipGetLastError(), what);
+    }
     return X0NE_OK;
 }
 
@@ -1281,17 +1281,19 @@ extern "C" x0ne_status x0ne_gpu_kv8_select(x0ne_gpu* g, const x0ne_kv8* c, uint6
         return bad(what, "bounds and q (16-byte aligned), lens and page_list are required");
     if (!work || work % 256 || work_bytes < x0ne_kv8_work_bytes(c, q_heads))
         return bad(what, "a workspace of x0ne_kv8_work_bytes (256-byte aligned) is required");
+    const uint32_t blocks = (c->seq_pages + SELECT_PAGES - 1) / SELECT_PAGES;
+    if (blocks > 65535) return bad(what, std::to_string(c->seq_pages) + " pages of a sequence (up to 65535 x 64)");
     if (!g) return fail(X0NE_ERR_GPU, "no device");
     if (c->seqs == 0) return X0NE_OK;
     const OnDevice on(g->device);
-    g->counts.launches++;
-    const bool wide = (uint64_t)c->seqs * c->kv_heads * ((c->seq_pages + 63) / 64) > V_WIDE;
-    const uint32_t each = wide ? 16 * SELECT_WAVES : 4 * SELECT_WAVES, blocks = (c->seq_pages + each - 1) / each;
-    if (blocks > 65535) return bad(what, std::to_string(c->seq_pages) + " pages of a sequence (up to 65535 x 64)");
-    hipLaunchKernelGGL(wide ? kv8_select_kernel<4> : kv8_select_kernel<1>, dim3(c->kv_heads, blocks, c->seqs),
-                       dim3(SELECT_THREADS), 0, g->stream, table_of(c), (const bf16_t*)bounds, (const bf16_t*)q,
-                       (const uint32_t*)lens, budget, (uint32_t*)page_list, (uint64_t*)(work + counter_bytes(c)),
-                       (uint32_t*)work, q_heads);
-    X0NE_HIP(hipGetLastError(), what);
+    for (uint64_t s = 0; s < c->seqs; s += seqs_at_once(c)) {
+        const Table t = table_of(c, s);
+        g->counts.launches++;
+        hipLaunchKernelGGL(kv8_select_kernel, dim3(c->kv_heads, blocks, t.seqs), dim3(SELECT_THREADS), 0, g->stream, t,
+                           (const bf16_t*)bounds, (const bf16_t*)q + s * q_heads * KV8_HEAD, (const uint32_t*)lens + s, budget,
+                           (uint32_t*)page_list + s * c->kv_heads * budget, (uint64_t*)(work + COUNTER_BYTES), (uint32_t*)work,
+                           q_heads);
+        X0NE_HIP(hipGetLastError(), what);
+    }
     return X0NE_OK;
 }
