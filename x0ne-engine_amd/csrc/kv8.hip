@@ -35,8 +35,8 @@ __device__ __forceinline__ uint32_t pack(float lo, float hi) {
 }
 __device__ __forceinline__ float half_of(const u32x4& x, int e) { return e & 1 ? bf_hi(x[e / 2]) : bf_lo(x[e / 2]); }
 
-// Values moved within a row of 16 lanes by DPP (0xB1, 0x4E: xor 1 and 2; 0x141: lane 7 - i of each half row; 0x128: 8
-// lanes round): every lane has a source, so no old value is kept.
+// Values moved within a row of 16 lanes by DPP (0xB1, 0x4E: xor 1 and 2; 0x141: lane 7 - i of each half row; 0x124, 0x128:
+// 4 and 8 lanes round): every lane has a source, so no old value is kept.
 template <int CTRL>
 __device__ __forceinline__ uint32_t row_move(uint32_t v) {
     return (uint32_t)__builtin_amdgcn_mov_dpp((int)v, CTRL, 0xF, 0xF, true);
@@ -840,10 +840,7 @@ constexpr uint32_t SELECT_BINS = 2048;
 constexpr uint32_t SELECT_PAGES = 4 * 4 * SELECT_WAVES;  // pages that a block scores: 16 lanes have 4
 
 struct SelectShared {
-    union {
-        double q[MAX_GROUP][KV8_HEAD];
-        uint32_t bin[SELECT_BINS];
-    };
+    uint32_t bin[SELECT_BINS];
     uint64_t key[SELECT_PAGES];  // of a pair whose pages one block scores
     uint64_t low[SELECT_WAVES], high[SELECT_WAVES];
     uint32_t part[SELECT_WAVES], count[SELECT_KEYS * SELECT_WAVES], equal[SELECT_KEYS * SELECT_WAVES];
@@ -903,7 +900,7 @@ __device__ __forceinline__ void select_keys(Get&& get, uint32_t n, uint32_t take
         sh.high[wave] = hi;
     }
     for (uint32_t j = t; j < SELECT_BINS; j += SELECT_THREADS) sh.bin[j] = 0;
-    __syncthreads();
+    lds_barrier();
 #pragma unroll
     for (uint32_t w = 0; w < SELECT_WAVES; ++w) {
         lo = min(lo, sh.low[w]);
@@ -915,37 +912,43 @@ __device__ __forceinline__ void select_keys(Get&& get, uint32_t n, uint32_t take
         const int shift = kv8_shift(lo, hi);
         if (pass) {
             for (uint32_t j = t; j < SELECT_BINS; j += SELECT_THREADS) sh.bin[j] = 0;
-            __syncthreads();
+            lds_barrier();
         }
         each([&](uint64_t x) {
             if (x >= lo && x <= hi) atomicAdd(&sh.bin[(uint32_t)((x - lo) >> shift)], 1u);
         });
-        __syncthreads();
+        lds_barrier();
         // Bins from the top, EACH to a thread: the one in which the count reaches `need`.
-        uint32_t mine = 0;
+        uint32_t bin[EACH], mine = 0;
 #pragma unroll
-        for (uint32_t j = 0; j < EACH; ++j) mine += sh.bin[SELECT_BINS - 1 - EACH * t - j];
+        for (uint32_t j = 0; j < EACH; ++j) mine += bin[j] = sh.bin[SELECT_BINS - 1 - EACH * t - j];
         const uint32_t upto = wave_up_to(mine);
         if (lane == 63) sh.part[wave] = upto;
-        __syncthreads();
+        lds_barrier();
         uint32_t above = upto - mine;
 #pragma unroll
         for (uint32_t w = 0; w < SELECT_WAVES; ++w) above += w < wave ? sh.part[w] : 0u;
         if (above < need && above + mine >= need) {
-            uint32_t b = SELECT_BINS - 1 - EACH * t;
-            while (above + sh.bin[b] < need) above += sh.bin[b--];
-            sh.found = b;
+            uint32_t j = 0, inside = bin[0];
+#pragma unroll
+            for (uint32_t b = 1; b < EACH; ++b) {  // past the bins that end before `need`
+                if (above + inside >= need) continue;
+                above += inside;
+                inside = bin[b];
+                j = b;
+            }
+            sh.found = SELECT_BINS - 1 - EACH * t - j;
             sh.above = above;
-            sh.inside = sh.bin[b];
+            sh.inside = inside;
         }
-        __syncthreads();
+        lds_barrier();
         need -= sh.above;
         kv8_narrow(lo, hi, shift, sh.found);
         if (sh.inside == need) {
             ties = false;
             break;
         }
-        __syncthreads();  // found, above and inside are read
+        lds_barrier();  // found, above and inside are read
     }
     // Indices in order: per row of 256 keys and wavefront the number taken, then its place.
     uint32_t placed = 0, equals = 0;
@@ -954,42 +957,43 @@ __device__ __forceinline__ void select_keys(Get&& get, uint32_t n, uint32_t take
         uint32_t equal_before[SELECT_KEYS];
         const uint64_t below = (1ull << lane) - 1;
         if (t < SELECT_KEYS * SELECT_WAVES) sh.count[t] = sh.equal[t] = 0;
-        __syncthreads();
+        lds_barrier();
         if (ties) {
             rows(first, [&](uint32_t j, bool in) {
                 const uint64_t m = __ballot(in && key[j] == lo);
                 equal_before[j] = (uint32_t)__popcll(m & below);
                 if (lane == 0) sh.equal[SELECT_WAVES * j + wave] = (uint32_t)__popcll(m);
             });
-            __syncthreads();
+            lds_barrier();
             const uint32_t own = sh.equal[lane], upto = wave_up_to(own);
             rows(first, [&](uint32_t j, bool) { equal_before[j] += equals + __builtin_amdgcn_readlane(upto - own, SELECT_WAVES * j + wave); });
             equals += __builtin_amdgcn_readlane(upto, 63);
         }
-        auto taken = [&](uint32_t j, bool in) {
-            return __ballot(in && (ties ? key[j] > lo || (key[j] == lo && equal_before[j] < need) : key[j] >= lo));
-        };
+        uint64_t taken[SELECT_KEYS];
         rows(first, [&](uint32_t j, bool in) {
-            const uint64_t m = taken(j, in);
-            if (lane == 0) sh.count[SELECT_WAVES * j + wave] = (uint32_t)__popcll(m);
+            taken[j] = __ballot(in && (ties ? key[j] > lo || (key[j] == lo && equal_before[j] < need) : key[j] >= lo));
+            if (lane == 0) sh.count[SELECT_WAVES * j + wave] = (uint32_t)__popcll(taken[j]);
         });
-        __syncthreads();
+        lds_barrier();
         const uint32_t own = sh.count[lane], upto = wave_up_to(own);
-        rows(first, [&](uint32_t j, bool in) {
-            const uint64_t m = taken(j, in);
+        rows(first, [&](uint32_t j, bool) {
             const uint32_t at = placed + __builtin_amdgcn_readlane(upto - own, SELECT_WAVES * j + wave);
-            if (m >> lane & 1) to[at + (uint32_t)__popcll(m & below)] = first + SELECT_THREADS * j + t;
+            if (taken[j] >> lane & 1) to[at + (uint32_t)__popcll(taken[j] & below)] = first + SELECT_THREADS * j + t;
         });
         placed += __builtin_amdgcn_readlane(upto, 63);
-        __syncthreads();  // the counts are read
+        if (n > AT_ONCE) lds_barrier();  // the counts are read
     }
 }
 
-// The pages of (sequence, kv head). 16 lanes have 8 dims each of a page's bounds (two 16-byte loads) of 4 pages, all in
-// flight at once (us, 2048 pages of 8 pairs: 24.2, with 1 page 33.6: more blocks to count), so a block scores 64 pages;
-// products and sums in f64, so that equal pages score equal and near ones in their order. The last block of its (sequence,
-// kv head) to count itself selects; a block that has them all need not count. The last page stands outside: it is always
-// kept.
+// The pages of (sequence, kv head). A block scores 64 pages, a wavefront 16 of them as 4 x 4: lane l has dims 8 (l / 4) ..
+// of page l % 4 of each four (two 16-byte loads of bounds each, all in flight at once; one four to a wavefront, with 4
+// times the blocks to count: 33.6 us for 24.2, 2048 pages of 8 pairs) and of query l % 4, so element d of the 8 is an
+// operand of a product of 4 pages and 4 queries over 4 dims, 4 of which (4 x 4 x 4, four blocks) the f64 matrix
+// instruction sums: max(q lo, q hi) = q+ hi + q- lo, q+ and q- being q where it is not below and where it is below 0, else
+// 0 (a NaN is in q+). Products of bf16 are exact and sums f64, in one order for all pages, so equal pages score equal and
+// near ones in their order (with 16 lanes to a page and vector f64: 33.5 us for 29.7, 16 sequences of up to 16000 keys).
+// The last block of its (sequence, kv head) to count itself selects; a block that has them all need not count. The last
+// page stands outside: it is always kept.
 __global__ void __launch_bounds__(SELECT_THREADS)
     kv8_select_kernel(Table t, const bf16_t* __restrict__ bounds, const bf16_t* __restrict__ q,
                       const uint32_t* __restrict__ lens, uint32_t budget, uint32_t* __restrict__ list,
@@ -1000,20 +1004,20 @@ __global__ void __launch_bounds__(SELECT_THREADS)
     const size_t pair = (size_t)s * t.kv_heads + kh;
     uint32_t* to = list + pair * budget;
     // What is needed of memory is requested at once: the length, the queries, the table's entries, whatever the length.
+    // Queries past the group repeat its last one, which leaves the maximum as it is.
     const uint32_t first = blockIdx.y * SELECT_PAGES;
     const uint32_t pages = (kv8_keys(lens[s], t.seq_pages) + KV8_PAGE - 1) / KV8_PAGE;
+    auto entry_at = [&](uint32_t p) { return t.pages[(size_t)s * t.seq_pages + min(p, t.seq_pages - 1)]; };
     uint32_t entry[4];
 #pragma unroll
-    for (uint32_t j = 0; j < 4; ++j) {
-        const uint32_t p = first + 16 * wave + 4 * j + g;
-        entry[j] = t.pages[(size_t)s * t.seq_pages + min(p, t.seq_pages - 1)];
-    }
-    for (uint32_t e = i; e < group * KV8_HEAD; e += SELECT_THREADS)
-        sh.q[0][e] = (double)bf2f(q[((size_t)s * q_heads + kh * group) * KV8_HEAD + e]);
-    u32x4 lo[4], hi[4];
+    for (uint32_t j = 0; j < 4; ++j) entry[j] = entry_at(first + 16 * wave + 4 * j + (lane & 3));
+    const uint32_t at = 16 * wave + 4 * (n >> 2) + g, its_entry = entry_at(first + at);
+    const bf16_t* head = q + ((size_t)s * q_heads + kh * group) * KV8_HEAD + 8 * (lane >> 2);
+    auto query = [&](uint32_t h) { return *reinterpret_cast<const u32x4*>(head + min(h + (lane & 3), group - 1) * KV8_HEAD); };
+    u32x4 x = query(0), lo[4], hi[4];
 #pragma unroll
     for (uint32_t j = 0; j < 4; ++j) {
-        const u32x4* b = reinterpret_cast<const u32x4*>(bounds + kv8_bound(entry[j] < t.pool ? entry[j] : 0u, t.kv_heads, kh)) + n;
+        const u32x4* b = reinterpret_cast<const u32x4*>(bounds + kv8_bound(entry[j] < t.pool ? entry[j] : 0u, t.kv_heads, kh)) + (lane >> 2);
         lo[j] = b[0];
         hi[j] = b[KV8_HEAD / 8];
     }
@@ -1024,35 +1028,36 @@ __global__ void __launch_bounds__(SELECT_THREADS)
     }
     const uint32_t scored = pages - 1;
     if (first >= scored) return;
-    __syncthreads();
-    // Four pages' sums over 16 lanes, transposed: at the first two steps a lane keeps two, then one of its sums and adds
-    // its partner's of those, so lane n ends with page n / 4's. Each sum is added in the same tree.
-    const bool up8 = n & 8, up4 = n & 4;
     uint64_t best = 0;
-    for (uint32_t h = 0; h < group; ++h) {
-        double x[8], sum[4];
+#pragma unroll 1
+    for (uint32_t h = 0; h < group; h += 4) {
+        // Converted again for every 4 queries: kept, the bounds' 64 doubles are half the registers (30.7 us for 29.7).
 #pragma unroll
-        for (int d = 0; d < 8; ++d) x[d] = sh.q[h][8 * n + d];
+        for (int j = 0; j < 4; ++j) asm("" : "+v"(lo[j]), "+v"(hi[j]));
+        double sum[4] = {0.0, 0.0, 0.0, 0.0};
 #pragma unroll
-        for (uint32_t j = 0; j < 4; ++j) {
-            sum[j] = 0.0;
+        for (int d = 0; d < 8; ++d) {
+            const float v = half_of(x, d);
+            const double up = v < 0.f ? 0.0 : (double)v, down = v < 0.f ? (double)v : 0.0;
 #pragma unroll
-            for (int d = 0; d < 8; ++d) {
-                const uint32_t w = x[d] < 0.0 ? lo[j][d / 2] : hi[j][d / 2];
-                sum[j] = fma(x[d], (double)(d & 1 ? bf_hi(w) : bf_lo(w)), sum[j]);
-            }
+            for (int j = 0; j < 4; ++j) sum[j] = __builtin_amdgcn_mfma_f64_4x4x4f64((double)half_of(hi[j], d), up, sum[j], 0, 0, 0);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) sum[j] = __builtin_amdgcn_mfma_f64_4x4x4f64((double)half_of(lo[j], d), down, sum[j], 0, 0, 0);
         }
+        if (h + 4 < group) x = query(h + 4);
+        // The result of page i, query j, block b is in lane 16 i + 4 b + j: the blocks' sum, in all four; lane n then takes
+        // the pages of four n / 4, so its page is 4 (n / 4) + g of the wavefront's.
 #pragma unroll
-        for (int j = 0; j < 2; ++j) sum[j] = (up8 ? sum[j + 2] : sum[j]) + row_move_d<0x128>(up8 ? sum[j] : sum[j + 2]);
-        double one = (up4 ? sum[1] : sum[0]) + row_move_d<0x141>(up4 ? sum[0] : sum[1]);
-        one += row_move_d<0x4E>(one);
-        one += row_move_d<0xB1>(one);
-        best = max(best, score_key(one));
+        for (int j = 0; j < 4; ++j) {
+            sum[j] += row_move_d<0x128>(sum[j]);
+            sum[j] += row_move_d<0x124>(sum[j]);
+        }
+        best = max(best, score_key(n & 8 ? n & 4 ? sum[3] : sum[2] : n & 4 ? sum[1] : sum[0]));
     }
+    best = max(best, row_move_u<0xB1>(best));
+    best = max(best, row_move_u<0x4E>(best));
     uint64_t* key = keys_of + pair * t.seq_pages;
-    const uint32_t mine = up8 ? up4 ? entry[3] : entry[2] : up4 ? entry[1] : entry[0];
-    if (mine >= t.pool) best = 0;
-    const uint32_t at = 16 * wave + 4 * (n >> 2) + g;
+    if (its_entry >= t.pool) best = 0;
     const bool puts = (n & 3) == 0 && first + at < scored;
     if (scored > SELECT_PAGES) {
         if (puts) __hip_atomic_store(key + first + at, best, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
