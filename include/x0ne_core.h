@@ -216,23 +216,24 @@ typedef struct {
 } x0ne_kv8;
 
 /* Writes rows of any mix of sequences: qkv [rows][(q_heads + 2 kv_heads) 128] bf16, row r at position
-   row_pos[r] of sequence row_seq[r] (u32 each; the rows name distinct positions). RMSNorm of each
-   head of q and k (weights q_norm, k_norm, 128 bf16) and rotate-half RoPE from rope_cs, the f64 (cos,
-   sin) table of `positions` positions (x0ne_rope_table_f64): q_out [rows][q_heads 128] bf16 has the
-   bits of x0ne_qk_norm_rope_kv_write_rows_bf16, the cache holds the codes of its k and v rows. A row
-   whose sequence is not below seqs, or whose position has no table entry or no page-table entry, is
-   padding: nothing of it is written. bounds (0: none): [pool][kv_heads][2][128] bf16, of every page
-   whose last position is among the rows the smallest and the largest key value of each dim over its
-   16 positions (zeros +0, NaN where a key is), for x0ne_gpu_kv8_select; the rows of such a page then
-   stand together, their positions ascending by 1 (as those of a prompt do; the page's other positions
-   are those of earlier calls). qkv, q_norm, k_norm, rope_cs, q_out and bounds are 16-byte aligned;
-   q_heads 1 to 16384, rows below 2^24. */
+   row_pos[r] of sequence row_seq[r] (u32 each; no two rows name the same slot of a page, by one
+   sequence's table or by two). RMSNorm of each head of q and k (weights q_norm, k_norm, 128 bf16) and
+   rotate-half RoPE from rope_cs, the f64 (cos, sin) table of `positions` positions
+   (x0ne_rope_table_f64): q_out [rows][q_heads 128] bf16, apart from qkv, has the bits of
+   x0ne_qk_norm_rope_kv_write_rows_bf16, the cache holds the codes of its k and v rows. A row whose
+   sequence is not below seqs, or whose position has no table entry or no page-table entry, is padding:
+   nothing of it is written. bounds (0: none): [pool][kv_heads][2][128] bf16, of every page whose last
+   position is among the rows the smallest and the largest key value of each dim over its 16 positions
+   (zeros +0, NaN where a key is), for x0ne_gpu_kv8_select; the rows of such a page then stand
+   together, their positions ascending by 1 (as those of a prompt do; the page's other positions are
+   those of earlier calls). qkv, q_norm, k_norm, rope_cs, q_out and bounds are 16-byte aligned; q_heads
+   1 to 16384, rows below 2^24. */
 x0ne_status x0ne_gpu_kv8_write(x0ne_gpu* g, const x0ne_kv8* c, uint64_t qkv, uint64_t rows, uint32_t q_heads,
                                uint64_t q_norm, uint64_t k_norm, float eps, uint64_t rope_cs, uint32_t positions,
                                uint64_t row_seq, uint64_t row_pos, uint64_t q_out, uint64_t bounds);
 /* Reads it back as bf16 pages (exact): sequence s's positions below lens[s] (u32; at most its pages')
    into the K plane [out_pool][kv_heads][16][128] and the V plane [out_pool][kv_heads][128][16] at the
-   pages that out_table [seqs][seq_pages] names, the layout that the bf16 kernels of this library take
+   pages that out_table [seqs][seq_pages] names (each once), the layout that the bf16 kernels of this library take
    (x0ne_attention_prefill_g*_bf16, x0ne_gpu_attention_split). Positions of a sequence's last page at
    or past its length are zero; pages past it, and entries of out_pool or more, are left alone. */
 x0ne_status x0ne_gpu_kv8_read(x0ne_gpu* g, const x0ne_kv8* c, uint64_t lens, uint64_t k, uint64_t v, uint64_t out_table,
