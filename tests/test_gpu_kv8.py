@@ -98,6 +98,18 @@ def test_bounds_of_pages_filled_over_several_calls(kernels, heads):
     check_write(kernels, rng, *heads, qkv, row_seq, row_pos, seq_pages, seqs, cache=c)
 
 
+@pytest.mark.parametrize("kv_heads", [1, 6, 7])
+def test_bounds_of_a_launch_of_many_blocks(kernels, kv_heads):
+    """Heads enough that a block takes four of them: a prompt that starts inside a page (each page's rows in two
+    blocks, the first with slots of an earlier call), then one whole page, then single rows that end pages."""
+    rng = np.random.default_rng(kv_heads)
+    q_heads = 2048 // kv_heads * kv_heads
+    c = R.fill(rng, kv_heads, [5, 16, 31, 47], 5)
+    row_seq = [0] * 43 + [1] * 5 + [1] * 16 + [2, 3]
+    row_pos = list(range(5, 48)) + list(range(16, 21)) + list(range(32, 48)) + [31, 47]
+    check_write(kernels, rng, q_heads, kv_heads, random_qkv(rng, len(row_seq), q_heads, kv_heads), row_seq, row_pos, 5, 4, cache=c)
+
+
 def test_rows_past_the_table_or_the_pool_are_left_alone(kernels):
     """Padding of every kind: no such sequence, past the sequence's pages, past the rope table, a page outside the
     pool (its q is written); the bounds of a page outside the pool are not."""

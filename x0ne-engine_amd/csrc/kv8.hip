@@ -204,14 +204,18 @@ __device__ __forceinline__ void put_bounds(u32x2 w, uint32_t byte, bf16_t* to, K
 //    a prompt, that is stored as such, else byte by byte.
 // A row of no sequence, or past the sequence's pages or the rope table, writes nothing.
 // Bounds of a page belong to the blocks of the row of its last slot. Rows that are one whole page have its keys at
-// hand; else each 16 lanes take a slot: a row of this call (of the 15 rows before) is computed again, since another
-// block writes its codes meanwhile, an older one is read from the cache.
+// hand; else each 16 lanes take a slot, whose codes are this block's own (through LDS) or of an earlier call (from the
+// cache); a row of this call before the block's, whose codes another block writes meanwhile, is computed again (all of the
+// call's rows computed again: 64 rows of 64 sequences 9.6 us for 7.4, 777 rows 13.1 for 12.8).
 template <int HEADS>
 __global__ void __launch_bounds__(256) kv8_write_kernel(const Write a) {
     constexpr uint32_t HD = KV8_HEAD;
     __shared__ union {
         uint32_t turned[WRITE_VALUES][KV8_PART / 4];
-        KeyValues keys;
+        struct {
+            KeyValues keys;
+            uint32_t code[HEADS][WRITE_ROWS][HD / 4], byte[HEADS][WRITE_ROWS];
+        };
     } sh;
     const uint32_t n = threadIdx.x & 15, r = threadIdx.x >> 4, r0 = blockIdx.x * WRITE_ROWS, last = a.rows - 1;
     const uint32_t kvh = a.t.kv_heads, heads = a.q_heads + kvh;
@@ -279,32 +283,58 @@ __global__ void __launch_bounds__(256) kv8_write_kernel(const Write a) {
                 if (i < count) put_bounds(code[i], byte[i], a.bounds + kv8_bound(page_n, kvh, h0 + i), sh.keys);
             return;
         }
-        for (uint64_t ends = __ballot(page_n != KV8_NONE && pos_n % KV8_PAGE == KV8_PAGE - 1) & 0xFFFFu; ends; ends &= ends - 1) {
+        uint64_t ends = __ballot(page_n != KV8_NONE && pos_n % KV8_PAGE == KV8_PAGE - 1) & 0xFFFFu;
+        if (!ends) return;
+#pragma unroll
+        for (uint32_t i = 0; i < HEADS; ++i) {
+            sh.code[i][r][n] = code[i][0];
+            sh.code[i][r][16 + n] = code[i][1];
+            if (n == 0) sh.byte[i][r] = byte[i];
+        }
+        lds_barrier();
+        for (; ends; ends &= ends - 1) {
             const uint32_t at = (uint32_t)__builtin_ctzll(ends), end = r0 + at;
             const uint32_t its_seq = __builtin_amdgcn_readlane(seq_n, at), its_pos = __builtin_amdgcn_readlane(pos_n, at);
             const uint32_t its_page = __builtin_amdgcn_readlane(page_n, at);
             const uint32_t from = end + r - 15, from_pos = its_pos + r - 15;  // slot r's row, if it is of this call
             const bool fresh = end + r >= 15 && a.row_seq[min(from, last)] == its_seq && a.row_pos[min(from, last)] == from_pos;
+            const bool here = fresh && from >= r0;
+#pragma unroll 1
+            for (uint32_t i0 = 0; i0 < count; i0 += 2) {
+                u32x2 v[2];
+                uint32_t b[2];
 #pragma unroll
-            for (int j = 0; j < 4; ++j) c[j] = a.cs[(size_t)from_pos * (HD / 2) + 4 * n + j];
-#pragma unroll
-            for (uint32_t i = 0; i < HEADS; ++i) {
-                const uint32_t h = h0 + min(i, count - 1);
-                const uint8_t* rec = a.codes + kv8_record(its_page, kvh, h) + r * HD;
-                code[i] = u32x2{*reinterpret_cast<const uint32_t*>(rec + 4 * n), *reinterpret_cast<const uint32_t*>(rec + 64 + 4 * n)};
-                byte[i] = a.scales[kv8_scale(its_page, kvh, h) + r];
-                x[i] = load_head(a.qkv + min(from, last) * stride + first + min(i, count - 1) * HD, n);
-            }
-#pragma unroll
-            for (uint32_t i = 0; i < HEADS; ++i) {
-                if (i >= count) break;
-                uint32_t again;
-                const u32x2 v = quantise(turn_head(x[i], root_of(square_sum(x[i]), a.eps), w, c), again);
-                if (fresh) {
-                    code[i] = v;
-                    byte[i] = again;
+                for (uint32_t i = 0; i < 2; ++i) {
+                    const uint32_t h = h0 + min(i0 + i, count - 1);
+                    const uint8_t* rec = a.codes + kv8_record(its_page, kvh, h) + r * HD;
+                    v[i] = u32x2{*reinterpret_cast<const uint32_t*>(rec + 4 * n), *reinterpret_cast<const uint32_t*>(rec + 64 + 4 * n)};
+                    b[i] = a.scales[kv8_scale(its_page, kvh, h) + r];
                 }
-                put_bounds(code[i], byte[i], a.bounds + kv8_bound(its_page, kvh, h0 + i), sh.keys);
+                if (__any(fresh && !here)) {
+                    u32x4 was[2];
+#pragma unroll
+                    for (uint32_t i = 0; i < 2; ++i) was[i] = load_head(a.qkv + min(from, last) * stride + first + min(i0 + i, count - 1) * HD, n);
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) c[j] = a.cs[(size_t)from_pos * (HD / 2) + 4 * n + j];
+#pragma unroll
+                    for (uint32_t i = 0; i < 2; ++i) {
+                        uint32_t again;
+                        const u32x2 x = quantise(turn_head(was[i], root_of(square_sum(was[i]), a.eps), w, c), again);
+                        if (fresh) {
+                            v[i] = x;
+                            b[i] = again;
+                        }
+                    }
+                }
+#pragma unroll
+                for (uint32_t i = 0; i < 2; ++i) {
+                    if (i0 + i >= count) break;
+                    if (here) {
+                        v[i] = u32x2{sh.code[i0 + i][from - r0][n], sh.code[i0 + i][from - r0][16 + n]};
+                        b[i] = sh.byte[i0 + i][from - r0];
+                    }
+                    put_bounds(v[i], b[i], a.bounds + kv8_bound(its_page, kvh, h0 + i0 + i), sh.keys);
+                }
             }
         }
         return;
@@ -1155,8 +1185,8 @@ extern "C" x0ne_status x0ne_gpu_kv8_write(x0ne_gpu* g, const x0ne_kv8* c, uint64
                positions,
                eps};
     // 4 heads to a block read cos and sin, and take square roots, half as often as 2, which are over sooner and, with
-    // bounds, keep the blocks of a row that ends a page short (us with 2 / 4: 64 rows of 64 sequences, 40 blocks of 4, 9.5 /
-    // 15.4; 777 rows of 72 heads, 882 blocks, 13.0 / 13.8; 2048 rows of 40 heads, 1280 blocks, 15.0 / 13.8; 8 heads 16.3).
+    // bounds, keep the blocks of a row that ends a page short (us with 2 / 4: 64 rows of 64 sequences, 40 blocks of 4, 7.4 /
+    // 10.9; 777 rows of 72 heads, 882 blocks, 12.8 / 13.9; 2048 rows of 40 heads, 1280 blocks, 15.0 / 13.8; 8 heads 16.3).
     const uint32_t tiles = (a.rows + WRITE_ROWS - 1) / WRITE_ROWS;
     const bool many = (uint64_t)tiles * ((q_heads + c->kv_heads) / WRITE_HEADS) >= 1024;
     const uint32_t each = many ? WRITE_HEADS : 2;
