@@ -395,6 +395,24 @@ def test_attention_keeps_poison_to_its_own(kernels):
     assert np.isnan(vals(out)[1, :4]).all() and np.isnan(vals(out)[2, 4:, 77]).all()
 
 
+@pytest.mark.parametrize("kv_heads,lens", [(2, [5, 0, 40, 700]), (1, [9000]), (8, [300] * 20)])
+def test_attention_of_queries_that_hold_an_infinity(kernels, kv_heads, lens):
+    """Keys whose dim 7 is positive and queries with -inf or +inf there: every score -inf or +inf, whose softmax is NaN;
+    the other heads and sequences have the bits they have without."""
+    rng = np.random.default_rng(23)
+    c = R.fill(rng, kv_heads, lens, -(-max(lens) // PAGE))
+    row = c.codes[:, :, :2048].reshape(c.pool, kv_heads, PAGE, HEAD)
+    row[..., 7] = np.maximum(row[..., 7] & 0x7F, 1)
+    clean = random_q(rng, len(lens), 4 * kv_heads)
+    q, bad = clean.copy(), np.zeros(clean.shape[:2], bool)
+    for s, h, x in [(0, 0, 0xFF80), (-1, -1, 0xFF80), (-1, 1, 0x7F80)]:
+        q[s, h, 7] = x
+        bad[s, h] = True
+    out = kernels.kv8_attention(c, q, 4 * kv_heads, lens)
+    check_attention(c, q, 4 * kv_heads, lens, out)
+    assert np.isnan(vals(out)[bad]).all() and (out[~bad] == kernels.kv8_attention(c, clean, 4 * kv_heads, lens)[~bad]).all()
+
+
 @pytest.mark.parametrize("budget", [1, 2, 5, 16, 70])
 def test_attention_over_a_page_list(kernels, budget):
     """Lists of chosen pages (with and without the last), shorter than the budget, entries of none among them."""
@@ -740,3 +758,41 @@ def test_more_pairs_than_counters(kernels):
     few = type(c)(c.codes[:, some], c.scales[:, some], four)
     assert (pages[:4, some] == R.select(few, R.all_bounds(few), vals(q4[:, some]), lens, budget)).all()
     check_attention(few, q4[:, some], 4, lens, out[:4, some])
+
+
+def test_two_gpus_streams_at_once(kernels):
+    """Two Gpus of one device, each with its stream and workspace, their calls issued in turn without a wait between:
+    each the bits it has alone."""
+    from x0ne_core import Arena, Gpu, Kv8
+    from x0ne_core.arena import Class
+    rng = np.random.default_rng(24)
+    pairs = []
+    for g, (kvh, q_heads, lens) in zip((kernels.gpu, Gpu()), [(8, 32, [6000, 50, 0]), (2, 8, [3000] * 9)]):
+        c = R.fill(rng, kvh, lens, 376)
+        q, a, budget = random_q(rng, len(lens), q_heads), Arena(), 9
+        size = g.kv8_work_bytes(Kv8(16, 16, 16, c.pool, kvh, *c.table.shape), q_heads)
+        bounds = R.all_bounds(c)
+        arrays = {"codes": c.codes, "scales": c.scales, "table": c.table, "q": q, "lens": np.array(lens, np.uint32),
+                  "bounds": bounds, "work": np.zeros(size, np.uint8)}
+        s = {k: a.alloc(k, v.nbytes, Class.CLIENT_DATA) for k, v in arrays.items()}
+        s.update({k: a.alloc(k, n, Class.CLIENT_DATA) for k, n in
+                  {"out": q.nbytes, "sparse": q.nbytes, "list": len(lens) * kvh * budget * 4}.items()})
+        a.freeze(g)
+        for k, v in arrays.items():
+            a.write(s[k], 0, v)
+        at = {k: a.ptr(v) for k, v in s.items()}
+        pairs.append((g, c, q, q_heads, lens, bounds, budget, size, a, s, at, Kv8(at["codes"], at["scales"], at["table"], c.pool, kvh, *c.table.shape)))
+    for _ in range(10):
+        for g, c, q, q_heads, lens, bounds, budget, size, a, s, at, kv in pairs:
+            g.kv8_select(kv, at["bounds"], at["q"], q_heads, at["lens"], budget, at["list"], at["work"], size)
+            g.kv8_attention(kv, at["q"], q_heads, at["lens"], at["out"], 0.088, at["work"], size)
+            g.kv8_attention(kv, at["q"], q_heads, at["lens"], at["sparse"], 0.088, at["work"], size, page_list=at["list"], budget=budget)
+    for g, *_ in pairs:
+        g.sync()
+    for g, c, q, q_heads, lens, bounds, budget, size, a, s, at, kv in pairs:
+        read = lambda k, n, t: a.read_array(s[k], 0, n, t)
+        pages = read("list", len(lens) * c.kv_heads * budget, np.uint32).reshape(len(lens), c.kv_heads, budget)
+        assert (pages == kernels.kv8_select(c, bounds, q, q_heads, lens, budget)).all()
+        assert (read("out", q.size, np.uint16).reshape(q.shape) == kernels.kv8_attention(c, q, q_heads, lens, scale=0.088)).all()
+        assert (read("sparse", q.size, np.uint16).reshape(q.shape) ==
+                kernels.kv8_attention(c, q, q_heads, lens, page_list=pages, scale=0.088)).all()

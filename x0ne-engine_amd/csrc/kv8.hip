@@ -457,6 +457,10 @@ __device__ __forceinline__ float2 get2(const float* p) {
     const uint64_t v = __hip_atomic_load((const uint64_t*)p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     return make_float2(__uint_as_float((uint32_t)v), __uint_as_float((uint32_t)(v >> 32)));
 }
+// A state without a key has the maximum -inf. One whose keys all score -inf (an infinity in the query) has the lowest
+// finite value and no weight: its softmax is 0 / 0.
+constexpr float LOWEST = -3.402823466e+38f;
+__device__ __forceinline__ float share(float top, float l) { return l != 0.f ? 1.f / l : top == -INFINITY ? 0.f : NAN; }
 // 2^(m - top), 0 for a state without a key.
 __device__ __forceinline__ float factor(float m, float top) {
     return __builtin_amdgcn_exp2f(m - (top == -INFINITY ? 0.f : top));
@@ -521,10 +525,10 @@ __device__ __forceinline__ void join(const Attend& a, const float* __restrict__ 
     // Each head's factors and sum by one wavefront, a lane per slice.
     for (uint32_t h = t / 64; h < a.group; h += WAVES) {
         const uint32_t z = t % 64;
-        const float m = z < active ? sh.m[h][z] : -INFINITY, f = factor(m, rows_max(row_max(m)));
+        const float m = z < active ? sh.m[h][z] : -INFINITY, top = rows_max(row_max(m)), f = factor(m, top);
         if (z < active) sh.m[h][z] = f;
         const float l = rows_sum(row_sum(z < active ? f * sh.l[h][z] : 0.f));
-        if (z == 0) sh.wl[0][h] = l;
+        if (z == 0) sh.wl[0][h] = share(top, l);
     }
     lds_barrier();
     auto sum = [&](uint32_t e) -> f32x4 {
@@ -540,7 +544,7 @@ __device__ __forceinline__ void join(const Attend& a, const float* __restrict__ 
     };
     auto store = [&](uint32_t e, f32x4 x) {
         const uint32_t h = e / (KV8_HEAD / 4);
-        const float l = sh.wl[0][h], r = l == 0.f ? 0.f : 1.f / l;
+        const float r = sh.wl[0][h];
         *reinterpret_cast<uint2*>(out + 4 * e) = make_uint2(pack(x[0] * r, x[1] * r), pack(x[2] * r, x[3] * r));
     };
     if (parts == 1) {
@@ -743,6 +747,7 @@ __global__ void __launch_bounds__(64 * WAVES, 2) kv8_attention_kernel(const Atte
 #pragma unroll
                 for (int e = 0; e < 4; ++e) mx = fmaxf(mx, sc[m][e]);
             mx = fmaxf(m_run, rows_max(mx));
+            if (whole || __any(here.valid != 0)) mx = fmaxf(mx, LOWEST);
             if (__any(mx > m_run)) {
                 const float alpha = factor(m_run, mx);
                 lsum *= alpha;
@@ -750,7 +755,7 @@ __global__ void __launch_bounds__(64 * WAVES, 2) kv8_attention_kernel(const Atte
                 for (int c = 0; c < 8; ++c) o[c] *= alpha;
                 m_run = mx;
             }
-            const float ref = m_run == -INFINITY ? 0.f : m_run;
+            const float ref = m_run == -INFINITY ? 0.f : m_run;  // a tile without a key
             u32x4 hi[2], lo[2];
 #pragma unroll
             for (int m = 0; m < 4; ++m) {
@@ -825,7 +830,7 @@ __global__ void __launch_bounds__(64 * WAVES, 2) kv8_attention_kernel(const Atte
                 x += f * *reinterpret_cast<const f32x4*>(&sh.wo[w][h][d]);
             }
             if (it.active == 1) {
-                const float r = l == 0.f ? 0.f : 1.f / l;
+                const float r = share(top, l);
                 *reinterpret_cast<uint2*>(out + h * KV8_HEAD + d) = make_uint2(pack(x[0] * r, x[1] * r), pack(x[2] * r, x[3] * r));
             } else {
                 float* st = state + ((size_t)h * a.slices + it.y) * STATE;
