@@ -220,28 +220,28 @@ class Gpu:
     def kv8_write(self, cache: Kv8, qkv: int, rows: int, q_heads: int, q_norm: int, k_norm: int, eps: float, rope_cs: int,
                   positions: int, row_seq: int, row_pos: int, q_out: int, bounds: int = 0):
         """QK-norm, RoPE and the quantised K/V write of rows of any mix of sequences (x0ne_gpu_kv8_write)."""
-        check(lib().x0ne_gpu_kv8_write(self.h, C.byref(cache), qkv, rows, q_heads, q_norm, k_norm, eps, rope_cs, positions,
+        check(lib().x0ne_gpu_kv8_write(self.h, cache, qkv, rows, q_heads, q_norm, k_norm, eps, rope_cs, positions,
                                        row_seq, row_pos, q_out, bounds), "kv8_write")
 
     def kv8_read(self, cache: Kv8, lens: int, k: int, v: int, out_table: int, out_pool: int):
         """The cache's positions below lens back as bf16 pages (x0ne_gpu_kv8_read)."""
-        check(lib().x0ne_gpu_kv8_read(self.h, C.byref(cache), lens, k, v, out_table, out_pool), "kv8_read")
+        check(lib().x0ne_gpu_kv8_read(self.h, cache, lens, k, v, out_table, out_pool), "kv8_read")
 
     def kv8_work_bytes(self, cache: Kv8, q_heads: int) -> int:
         """Bytes of the zeroed workspace of kv8_attention and kv8_select; 0 for a cache they refuse."""
-        return lib().x0ne_kv8_work_bytes(C.byref(cache), q_heads)
+        return lib().x0ne_kv8_work_bytes(cache, q_heads)
 
     def kv8_attention(self, cache: Kv8, q: int, q_heads: int, lens: int, out: int, scale: float, work: int, work_bytes: int,
                       page_list: int = 0, budget: int = 0):
         """Decode attention of one query per sequence, over every page or those of page_list
         (x0ne_gpu_kv8_attention)."""
-        check(lib().x0ne_gpu_kv8_attention(self.h, C.byref(cache), q, q_heads, lens, page_list, budget, out, scale, work,
+        check(lib().x0ne_gpu_kv8_attention(self.h, cache, q, q_heads, lens, page_list, budget, out, scale, work,
                                            work_bytes), "kv8_attention")
 
     def kv8_select(self, cache: Kv8, bounds: int, q: int, q_heads: int, lens: int, budget: int, page_list: int, work: int,
                    work_bytes: int):
         """The budget pages per sequence and kv head worth attending, by their bounds (x0ne_gpu_kv8_select)."""
-        check(lib().x0ne_gpu_kv8_select(self.h, C.byref(cache), bounds, q, q_heads, lens, budget, page_list, work, work_bytes),
+        check(lib().x0ne_gpu_kv8_select(self.h, cache, bounds, q, q_heads, lens, budget, page_list, work, work_bytes),
               "kv8_select")
 
     def capture(self, launches) -> Graph:
