@@ -193,6 +193,24 @@ def test_read_under_a_table_far_wider_than_the_sequences(kernels):
     check_read(kernels, c, lens, out_table, k, v)
 
 
+def test_read_of_more_records_than_wavefronts(kernels):
+    """100000 pages of 3 kv heads: a wavefront takes several. The pages are five in turn, most go nowhere."""
+    rng = np.random.default_rng(25)
+    pages, kvh = 100000, 3
+    c = R.fill(rng, kvh, [80], 5, spare=0)
+    c = type(c)(c.codes, c.scales, np.resize(c.table, (1, pages)))
+    at = [0, 1, 43690, 43691, 87380, 87381, 87382, 99998, 99999]
+    out_table = np.full((1, pages), NONE, np.uint32)
+    out_table[0, at] = np.arange(len(at))
+    lens = [pages * PAGE - 5]
+    k, v = kernels.kv8_read(c, lens, out_table, len(at))
+    for i, p in enumerate(at):
+        want_k, want_v = R.page_values(c, int(c.table[0, p]))
+        if p == pages - 1:
+            want_k[:, 11:], want_v[:, 11:] = 0, 0
+        assert (vals(k[i]).reshape(kvh, PAGE, HEAD) == want_k).all() and (vals(v[i]).reshape(kvh, HEAD, PAGE) == want_v.transpose(0, 2, 1)).all(), p
+
+
 def check_read(kernels, c, lens, out_table, k, v):
     want_k, want_v = np.full(k.shape, kernels.SENTINEL, np.uint16), np.full(v.shape, kernels.SENTINEL, np.uint16)
     for s, n in enumerate(lens):

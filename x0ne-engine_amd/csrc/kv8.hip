@@ -563,7 +563,7 @@ __device__ __forceinline__ void join(const Attend& a, const float* __restrict__ 
 
 // A slice of a sequence: its tiles are cut into `active` slices of `per` tiles, by its own length and the call's `slices`
 // and `rounds` only. A block walks slices of its kv head and its 64 sequences: lane l of each wavefront holds a sequence's
-// length and the slices up to and with it.
+// length, its slices' number and size (the divisions, once for all lanes) and the slices up to and with it.
 struct Item {
     uint32_t s, y, keys, pages, np, per, active, t0, t_end;  // sequence and slice; this wavefront's tiles t0, t0 + WAVES ..
     __device__ __forceinline__ bool any() const { return t0 < t_end; }
@@ -591,31 +591,34 @@ __global__ void __launch_bounds__(64 * WAVES, 2) kv8_attention_kernel(const Atte
     __shared__ Shared<WAVES> sh;
     const uint32_t kh = blockIdx.x, s0 = blockIdx.z * 64, step = WAVES;
     const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), n = lane & 15, g = lane >> 4;
-    auto shape = [&](uint32_t keys) -> Item {
+    auto shape = [&](uint32_t keys) -> Item {  // all but its slices
         Item it = {};
         it.keys = keys;
         it.pages = (keys + KV8_PAGE - 1) / KV8_PAGE;
         it.np = a.list ? min(a.budget, it.pages) : it.pages;
-        const uint32_t tiles = (it.np + TILE_PAGES - 1) / TILE_PAGES, rounds = (tiles + WAVES - 1) / WAVES;
-        it.active = max(1u, min(a.slices, (rounds + a.rounds - 1) / a.rounds));
-        it.per = WAVES * max(1u, (rounds + it.active - 1) / it.active);
-        it.active = max(1u, (tiles + it.per - 1) / it.per);
-        it.t_end = tiles;
+        it.t_end = (it.np + TILE_PAGES - 1) / TILE_PAGES;
         return it;
     };
     uint32_t my_keys = s0 + lane < a.t.seqs ? kv8_keys(a.lens[s0 + lane], a.t.seq_pages) : 0u, my_seq = lane;
-    uint32_t mine = s0 + lane < a.t.seqs ? shape(my_keys).active : 0u;
-    uint32_t upto = wave_up_to(mine);
+    const uint32_t tiles = shape(my_keys).t_end, rounds = (tiles + WAVES - 1) / WAVES;
+    uint32_t active = max(1u, min(a.slices, (rounds + a.rounds - 1) / a.rounds));
+    uint32_t per = WAVES * max(1u, (rounds + active - 1) / active);
+    active = s0 + lane < a.t.seqs ? max(1u, (tiles + per - 1) / per) : 0u;
+    uint32_t upto = wave_up_to(active);
     const uint32_t total = __builtin_amdgcn_readlane(upto, 63), blocks = gridDim.y;
     if (total > blocks) {  // several slices per block: the longest sequences' first
         uint32_t rank = 0;
-        for (int j = 0; j < 64; ++j) {
+        const uint32_t there = min(64u, a.t.seqs - s0);
+#pragma unroll 1
+        for (uint32_t j = 0; j < there; ++j) {
             const uint32_t other = __builtin_amdgcn_readlane(my_keys, j);
-            rank += other > my_keys || (other == my_keys && (uint32_t)j < lane);
+            rank += other > my_keys || (other == my_keys && j < lane);
         }
         my_seq = (uint32_t)__builtin_amdgcn_ds_permute((int)(4 * rank), (int)lane);
         my_keys = (uint32_t)__builtin_amdgcn_ds_permute((int)(4 * rank), (int)my_keys);
-        upto = wave_up_to((uint32_t)__builtin_amdgcn_ds_permute((int)(4 * rank), (int)mine));
+        per = (uint32_t)__builtin_amdgcn_ds_permute((int)(4 * rank), (int)per);
+        active = (uint32_t)__builtin_amdgcn_ds_permute((int)(4 * rank), (int)active);
+        upto = wave_up_to(active);
     }
     // A block's slice of round r, the rounds to and fro over the blocks.
     auto item = [&](uint32_t r) -> Item {
@@ -624,6 +627,8 @@ __global__ void __launch_bounds__(64 * WAVES, 2) kv8_attention_kernel(const Atte
         const uint32_t at = (uint32_t)__popcll(__ballot(upto <= i));
         Item it = shape(__builtin_amdgcn_readlane(my_keys, at));
         it.s = s0 + __builtin_amdgcn_readlane(my_seq, at);
+        it.per = __builtin_amdgcn_readlane(per, at);
+        it.active = __builtin_amdgcn_readlane(active, at);
         it.y = i - (__builtin_amdgcn_readlane(upto, at) - it.active);
         it.t0 = it.y * it.per + wave;
         it.t_end = min(it.t_end, (it.y + 1) * it.per);
@@ -1032,9 +1037,9 @@ __device__ __forceinline__ void select_keys(Get&& get, uint32_t n, uint32_t take
 __global__ void __launch_bounds__(SELECT_THREADS)
     kv8_select_kernel(Table t, const bf16_t* __restrict__ bounds, const bf16_t* __restrict__ q,
                       const uint32_t* __restrict__ lens, uint32_t budget, uint32_t* __restrict__ list,
-                      uint64_t* __restrict__ keys_of, uint32_t* __restrict__ counter_of, uint32_t q_heads) {
+                      uint64_t* __restrict__ keys_of, uint32_t* __restrict__ counter_of, uint32_t group) {
     __shared__ SelectShared sh;
-    const uint32_t kh = blockIdx.x, s = blockIdx.z, i = threadIdx.x, group = q_heads / t.kv_heads;
+    const uint32_t kh = blockIdx.x, s = blockIdx.z, i = threadIdx.x;
     const uint32_t lane = i & 63, wave = __builtin_amdgcn_readfirstlane(i >> 6), n = lane & 15, g = lane >> 4;
     const size_t pair = (size_t)s * t.kv_heads + kh;
     uint32_t* to = list + pair * budget;
@@ -1047,7 +1052,7 @@ __global__ void __launch_bounds__(SELECT_THREADS)
 #pragma unroll
     for (uint32_t j = 0; j < 4; ++j) entry[j] = entry_at(first + 16 * wave + 4 * j + (lane & 3));
     const uint32_t at = 16 * wave + 4 * (n >> 2) + g, its_entry = entry_at(first + at);
-    const bf16_t* head = q + ((size_t)s * q_heads + kh * group) * KV8_HEAD + 8 * (lane >> 2);
+    const bf16_t* head = q + pair * group * KV8_HEAD + 8 * (lane >> 2);
     auto query = [&](uint32_t h) { return *reinterpret_cast<const u32x4*>(head + min(h + (lane & 3), group - 1) * KV8_HEAD); };
     u32x4 x = query(0), lo[4], hi[4];
 #pragma unroll
@@ -1332,7 +1337,7 @@ extern "C" x0ne_status x0ne_gpu_kv8_select(x0ne_gpu* g, const x0ne_kv8* c, uint6
         hipLaunchKernelGGL(kv8_select_kernel, dim3(c->kv_heads, blocks, t.seqs), dim3(SELECT_THREADS), 0, g->stream, t,
                            (const bf16_t*)bounds, (const bf16_t*)q + s * q_heads * KV8_HEAD, (const uint32_t*)lens + s, budget,
                            (uint32_t*)page_list + s * c->kv_heads * budget, (uint64_t*)(work + COUNTER_BYTES), (uint32_t*)work,
-                           q_heads);
+                           q_heads / c->kv_heads);
         X0NE_HIP(hipGetLastError(), what);
     }
     return X0NE_OK;
