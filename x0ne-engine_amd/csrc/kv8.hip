@@ -1234,12 +1234,13 @@ extern "C" x0ne_status x0ne_gpu_kv8_read(x0ne_gpu* g, const x0ne_kv8* c, uint64_
 //  - Many: blocks that fill the card walk the slices, longest first. A slice of one round costs about four (its lookups,
 //    states and count are not hidden), so slices are two thirds of what a block has to do if every sequence fills its
 //    table (64 sequences of up to 6000 keys, blocks of 8, 2 / 4 / 8 / 12 rounds: 108 / 95 / 87 / 77; 16 of up to 8192,
-//    2 / 4 / 6 / 8: 48 / 45 / 36 / 40), up to 16, and fewer for fewer pairs, whose lengths may be far below their tables'.
+//    3 / 4 / 5 / 6 / 8: 44 / 47 / 37 / 38 / 44), up to 16, and fewer for fewer pairs, whose lengths may be far below
+//    their tables'.
 //  - Blocks of 8 wavefronts, one on a CU, join fewer states than two of 4 and start fewer slices (us with 4 / 8: 32768
-//    keys 21.1 / 19.2, 64 sequences 83 / 77, 16 sequences 35 / 36); where the pages, all attended, are less than two
-//    rounds of 8 for each CU, 4 (128 pages for each of 8 pairs 9 / 11).
+//    keys 21.1 / 19.0, 64 sequences 84 / 73, 16 sequences 35 / 35); where the pages, all attended, are less than two
+//    rounds of 8 for each CU, 4 (128 pages for each of 8 pairs, with their selection, 21.9 / 24.1).
 //  - Loads of more than the Infinity Cache holds bypass it (64 sequences of up to 6000 keys 76.6 -> 72.9 us); 67 MB, read
-//    again before 256 MB of others, come from it (32768 keys 19.2 us with it, 22.3 without).
+//    again before 256 MB of others, come from it (32768 keys 19 us with it, 22 without).
 struct Cut {
     uint32_t waves, slices, rounds, blocks;
     bool stream;
