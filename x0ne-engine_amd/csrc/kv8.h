@@ -75,3 +75,52 @@ KV8_BOTH void kv8_narrow(uint64_t& lo, uint64_t& hi, int shift, uint32_t bin) {
     lo += (uint64_t)bin << shift;
     if (hi - lo > span) hi = lo + span;
 }
+
+// How decode attention cuts sequences: at most `slices` slices of at least `rounds` rounds (a tile of KV8_TILE pages for
+// each of a block's `waves` wavefronts), over `blocks` blocks for each kv head and 64 sequences.
+//  - Few pairs of sequence and kv head: slices for one block on each of 256 CUs; more bring more states to join than
+//    overlap gains (us, 32768 keys, 8 pairs, blocks of 4, 16 / 32 / 64 slices: 27.2 / 21.7 / 26.8).
+//  - Many: blocks that fill the card walk the slices, longest first. A slice of one round costs about four (its lookups,
+//    states and count are not hidden), so slices are two thirds of what a block has to do if every sequence fills its
+//    table (64 sequences of up to 6000 keys, blocks of 8, 2 / 4 / 8 / 12 rounds: 108 / 95 / 87 / 77; 16 of up to 8192,
+//    3 / 4 / 5 / 6 / 8: 44 / 47 / 37 / 38 / 44), up to 16, and fewer for fewer pairs, whose lengths may be far below
+//    their tables'.
+//  - Blocks of 8 wavefronts, one on a CU, join fewer states than two of 4 and start fewer slices (us with 4 / 8: 32768
+//    keys 21.1 / 19.0, 64 sequences 84 / 73, 16 sequences 35 / 35); where the pages, all attended, are less than two
+//    rounds of 8 for each CU, 4 (128 pages for each of 8 pairs, with their selection, 21.9 / 24.1).
+//  - Loads of more than the Infinity Cache holds bypass it (64 sequences of up to 6000 keys 76.6 -> 72.9 us); 67 MB, read
+//    again before 256 MB of others, come from it (32768 keys 19 us with it, 22 without).
+constexpr uint64_t KV8_STREAM = 256ull << 20;  // the Infinity Cache's bytes
+constexpr uint32_t KV8_TILE = 4;               // pages of a wavefront's tile
+constexpr uint32_t KV8_SLICES = 64;            // the most slices of a sequence
+struct Kv8Cut {
+    uint32_t waves, slices, rounds, blocks;
+    bool stream;
+};
+inline Kv8Cut kv8_cut(uint32_t kv_heads, uint32_t seqs, uint32_t seq_pages, uint32_t budget) {
+    auto least = [](uint64_t a, uint64_t b) { return a < b ? a : b; };
+    auto most_of = [](uint64_t a, uint64_t b) { return a > b ? a : b; };
+    const uint64_t pairs = most_of(1, (uint64_t)seqs * kv_heads), parts = (seqs + 63) / 64, together = least(seqs, 64);
+    const uint32_t most = budget && budget < seq_pages ? budget : seq_pages;  // pages a sequence attends
+    Kv8Cut cut;
+    cut.waves = pairs * ((most + 31) / 32) >= 512 ? 8 : 4;
+    cut.stream = pairs * most * (KV8_RECORD + KV8_SCALES) > KV8_STREAM;  // 8 wavefronts then
+    cut.slices = (uint32_t)least(KV8_SLICES, most_of(16, 256 / pairs));
+    cut.blocks = (uint32_t)most_of(1, 2048 / cut.waves / most_of(1, parts * kv_heads));
+    const uint64_t fullest = (uint64_t)((most + KV8_TILE * cut.waves - 1) / (KV8_TILE * cut.waves)) * together;
+    cut.rounds = (uint32_t)most_of(1, least(least(16, pairs / 24), 2 * fullest / (3 * cut.blocks)));
+    cut.blocks = (uint32_t)most_of(1, least(cut.blocks, cut.slices * together));
+    return cut;
+}
+// The slices of a sequence of `tiles` tiles, and the tiles of each: at least one slice, by its own length and the cut only.
+KV8_BOTH uint32_t kv8_slices(uint32_t tiles, uint32_t waves, uint32_t slices, uint32_t cut_rounds, uint32_t& per) {
+    const uint32_t rounds = (tiles + waves - 1) / waves, wanted = (rounds + cut_rounds - 1) / cut_rounds;
+    const uint32_t few = wanted < slices ? wanted : slices, active = few > 1 ? few : 1, each = (rounds + active - 1) / active;
+    per = waves * (each > 1 ? each : 1);
+    const uint32_t n = (tiles + per - 1) / per;
+    return n > 1 ? n : 1;
+}
+// The slice that a block takes in its turn r, among those of its kv head and 64 sequences: to and fro over the blocks.
+KV8_BOTH uint32_t kv8_turn(uint32_t r, uint32_t block, uint32_t blocks) {
+    return r * blocks + (r & 1 ? blocks - 1 - block : block);
+}

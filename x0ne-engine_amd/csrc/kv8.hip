@@ -381,7 +381,6 @@ __device__ __forceinline__ void put(T* p, T x) {
     else
         *p = x;
 }
-constexpr uint64_t STREAM_BYTES = 256ull << 20;  // the Infinity Cache
 
 // Eight codes as bf16, times the power of two `scale`: exact.
 __device__ __forceinline__ u32x4 decode(uint32_t lo, uint32_t hi, float scale) {
@@ -466,8 +465,6 @@ __device__ __forceinline__ float factor(float m, float top) {
     return __builtin_amdgcn_exp2f(m - (top == -INFINITY ? 0.f : top));
 }
 
-constexpr uint32_t TILE_PAGES = 4;
-constexpr uint32_t MAX_SLICES = 64;
 constexpr uint32_t STATE = KV8_HEAD + 4;  // floats of a partial state: m, l, two unused, o
 constexpr uint32_t MAX_GROUP = 16;
 
@@ -487,7 +484,7 @@ template <uint32_t WAVES>
 struct Shared {
     float wm[WAVES][MAX_GROUP], wl[WAVES][MAX_GROUP];
     float wo[WAVES][MAX_GROUP][KV8_HEAD + 4];
-    float m[MAX_GROUP][MAX_SLICES], l[MAX_GROUP][MAX_SLICES];  // the join's: each slice's maximum (then factor) and sum
+    float m[MAX_GROUP][KV8_SLICES], l[MAX_GROUP][KV8_SLICES];  // the join's: each slice's maximum (then factor) and sum
     uint32_t last;
 };
 
@@ -596,14 +593,12 @@ __global__ void __launch_bounds__(64 * WAVES, 2) kv8_attention_kernel(const Atte
         it.keys = keys;
         it.pages = (keys + KV8_PAGE - 1) / KV8_PAGE;
         it.np = a.list ? min(a.budget, it.pages) : it.pages;
-        it.t_end = (it.np + TILE_PAGES - 1) / TILE_PAGES;
+        it.t_end = (it.np + KV8_TILE - 1) / KV8_TILE;
         return it;
     };
     uint32_t my_keys = s0 + lane < a.t.seqs ? kv8_keys(a.lens[s0 + lane], a.t.seq_pages) : 0u, my_seq = lane;
-    const uint32_t tiles = shape(my_keys).t_end, rounds = (tiles + WAVES - 1) / WAVES;
-    uint32_t active = max(1u, min(a.slices, (rounds + a.rounds - 1) / a.rounds));
-    uint32_t per = WAVES * max(1u, (rounds + active - 1) / active);
-    active = s0 + lane < a.t.seqs ? max(1u, (tiles + per - 1) / per) : 0u;
+    uint32_t per, active = kv8_slices(shape(my_keys).t_end, WAVES, a.slices, a.rounds, per);
+    if (s0 + lane >= a.t.seqs) active = 0;
     uint32_t upto = wave_up_to(active);
     const uint32_t total = __builtin_amdgcn_readlane(upto, 63), blocks = gridDim.y;
     if (total > blocks) {  // several slices per block: the longest sequences' first
@@ -622,7 +617,7 @@ __global__ void __launch_bounds__(64 * WAVES, 2) kv8_attention_kernel(const Atte
     }
     // A block's slice of round r, the rounds to and fro over the blocks.
     auto item = [&](uint32_t r) -> Item {
-        const uint32_t i = r * blocks + (r & 1 ? blocks - 1 - blockIdx.y : blockIdx.y);
+        const uint32_t i = kv8_turn(r, blockIdx.y, blocks);
         if (i >= total) return Item{};
         const uint32_t at = (uint32_t)__popcll(__ballot(upto <= i));
         Item it = shape(__builtin_amdgcn_readlane(my_keys, at));
@@ -641,7 +636,7 @@ __global__ void __launch_bounds__(64 * WAVES, 2) kv8_attention_kernel(const Atte
         uint32_t page, valid;
     };
     auto logical_at = [&](const Item& it, uint32_t t) -> uint32_t {
-        const uint32_t at = TILE_PAGES * t + g;
+        const uint32_t at = KV8_TILE * t + g;
         if (t >= it.t_end || at >= it.np) return KV8_NONE;
         return a.list ? a.list[((size_t)it.s * a.t.kv_heads + kh) * a.budget + at] : at;
     };
@@ -1219,7 +1214,7 @@ extern "C" x0ne_status x0ne_gpu_kv8_read(x0ne_gpu* g, const x0ne_kv8* c, uint64_
     g->counts.launches++;
     const uint64_t blocks = std::min<uint64_t>(65536, ((uint64_t)c->seq_pages * c->kv_heads + 3) / 4);
     // Bypassing the Infinity Cache with more than it holds: 16 sequences of up to 8192 positions 88.5 -> 85.3 us.
-    const bool stream = (uint64_t)c->seqs * c->seq_pages * c->kv_heads * (3 * KV8_RECORD) > STREAM_BYTES;
+    const bool stream = (uint64_t)c->seqs * c->seq_pages * c->kv_heads * (3 * KV8_RECORD) > KV8_STREAM;
     hipLaunchKernelGGL(stream ? kv8_read_kernel<true> : kv8_read_kernel<false>, dim3((uint32_t)blocks, c->seqs), dim3(256), 0, g->stream,
                        whole_table(c), (const uint8_t*)c->codes, (const uint8_t*)c->scales, (const uint32_t*)lens,
                        (bf16_t*)k, (bf16_t*)v, (const uint32_t*)out_table, out_pool);
@@ -1227,37 +1222,7 @@ extern "C" x0ne_status x0ne_gpu_kv8_read(x0ne_gpu* g, const x0ne_kv8* c, uint64_
     return X0NE_OK;
 }
 
-// How sequences are cut: at most `slices` slices of at least `rounds` rounds (a tile for each of a block's `waves`
-// wavefronts), over `blocks` blocks for each kv head and 64 sequences.
-//  - Few pairs of sequence and kv head: slices for one block on each of 256 CUs; more bring more states to join than
-//    overlap gains (us, 32768 keys, 8 pairs, blocks of 4, 16 / 32 / 64 slices: 27.2 / 21.7 / 26.8).
-//  - Many: blocks that fill the card walk the slices, longest first. A slice of one round costs about four (its lookups,
-//    states and count are not hidden), so slices are two thirds of what a block has to do if every sequence fills its
-//    table (64 sequences of up to 6000 keys, blocks of 8, 2 / 4 / 8 / 12 rounds: 108 / 95 / 87 / 77; 16 of up to 8192,
-//    3 / 4 / 5 / 6 / 8: 44 / 47 / 37 / 38 / 44), up to 16, and fewer for fewer pairs, whose lengths may be far below
-//    their tables'.
-//  - Blocks of 8 wavefronts, one on a CU, join fewer states than two of 4 and start fewer slices (us with 4 / 8: 32768
-//    keys 21.1 / 19.0, 64 sequences 84 / 73, 16 sequences 35 / 35); where the pages, all attended, are less than two
-//    rounds of 8 for each CU, 4 (128 pages for each of 8 pairs, with their selection, 21.9 / 24.1).
-//  - Loads of more than the Infinity Cache holds bypass it (64 sequences of up to 6000 keys 76.6 -> 72.9 us); 67 MB, read
-//    again before 256 MB of others, come from it (32768 keys 19 us with it, 22 without).
-struct Cut {
-    uint32_t waves, slices, rounds, blocks;
-    bool stream;
-};
-static Cut cut_of(const x0ne_kv8* c, uint32_t budget = 0) {
-    const uint64_t pairs = std::max<uint64_t>(1, (uint64_t)c->seqs * c->kv_heads), parts = (c->seqs + 63) / 64;
-    const uint32_t most = budget ? std::min(budget, c->seq_pages) : c->seq_pages;  // pages a sequence attends
-    Cut cut;
-    cut.waves = pairs * ((most + 31) / 32) >= 512 ? 8 : 4;
-    cut.stream = pairs * most * (KV8_RECORD + KV8_SCALES) > STREAM_BYTES;  // 8 wavefronts then
-    cut.slices = (uint32_t)std::min<uint64_t>(MAX_SLICES, std::max<uint64_t>(16, 256 / pairs));
-    cut.blocks = (uint32_t)std::max<uint64_t>(1, 2048 / cut.waves / std::max<uint64_t>(1, parts * c->kv_heads));
-    const uint64_t fullest = (uint64_t)((most + 4 * cut.waves - 1) / (4 * cut.waves)) * std::min(c->seqs, 64u);
-    cut.rounds = (uint32_t)std::max<uint64_t>(1, std::min(std::min<uint64_t>(16, pairs / 24), 2 * fullest / (3 * cut.blocks)));
-    cut.blocks = std::max(1u, std::min(cut.blocks, cut.slices * std::min(c->seqs, 64u)));
-    return cut;
-}
+static Kv8Cut cut_of(const x0ne_kv8* c, uint32_t budget = 0) { return kv8_cut(c->kv_heads, c->seqs, c->seq_pages, budget); }
 
 // The workspace: a counter per (sequence, kv head), then the states of attention or the scores of selection. The counters
 // are as many for every cache, so that no call's states lie where another's counters are: caches of any shapes share a
@@ -1290,7 +1255,7 @@ extern "C" x0ne_status x0ne_gpu_kv8_attention(x0ne_gpu* g, const x0ne_kv8* c, ui
     if (!g) return fail(X0NE_ERR_GPU, "no device");
     if (c->seqs == 0) return X0NE_OK;
     const OnDevice on(g->device);
-    const Cut cut = cut_of(c, budget);
+    const Kv8Cut cut = cut_of(c, budget);
     const auto kernel = cut.waves == 4 ? kv8_attention_kernel<4, false> : cut.stream ? kv8_attention_kernel<8, true> : kv8_attention_kernel<8, false>;
     for (uint64_t s = 0; s < c->seqs; s += seqs_at_once(c)) {
         Attend a = {};
