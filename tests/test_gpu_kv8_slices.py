@@ -1,5 +1,7 @@
-"""Decode attention over the 8-bit paged K/V cache where blocks walk several slices: batches whose blocks count and join
-slices while they hold further ones (tests/test_cpu_kv8_slices.py holds the shapes to that)."""
+"""Decode attention over the 8-bit paged K/V cache where blocks walk several slices, with outputs that show every page
+and key: batches whose blocks count and join slices while they hold further ones (tests/test_cpu_kv8_slices.py holds
+the shapes to that), a scale of 0 over values that count keys, and flat scores within a bound in which a single
+page stands out."""
 import numpy as np
 import pytest
 
@@ -61,3 +63,127 @@ def test_attention_of_blocks_that_walk_slices(kernels, group, kv_heads, kinds, s
         out = kernels.kv8_attention(c, q[of], q_heads, lens, page_list=None if pages is None else pages[of], calls=calls)
         assert (out == out[:n][of]).all(), "sequences of one kind differ"
     check_attention(kinds_only(c, n), q, q_heads, kinds, out[:n], page_list=pages)
+
+
+# -- values that count keys --
+
+# (group, kv heads, lengths, pages of a table)
+COUNTED = [
+    (4, 2, [20000], 1259),
+    (1, 1, [4097, 64, 65, 63, 1], 270),
+    (3, 2, [9000, 8191, 8192, 8193], 572),
+    (7, 1, [n for m in range(1, 33) for n in (64 * m - 1, 64 * m, 64 * m + 1)][:62], 128),
+    (2, 8, [2000, 1990, 1951, 2000] * 10, 126),
+    (2, 2, [2000, 1985, 1984, 1983] * 10, 126),
+    (8, 8, [6000, 5500, 6000, 5999] * 10, 376),
+    (5, 8, [6000, 6000, 5900, 60] * 5, 376),
+    (1, 4, [4700, 4800, 17, 4000] * 8, 300),
+    (1, 8, [16384, 777, 40] + [33] * 5, 1100),
+]
+COUNT_OFF = 2.0 ** -8 + 2.0 ** -21  # the rounding to bf16 and, in f32, of 1 / n and its product: a few 2^-24
+
+
+def counting(rng, kv_heads, lens, seq_pages):
+    """A cache of 128 pages whose values are 1 in one dim and 0 in the others: dim (a_h p + b_h) % 127 in page p < 127,
+    so that each kv head deals the pages to its dims in its own order, and 127 in page 127. Tables use the first 127 pages
+    about as often, and 127 for every sequence's last: (cache, dim of each page [kv_heads][128])."""
+    page = np.arange(128)
+    a, b = rng.integers(1, 127, (2, kv_heads))
+    dims = np.where(page < 127, (a[:, None] * page + b[:, None]) % 127, 127)
+    v = np.zeros((128, kv_heads, PAGE, HEAD))
+    for h in range(kv_heads):
+        v[page, h, :, dims[h]] = 1.0
+    c = R.fill(rng, kv_heads, [128 * PAGE], 128, spare=0)
+    vc, vs = R.quantise(v)
+    c.codes[:, :, 2048:] = vc.transpose(0, 1, 3, 2).reshape(128, kv_heads, 2048)
+    c.scales[:, :, PAGE:] = vs
+    table = np.stack([np.concatenate([rng.permutation(127) for _ in range(-(-seq_pages // 127))])[:seq_pages] for _ in lens])
+    for s, n in enumerate(lens):
+        table[s, -(-n // PAGE) - 1] = 127
+    return type(c)(c.codes, c.scales, table.astype(np.uint32)), dims
+
+
+def counts(c, dims, s, n):
+    """Keys of sequence s below n in each dim, [kv_heads][128], and of each of its pages: [pages]."""
+    keys = np.minimum(PAGE, n - PAGE * np.arange(-(-n // PAGE)))
+    at = dims[:, c.table[s, :len(keys)]]
+    return np.stack([np.bincount(at[h], keys, HEAD) for h in range(len(dims))]), keys
+
+
+@pytest.mark.parametrize("group,kv_heads,lens,seq_pages", COUNTED)
+def test_every_page_and_key_counts_once(kernels, group, kv_heads, lens, seq_pages):
+    """At a scale of 0 every key weighs 1 and the sums are whole numbers, exact in f32: an output is its dim's keys over
+    the sequence's, within the final roundings. A page left out, taken twice or for another moves some dim by more, and
+    so does a key of the last page or one behind the length."""
+    rng = np.random.default_rng(len(lens) * 100 + kv_heads)
+    c, dims = counting(rng, kv_heads, lens, seq_pages)
+    q = random_q(rng, len(lens), group * kv_heads)
+    out = vals(kernels.kv8_attention(c, q, group * kv_heads, lens, scale=0.0, calls=2)).reshape(len(lens), kv_heads, group, HEAD)
+    for s, n in enumerate(lens):
+        want = counts(c, dims, s, n)[0][:, None] / n
+        assert (np.abs(out[s] - want) <= COUNT_OFF * want).all(), f"sequence {s} of {n} keys"
+
+
+# -- flat scores --
+
+# (group, kv heads, lengths, pages of a table, the most tiles a wavefront takes of a slice)
+FLAT = [
+    (4, 2, [20000], 1259, 2),
+    (4, 2, [9000, 8191], 572, 1),
+    (8, 1, [4097, 1025], 270, 1),
+    (4, 8, [6000, 5500, 6000, 5999] * 10, 376, 6),
+    (2, 2, [2000, 1990, 1951, 2000] * 10, 126, 1),
+]
+FLAT_Q = 0.1
+
+
+def flat_tolerance(keys_v, weights, q, k, scale, rounds):
+    """How far the outputs of one kv head [group][128] may be from their 64-bit values, by the kernel's steps. A score in
+    units of log 2 is a sum of 128 exact products in f32 in any order (130 roundings), times a factor of three roundings
+    and less a maximum (two more, of numbers up to the largest score twice): its weight is off by ln 2 times that. Each
+    of a wavefront's `rounds` tiles may rescale what is before it, as do the joins of wavefronts and of slices: an exponential
+    (1 ulp, 2^-23) and a product each. A weight is two bf16 parts (2^-17 of it). The value sums round at most 33 times a
+    matrix instruction, 4 of which a dim's sum takes of each tile (2 by 32 keys, of both parts), and once per wavefront
+    and slice (8 + 64); the sum of the weights 16 times a tile and once per lane, wavefront and slice. Those go with the sum of
+    |v| under the weights; what the denominator has, with the output; then a division and a product, and the rounding
+    to bf16."""
+    reach = float((np.abs(q) @ np.abs(k).T).max()) * abs(scale) * np.log2(np.e)
+    share = weights / weights.sum(-1, keepdims=True)
+    spread, want = share @ np.abs(keys_v), share @ keys_v
+    weight = np.log(2) * 135 * 2.0 ** -24 * reach + (rounds + 3) * 3 * 2.0 ** -23
+    return (spread * (weight + 2.0 ** -17 + (132 * rounds + 80) * 2.0 ** -24)
+            + np.abs(want) * (weight + (16 * rounds + 80) * 2.0 ** -24 + 2.0 ** -22 + 2.0 ** -8))
+
+
+def flat_case(group, kv_heads, lens, seq_pages):
+    """(cache, queries, number of kinds): random keys and values, every page of a sequence another of the pool."""
+    rng = np.random.default_rng(len(lens) * 10 + group)
+    n = min(len(lens), 4)
+    c = R.fill(rng, kv_heads, [seq_pages * PAGE], seq_pages, spare=0)
+    tables = np.stack([rng.permutation(seq_pages) for _ in range(n)]).astype(np.uint32)
+    return type(c)(c.codes, c.scales, tables), random_q(rng, n, group * kv_heads, FLAT_Q), n
+
+
+def flat_weights(c, q, s, h, n, scale):
+    """Of kv head h of sequence s: keys, values [n][128], the weights [group][n]."""
+    k, v = (x[h] for x in R.sequence(c, s, n))
+    x = q @ k.T * scale
+    return k, v, np.exp(x - x.max(-1, keepdims=True))
+
+
+@pytest.mark.parametrize("group,kv_heads,lens,seq_pages,rounds", FLAT)
+def test_attention_of_flat_scores_misses_no_page(kernels, group, kv_heads, lens, seq_pages, rounds):
+    from x0ne_core.ops import attn_scale
+    c, q, n = flat_case(group, kv_heads, lens, seq_pages)
+    of, scale = np.arange(len(lens)) % n, attn_scale(HEAD)
+    out = kernels.kv8_attention(type(c)(c.codes, c.scales, c.table[of]), q[of], group * kv_heads, lens, calls=2)
+    assert (out == out[:n][of]).all()
+    got, qv, worst = vals(out[:n]).reshape(n, kv_heads, group, HEAD), vals(q).reshape(n, kv_heads, group, HEAD), 0.0
+    for s in range(n):
+        for h in range(kv_heads):
+            k, v, w = flat_weights(c, qv[s, h], s, h, lens[s], scale)
+            tol = flat_tolerance(v, w, qv[s, h], k, scale, rounds)
+            off = np.abs(got[s, h] - w @ v / w.sum(-1, keepdims=True))
+            worst = max(worst, float((off / tol).max()))
+            assert (off <= tol).all(), f"sequence {s} of {lens[s]} keys, kv head {h}: {(off / tol).max()} of the tolerance"
+    print(f"MEASURE kv8 attention, flat scores {group}/{kv_heads} {lens[:4]}: worst {worst:.3f} of the tolerance")
