@@ -187,3 +187,34 @@ def test_attention_of_flat_scores_misses_no_page(kernels, group, kv_heads, lens,
             worst = max(worst, float((off / tol).max()))
             assert (off <= tol).all(), f"sequence {s} of {lens[s]} keys, kv head {h}: {(off / tol).max()} of the tolerance"
     print(f"MEASURE kv8 attention, flat scores {group}/{kv_heads} {lens[:4]}: worst {worst:.3f} of the tolerance")
+
+
+# -- values of every size --
+
+@pytest.mark.parametrize("power", [-124, -112, -100, 60, 115, None])
+def test_attention_of_tiny_and_large_values(kernels, power):
+    """Values around 2^power, and rows of sizes from 2^-40 to 2^40 beside each other (None), under ordinary scores:
+    within flat_tolerance's bound. A weight times its row's power of two lies below bf16's normal numbers for tiny
+    rows, where its second part is off by up to 2^-134 of the row's code, as is the output's own rounding."""
+    from x0ne_core.ops import attn_scale
+    rng = np.random.default_rng(200 + (power or 0))
+    lens, kv_heads, group = [300, 40, 1, 700], 2, 4
+    c = R.fill(rng, kv_heads, lens, 44)
+    x = rng.standard_normal((c.pool, kv_heads, PAGE, HEAD))
+    x *= 2.0 ** (power if power is not None else rng.integers(-40, 41, (c.pool, kv_heads, PAGE, 1)))
+    vc, vs = R.quantise(vals(bits(x)).reshape(x.shape))
+    c.codes[:, :, 2048:] = vc.transpose(0, 1, 3, 2).reshape(c.pool, kv_heads, 2048)
+    c.scales[:, :, PAGE:] = vs
+    q, scale = random_q(rng, len(lens), group * kv_heads), attn_scale(HEAD)
+    got = vals(kernels.kv8_attention(c, q, group * kv_heads, lens)).reshape(len(lens), kv_heads, group, HEAD)
+    qv, worst = vals(q).reshape(len(lens), kv_heads, group, HEAD), 0.0
+    for s, n in enumerate(lens):
+        page = c.table[s, np.arange(n) // PAGE]
+        for h in range(kv_heads):
+            k, v, w = flat_weights(c, qv[s, h], s, h, n, scale)
+            e = R.powers(c.scales[page, h, PAGE + np.arange(n) % PAGE])[:, None]
+            tol = flat_tolerance(v, w, qv[s, h], k, scale, 1) + 2.0 ** -134 * (1 + (np.abs(v) / e).sum(0) / w.sum(-1, keepdims=True))
+            off = np.abs(got[s, h] - w @ v / w.sum(-1, keepdims=True))
+            worst = max(worst, float((off / tol).max()))
+            assert (off <= tol).all(), f"sequence {s} of {n} keys, kv head {h}: {(off / tol).max()} of the tolerance"
+    print(f"MEASURE kv8 attention, values around 2^{power}: worst {worst:.3f} of the tolerance")
