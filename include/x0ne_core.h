@@ -238,10 +238,11 @@ x0ne_status x0ne_gpu_kv8_write(x0ne_gpu* g, const x0ne_kv8* c, uint64_t qkv, uin
    or past its length are zero; pages past it, and entries of out_pool or more, are left alone. */
 x0ne_status x0ne_gpu_kv8_read(x0ne_gpu* g, const x0ne_kv8* c, uint64_t lens, uint64_t k, uint64_t v, uint64_t out_table,
                               uint32_t out_pool);
-/* Bytes of the workspace of x0ne_gpu_kv8_attention and _select for this cache (0 where they refuse
-   it): 256-byte aligned, zeroed once before its first call and left ready for the next one by each,
-   whatever that one's cache. Calls that share it must not overlap (those of one Gpu, and its graphs,
-   run one after the other). */
+/* Bytes of the workspace of x0ne_gpu_kv8_attention and _select for a cache of these numbers (its
+   addresses are not looked at; 0 where the calls refuse the numbers, but for _select's own limit of
+   seq_pages): 256-byte aligned, zeroed once before its first call and left ready for the next one by
+   each, whatever that one's cache. Calls that share it must not overlap (those of one Gpu, and its
+   graphs, run one after the other). */
 uint64_t x0ne_kv8_work_bytes(const x0ne_kv8* c, uint32_t q_heads);
 /* Decode attention of one query per sequence: out [seqs][q_heads 128] bf16 = softmax(scale q k) v over
    the keys below lens[s] (u32; at most its pages'), q [seqs][q_heads 128] bf16 from the same layout,

@@ -105,3 +105,11 @@ def test_caches_of_all_shapes_have_their_counters_in_the_same_place():
     for kv_heads, seqs in [(1, 1), (8, 1), (8, 16), (8, 64), (2, 700), (1024, 64)]:
         size = [f(C.byref(_lib.Kv8C(16, 16, 16, 8, kv_heads, seqs, pages)), kv_heads) for pages in (1 << 20, 1 << 21)]
         assert size[0] - (size[1] - size[0]) == 4 * 65536, (kv_heads, seqs, size)
+
+
+def test_the_workspace_is_sized_before_the_cache_has_addresses():
+    from x0ne_core import _lib
+    f, numbers = _lib.lib().x0ne_kv8_work_bytes, (8, 2, 3, 4)
+    assert f(C.byref(_lib.Kv8C(0, 0, 0, *numbers)), 8) == f(C.byref(_lib.Kv8C(4096, 4096, 4096, *numbers)), 8) > 4 * 65536
+    for refused in [(0, 2, 3, 4), (8, 0, 3, 4), (8, 1025, 3, 4), (8, 2, 65536, 4), (8, 2, 3, 0), (8, 2, 3, 1 << 24)]:
+        assert f(C.byref(_lib.Kv8C(0, 0, 0, *refused)), 8) == 0, refused

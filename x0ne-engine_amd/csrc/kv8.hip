@@ -1134,15 +1134,20 @@ struct OnDevice {
 
 x0ne_status bad(const char* what, const std::string& why) { return fail(X0NE_ERR_FORMAT, std::string(what) + ": " + why); }
 
-x0ne_status check_cache(const char* what, const x0ne_kv8* c) {
+x0ne_status check_shape(const char* what, const x0ne_kv8* c) {
     if (!c) return bad(what, "no cache");
-    if (!c->codes || !c->scales || !c->page_table || c->codes % 16 || c->scales % 16 || c->page_table % 4)
-        return bad(what, "codes and scales (16-byte aligned) and page_table are required");
     if (c->pool == 0 || c->kv_heads == 0 || c->kv_heads > 1024 || c->seqs > 65535 || c->seq_pages == 0 ||
         c->seq_pages >= (1u << 24))
         return bad(what, std::to_string(c->pool) + " pages of " + std::to_string(c->kv_heads) + " kv heads, " +
                              std::to_string(c->seqs) + " sequences of " + std::to_string(c->seq_pages) +
                              " pages (1 to 1024 kv heads, up to 65535 sequences, 1 to 2^24 - 1 pages)");
+    return X0NE_OK;
+}
+
+x0ne_status check_cache(const char* what, const x0ne_kv8* c) {
+    X0NE_TRY(check_shape(what, c));
+    if (!c->codes || !c->scales || !c->page_table || c->codes % 16 || c->scales % 16 || c->page_table % 4)
+        return bad(what, "codes and scales (16-byte aligned) and page_table are required");
     return X0NE_OK;
 }
 
@@ -1152,7 +1157,6 @@ x0ne_status check_heads(const char* what, const x0ne_kv8* c, uint32_t q_heads) {
                              " kv heads (1 to 16 per kv head)");
     return X0NE_OK;
 }
-
 
 Table whole_table(const x0ne_kv8* c) {
     return Table{(const uint32_t*)c->page_table, c->seqs, c->seq_pages, c->pool, c->kv_heads};
@@ -1235,7 +1239,7 @@ static Table table_of(const x0ne_kv8* c, uint64_t first) {  // of a launch's seq
 }
 
 extern "C" uint64_t x0ne_kv8_work_bytes(const x0ne_kv8* c, uint32_t q_heads) {
-    if (check_cache("kv8 workspace", c) != X0NE_OK || check_heads("kv8 workspace", c, q_heads) != X0NE_OK) return 0;
+    if (check_shape("kv8 workspace", c) != X0NE_OK || check_heads("kv8 workspace", c, q_heads) != X0NE_OK) return 0;
     const uint64_t states = (uint64_t)c->seqs * q_heads * cut_of(c).slices * STATE * 4;
     const uint64_t scores = (uint64_t)c->seqs * c->kv_heads * c->seq_pages * 8;
     return COUNTER_BYTES + std::max(states, scores);

@@ -424,7 +424,8 @@ impl Gpu {
         check(unsafe { sys::x0ne_gpu_kv8_read(self.h.0, c, lens, k, v, out_table, out_pool) })
     }
 
-    /// Bytes of the zeroed workspace of `kv8_attention` and `kv8_select`; 0 for a cache they refuse.
+    /// Bytes of the zeroed workspace of `kv8_attention` and `kv8_select`, by the cache's numbers (its addresses
+    /// may still be 0); 0 for numbers they refuse.
     pub fn kv8_work_bytes(c: &sys::x0ne_kv8, q_heads: u32) -> u64 {
         // SAFETY: reads the cache's numbers only.
         unsafe { sys::x0ne_kv8_work_bytes(c, q_heads) }

@@ -228,7 +228,8 @@ class Gpu:
         check(lib().x0ne_gpu_kv8_read(self.h, cache, lens, k, v, out_table, out_pool), "kv8_read")
 
     def kv8_work_bytes(self, cache: Kv8, q_heads: int) -> int:
-        """Bytes of the zeroed workspace of kv8_attention and kv8_select; 0 for a cache they refuse."""
+        """Bytes of the zeroed workspace of kv8_attention and kv8_select, by the cache's numbers (its addresses may still be
+        0); 0 for numbers they refuse."""
         return lib().x0ne_kv8_work_bytes(cache, q_heads)
 
     def kv8_attention(self, cache: Kv8, q: int, q_heads: int, lens: int, out: int, scale: float, work: int, work_bytes: int,

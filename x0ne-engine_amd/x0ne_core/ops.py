@@ -1106,7 +1106,7 @@ class Kernels:
         """x0ne_gpu_kv8_attention, `calls` times over one workspace: out [seqs][q_heads][128] bf16 bits of the last."""
         seqs = pages.table.shape[0]
         n = seqs * q_heads * HEAD_DIM
-        size = self.gpu.kv8_work_bytes(Kv8(16, 16, 16, pages.pool, pages.kv_heads, *pages.table.shape), q_heads)
+        size = self.gpu.kv8_work_bytes(Kv8(0, 0, 0, pages.pool, pages.kv_heads, *pages.table.shape), q_heads)
         extra = {"q": np.asarray(q, np.uint16), "lens": np.asarray(lens, np.uint32), "work": np.zeros(size, np.uint8),
                  "out": np.full(n, self.SENTINEL, np.uint16)}
         if page_list is not None:
@@ -1123,7 +1123,7 @@ class Kernels:
         """x0ne_gpu_kv8_select, `calls` times over one workspace: the page list [seqs][kv_heads][budget] (uint32)."""
         seqs = pages.table.shape[0]
         n = seqs * pages.kv_heads * budget
-        size = self.gpu.kv8_work_bytes(Kv8(16, 16, 16, pages.pool, pages.kv_heads, *pages.table.shape), q_heads)
+        size = self.gpu.kv8_work_bytes(Kv8(0, 0, 0, pages.pool, pages.kv_heads, *pages.table.shape), q_heads)
         extra = {"q": np.asarray(q, np.uint16), "lens": np.asarray(lens, np.uint32), "work": np.zeros(size, np.uint8),
                  "bounds": np.asarray(bounds, np.uint16), "list": np.full(n, 0xA5A5A5A5, np.uint32)}
         a, kv, s = self._kv8(pages, extra)
