@@ -1038,10 +1038,18 @@ __global__ void __launch_bounds__(SELECT_THREADS)
     const uint32_t lane = i & 63, wave = __builtin_amdgcn_readfirstlane(i >> 6), n = lane & 15, g = lane >> 4;
     const size_t pair = (size_t)s * t.kv_heads + kh;
     uint32_t* to = list + pair * budget;
-    // What is needed of memory is requested at once: the length, the queries, the table's entries, whatever the length.
-    // Queries past the group repeat its last one, which leaves the maximum as it is.
     const uint32_t first = blockIdx.y * SELECT_PAGES;
     const uint32_t pages = (kv8_keys(lens[s], t.seq_pages) + KV8_PAGE - 1) / KV8_PAGE;
+    if (pages <= budget || budget == 1) {
+        if (blockIdx.y == 0)
+            for (uint32_t j = i; j < budget; j += SELECT_THREADS) to[j] = j >= pages ? KV8_NONE : budget == 1 ? pages - 1 : j;
+        return;
+    }
+    const uint32_t scored = pages - 1;
+    if (first >= scored) return;
+    // Behind the length, the table's entries and the first queries at once; behind the entries, the bounds. Nothing is
+    // read for pages past the sequence's block of 64: a table may be far wider than its sequence. Queries past the group
+    // repeat its last one, which leaves the maximum as it is.
     auto entry_at = [&](uint32_t p) { return t.pages[(size_t)s * t.seq_pages + min(p, t.seq_pages - 1)]; };
     uint32_t entry[4];
 #pragma unroll
@@ -1056,13 +1064,6 @@ __global__ void __launch_bounds__(SELECT_THREADS)
         lo[j] = b[0];
         hi[j] = b[KV8_HEAD / 8];
     }
-    if (pages <= budget || budget == 1) {
-        if (blockIdx.y == 0)
-            for (uint32_t j = i; j < budget; j += SELECT_THREADS) to[j] = j >= pages ? KV8_NONE : budget == 1 ? pages - 1 : j;
-        return;
-    }
-    const uint32_t scored = pages - 1;
-    if (first >= scored) return;
     uint64_t best = 0;
 #pragma unroll 1
     for (uint32_t h = 0; h < group; h += 4) {
