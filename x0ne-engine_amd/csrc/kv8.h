@@ -80,16 +80,25 @@ KV8_BOTH void kv8_narrow(uint64_t& lo, uint64_t& hi, int shift, uint32_t bin) {
 // each of a block's `waves` wavefronts), over `blocks` blocks for each kv head and 64 sequences.
 //  - Few pairs of sequence and kv head: slices for one block on each of 256 CUs; more bring more states to join than
 //    overlap gains (us, 32768 keys, 8 pairs, blocks of 4, 16 / 32 / 64 slices: 27.2 / 21.7 / 26.8).
-//  - Many: blocks that fill the card walk the slices, longest first. A slice of one round costs about four (its lookups,
-//    states and count are not hidden), so slices are two thirds of what a block has to do if every sequence fills its
-//    table (64 sequences of up to 6000 keys, blocks of 8, 2 / 4 / 8 / 12 rounds: 108 / 95 / 87 / 77; 16 of up to 8192,
-//    3 / 4 / 5 / 6 / 8: 44 / 47 / 37 / 38 / 44), up to 16, and fewer for fewer pairs, whose lengths may be far below
-//    their tables'.
+//  - Many: blocks that fill the card walk the slices, longest first. A slice of one round costs about four (its lookups
+//    are waited for, its states and count are not hidden), so slices are two thirds of what a block has to do if every
+//    sequence fills its table, or 8192 positions of it (pairs / 24), and up to 16: known before the lengths are, and the
+//    same under tables far wider than the sequences (16 sequences of up to 8192 keys 35 us under 513, 2048 and 8192 pages;
+//    16 rounds 67). An estimate: where the slices happen to fill the blocks evenly, fewer or more rounds are faster. us
+//    by rounds, 8 kv heads, lengths spread evenly up to 8192, the estimate's in brackets:
+//      rounds           2     3     4     5     6     8    12    16
+//       8 sequences  [25.7]  18.5  19.7  22.0  24.4  29.1  36.8  46.5
+//      13             33.9   38.1 [36.1] 30.7  32.7  37.2  43.2  57.0
+//      16             46.3   41.7  44.6 [35.0] 36.7  42.5  53.2  66.8
+//      20             47.9   47.1  50.1  49.7 [55.8] 44.8  54.9  68.0
+//      32 ([10] 67.3) 75.5   70.3  70.0  63.5  66.3  68.8  63.7  74.5
+//    and it does not see one long sequence among short ones: 32768 keys among 63 of 200 under 2048 pages takes 16 rounds, 4
+//    slices, and 77.7 us; 4 rounds 36.5.
 //  - Blocks of 8 wavefronts, one on a CU, join fewer states than two of 4 and start fewer slices (us with 4 / 8: 32768
 //    keys 21.1 / 19.0, 64 sequences 84 / 73, 16 sequences 35 / 35); where the pages, all attended, are less than two
 //    rounds of 8 for each CU, 4 (128 pages for each of 8 pairs, with their selection, 21.9 / 24.1).
-//  - Loads of more than the Infinity Cache holds bypass it (64 sequences of up to 6000 keys 76.6 -> 72.9 us); 67 MB, read
-//    again before 256 MB of others, come from it (32768 keys 19 us with it, 22 without).
+//  - Loads of more than the Infinity Cache holds, by the tables' width, bypass it (64 sequences of up to 6000 keys 76.6 ->
+//    72.9 us); 67 MB, read again before 256 MB of others, come from it (32768 keys 19 us with it, 22 without).
 constexpr uint64_t KV8_STREAM = 256ull << 20;  // the Infinity Cache's bytes
 constexpr uint32_t KV8_TILE = 4;               // pages of a wavefront's tile
 constexpr uint32_t KV8_SLICES = 64;            // the most slices of a sequence

@@ -199,7 +199,8 @@ __device__ __forceinline__ void put_bounds(u32x2 w, uint32_t byte, bf16_t* to, K
 // page: the arithmetic of x0ne_qk_norm_rope_kv_write_rows_bf16, so q_out has its bits and the codes are those of its k
 // row. A block takes 16 rows, 16 lanes to a row, and by blockIdx.y
 //  - HEADS heads of q, or of k behind those: their loads are all requested at once, cos and sin are read once, and the
-//    f64 square roots and divisions are one for all (lane i computes head i's);
+//    f64 square roots and divisions are one for all (lane i computes head i's). Of k, and of values, the page lookups of a
+//    thread's row and of row n (to tell a whole page) come one after the other, each waited for, behind those loads;
 //  - then the values of WRITE_VALUES kv heads, turned dim-major in LDS: where the block's rows are one whole page, as in
 //    a prompt, that is stored as such, else byte by byte.
 // A row of no sequence, or past the sequence's pages or the rope table, writes nothing.
@@ -489,8 +490,9 @@ struct Shared {
 };
 
 // The slices' states of a group's heads joined, in slice order within each part: a thread has four dims of one head
-// and, for a group of at most 4 heads, every second, fourth .. slice (the parts meet in LDS). All of a thread's
-// loads of up to JOIN_AHEAD slices are requested before the maxima are known, so they cost one round trip.
+// and, where a group's 32 threads a head are at most a quarter or half of the block (2 and 4 heads for 4 wavefronts, 4 and 8
+// for 8), every fourth or second slice (the parts meet in LDS). All of a thread's loads of up to JOIN_AHEAD slices are
+// requested before the maxima are known, so they cost one round trip.
 constexpr uint32_t JOIN_AHEAD = 8;
 template <uint32_t WAVES>
 __device__ __forceinline__ void join(const Attend& a, const float* __restrict__ st, bf16_t* __restrict__ out,
@@ -545,7 +547,7 @@ __device__ __forceinline__ void join(const Attend& a, const float* __restrict__ 
         *reinterpret_cast<uint2*>(out + 4 * e) = make_uint2(pack(x[0] * r, x[1] * r), pack(x[2] * r, x[3] * r));
     };
     if (parts == 1) {
-        for (uint32_t e = first; e < quads; e += THREADS) store(e, sum(e));  // twice for more than 8 heads
+        for (uint32_t e = first; e < quads; e += THREADS) store(e, sum(e));  // twice for more than 8 heads of 4 wavefronts
         return;
     }
     float* mine = &sh.wo[0][0][0] + 4 * t;
@@ -576,12 +578,15 @@ struct Item {
 //    page g, and with the value of dim 16 c + n at those keys as row n of product c (one 16-byte load: V is dim-major)
 //    the weights are an operand as they lie, without a move between lanes.
 //  - Dims of a product's k step j are 32 g + 8 j ..: a lane's keys come as two 16-byte loads.
-//  - Weights enter as bf16 hi + lo (2^-17 of the weight): one bf16 would add as much error as the output's rounding.
+//  - Weights enter as bf16 hi + lo (2^-17 of the weight, 2^-134 where its value's power of two is tiny): one bf16 would add
+//    as much error as the output's rounding. Their sum takes them whole.
 // The next tile's keys are requested behind the scores, its values behind the value products; the next slice's first
-// tile and queries likewise, so the memory is busy while a slice's states are joined. The running maximum and sum are
-// f32. A slice's state (m, l, o) is joined by the last block of its (sequence, kv head) to count itself, slices in
-// order; a sequence of one slice is written at once. Keys past the length, entries behind a list and pages that are
-// not there weigh 0, their values are taken as 0.
+// tile and queries likewise, so the memory is busy while a slice's states are joined. It is not at a slice's start: the
+// list and table entries of the slice after it are waited for there, one behind the other, and with them this slice's
+// first tile, before its first product. The running maximum and sum are f32, and the sums of weighted values, not yet
+// divided: values near bf16's largest over several keys pass f32. A slice's state (m, l, o) is joined by the last block
+// of its (sequence, kv head) to count itself, slices in order; a sequence of one slice is written at once. Keys past the
+// length, entries behind a list and pages that are not there weigh 0, their values are taken as 0.
 template <uint32_t WAVES, bool STREAM>
 __global__ void __launch_bounds__(64 * WAVES, 2) kv8_attention_kernel(const Attend a) {
     constexpr uint32_t THREADS = 64 * WAVES;
