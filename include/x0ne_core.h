@@ -249,8 +249,8 @@ uint64_t x0ne_kv8_work_bytes(const x0ne_kv8* c, uint32_t q_heads);
    q head h reading kv head h / (q_heads / kv_heads), 1 to 16 q heads per kv head. Scores, softmax and
    sums in f32; a weight times the scale of its value enters the products as two bf16 parts (2^-17 of
    it), and weighted values are summed before they are divided (values near bf16's largest over several
-   keys give infinities). A sequence without keys gives zeros; out may be q. page_list (0, with budget 0:
-   every page): [seqs][kv_heads][budget] u32, the logical pages that the queries of a kv head attend:
+   keys give infinities or NaN). A sequence without keys gives zeros; out may be q. page_list (0, with
+   budget 0: every page): [seqs][kv_heads][budget] u32, the logical pages that the queries of a kv head attend:
    the first min(budget, pages of the sequence) entries, each page once, entries past the sequence's
    pages skipped. A row's bits depend on the sequence itself and the seqs, seq_pages, heads and budget of the
    call, not on the other sequences. */

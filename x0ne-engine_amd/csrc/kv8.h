@@ -85,13 +85,14 @@ KV8_BOTH void kv8_narrow(uint64_t& lo, uint64_t& hi, int shift, uint32_t bin) {
 //    sequence fills its table, or 8192 positions of it (pairs / 24), and up to 16: known before the lengths are, and the
 //    same under tables far wider than the sequences (16 sequences of up to 8192 keys 35 us under 513, 2048 and 8192 pages;
 //    16 rounds 67). An estimate: where the slices happen to fill the blocks evenly, fewer or more rounds are faster. us
-//    by rounds, 8 kv heads, lengths spread evenly up to 8192, the estimate's in brackets:
+//    by rounds, 8 kv heads, lengths spread evenly up to 8192 (64: 6000), the estimate's in brackets:
 //      rounds           2     3     4     5     6     8    12    16
 //       8 sequences  [25.7]  18.5  19.7  22.0  24.4  29.1  36.8  46.5
 //      13             33.9   38.1 [36.1] 30.7  32.7  37.2  43.2  57.0
 //      16             46.3   41.7  44.6 [35.0] 36.7  42.5  53.2  66.8
 //      20             47.9   47.1  50.1  49.7 [55.8] 44.8  54.9  68.0
 //      32 ([10] 67.3) 75.5   70.3  70.0  63.5  66.3  68.8  63.7  74.5
+//      64            107.6   99.7  94.1  97.0  92.5  86.3  72.7 [72.6]
 //    and it does not see one long sequence among short ones: 32768 keys among 63 of 200 under 2048 pages takes 16 rounds, 4
 //    slices, and 77.7 us; 4 rounds 36.5.
 //  - Blocks of 8 wavefronts, one on a CU, join fewer states than two of 4 and start fewer slices (us with 4 / 8: 32768
