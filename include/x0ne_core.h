@@ -266,6 +266,63 @@ x0ne_status x0ne_gpu_kv8_attention(x0ne_gpu* g, const x0ne_kv8* c, uint64_t q, u
 x0ne_status x0ne_gpu_kv8_select(x0ne_gpu* g, const x0ne_kv8* c, uint64_t bounds, uint64_t q, uint32_t q_heads,
                                 uint64_t lens, uint32_t budget, uint64_t page_list, uint64_t work, uint64_t work_bytes);
 
+/* ---- weights in 4 bits: no counterpart in the reference, whose weights are bf16 ----
+   A group of 32, 64 or 128 consecutive weights w of a row is held as e2m1 codes (magnitudes 0, .5, 1,
+   1.5, 2, 3, 4, 6 as codes 0 to 7, the sign in bit 3) of w / s and one bf16 scale s, the nearest to
+   max |w| / 6 and at least 2^-126; a code is the nearest to w / s, the even one of two as near. A group
+   with a weight that is not finite has the scale NaN. The last group of a row may be shorter. Device
+   addresses, 16-byte aligned: codes [ceil(rows / 16)][ceil(cols / 128)] tiles of 1 KiB, [4 q][16 rows]
+   [4 s][4 b], byte b the columns 32 s + 8 q + 2 b (low 4 bits) and the next of a tile; scales
+   [ceil(rows / 16)][ceil(cols / 128)][16 rows][128 / group] bf16. Rows and columns past the matrix are
+   held as weights of 0. 4 + 16 / group bits for a weight instead of 16. (OCP MXFP4 is such a form:
+   groups of 32 whose scales are powers of two.) rows and cols 1 to 2^24, cols a multiple of 8, else
+   X0NE_ERR_FORMAT, as for a required address that is 0 or not aligned as stated. The calls run on the
+   Gpu's stream, allocate nothing, and may be captured into a graph. */
+typedef struct {
+    uint64_t codes, scales;
+    uint32_t rows, cols, group;
+    uint32_t reserved; /* 0 */
+} x0ne_w4;
+/* Bytes of the codes and of the scales of a matrix of these numbers (its addresses are not looked at;
+   0 where the calls refuse the numbers). */
+uint64_t x0ne_w4_code_bytes(const x0ne_w4* w);
+uint64_t x0ne_w4_scale_bytes(const x0ne_w4* w);
+/* Brings a row-major bf16 matrix [rows][cols] (16-byte aligned) into 4 bits. */
+x0ne_status x0ne_gpu_w4_quantise(x0ne_gpu* g, const x0ne_w4* w, uint64_t from);
+/* What the codes stand for, bf16(code s), row-major [rows][cols] (16-byte aligned): the layout that
+   x0ne_gpu_gemv takes, which serves the many rows of a prompt. */
+x0ne_status x0ne_gpu_w4_read(x0ne_gpu* g, const x0ne_w4* w, uint64_t to);
+/* Y = X W^T, X [n][cols] bf16 row-major (16-byte aligned): products and sums in f32, a group's sum
+   times its scale, rounded once. out X0NE_W4_BF16, X0NE_W4_F32: Y [n][rows]; X0NE_W4_SWIGLU: W is
+   [gate; up] (rows a multiple of 32) and Y [n][rows / 2] bf16 = silu(gate) up of the f32 sums. Y is
+   4-byte aligned and not in X. n up to 65535 x 16; X below 4 GiB. The same call gives the same bits. */
+enum { X0NE_W4_BF16 = 0, X0NE_W4_F32 = 1, X0NE_W4_SWIGLU = 2 };
+x0ne_status x0ne_gpu_w4_gemv(x0ne_gpu* g, const x0ne_w4* w, uint64_t x, uint64_t n, uint64_t y, uint32_t out);
+
+/* ---- log probabilities: no counterpart in the reference beside the engine's run ----
+   Of rows of logits l, f32 or bf16 (bf16 = 1), row r at logits + r stride elements, vocab of them: with
+   x = scale l, log p = x - log sum e^x. Device addresses; what is 0 is not computed.
+   tokens [rows][per_row] u32: token_lp [rows][per_row] f32 their log p, NaN for an id of vocab or more.
+   entropy [rows] f32: - sum p log p (a p of 0 adds 0).
+   top (0 to 64): top_ids [rows][top] u32 the ids of the largest logits, falling, the lower id first of
+   equal ones, top_lp [rows][top] f32 their log p. Logits of -infinity are no alternatives: behind the
+   last one stand 0xFFFFFFFF and -infinity. A row with NaN or +infinity (also as scale l), or with nothing
+   above -infinity, has no distribution: NaN and 0xFFFFFFFF throughout. f32 arithmetic.
+   work: 256-byte aligned, x0ne_logprobs_work_bytes of it, zeroed once before its first call and left
+   ready for the next by each; calls of all shapes, and those of the 8-bit cache, may share it in turn.
+   Up to 2^24 rows, logits of a row and tokens to a row, stride below 2^32, logits aligned to one, other
+   addresses to 4 bytes, scale positive and finite, else X0NE_ERR_FORMAT. A call of no rows does nothing.
+   It runs on the Gpu's stream, allocates nothing, and may be captured into a graph. */
+typedef struct {
+    uint64_t logits, stride, tokens, token_lp, entropy, top_ids, top_lp, work, work_bytes;
+    uint32_t rows, vocab, per_row, top, bf16;
+    float scale;
+} x0ne_logprobs;
+/* Bytes of the workspace of a call of these numbers (its addresses are not looked at; 0 where the call
+   refuses the numbers). */
+uint64_t x0ne_logprobs_work_bytes(const x0ne_logprobs* d);
+x0ne_status x0ne_gpu_logprobs(x0ne_gpu* g, const x0ne_logprobs* d);
+
 /* Graph capture (gpu.rs:1170-1238): every launch between begin and end is recorded, then
    replayed by x0ne_gpu_launch_graph on the Gpu that captured it (another Gpu is refused with
    X0NE_ERR_GPU, gpu.rs:1225-1230). */

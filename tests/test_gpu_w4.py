@@ -1,0 +1,196 @@
+"""Weights in 4 bits (x0ne_gpu_w4_*) against their plain 64-bit form (w4_reference.py): codes, scales and the read-back
+bit for bit, products within a derived tolerance, and bit for bit where every sum is exact."""
+import numpy as np
+import pytest
+
+import w4_reference as R
+from w4_reference import bits, vals
+
+pytestmark = pytest.mark.gpu
+
+
+def trained(rng, rows, cols):
+    """Weights of uneven rows and a few far values."""
+    w = rng.standard_normal((rows, cols)) * 0.02 * (0.5 + rng.random((rows, 1)))
+    return bits(np.where(rng.random((rows, cols)) < 0.002, 8.0 * w, w))
+
+
+# -- the form --
+
+def check_form(kernels, w, group):
+    rows, cols = w.shape
+    code, s = R.quantise(vals(w), group)
+    want_codes, want_scales = R.lay(code, s)
+    codes, scales = kernels.w4_quantise(w, group)
+    bad = np.isnan(vals(want_scales))
+    assert (np.isnan(vals(scales)) == bad).all() and (scales[~bad] == want_scales[~bad]).all()
+    # A zero's sign is not stated.
+    flat = lambda c: np.stack([np.where(h == 8, 0, h) for h in (c & 15, c >> 4)])
+    assert (flat(codes) == flat(want_codes)).all(), f"{int((flat(codes) != flat(want_codes)).sum())} codes differ"
+    got, want = kernels.w4_read(codes, scales, rows, cols, group), R.values(code, s)[:rows, :cols]
+    nan = np.isnan(want)
+    assert (np.isnan(vals(got)) == nan).all() and (vals(got)[~nan] == vals(bits(want))[~nan]).all()
+    return codes, scales
+
+
+@pytest.mark.parametrize("rows,cols", [(1, 8), (16, 128), (15, 120), (17, 136), (33, 1000), (1000, 1096), (70, 2056)])
+@pytest.mark.parametrize("group", [32, 64, 128])
+def test_matrices_of_all_sizes(kernels, rows, cols, group):
+    check_form(kernels, trained(np.random.default_rng(rows + cols + group), rows, cols), group)
+
+
+@pytest.mark.parametrize("group", [32, 64, 128])
+def test_weights_of_all_sizes(kernels, group):
+    """Every bf16 pattern, infinities and NaN among them, in groups of its own size and in groups of all sizes; groups of
+    zeros of both signs; the smallest and the largest."""
+    rng = np.random.default_rng(group)
+    every = np.arange(1 << 16).astype(np.uint16).reshape(256, 256)
+    check_form(kernels, every, group)
+    check_form(kernels, rng.permutation(every.ravel()).reshape(256, 256), group)
+    finite = every.ravel()[np.isfinite(vals(every.ravel()))]
+    check_form(kernels, rng.permutation(finite)[:256 * 248].reshape(256, 248), group)
+    ends = rng.choice(np.array([0, 0x8000, 1, 0x8001, 0x7F, 0x80, 0x7F7F, 0xFF7F], np.uint16), (48, 256))
+    check_form(kernels, ends, group)
+    check_form(kernels, np.where(rng.random((16, 256)) < 0.5, 0x8000, 0).astype(np.uint16), group)
+
+
+@pytest.mark.parametrize("group", [32, 64, 128])
+def test_weights_at_the_middles_of_codes(kernels, group):
+    """Scales of 8 bits whose group's weights are middles of codes times it where those are bf16, and their neighbours."""
+    rng = np.random.default_rng(group + 1)
+    middles = (R.GRID[1:] + R.GRID[:-1]) / 2
+    rows = []
+    for s in rng.choice(np.arange(128, 256), 64, replace=False):
+        row = bits(rng.choice(np.concatenate([middles, R.GRID]), 128) * s / 64).astype(np.int64) + rng.integers(-1, 2, 128)
+        row = np.maximum(row, 0)
+        row[::group] = bits(np.array([6.0 * s / 64]))[0]
+        rows.append(row)
+    w = np.array(rows).astype(np.uint16)
+    check_form(kernels, np.where(rng.random(w.shape) < 0.5, w | 0x8000, w).astype(np.uint16), group)
+
+
+# -- products --
+
+def held(rng, rows, cols, group):
+    """Random codes and scales of uneven size: (codes, scales as they lie, their values)."""
+    code = np.zeros((-(-rows // 16) * 16, -(-cols // 128) * 128), np.int64)
+    code[:rows, :cols] = rng.integers(0, 16, (rows, cols))
+    s = vals(bits(np.exp(rng.standard_normal((code.shape[0], code.shape[1] // group))) * 0.01))
+    return (*R.lay(code, s), R.values(code, s)[:rows, :cols])
+
+
+def silu(x):
+    return x / (1.0 + np.exp(-x))
+
+
+def check_product(w, x, y, out, group):
+    """Each f32 sum within one rounding of 2^-23 (an addition that truncates) for each addition of its longest chain: the
+    32 products of an instruction and the instructions of a group, the groups of a wavefront's tiles, the wavefronts.
+    Then 2^-8 for a rounding to bf16, and for SwiGLU the sums' errors through a slope of at most 1.1, and 8 roundings."""
+    chain = (group + w.shape[1] // 32 + 32) * 2.0 ** -23
+    want, size = x @ w.T, np.abs(x) @ np.abs(w).T
+    tol = chain * size
+    if out == "swiglu":
+        h = w.shape[0] // 2
+        gate, up, dg, du = want[:, :h], want[:, h:], tol[:, :h], tol[:, h:]
+        want = silu(gate) * up
+        tol = 1.1 * dg * (np.abs(up) + du) + np.abs(silu(gate)) * du + 8 * 2.0 ** -24 * np.abs(want)
+    if out != "f32":
+        tol = tol * (1 + 2.0 ** -8) + 2.0 ** -8 * np.abs(want)
+        y = vals(y)
+    worst = (np.abs(y - want) / (tol + 1e-30)).max()
+    print(f"MEASURE w4 product {w.shape} x {len(x)} {out}: worst {worst:.3f} of the tolerance")
+    assert worst <= 1.0
+
+
+@pytest.mark.parametrize("out", ["bf16", "f32", "swiglu"])
+@pytest.mark.parametrize("group", [32, 64, 128])
+@pytest.mark.parametrize("rows,cols,n", [(32, 8, 1), (32, 128, 1), (96, 1000, 2), (64, 2048, 3), (160, 4104, 5), (4096, 1024, 1),
+                                         (544, 640, 16), (544, 648, 17), (288, 1992, 31), (96, 1096, 33), (64, 512, 64), (96, 264, 65),
+                                         (32, 136, 200)])
+def test_products(kernels, rows, cols, n, group, out):
+    rng = np.random.default_rng(rows + cols + n + group)
+    codes, scales, w = held(rng, rows, cols, group)
+    x = bits(rng.standard_normal((n, cols)) * np.where(rng.random(cols) < 0.02, 20.0, 1.0))
+    check_product(w, vals(x), kernels.w4_gemv(codes, scales, rows, cols, group, x, out), out, group)
+
+
+@pytest.mark.parametrize("out", ["bf16", "f32"])
+@pytest.mark.parametrize("rows,n", [(1, 1), (1, 64), (15, 4), (17, 1), (31, 16), (1000, 9), (2049, 61)])
+def test_products_of_uneven_rows(kernels, rows, n, out):
+    rng = np.random.default_rng(rows + n)
+    codes, scales, w = held(rng, rows, 520, 64)
+    x = bits(rng.standard_normal((n, 520)))
+    check_product(w, vals(x), kernels.w4_gemv(codes, scales, rows, 520, 64, x, out), out, 64)
+
+
+@pytest.mark.parametrize("rows,cols,n", [(5120, 25600, 16), (24576, 4096, 1), (20000, 2048, 40), (6144, 4096, 64), (1024, 16384, 7)])
+def test_products_of_large_matrices(kernels, rows, cols, n):
+    """A sample of the rows, and all of them against the read-back by a long f32 sum on the host."""
+    rng = np.random.default_rng(rows + n)
+    codes, scales, w = held(rng, rows, cols, 128)
+    x = bits(rng.standard_normal((n, cols)))
+    y = kernels.w4_gemv(codes, scales, rows, cols, 128, x, "f32")
+    check_product(w, vals(x), y, "f32", 128)
+
+
+@pytest.mark.parametrize("rows,cols,n,group", [(32, 8, 1, 32), (64, 1160, 1, 32), (64, 4096, 2, 64), (2080, 640, 16, 128), (48, 2000, 23, 32),
+                                               (8256, 384, 37, 64), (16, 25600, 5, 32), (6144, 1024, 64, 128), (70000, 256, 3, 32)])
+def test_products_whose_sums_are_exact(kernels, rows, cols, n, group):
+    """Whole x up to 7, codes whole multiples of .5 and scales 1, 2 and 4: every sum is exact in f32 (below 2^24 halves),
+    so that each weight, scale and x shows in its place."""
+    rng = np.random.default_rng(rows + cols + n)
+    code = np.zeros((-(-rows // 16) * 16, -(-cols // 128) * 128), np.int64)
+    code[:rows, :cols] = rng.integers(0, 16, (rows, cols))
+    s = 2.0 ** rng.integers(0, 3, (code.shape[0], code.shape[1] // group))
+    x = rng.integers(-7, 8, (n, cols)).astype(np.float64)
+    assert 7 * 6 * 4 * 2 * cols < 1 << 24
+    codes, scales = R.lay(code, s)
+    y = kernels.w4_gemv(codes, scales, rows, cols, group, bits(x), "f32")
+    assert (y == x @ R.values(code, s)[:rows, :cols].T).all()
+
+
+@pytest.mark.parametrize("n", [1, 6, 20, 64])
+def test_infinities_and_nan_stay_in_their_rows(kernels, n):
+    """A token with an infinity or NaN, a group whose scale is NaN: only their own outputs show it."""
+    rng = np.random.default_rng(n)
+    rows, cols = 100, 1000
+    codes, scales, w = held(rng, rows, cols, 32)
+    code, s = R.quantise(vals(trained(rng, rows, cols)), 32)
+    s[7, 3] = np.nan
+    codes, scales = R.lay(code, s)
+    w = R.values(code, s)[:rows, :cols]
+    x = rng.standard_normal((n, cols))
+    if n > 1:
+        x[n // 2, 999], x[n - 1, 0] = np.nan, np.inf
+    x = vals(bits(x))
+    y = kernels.w4_gemv(codes, scales, rows, cols, 32, bits(x), "f32")
+    fine_rows, fine_tokens = np.arange(rows) != 7, np.isfinite(x).all(1)
+    assert np.isnan(y[:, 7]).all() and np.isfinite(y[fine_tokens][:, fine_rows]).all()
+    if n > 1:
+        assert np.isnan(y[n // 2]).all() and not np.isfinite(y[n - 1]).any()
+    check_product(w[fine_rows], x[fine_tokens], y[fine_tokens][:, fine_rows], "f32", 32)
+
+
+def test_swiglu_of_far_gates(kernels):
+    """Gates of -3e4 to 3e4 and -0: silu(gate) up without an infinity or NaN."""
+    gates = np.array([-30000.0, -200.0, -104.0, -88.5, -50.0, -1e-3, 0.0, 1e-3, 50.0, 88.5, 200.0, 30000.0, 1.0, 2.0, 3.0, 4.0])
+    code = np.zeros((32, 128), np.int64)
+    code[:16, 0], code[16:, 1] = 2, 2
+    codes, scales = R.lay(code, np.ones((32, 4)))
+    x = np.zeros((16, 128))
+    x[:, 0], x[:, 1] = gates, 1.5
+    x = vals(bits(x))
+    y = vals(kernels.w4_gemv(codes, scales, 32, 128, 32, bits(x), "swiglu"))
+    with np.errstate(over="ignore"):
+        want = silu(x[:, 0]) * 1.5
+    assert (np.abs(y - want[:, None]) <= 2.0 ** -7 * np.abs(want)[:, None] + 1e-37).all()
+
+
+@pytest.mark.parametrize("rows,cols,n,out", [(4096, 1024, 1, "bf16"), (2048, 2048, 33, "swiglu")])
+def test_the_same_call_gives_the_same_bits(kernels, rows, cols, n, out):
+    rng = np.random.default_rng(n)
+    codes, scales, _ = held(rng, rows, cols, 64)
+    x = bits(rng.standard_normal((n, cols)))
+    first = kernels.w4_gemv(codes, scales, rows, cols, 64, x, out)
+    assert (kernels.w4_gemv(codes, scales, rows, cols, 64, x, out, calls=5) == first).all()

@@ -19,6 +19,18 @@ x0ne_status fail(x0ne_status s, const std::string& msg);
 // X0NE_ERR_GPU with the runtime's error text, for a failed HIP call.
 x0ne_status gpu_fail(hipError_t e, const char* what);
 
+// The Gpu's device is current while a call launches, whatever the caller's is.
+struct OnDevice {
+    int before = -1;
+    explicit OnDevice(int device) {
+        int now = device;
+        if (hipGetDevice(&now) == hipSuccess && now != device && hipSetDevice(device) == hipSuccess) before = now;
+    }
+    ~OnDevice() {
+        if (before >= 0) (void)hipSetDevice(before);
+    }
+};
+
 struct Counts {
     std::atomic<uint64_t> launches{0}, graph_launches{0}, gemms{0}, htod{0}, dtoh{0}, memsets{0}, syncs{0};
 };

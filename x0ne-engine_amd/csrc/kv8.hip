@@ -1126,18 +1126,6 @@ __global__ void __launch_bounds__(SELECT_THREADS)
 
 // ---- host ----
 
-// The Gpu's device is current while a call launches, whatever the caller's is.
-struct OnDevice {
-    int before = -1;
-    explicit OnDevice(int device) {
-        int now = device;
-        if (hipGetDevice(&now) == hipSuccess && now != device && hipSetDevice(device) == hipSuccess) before = now;
-    }
-    ~OnDevice() {
-        if (before >= 0) (void)hipSetDevice(before);
-    }
-};
-
 x0ne_status bad(const char* what, const std::string& why) { return fail(X0NE_ERR_FORMAT, std::string(what) + ": " + why); }
 
 x0ne_status check_shape(const char* what, const x0ne_kv8* c) {

@@ -1,5 +1,5 @@
 //! The kernel-launch API of x0ne-core/runtime/src/gpu.rs over libx0ne_core.so: `Gpu::{new, launch,
-//! gemm, kv8_*, capture, launch_graph, split_plan, allocate, counts, mem_info, sync}`, `Arg`,
+//! gemm, kv8_*, w4_*, logprobs, capture, launch_graph, split_plan, allocate, counts, mem_info, sync}`, `Arg`,
 //! `check_args` and the `launch!` macro, with the reference's names, argument meanings and
 //! errors. The kernels are this library's gfx950 code; its table (x0ne_kernel_name,
 //! x0ne_kernel_params) stands for `x0ne_core_kernels::{KERNEL_NAMES, KERNEL_PARAMS}`, and every
@@ -459,6 +459,62 @@ impl Gpu {
         check(unsafe {
             sys::x0ne_gpu_kv8_select(self.h.0, c, bounds, q, q_heads, lens, budget, page_list, work, work_bytes)
         })
+    }
+
+    /// Bytes of the codes and of the scales of a matrix in 4 bits, by its numbers (its addresses may still be 0); 0
+    /// for numbers that the calls refuse.
+    pub fn w4_bytes(w: &sys::x0ne_w4) -> (u64, u64) {
+        // SAFETY: reads the matrix's numbers only.
+        unsafe { (sys::x0ne_w4_code_bytes(w), sys::x0ne_w4_scale_bytes(w)) }
+    }
+
+    /// A row-major bf16 matrix into 4 bits (`x0ne_gpu_w4_quantise`). No counterpart in the reference.
+    ///
+    /// # Safety
+    ///
+    /// Every address of `w` and of the arguments is device memory of this device of the size that
+    /// `include/x0ne_core.h` states, allocated until the call is done on the stream.
+    pub unsafe fn w4_quantise(&self, w: &sys::x0ne_w4, from: u64) -> Result<()> {
+        // SAFETY: a live device handle and matrix; the addresses are the caller's contract.
+        check(unsafe { sys::x0ne_gpu_w4_quantise(self.h.0, w, from) })
+    }
+
+    /// What the codes stand for as a row-major bf16 matrix (`x0ne_gpu_w4_read`).
+    ///
+    /// # Safety
+    ///
+    /// As [`Gpu::w4_quantise`].
+    pub unsafe fn w4_read(&self, w: &sys::x0ne_w4, to: u64) -> Result<()> {
+        // SAFETY: as w4_quantise.
+        check(unsafe { sys::x0ne_gpu_w4_read(self.h.0, w, to) })
+    }
+
+    /// Y = X W^T of `n` rows of X (`x0ne_gpu_w4_gemv`); `out` is `X0NE_W4_BF16` (0), `_F32` (1) or `_SWIGLU` (2).
+    ///
+    /// # Safety
+    ///
+    /// As [`Gpu::w4_quantise`].
+    pub unsafe fn w4_gemv(&self, w: &sys::x0ne_w4, x: u64, n: usize, y: u64, out: u32) -> Result<()> {
+        // SAFETY: as w4_quantise.
+        check(unsafe { sys::x0ne_gpu_w4_gemv(self.h.0, w, x, n as u64, y, out) })
+    }
+
+    /// Bytes of the zeroed workspace of `logprobs`, by the descriptor's numbers; 0 for numbers it refuses.
+    pub fn logprobs_work_bytes(d: &sys::x0ne_logprobs) -> u64 {
+        // SAFETY: reads the descriptor's numbers only.
+        unsafe { sys::x0ne_logprobs_work_bytes(d) }
+    }
+
+    /// Log probabilities of given tokens, entropy and top alternatives of rows of logits
+    /// (`x0ne_gpu_logprobs`).
+    ///
+    /// # Safety
+    ///
+    /// As [`Gpu::w4_quantise`], of the descriptor's addresses; `d.work` was zeroed before its first
+    /// call and no other call uses it meanwhile.
+    pub unsafe fn logprobs(&self, d: &sys::x0ne_logprobs) -> Result<()> {
+        // SAFETY: a live device handle and descriptor; the addresses are the caller's contract.
+        check(unsafe { sys::x0ne_gpu_logprobs(self.h.0, d) })
     }
 
     /// Captures every launch `f` issues on the stream into one graph and instantiates it

@@ -101,6 +101,37 @@ pub struct x0ne_kv8 {
 }
 
 #[repr(C)]
+#[derive(Clone, Copy, Default, Debug)]
+pub struct x0ne_w4 {
+    pub codes: u64,
+    pub scales: u64,
+    pub rows: u32,
+    pub cols: u32,
+    pub group: u32,
+    pub reserved: u32,
+}
+
+#[repr(C)]
+#[derive(Clone, Copy, Default, Debug)]
+pub struct x0ne_logprobs {
+    pub logits: u64,
+    pub stride: u64,
+    pub tokens: u64,
+    pub token_lp: u64,
+    pub entropy: u64,
+    pub top_ids: u64,
+    pub top_lp: u64,
+    pub work: u64,
+    pub work_bytes: u64,
+    pub rows: u32,
+    pub vocab: u32,
+    pub per_row: u32,
+    pub top: u32,
+    pub bf16: u32,
+    pub scale: f32,
+}
+
+#[repr(C)]
 #[derive(Clone, Copy, Default)]
 pub struct x0ne_gemv_fused {
     pub w: u64,
@@ -178,6 +209,13 @@ extern "C" {
                                   -> c_int;
     pub fn x0ne_gpu_kv8_select(g: *mut x0ne_gpu, c: *const x0ne_kv8, bounds: u64, q: u64, q_heads: u32, lens: u64,
                                budget: u32, page_list: u64, work: u64, work_bytes: u64) -> c_int;
+    pub fn x0ne_w4_code_bytes(w: *const x0ne_w4) -> u64;
+    pub fn x0ne_w4_scale_bytes(w: *const x0ne_w4) -> u64;
+    pub fn x0ne_gpu_w4_quantise(g: *mut x0ne_gpu, w: *const x0ne_w4, from: u64) -> c_int;
+    pub fn x0ne_gpu_w4_read(g: *mut x0ne_gpu, w: *const x0ne_w4, to: u64) -> c_int;
+    pub fn x0ne_gpu_w4_gemv(g: *mut x0ne_gpu, w: *const x0ne_w4, x: u64, n: u64, y: u64, out: u32) -> c_int;
+    pub fn x0ne_logprobs_work_bytes(d: *const x0ne_logprobs) -> u64;
+    pub fn x0ne_gpu_logprobs(g: *mut x0ne_gpu, d: *const x0ne_logprobs) -> c_int;
     pub fn x0ne_gpu_capture_begin(g: *mut x0ne_gpu) -> c_int;
     pub fn x0ne_gpu_capture_end(g: *mut x0ne_gpu, out: *mut *mut x0ne_graph) -> c_int;
     pub fn x0ne_gpu_launch_graph(g: *mut x0ne_gpu, graph: *const x0ne_graph) -> c_int;

@@ -87,6 +87,18 @@ class Kv8C(C.Structure):
                [(n, C.c_uint32) for n in ("pool", "kv_heads", "seqs", "seq_pages")]
 
 
+class W4C(C.Structure):
+    """x0ne_w4: a matrix of weights in 4 bits."""
+    _fields_ = [("codes", C.c_uint64), ("scales", C.c_uint64)] + [(n, C.c_uint32) for n in ("rows", "cols", "group", "reserved")]
+
+
+class LogProbsC(C.Structure):
+    """x0ne_logprobs: rows of logits and what is asked of them."""
+    _fields_ = [(n, C.c_uint64) for n in ("logits", "stride", "tokens", "token_lp", "entropy", "top_ids", "top_lp", "work",
+                                          "work_bytes")] + \
+               [(n, C.c_uint32) for n in ("rows", "vocab", "per_row", "top", "bf16")] + [("scale", C.c_float)]
+
+
 class EngineOptionsC(C.Structure):
     _fields_ = [("max_ctx", C.c_uint64), ("page_seed", C.c_uint64), ("sums", C.c_uint32),
                 ("prefill_chunk", C.c_uint32), ("max_batch", C.c_uint32), ("reserved", C.c_uint32)]
@@ -130,6 +142,13 @@ SIGNATURES = {
     "x0ne_kv8_work_bytes": ([C.POINTER(Kv8C), U32], U64),
     "x0ne_gpu_kv8_attention": ([P, C.POINTER(Kv8C), U64, U32, U64, U64, U32, U64, F32, U64, U64], ST),
     "x0ne_gpu_kv8_select": ([P, C.POINTER(Kv8C), U64, U64, U32, U64, U32, U64, U64, U64], ST),
+    "x0ne_w4_code_bytes": ([C.POINTER(W4C)], U64),
+    "x0ne_w4_scale_bytes": ([C.POINTER(W4C)], U64),
+    "x0ne_gpu_w4_quantise": ([P, C.POINTER(W4C), U64], ST),
+    "x0ne_gpu_w4_read": ([P, C.POINTER(W4C), U64], ST),
+    "x0ne_gpu_w4_gemv": ([P, C.POINTER(W4C), U64, U64, U64, U32], ST),
+    "x0ne_logprobs_work_bytes": ([C.POINTER(LogProbsC)], U64),
+    "x0ne_gpu_logprobs": ([P, C.POINTER(LogProbsC)], ST),
     "x0ne_gpu_capture_begin": ([P], ST),
     "x0ne_gpu_capture_end": ([P, C.POINTER(P)], ST),
     "x0ne_gpu_launch_graph": ([P, P], ST),

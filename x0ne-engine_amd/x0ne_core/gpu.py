@@ -5,7 +5,7 @@ import ctypes as C
 from dataclasses import dataclass
 from enum import IntEnum
 
-from ._lib import ArgC, Counts, GemvFusedC, Kv8C, SplitPlanC, check, lib
+from ._lib import ArgC, Counts, FormatError, GemvFusedC, Kv8C, LogProbsC, SplitPlanC, W4C, check, lib
 
 
 class Param(IntEnum):
@@ -106,6 +106,27 @@ class SplitPlan:
 class Kv8(Kv8C):
     """An 8-bit paged K/V cache (x0ne_kv8) at device addresses: codes [pool][kv_heads][4096], scales
     [pool][kv_heads][32], page_table [seqs][seq_pages]."""
+
+
+class W4(W4C):
+    """A matrix of weights in 4 bits (x0ne_w4) at device addresses: codes and scales of rows x cols weights in groups of
+    32, 64 or 128."""
+
+    def code_bytes(self) -> int:
+        return lib().x0ne_w4_code_bytes(self)
+
+    def scale_bytes(self) -> int:
+        return lib().x0ne_w4_scale_bytes(self)
+
+
+W4_OUT = {"bf16": 0, "f32": 1, "swiglu": 2}
+
+
+class LogProbs(LogProbsC):
+    """Rows of logits and what is asked of them (x0ne_logprobs), at device addresses; the scale is 1 unless given."""
+
+    def __init__(self, scale: float = 1.0, **fields):
+        super().__init__(scale=scale, **fields)
 
 
 class Graph:
@@ -244,6 +265,28 @@ class Gpu:
         """The budget pages per sequence and kv head worth attending, by their bounds (x0ne_gpu_kv8_select)."""
         check(lib().x0ne_gpu_kv8_select(self.h, cache, bounds, q, q_heads, lens, budget, page_list, work, work_bytes),
               "kv8_select")
+
+    def w4_quantise(self, w: W4, source: int):
+        """A row-major bf16 matrix into 4 bits (x0ne_gpu_w4_quantise)."""
+        check(lib().x0ne_gpu_w4_quantise(self.h, w, source), "w4_quantise")
+
+    def w4_read(self, w: W4, to: int):
+        """What the codes stand for as a row-major bf16 matrix (x0ne_gpu_w4_read)."""
+        check(lib().x0ne_gpu_w4_read(self.h, w, to), "w4_read")
+
+    def w4_gemv(self, w: W4, x: int, n: int, y: int, out: str = "bf16"):
+        """Y = X W^T of n rows of X (x0ne_gpu_w4_gemv); out "bf16", "f32", or "swiglu" of a [gate; up] W."""
+        if out not in W4_OUT:
+            raise FormatError(f"w4_gemv: no output {out!r} (bf16, f32 or swiglu)")
+        check(lib().x0ne_gpu_w4_gemv(self.h, w, x, n, y, W4_OUT[out]), "w4_gemv")
+
+    def logprobs_work_bytes(self, d: LogProbs) -> int:
+        """Bytes of the zeroed workspace of logprobs, by the descriptor's numbers; 0 for numbers it refuses."""
+        return lib().x0ne_logprobs_work_bytes(d)
+
+    def logprobs(self, d: LogProbs):
+        """Log probabilities of given tokens, entropy and top alternatives of rows of logits (x0ne_gpu_logprobs)."""
+        check(lib().x0ne_gpu_logprobs(self.h, d), "logprobs")
 
     def capture(self, launches) -> Graph:
         """Gpu::capture (gpu.rs:1170-1217): records the launches `launches()` makes."""

@@ -15,7 +15,7 @@ import numpy as np
 
 from ._lib import FormatError, GpuError
 from .arena import Arena, Class
-from .gpu import Arg, Gpu, Kv8, SplitPlan, split_state_bytes
+from .gpu import Arg, Gpu, Kv8, LogProbs, SplitPlan, W4, split_state_bytes
 
 HEAD_DIM = 128
 PAGE = 16
@@ -1132,3 +1132,77 @@ class Kernels:
                                 a.ptr(s["work"]), size)
         self.gpu.sync()
         return a.read_array(s["list"], 0, n, np.uint32).reshape(seqs, pages.kv_heads, budget)
+
+    # -- weights in 4 bits, log probabilities (w4.hip, logprobs.hip) --
+    def _arrays(self, arrays: dict):
+        """An arena with these arrays: (arena, device address of each, a function that reads one back)."""
+        a = self._arena()
+        arrays = {k: np.ascontiguousarray(v) for k, v in arrays.items()}
+        s = {k: a.alloc(k, max(v.nbytes, 16), Class.CLIENT_DATA) for k, v in arrays.items()}
+        self._freeze(a)
+        for k, v in arrays.items():
+            if v.nbytes:
+                a.write(s[k], 0, v)
+        return a, {k: a.ptr(v) for k, v in s.items()}, \
+            lambda k: a.read_array(s[k], 0, arrays[k].size, arrays[k].dtype).reshape(arrays[k].shape) if arrays[k].size else arrays[k]
+
+    def w4_quantise(self, w, group: int):
+        """x0ne_gpu_w4_quantise of w [rows][cols] (bf16 bits): (codes, scales as bf16 bits), as they lie."""
+        w = np.asarray(w, np.uint16)
+        d = W4(0, 0, *w.shape, group)
+        a, at, back = self._arrays({"w": w, "codes": np.full(d.code_bytes(), 0xA5, np.uint8),
+                                    "scales": np.full(d.scale_bytes() // 2, self.SENTINEL, np.uint16)})
+        self.gpu.w4_quantise(W4(at["codes"], at["scales"], *w.shape, group), at["w"])
+        self.gpu.sync()
+        return back("codes"), back("scales")
+
+    def w4_read(self, codes, scales, rows: int, cols: int, group: int) -> np.ndarray:
+        """x0ne_gpu_w4_read: [rows][cols] bf16 bits."""
+        a, at, back = self._arrays({"codes": codes, "scales": scales, "to": np.full((rows + 1, cols), self.SENTINEL, np.uint16)})
+        self.gpu.w4_read(W4(at["codes"], at["scales"], rows, cols, group), at["to"])
+        self.gpu.sync()
+        to = back("to")
+        if (to[rows] != self.SENTINEL).any():
+            raise GpuError("w4_read: a row behind the last was written")
+        return to[:rows]
+
+    def w4_gemv(self, codes, scales, rows: int, cols: int, group: int, x, out: str = "bf16", calls: int = 1) -> np.ndarray:
+        """x0ne_gpu_w4_gemv of x [n][cols] (bf16 bits): [n][rows], or [n][rows / 2] of "swiglu", bf16 bits or f32."""
+        x = np.asarray(x, np.uint16)
+        shape = (x.shape[0] + 1, rows // 2 if out == "swiglu" else rows)
+        y = np.full(shape, -1.25, np.float32) if out == "f32" else np.full(shape, self.SENTINEL, np.uint16)
+        a, at, back = self._arrays({"codes": codes, "scales": scales, "x": x, "y": y})
+        for _ in range(calls):
+            self.gpu.w4_gemv(W4(at["codes"], at["scales"], rows, cols, group), at["x"], x.shape[0], at["y"], out)
+        self.gpu.sync()
+        got = back("y")
+        if (got[-1] != y[-1]).any():
+            raise GpuError("w4_gemv: a row behind the last was written")
+        return got[:-1]
+
+    def logprobs(self, logits, tokens=None, top: int = 0, entropy: bool = True, scale: float = 1.0, vocab: int | None = None,
+                 calls: int = 1):
+        """x0ne_gpu_logprobs of logits [rows][stride] (f32, or bf16 bits as uint16), the first vocab of each row, tokens
+        [rows][per_row]: (token_lp, entropy, top_ids, top_lp), None for what is not asked."""
+        bf16 = logits.dtype == np.uint16
+        rows, stride = logits.shape
+        numbers = dict(rows=rows, stride=stride, vocab=stride if vocab is None else vocab, top=top, bf16=int(bf16), scale=scale,
+                       per_row=0 if tokens is None else tokens.shape[1])
+        size = self.gpu.logprobs_work_bytes(LogProbs(**numbers))
+        arrays = {"logits": logits, "work": np.zeros(size, np.uint8), "entropy": np.full(rows + 1, -7.0, np.float32),
+                  "top_ids": np.full((rows + 1, top), 0xA5A5A5A5, np.uint32), "top_lp": np.full((rows + 1, top), -7.0, np.float32),
+                  "token_lp": np.full((rows + 1, numbers["per_row"]), -7.0, np.float32)}
+        if tokens is not None:
+            arrays["tokens"] = np.asarray(tokens, np.uint32)
+        a, at, back = self._arrays(arrays)
+        d = LogProbs(logits=at["logits"], entropy=at["entropy"] if entropy else 0, work=at["work"], work_bytes=size,
+                     tokens=at.get("tokens", 0), token_lp=at["token_lp"] if tokens is not None else 0,
+                     top_ids=at["top_ids"] if top else 0, top_lp=at["top_lp"] if top else 0, **numbers)
+        for _ in range(calls):
+            self.gpu.logprobs(d)
+        self.gpu.sync()
+        got = {k: back(k) for k in ("token_lp", "entropy", "top_ids", "top_lp")}
+        if any((v[-1:] != arrays[k][-1:]).any() for k, v in got.items()):
+            raise GpuError("logprobs: a row behind the last was written")
+        return (got["token_lp"][:-1] if tokens is not None else None, got["entropy"][:-1] if entropy else None,
+                got["top_ids"][:-1] if top else None, got["top_lp"][:-1] if top else None)
