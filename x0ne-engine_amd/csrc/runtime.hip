@@ -100,6 +100,13 @@ extern "C" x0ne_status x0ne_gpu_new(x0ne_gpu** out) {
         delete g;
         return gpu_fail(e, "hipStreamCreateWithFlags");
     }
+    e = hipMalloc((void**)&g->counters, GPU_COUNTERS * 4);
+    if (e == hipSuccess) e = hipMemset(g->counters, 0, GPU_COUNTERS * 4);
+    if (e == hipSuccess) e = hipDeviceSynchronize();
+    if (e != hipSuccess) {
+        x0ne_gpu_free(g);
+        return gpu_fail(e, "the counters");
+    }
     *out = g;
     return X0NE_OK;
 }
@@ -114,6 +121,7 @@ extern "C" void x0ne_gpu_free(x0ne_gpu* g) {
         (void)hipStreamDestroy(g->stream);
     }
     if (g->tile_parts) (void)hipFree(g->tile_parts);
+    if (g->counters) (void)hipFree(g->counters);
     delete g;
 }
 
@@ -286,7 +294,7 @@ namespace x0ne {
 // The Gpu's own workspace for the tiled GEMM's slices, allocated at the first call whose plan has
 // slices or when a capture begins (a capture must not allocate); null without the memory for it: the
 // Gpu's GEMMs then stay unsplit.
-static float* own_parts(x0ne_gpu* g) {
+float* own_parts(x0ne_gpu* g) {
     if (!g->tile_parts && !g->tile_parts_refused && !g->capturing) {
         // Another thread may have a capture of its own Gpu open: this thread's mode is relaxed for the
         // allocation, so that it is neither refused nor ends that capture.

@@ -124,63 +124,225 @@ __global__ void __launch_bounds__(256) w4_read_kernel(Form f, bf16_t* __restrict
     }
 }
 
-// Y = X W^T of 16 rows of X and 16 of W to a block (SwiGLU: 16 gate rows and the 16 up rows that go with them), the
-// tiles of a panel to its wavefronts in turn. X is the A operand, W the B operand: a lane's four sums are four tokens of
-// one row of W, whose scale of a group is one value.
-template <int G, int OUT>
-__global__ void __launch_bounds__(256) w4_gemv_kernel(Form f, const bf16_t* __restrict__ x, uint32_t n, void* __restrict__ y) {
-    constexpr int PANELS = OUT == X0NE_W4_SWIGLU ? 2 : 1;
-    __shared__ f32x4 part[4][PANELS][64];
-    const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const uint32_t token = blockIdx.y * 16 + (lane & 15), panels = (f.rows + 15) / 16;
-    f32x4 sum[PANELS] = {};
-    for (uint32_t t = wave; t < f.tiles; t += 4) {
-        bf16x8 a[4];
+// Word 3 of a raw buffer's descriptor (gfx9: 32-bit data format). A load at or past its bytes gives zeros.
+constexpr uint32_t RSRC_WORD3 = 0x00020000, OFF_NONE = 0xFFFFFFF0u;
+
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t rsrc(const void* base, uint32_t bytes) {
+    return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(base), 0, (int)bytes, (int)RSRC_WORD3);
+}
+// The cache policy of what is read once (non-temporal).
+constexpr int NT = 2;
+template <int POLICY = 0>
+__device__ __forceinline__ u32x4 load16(__amdgpu_buffer_rsrc_t r, uint32_t off) {
+    return __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(r, (int)off, 0, POLICY));
+}
+
+// A tile of a panel in flight: a lane's codes and its row's scales.
+template <int G>
+struct Piece {
+    u32x4 codes;
+    uint32_t scales[G == 32 ? 2 : 1];
+};
+
+// How a launch's blocks share the work: a unit is `rounds` rounds of a tile to each wavefront, and block b takes the rounds
+// from b run to (b + 1) run - 1 of all units' one behind the other.
+struct Cut {
+    uint32_t all, rounds, run, blocks, groups;
+    float* parts;        // [blocks][2][P TT][4][64]: of a block's first unit, and of its last, where they are cut
+    uint32_t* counters;  // one per unit: zero, left at zero
+};
+
+// Y = X W^T. A block of V wavefronts takes a run of the tiles of units of P panels (SwiGLU: half of them gate, the others up)
+// and 4 XL rows of X; its wavefronts take the run's tiles in turn, so that it reads V KiB in a row. X is the A operand, W the B operand: a
+// lane's four sums are four tokens of one row of W, whose scale of a group is one value.
+// A load of X takes 4 rows of a tile's 256 bytes, neighbouring lanes on one row, and passes through the wavefront's own
+// LDS, 16-byte chunks placed by an XOR of the row, into the operand's order.
+template <int G, int OUT, int XL, int P, int V, int U, int POLICY, bool EVEN>
+__global__ void __launch_bounds__(64 * V) w4_gemv_kernel(Form f, const bf16_t* __restrict__ x, uint32_t n, void* __restrict__ y, Cut cut) {
+    constexpr int PAIR = OUT == X0NE_W4_SWIGLU ? 2 : 1, PER = 128 / G, TT = (XL + 3) / 4, TOKENS = XL < 4 ? 4 * XL : 16 * TT;
+    // A wavefront's X tile, then its sums of a unit.
+    constexpr int OWN = XL * 64 > P * TT * 64 ? XL * 64 : P * TT * 64;
+    __shared__ u32x4 lds[V][OWN];
+    __shared__ uint32_t last;
+    // Blocks go round the 8 XCDs in the order of their ids: those of a run for the groups of rows of X are neighbours on one,
+    // so that its weights come from memory once.
+    const uint32_t group = (blockIdx.x >> 3) % cut.groups, block = (blockIdx.x >> 3) / cut.groups * 8 + (blockIdx.x & 7);
+    const uint32_t first = block * cut.run, end = min(first + cut.run, cut.all);
+    const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const uint32_t token0 = group * TOKENS, panels = (f.rows + 15) / 16;
+    const __amdgpu_buffer_rsrc_t xr = rsrc(x, n * f.cols * 2);
+    u32x4* mine = lds[wave];
+    // Panel p of unit u: SwiGLU's odd ones are the up rows of the even ones.
+    auto panel_of = [&](uint32_t u, int p) { return u * (P / PAIR) + p / PAIR + p % PAIR * (panels / 2); };
+
+    Piece<G> w[U][P];
+    u32x4 a[U][XL];
+    auto load = [&](int slot, bool more, uint32_t u, uint32_t t) {
 #pragma unroll
-        for (int s = 0; s < 4; ++s) {
-            const uint32_t col = t * TILE_COLS + 32 * s + 8 * (lane >> 4);
-            u32x4 v = {0, 0, 0, 0};
-            if (token < n && col < f.cols) v = *reinterpret_cast<const u32x4*>(x + (size_t)token * f.cols + col);
-            a[s] = __builtin_bit_cast(bf16x8, v);
+        for (int p = 0; p < P; ++p) {
+            const uint32_t panel = panel_of(u, p);
+            const bool there = more && panel < panels;
+            const size_t tile = (size_t)panel * f.tiles;
+            const auto cr = rsrc(f.codes + (there ? tile * TILE_BYTES : 0), there ? f.tiles * TILE_BYTES : 0);
+            const auto sr = rsrc(f.scales + (there ? tile * (16 * PER) : 0), there ? f.tiles * (32 * PER) : 0);
+            w[slot][p].codes = load16<POLICY>(cr, t * TILE_BYTES + 16 * lane);
+            const int at = (int)((t * 16 + (lane & 15)) * 2 * PER);
+            if (PER == 4) {
+                const auto v = __builtin_amdgcn_raw_buffer_load_b64(sr, at, 0, POLICY);
+                w[slot][p].scales[0] = v[0];
+                w[slot][p].scales[PER / 4] = v[1];
+            } else if (PER == 2)
+                w[slot][p].scales[0] = __builtin_amdgcn_raw_buffer_load_b32(sr, at, 0, POLICY);
+            else
+                w[slot][p].scales[0] = (uint32_t)(uint16_t)__builtin_amdgcn_raw_buffer_load_b16(sr, at, 0, POLICY);
         }
+        const uint32_t col = t * TILE_COLS + 8 * (lane & 15);
 #pragma unroll
-        for (int p = 0; p < PANELS; ++p) {
-            const size_t tile = (size_t)(blockIdx.x + p * (panels / 2)) * f.tiles + t;
-            const u32x4 c = *reinterpret_cast<const u32x4*>(f.codes + tile * TILE_BYTES + 16 * lane);
-            f32x4 acc = {};
+        for (int i = 0; i < XL; ++i) {
+            const uint32_t token = token0 + 4 * i + (lane >> 4);
+            a[slot][i] = load16(xr, more && token < n && col < f.cols ? (token * f.cols + col) * 2 : OFF_NONE);
+        }
+    };
+
+    f32x4 sum[P][TT] = {};
+    auto multiply = [&](int slot) {
+#pragma unroll
+        for (int i = 0; i < XL; ++i) {
+            const uint32_t r = 4 * i + (lane >> 4);
+            mine[r * 16 + ((lane ^ r) & 15)] = a[slot][i];
+        }
+        bf16x8 frag[TT][4];
+#pragma unroll
+        for (int i = 0; i < TT; ++i)
 #pragma unroll
             for (int s = 0; s < 4; ++s) {
-                acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a[s], decode8(c[s]), acc, 0, 0, 0);
-                if ((s + 1) % (G / 32) == 0) {
-                    const float scale = scale_of<G>(f.scales, tile, lane & 15, s);
+                const uint32_t r = (16 * i + (lane & 15)) & (4 * XL - 1);
+                frag[i][s] = __builtin_bit_cast(bf16x8, mine[r * 16 + ((4 * s + (lane >> 4)) ^ (r & 15))]);
+            }
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) sum[p][i] = fmaf(acc[i], scale, sum[p][i]);
-                    acc = f32x4{};
+        for (int p = 0; p < P; ++p) {
+            f32x4 acc[TT] = {};
+#pragma unroll
+            for (int s = 0; s < 4; ++s) {
+                const bf16x8 b = decode8(w[slot][p].codes[s]);
+#pragma unroll
+                for (int i = 0; i < TT; ++i) acc[i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(frag[i][s], b, acc[i], 0, 0, 0);
+                if ((s + 1) % (G / 32) == 0) {
+                    const int g = s * 32 / G;
+                    const uint32_t word = w[slot][p].scales[PER == 4 ? g / 2 : 0];
+                    const float scale = g & 1 ? bf_hi(word) : bf_lo(word);
+#pragma unroll
+                    for (int i = 0; i < TT; ++i) {
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) sum[p][i][j] = fmaf(acc[i][j], scale, sum[p][i][j]);
+                        acc[i] = f32x4{};
+                    }
                 }
             }
         }
-    }
+    };
+
+    auto write = [&](uint32_t u, uint32_t o, const f32x4* r) {
+        const uint32_t p = o / TT * PAIR, i = o % TT;
+        const uint32_t row = panel_of(u, p) * 16 + (lane & 15), out_rows = f.rows / PAIR;
 #pragma unroll
-    for (int p = 0; p < PANELS; ++p) part[wave][p][lane] = sum[p];
-    __syncthreads();
-    if (wave != 0) return;
+        for (int j = 0; j < 4; ++j) {
+            const uint32_t to = token0 + 16 * i + 4 * (lane >> 4) + j;
+            if (row >= out_rows || to >= min(n, token0 + TOKENS)) continue;
+            const size_t at = (size_t)to * out_rows + row;
+            if (OUT == X0NE_W4_F32)
+                static_cast<float*>(y)[at] = r[0][j];
+            else if (OUT == X0NE_W4_BF16)
+                static_cast<bf16_t*>(y)[at] = f2bf(r[0][j]);
+            else
+                static_cast<bf16_t*>(y)[at] = f2bf(r[0][j] / (1.0f + expf(-r[0][j])) * r[PAIR - 1][j]);
+        }
+    };
+    // The wavefronts' sums of a unit, and those of the other blocks that have tiles of it: each leaves its part, and the
+    // last to count itself adds them in the blocks' order.
+    auto finish = [&](uint32_t u) {
 #pragma unroll
-    for (int p = 0; p < PANELS; ++p)
+        for (int p = 0; p < P; ++p)
 #pragma unroll
-        for (int v = 1; v < 4; ++v) sum[p] += part[v][p][lane];
-    const uint32_t row = blockIdx.x * 16 + (lane & 15), out_rows = f.rows / PANELS;
-    if (row >= out_rows) return;
+            for (int i = 0; i < TT; ++i) {
+                mine[(p * TT + i) * 64 + lane] = __builtin_bit_cast(u32x4, sum[p][i]);
+                sum[p][i] = f32x4{};
+            }
+        lds_barrier();
+        const uint32_t begin = u * cut.rounds, behind = begin + cut.rounds;
+        const bool whole = !EVEN || (begin >= first && behind <= end);
+        float* parts = cut.parts + (size_t)group * cut.blocks * (2 * P * TT * 256);
+        float* part = parts + (size_t)(2 * block + (begin > first)) * (P * TT * 256);
+        for (uint32_t o = wave; o < P / PAIR * TT; o += V) {
+            const uint32_t p = o / TT * PAIR, i = o % TT;
+            f32x4 r[PAIR] = {};
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const uint32_t to = blockIdx.y * 16 + 4 * (lane >> 4) + i;
-        if (to >= n) break;
-        const size_t at = (size_t)to * out_rows + row;
-        if (OUT == X0NE_W4_F32)
-            static_cast<float*>(y)[at] = sum[0][i];
-        else if (OUT == X0NE_W4_BF16)
-            static_cast<bf16_t*>(y)[at] = f2bf(sum[0][i]);
-        else
-            static_cast<bf16_t*>(y)[at] = f2bf(sum[0][i] / (1.0f + expf(-sum[0][i])) * sum[PANELS - 1][i]);
+            for (int v = 0; v < V; ++v)
+#pragma unroll
+                for (int k = 0; k < PAIR; ++k) r[k] += __builtin_bit_cast(f32x4, lds[v][((p + k) * TT + i) * 64 + lane]);
+            if (whole) {
+                write(u, o, r);
+                continue;
+            }
+#pragma unroll
+            for (int k = 0; k < PAIR; ++k)
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                    __hip_atomic_store(part + (((p + k) * TT + i) * 4 + j) * 64 + lane, r[k][j], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        }
+        if (whole) {
+            lds_barrier();
+            return;
+        }
+        const uint32_t b1 = begin / cut.run, b2 = (behind - 1) / cut.run;
+        // The parts acknowledged, then the count.
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        __syncthreads();
+        uint32_t* counter = cut.counters + group * (cut.all / cut.rounds) + u;
+        if (threadIdx.x == 0) last = __hip_atomic_fetch_add(counter, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == b2 - b1;
+        __syncthreads();
+        if (!last) return;
+        if (threadIdx.x == 0) __hip_atomic_store(counter, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);  // for the next call
+        for (uint32_t o = wave; o < P / PAIR * TT; o += V) {
+            const uint32_t p = o / TT * PAIR, i = o % TT;
+            f32x4 r[PAIR] = {};
+            for (uint32_t b = b1; b <= b2; ++b) {
+                const float* from = parts + (size_t)(2 * b + (b == b1 && begin > b * cut.run)) * (P * TT * 256);
+#pragma unroll
+                for (int k = 0; k < PAIR; ++k)
+#pragma unroll
+                    for (int j = 0; j < 4; ++j)
+                        r[k][j] += __hip_atomic_load(from + (((p + k) * TT + i) * 4 + j) * 64 + lane, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            }
+            write(u, o, r);
+        }
+    };
+
+    if (first >= end) return;
+    // U rounds in flight, over the ends of units too. A round past the run's end is one of zeros, so that the loop has no
+    // other way out: with one, the compiler moved the loads' registers and waited for all of them.
+    uint32_t unit = first / cut.rounds, round = first % cut.rounds, next = first, next_u = unit, next_round = round;
+    auto load_next = [&](int slot) {
+        load(slot, next < end, next_u, next_round * V + wave);
+        ++next;
+        const bool over = ++next_round == cut.rounds;
+        next_u += over;
+        next_round = over ? 0 : next_round;
+    };
+#pragma unroll
+    for (int slot = 0; slot < U; ++slot) load_next(slot);
+    for (uint32_t at = first; at < end; at += U) {
+#pragma unroll
+        for (int slot = 0; slot < U; ++slot) {
+            multiply(slot);
+            load_next(slot);
+            const bool over = ++round == cut.rounds;
+            if (over || at + slot + 1 == end) {
+                if (at + slot < end) finish(unit);
+                unit += over;
+                round = over ? 0 : round;
+            }
+        }
     }
 }
 
@@ -189,13 +351,14 @@ __global__ void __launch_bounds__(256) w4_gemv_kernel(Form f, const bf16_t* __re
 x0ne_status bad(const char* what, const std::string& why) { return fail(X0NE_ERR_FORMAT, std::string(what) + ": " + why); }
 
 constexpr uint32_t MOST = 1u << 24;
+constexpr uint64_t MOST_WEIGHTS = 1ull << 40;  // more than memory holds; tiles are counted in 32 bits
 
 x0ne_status check_shape(const char* what, const x0ne_w4* w) {
     if (!w) return bad(what, "no matrix");
-    if (w->rows == 0 || w->rows > MOST || w->cols == 0 || w->cols > MOST || w->cols % 8 ||
+    if (w->rows == 0 || w->rows > MOST || w->cols == 0 || w->cols > MOST || w->cols % 8 || (uint64_t)w->rows * w->cols > MOST_WEIGHTS ||
         (w->group != 32 && w->group != 64 && w->group != 128))
         return bad(what, std::to_string(w->rows) + " rows of " + std::to_string(w->cols) + " columns in groups of " +
-                             std::to_string(w->group) + " (1 to 2^24 rows and columns, columns a multiple of 8, groups of 32, 64 or 128)");
+                             std::to_string(w->group) + " (1 to 2^24 rows and columns and up to 2^40 weights, columns a multiple of 8, groups of 32, 64 or 128)");
     return X0NE_OK;
 }
 
@@ -261,12 +424,33 @@ extern "C" x0ne_status x0ne_gpu_w4_read(x0ne_gpu* g, const x0ne_w4* w, uint64_t 
     });
 }
 
+static Cut cut_of(const Form& f, uint32_t P, uint32_t V, uint32_t groups, uint32_t slots, bool even, x0ne_gpu* g) {
+    const uint32_t units = ((f.rows + 15) / 16 + P - 1) / P, rounds = (f.tiles + V - 1) / V, each = std::max(1u, slots / groups);
+    Cut c = {units * rounds, rounds, even ? (units * rounds + each - 1) / each : (units + each - 1) / each * rounds, 0, groups, nullptr, nullptr};
+    c.blocks = (c.all + c.run - 1) / c.run;
+    if (even) c.parts = own_parts(g), c.counters = g->counters;
+    return c;
+}
+
+template <int OUT, int XL, int P, int V, int U, int POLICY, bool EVEN>
+static void launch_gemv(x0ne_gpu* g, const x0ne_w4* w, const bf16_t* x, uint32_t n, void* y, uint32_t per_cu) {
+    const auto kernel = w->group == 32   ? w4_gemv_kernel<32, OUT, XL, P, V, U, POLICY, EVEN>
+                        : w->group == 64 ? w4_gemv_kernel<64, OUT, XL, P, V, U, POLICY, EVEN>
+                                         : w4_gemv_kernel<128, OUT, XL, P, V, U, POLICY, EVEN>;
+    const Form f = form_of(w);
+    const Cut cut = cut_of(f, P, V, (n + 4 * XL - 1) / (4 * XL), per_cu * g->cus, EVEN, g);
+    hipLaunchKernelGGL(kernel, dim3((cut.blocks + 7) / 8 * 8 * cut.groups), dim3(64 * V), 0, g->stream, f, x, n, y, cut);
+}
+
 template <int OUT>
-static void launch_gemv(const x0ne_gpu* g, const x0ne_w4* w, const bf16_t* x, uint32_t n, void* y) {
-    const auto kernel = w->group == 32 ? w4_gemv_kernel<32, OUT> : w->group == 64 ? w4_gemv_kernel<64, OUT> : w4_gemv_kernel<128, OUT>;
-    const uint32_t panels = (w->rows + 15) / 16;
-    hipLaunchKernelGGL(kernel, dim3(OUT == X0NE_W4_SWIGLU ? panels / 2 : panels, (n + 15) / 16), dim3(256), 0, g->stream, form_of(w), x,
-                       n, y);
+static void launch_gemv(x0ne_gpu* g, const x0ne_w4* w, const bf16_t* x, uint32_t n, void* y) {
+    constexpr int PAIR = OUT == X0NE_W4_SWIGLU ? 2 : 1;
+    if (n <= 4)
+        launch_gemv<OUT, 1, PAIR, 8, 2, NT, false>(g, w, x, n, y, 3);
+    else if (n <= 16 && (w->rows + 63) / 64 <= GPU_COUNTERS && own_parts(g))
+        launch_gemv<OUT, 4, 4, 8, 1, NT, true>(g, w, x, n, y, 1);
+    else
+        launch_gemv<OUT, 4, 4, 8, 1, 0, false>(g, w, x, n, y, 2);
 }
 
 extern "C" x0ne_status x0ne_gpu_w4_gemv(x0ne_gpu* g, const x0ne_w4* w, uint64_t x, uint64_t n, uint64_t y, uint32_t out) {
