@@ -306,12 +306,12 @@ x0ne_status x0ne_gpu_w4_gemv(x0ne_gpu* g, const x0ne_w4* w, uint64_t x, uint64_t
    entropy [rows] f32: - sum p log p (a p of 0 adds 0).
    top (0 to 64): top_ids [rows][top] u32 the ids of the largest logits, falling, the lower id first of
    equal ones, top_lp [rows][top] f32 their log p. Logits of -infinity are no alternatives: behind the
-   last one stand 0xFFFFFFFF and -infinity. A row with NaN or +infinity (also as scale l), or with nothing
-   above -infinity, has no distribution: NaN and 0xFFFFFFFF throughout. f32 arithmetic.
-   work: 256-byte aligned, x0ne_logprobs_work_bytes of it, zeroed once before its first call and left
-   ready for the next by each; calls of all shapes, and those of the 8-bit cache, may share it in turn.
+   last one stand 0xFFFFFFFF and -infinity. A row with NaN or +infinity, or with nothing above -infinity, has
+   no distribution: NaN and 0xFFFFFFFF throughout. f32 arithmetic, log p as scale (l - max l) - log z.
+   work: 256-byte aligned, x0ne_logprobs_work_bytes of it. Nothing in it is kept from call to call; calls
+   of all shapes, and those of the 8-bit cache (which want it zeroed once), may share it in turn.
    Up to 2^24 rows, logits of a row and tokens to a row, stride below 2^32, logits aligned to one, other
-   addresses to 4 bytes, scale positive and finite, else X0NE_ERR_FORMAT. A call of no rows does nothing.
+   addresses to 4 bytes, scale from 2^-100 to 2^100, else X0NE_ERR_FORMAT. A call of no rows does nothing.
    It runs on the Gpu's stream, allocates nothing, and may be captured into a graph. */
 typedef struct {
     uint64_t logits, stride, tokens, token_lp, entropy, top_ids, top_lp, work, work_bytes;

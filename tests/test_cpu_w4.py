@@ -116,7 +116,7 @@ def test_logprobs_refusals_come_before_any_device():
     f = _lib.lib().x0ne_gpu_logprobs
     for change in BAD_NUMBERS + [
             dict(logits=0), dict(logits=4098), dict(logits=4097, bf16=1), dict(stride=999), dict(stride=1 << 32), dict(scale=0.0),
-            dict(scale=-1.0), dict(scale=float("inf")), dict(scale=float("nan")), dict(tokens=0), dict(tokens=258),
+            dict(scale=-1.0), dict(scale=2.0 ** -101), dict(scale=2.0 ** 101), dict(scale=float("inf")), dict(scale=float("nan")), dict(tokens=0), dict(tokens=258),
             dict(token_lp=0), dict(token_lp=258), dict(entropy=257), dict(top_ids=0), dict(top_ids=258), dict(top_lp=0),
             dict(top_lp=258), dict(work=0), dict(work=4224), dict(work_bytes=4 * 65536 - 1)]:
         status = f(None, C.byref(asked(**change)))

@@ -114,7 +114,7 @@ def test_scales_and_far_logits(kernels, scale):
     x[2] -= 1000.0
     x[3] *= 1e-3
     x[4] *= 50.0
-    x[5] = 3.0e38 * np.sign(x[5])  # scale l may be infinite: no distribution
+    x[5] = 3.0e38 * np.sign(x[5])  # scale l may be past f32
     check(kernels, x, rng.integers(0, 9000, (6, 2)), 8, scale)
 
 
@@ -141,8 +141,11 @@ def test_more_rows_than_counters(kernels):
     x = np.tile(logits(rng, 7, 4100), (10000, 1))
     got = kernels.logprobs(x, np.tile(np.arange(7)[:, None] * 500, (10000, 1)), 2, calls=2)
     want = check(kernels, x[:7], np.arange(7)[:, None] * 500, 2)
-    for g, w in zip(got, want):
-        assert (g.reshape(10000, *w.shape) == w[None]).all()
+    for name, g, w in zip(("token_lp", "entropy", "top_ids", "top_lp"), got, want):
+        g = g.reshape(10000, *w.shape)
+        assert (g == g[:1]).all()
+        # Fewer rows are cut into other slices: each within its tolerance of the exact value (M at most 30, H at most 9).
+        assert (g[0] == w).all() if name == "top_ids" else (np.abs(g[0] - w) <= 2 * (64 + 8 * 30) * 10 * 2.0 ** -24).all()
 
 
 def test_a_large_vocabulary(kernels):
@@ -211,7 +214,7 @@ def test_a_step_from_the_head_to_its_log_probabilities_in_a_graph(kernels, n):
     g.w4_quantise(d, at["w"])
     want_other = R.logprobs(other.astype(np.float64), 1.0, None, 64)[2]
     graph = g.capture(step)
-    assert graph.nodes() == 2
+    assert graph.nodes() == 3
     for _ in range(4):
         x = bits(rng.standard_normal((n, hidden)) * 3)
         a.write(sl["x"], 0, x)

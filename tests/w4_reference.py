@@ -68,7 +68,6 @@ def logprobs(x, scale, tokens=None, top=0):
     rows, vocab = x.shape
     with np.errstate(invalid="ignore", divide="ignore", over="ignore"):
         y = x * float(np.float32(scale))
-        y = np.where(np.abs(y) < 2.0 ** 128, y, np.copysign(np.inf, y) + 0.0 * np.where(np.isnan(y), y, 0.0))  # as f32 has it
         m = y.max(-1, keepdims=True)
         ok = np.isfinite(y.sum(-1)) | (np.isfinite(m[:, 0]) & ~np.isnan(y).any(-1))
         p = np.exp(y - m)

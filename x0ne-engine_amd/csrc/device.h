@@ -75,6 +75,16 @@ __device__ __forceinline__ float wave_max(float v) {
     return v;
 }
 
+// The sums of lanes 0 .. i, by DPP: within the rows of 16, then lane 15 of rows 0 and 2, then lane 31.
+__device__ __forceinline__ uint32_t wave_up_to(uint32_t x) {
+    x += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x111, 0xF, 0xF, false);
+    x += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x112, 0xF, 0xF, false);
+    x += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x114, 0xF, 0xF, false);
+    x += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x118, 0xF, 0xF, false);
+    x += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x142, 0xA, 0xF, false);
+    return x + (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x143, 0xC, 0xF, false);
+}
+
 // A barrier for data exchanged through LDS only: this wavefront's LDS operations are complete,
 // then all wavefronts meet. Unlike __syncthreads() it does not wait for outstanding global loads
 // (the workgroup fence does), so loads requested before it stay in flight across it.

@@ -49,15 +49,6 @@ template <int CTRL>
 __device__ __forceinline__ double row_move_d(double v) {
     return __longlong_as_double((long long)row_move_u<CTRL>((uint64_t)__double_as_longlong(v)));
 }
-// The sums of lanes 0 .. i, by DPP: within the rows of 16, then lane 15 of rows 0 and 2, then lane 31.
-__device__ __forceinline__ uint32_t wave_up_to(uint32_t x) {
-    x += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x111, 0xF, 0xF, false);
-    x += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x112, 0xF, 0xF, false);
-    x += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x114, 0xF, 0xF, false);
-    x += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x118, 0xF, 0xF, false);
-    x += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x142, 0xA, 0xF, false);
-    return x + (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x143, 0xC, 0xF, false);
-}
 __device__ __forceinline__ float row_max(float v) {
     v = fmaxf(v, __uint_as_float(row_move<0xB1>(__float_as_uint(v))));
     v = fmaxf(v, __uint_as_float(row_move<0x4E>(__float_as_uint(v))));

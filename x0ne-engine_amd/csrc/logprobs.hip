@@ -1,10 +1,9 @@
 // Log probabilities of rows of logits: those of given tokens, the entropy, and the top alternatives.
 //
-// With x = scale logit, m = max x, z = sum e^(x - m), t = sum (x - m) e^(x - m): log p = (x - m) - log z and the entropy
-// is log z - t / z. One pass: a block holds SLICE logits of a row in registers, forms (m, z, t) of them and picks its
-// top ones; the last block of a row to count itself joins the slices.
+// With l the logits, m = max l, z = sum e^(scale (l - m)), t = sum (l - m) e^(scale (l - m)): log p = scale (l - m) - log z
+// and the entropy is log z - scale t / z. One pass over the logits: a block holds a slice of a row in registers, 16 logits to a
+// thread, forms (m, z, t) of them and picks its top ones. A second, small kernel joins the slices of a row.
 #include <algorithm>
-#include <cmath>
 #include <string>
 
 #include "device.h"
@@ -14,9 +13,11 @@ using namespace x0ne;
 
 namespace {
 
-constexpr uint32_t THREADS = 256, EACH = 16, SLICE = THREADS * EACH, WAVES = THREADS / 64;
+constexpr uint32_t EACH = 16;  // logits to a thread
 constexpr uint32_t MOST_TOP = 64;
-constexpr float LOG2E = 1.44269504088896340736f;
+constexpr uint32_t CANDIDATES = 512;
+constexpr uint32_t RANKED = 128;  // so many keys are ranked without a floor
+constexpr float LOG2E = 1.44269504088896340736f, LOWEST = -3.40282347e38f;
 constexpr uint32_t NONE = 0xFFFFFFFFu;
 
 struct Args {
@@ -27,80 +28,192 @@ struct Args {
     float* entropy;
     uint32_t* top_ids;
     float* top_lp;
-    uint32_t* counter;  // one per row of the launch
-    float4* state;      // [rows][slices]: m, z, t
-    uint64_t* best;     // [rows][slices][top]
-    uint32_t rows, vocab, slices, per_row, top;
+    float4* state;   // [rows][slices]: m, z, t
+    uint64_t* best;  // [rows][top][slices]
+    uint32_t vocab, slices, length, per_row, top;  // logits of a slice
     float scale;
 };
 
-// Logits in order, zeros alike, and lower ids first among equals; 0 stands for none (minus infinity is no alternative).
+// Logits in order, zeros alike, and lower ids first among equals. No key of a logit above -infinity is 0.
 __device__ __forceinline__ uint64_t key_of(float x, uint32_t id) {
     const uint32_t b = __float_as_uint(x + 0.0f);
-    const uint32_t order = b ^ ((uint32_t)((int32_t)b >> 31) | 0x80000000u);
-    return x > -INFINITY ? (uint64_t)order << 32 | ~id : 0;
+    return (uint64_t)(b ^ ((uint32_t)((int32_t)b >> 31) | 0x80000000u)) << 32 | (uint32_t)~id;
 }
 __device__ __forceinline__ float logit_of(uint64_t key) {
     const uint32_t order = (uint32_t)(key >> 32);
     return __uint_as_float(order ^ (order & 0x80000000u ? 0x80000000u : 0xFFFFFFFFu));
 }
 
-struct Shared {
-    uint64_t key[SLICE];
-    uint64_t floor[WAVES];
-    uint64_t top[MOST_TOP];
-    float4 state[WAVES];
-    uint32_t count;
-    uint32_t last;
+// A value joined with that of another lane of its row of 16 by DPP (0xB1, 0x4E: xor 1 and 2; 0x141, 0x140: lane 7 - i of each
+// half row, lane 15 - i), and of other rows by the row swaps: after a step all lanes of 2, 4, 8, 16, 32, 64 have the same.
+template <int CTRL>
+__device__ __forceinline__ float moved(float x) {
+    return __uint_as_float((uint32_t)__builtin_amdgcn_mov_dpp((int)__float_as_uint(x), CTRL, 0xF, 0xF, true));
+}
+template <int STEP, class Op>
+__device__ __forceinline__ float fold(float x, Op op) {
+    if (STEP == 0) return op(x, moved<0xB1>(x));
+    if (STEP == 1) return op(x, moved<0x4E>(x));
+    if (STEP == 2) return op(x, moved<0x141>(x));
+    if (STEP == 3) return op(x, moved<0x140>(x));
+    const auto a = STEP == 4 ? __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false)
+                             : __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return op(__uint_as_float(a[0]), __uint_as_float(a[1]));
+}
+template <class Op>
+__device__ __forceinline__ float fold_all(float x, Op op) {
+    return fold<5>(fold<4>(fold<3>(fold<2>(fold<1>(fold<0>(x, op), op), op), op), op), op);
+}
+struct Most {
+    __device__ __forceinline__ float operator()(float a, float b) const { return fmaxf(a, b); }
+};
+struct Least {
+    __device__ __forceinline__ float operator()(float a, float b) const { return fminf(a, b); }
+};
+struct Sum {
+    __device__ __forceinline__ float operator()(float a, float b) const { return a + b; }
 };
 
-// The `top` largest of the block's keys (key(i) of each thread for i < EACH, all different but for 0), in order, into
-// sh.top, 0 behind the last. The top-th largest of a wavefront's lanes' largest keys is a floor that at least `top` keys
-// reach; those that reach the highest of the wavefronts' floors, few more than `top`, are ranked by counting.
-template <class Key>
-__device__ __forceinline__ void pick(Key key, uint32_t top, Shared& sh) {
-    const uint32_t wave = threadIdx.x >> 6;
-    uint64_t mine = 0;
-#pragma unroll
-    for (uint32_t i = 0; i < EACH; ++i) mine = max(mine, key(i));
-    uint32_t above = 0;
-    for (uint32_t l = 0; l < 64; ++l) above += (uint64_t)__shfl((unsigned long long)mine, (int)l, 64) > mine;
-    if (threadIdx.x == 0) sh.count = 0;
-    if (threadIdx.x < WAVES) sh.floor[threadIdx.x] = 0;
-    if (threadIdx.x < top) sh.top[threadIdx.x] = 0;
+template <uint32_t THREADS>
+struct Shared {
+    uint64_t key[CANDIDATES + 16];
+    uint64_t top[MOST_TOP];
+    float4 state[THREADS / 64];
+    float group[128];
+    float floor;
+    uint32_t count;
+};
+
+// A floor that at least `top` of the block's logits reach, by the largest of each thread's: its lanes are taken in 64 groups,
+// for more than 32 in 128, and the floor is the top-th largest of the groups' largest. On ordinary rows few more reach it.
+// -infinity is no alternative: the floor is above it.
+template <uint32_t THREADS>
+__device__ __forceinline__ float floor_of(float most, uint32_t top, Shared<THREADS>& sh) {
+    constexpr int STEPS = THREADS == 256 ? 1 : THREADS == 512 ? 2 : 3;  // to a 128th of the block
+    const uint32_t groups = top > 32 ? 128 : 64;
+    float g = fold<0>(most, Most());
+    if (STEPS > 1) g = fold<1>(g, Most());
+    if (STEPS > 2) g = fold<2>(g, Most());
+    if (groups == 64) g = fold<STEPS>(g, Most());
+    sh.group[threadIdx.x / (THREADS / groups)] = g;
     __syncthreads();
-    if (mine && above == top - 1) sh.floor[wave] = mine;
-    __syncthreads();
-    uint64_t floor = 1;
+    if (threadIdx.x < 64) {
+        float h = groups == 128 ? sh.group[64 + threadIdx.x] : -INFINITY;
+        g = sh.group[threadIdx.x];
+        if (top > 1) {
+            uint32_t over_g = 0, over_h = 0;
+#pragma unroll 1
+            for (uint32_t o = 0; o < groups; o += 16) {
 #pragma unroll
-    for (uint32_t w = 0; w < WAVES; ++w) floor = max(floor, sh.floor[w]);
-    if (mine >= floor) {
-#pragma unroll
-        for (uint32_t i = 0; i < EACH; ++i) {
-            const uint64_t k = key(i);
-            if (k >= floor) sh.key[atomicAdd(&sh.count, 1u)] = k;
-        }
+                for (uint32_t i = 0; i < 16; ++i) {
+                    over_g += sh.group[o + i] > g;
+                    over_h += sh.group[o + i] > h;
+                }
+            }
+            g = fold_all(fminf(over_g < top ? g : INFINITY, over_h < top ? h : INFINITY), Least());
+        } else
+            g = fold_all(g, Most());
+        if (threadIdx.x == 0) sh.floor = fmaxf(g, LOWEST);
     }
     __syncthreads();
-    const uint32_t count = sh.count;
-    for (uint32_t c = threadIdx.x; c < count; c += THREADS) {
+    return sh.floor;
+}
+
+// Room for a thread's `own` keys among the block's candidates: where they go. All threads take part.
+template <uint32_t THREADS>
+__device__ __forceinline__ uint32_t room(uint32_t own, Shared<THREADS>& sh) {
+    const uint32_t up_to = wave_up_to(own);
+    uint32_t base = 0;
+    if ((threadIdx.x & 63) == 63) base = __hip_atomic_fetch_add(&sh.count, up_to, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
+    return (uint32_t)__builtin_amdgcn_readlane((int)base, 63) + up_to - own;
+}
+
+// The `top` largest of the first `found` of sh.key, in order, into sh.top, by counting the larger ones of each.
+template <uint32_t THREADS>
+__device__ __forceinline__ void rank(uint32_t found, uint32_t top, Shared<THREADS>& sh) {
+    if (threadIdx.x < 16) sh.key[found + threadIdx.x] = 0;
+    __syncthreads();
+    for (uint32_t c = threadIdx.x; c < found; c += THREADS) {
         const uint64_t k = sh.key[c];
-        uint32_t rank = 0;
-        for (uint32_t o = 0; o < count; ++o) rank += sh.key[o] > k;
-        if (rank < top) sh.top[rank] = k;
+        uint32_t above = 0;
+#pragma unroll 1
+        for (uint32_t o = 0; o < found; o += 16) {
+#pragma unroll
+            for (uint32_t i = 0; i < 16; ++i) above += sh.key[o + i] > k;
+        }
+        if (k && above < top) sh.top[above] = k;
     }
     __syncthreads();
 }
 
-// (m, z, t) of two sets. A set of nothing but -infinity has m = -infinity and z = t = 0, or NaN.
-__device__ __forceinline__ float4 join(float4 a, float4 b) {
+// The `top` largest of the block's logits x[i] of ids id(i), in order, as keys into sh.top, 0 behind the last; `most` is the
+// largest of x. What reaches the floor is ranked by counting. Where that is too much (equal logits, parts that are masked
+// throughout), the floor is raised by bisection over the keys: all differ, so some floor leaves from top to CANDIDATES.
+template <uint32_t THREADS, class Id>
+__device__ __forceinline__ void pick(const float (&x)[EACH], float most, Id id, uint32_t top, Shared<THREADS>& sh) {
+    if (threadIdx.x == 0) sh.count = 0;
+    if (threadIdx.x < MOST_TOP) sh.top[threadIdx.x] = 0;
+    const float floor = floor_of<THREADS>(most, top, sh);
+    uint32_t own = 0;
+#pragma unroll
+    for (uint32_t i = 0; i < EACH; ++i) own += x[i] >= floor;
+    uint32_t at = room(own, sh);
+    if (own) {
+#pragma unroll
+        for (uint32_t i = 0; i < EACH; ++i)
+            if (x[i] >= floor && at < CANDIDATES) sh.key[at++] = key_of(x[i], id(i));
+    }
+    __syncthreads();
+    if (sh.count > CANDIDATES) {
+        uint64_t low = key_of(floor, NONE), high = ~0ull;
+        for (bool found = false; !found;) {
+            const uint64_t mid = low + (high - low) / 2;
+            __syncthreads();
+            if (threadIdx.x == 0) sh.count = 0;
+            __syncthreads();
+            own = 0;
+            uint32_t zero = 0;
+            asm volatile("" : "+v"(zero));  // the keys are formed here and not kept from turn to turn
+#pragma unroll
+            for (uint32_t i = 0; i < EACH; ++i) own += x[i] >= floor && key_of(x[i], id(i) + zero) >= mid;
+            at = room(own, sh);
+            __syncthreads();
+            const uint32_t count = sh.count;
+            if (count >= top)
+                low = mid;
+            else
+                high = mid;
+            found = (count >= top && count <= CANDIDATES) || high - low < 2;
+            if (found && own) {
+#pragma unroll
+                for (uint32_t i = 0; i < EACH; ++i) {
+                    const uint64_t k = key_of(x[i], id(i) + zero);
+                    if (x[i] >= floor && k >= mid && at < CANDIDATES) sh.key[at++] = k;
+                }
+            }
+        }
+        __syncthreads();
+    }
+    rank<THREADS>(min(sh.count, CANDIDATES), top, sh);
+}
+
+// (m, z, t) of two sets: one at the larger m as it is, one so far below it that nothing is left without an infinity times
+// zero. A set of nothing but -infinity has m = -infinity and z = t = 0, or NaN.
+__device__ __forceinline__ float4 join(float4 a, float4 b, float scale2) {
     const float m = fmaxf(a.x, b.x), da = a.x - m, db = b.x - m;
     float4 r = {m, 0.f, 0.f, 0.f};
-    const float pa = __builtin_amdgcn_exp2f(da * LOG2E), pb = __builtin_amdgcn_exp2f(db * LOG2E);
-    // A set at m as it is, and one so far below it that nothing is left without an infinity times zero.
+    const float pa = __builtin_amdgcn_exp2f(da * scale2), pb = __builtin_amdgcn_exp2f(db * scale2);
     r.y = (a.x == m ? a.y : pa * a.y) + (b.x == m ? b.y : pb * b.y);
-    r.z = (a.x == m ? a.z : pa > 0.f ? pa * (a.z + da * a.y) : pa * a.y) + (b.x == m ? b.z : pb > 0.f ? pb * (b.z + db * b.y) : pb * b.y);
+    r.z = (a.x == m ? a.z : pa > 0.f ? pa * (a.z + da * a.y) : 0.f) + (b.x == m ? b.z : pb > 0.f ? pb * (b.z + db * b.y) : 0.f);
     return r;
+}
+
+// Joined over the first `lanes` lanes.
+__device__ __forceinline__ float4 join_lanes(float4 all, int lanes, float scale2) {
+#pragma unroll 1
+    for (int o = 1; o < lanes; o <<= 1)
+        all = join(all, float4{__shfl_xor(all.x, o, 64), __shfl_xor(all.y, o, 64), __shfl_xor(all.z, o, 64), 0.f}, scale2);
+    return all;
 }
 
 typedef float f32x4a __attribute__((ext_vector_type(4), aligned(4)));
@@ -111,21 +224,48 @@ __device__ __forceinline__ float logit_at(const void* row, uint32_t i) {
     return BF16 ? bf2f(static_cast<const bf16_t*>(row)[i]) : static_cast<const float*>(row)[i];
 }
 
+// What is asked of row r, whose (m, z, t) is `all` and whose top keys are in sh.top; `given` is the logit of the thread's
+// first token.
+template <bool BF16, uint32_t THREADS>
+__device__ __forceinline__ void answer(const Args& a, const void* row, uint32_t r, float4 all, uint32_t token, float given, Shared<THREADS>& sh) {
+    // z is NaN with a NaN or an infinity among the logits, 0 where all are -infinity: no distribution.
+    const bool none = !(all.y > 0.f);
+    const float log_z = none ? NAN : logf(all.y);
+    auto log_p = [&](float l) { return (0.5f * l - 0.5f * all.x) * (2.f * a.scale) - log_z; };  // a difference may be past f32
+    if (a.entropy && threadIdx.x == 0) a.entropy[r] = log_z - a.scale * (all.z / all.y);
+    const uint64_t tokens = (uint64_t)r * a.per_row;
+    if (threadIdx.x < a.per_row) a.token_lp[tokens + threadIdx.x] = token < a.vocab ? log_p(given) : NAN;
+    for (uint32_t i = threadIdx.x + THREADS; i < a.per_row; i += THREADS) {
+        const uint32_t id = a.tokens[tokens + i];
+        a.token_lp[tokens + i] = id < a.vocab ? log_p(logit_at<BF16>(row, id)) : NAN;
+    }
+    if (threadIdx.x < a.top) {
+        const uint64_t k = sh.top[threadIdx.x], at = (uint64_t)r * a.top + threadIdx.x;
+        a.top_ids[at] = none || !k ? NONE : ~(uint32_t)k;
+        a.top_lp[at] = none ? NAN : k ? log_p(logit_of(k)) : -INFINITY;
+    }
+}
+
 template <bool BF16>
-__global__ void __launch_bounds__(256) logprobs_kernel(Args a) {
-    __shared__ Shared sh;
+__device__ __forceinline__ const void* row_of(const Args& a, uint32_t r) {
+    return static_cast<const uint8_t*>(a.logits) + r * a.stride * (BF16 ? 2 : 4);
+}
+
+template <bool BF16, uint32_t THREADS>
+__global__ void __launch_bounds__(THREADS, 8) logprobs_slices_kernel(Args a) {
+    constexpr uint32_t WAVES = THREADS / 64;
+    constexpr uint32_t PIECE = BF16 ? 8 : 4;  // logits of a 16-byte load
+    __shared__ Shared<THREADS> sh;
     const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const uint32_t r = blockIdx.x / a.slices, slice = blockIdx.x % a.slices;
-    const void* row = static_cast<const uint8_t*>(a.logits) + r * a.stride * (BF16 ? 2 : 4);
-    constexpr uint32_t PIECE = BF16 ? 8 : 4;  // logits of a 16-byte load
+    const void* row = row_of<BF16>(a, r);
+    const uint32_t start = slice * a.length, behind = min(start + a.length, a.vocab), first = start + threadIdx.x * PIECE;
+    auto id_of = [&](uint32_t i) { return first + i / PIECE * (THREADS * PIECE) + i % PIECE; };  // of x[i]
     float x[EACH];
-    const uint32_t first = slice * SLICE + threadIdx.x * PIECE;
-    // The id of x[i].
-    auto id_of = [&](uint32_t i) { return first + i / PIECE * (THREADS * PIECE) + i % PIECE; };
 #pragma unroll
     for (uint32_t v = 0; v < EACH / PIECE; ++v) {
         const uint32_t id = id_of(v * PIECE);
-        if (id < a.vocab && a.vocab - id >= PIECE) {
+        if (start + (v + 1) * THREADS * PIECE <= behind || id + PIECE <= behind) {  // all threads', or this one's
             if (BF16) {
                 const u32x4a w = *reinterpret_cast<const u32x4a*>(static_cast<const bf16_t*>(row) + id);
 #pragma unroll
@@ -137,99 +277,99 @@ __global__ void __launch_bounds__(256) logprobs_kernel(Args a) {
             }
         } else {
 #pragma unroll
-            for (uint32_t e = 0; e < PIECE; ++e) x[v * PIECE + e] = id + e < a.vocab ? logit_at<BF16>(row, id + e) : -INFINITY;
+            for (uint32_t e = 0; e < PIECE; ++e) x[v * PIECE + e] = id + e < behind ? logit_at<BF16>(row, id + e) : -INFINITY;
         }
     }
-    float m = -INFINITY;
+    const float scale2 = a.scale * LOG2E;
+    float most = x[0];
 #pragma unroll
-    for (uint32_t i = 0; i < EACH; ++i) m = fmaxf(m, x[i]);
-    m = wave_max(m) * a.scale;
-    const float base = m == -INFINITY ? 0.f : m;
+    for (uint32_t i = 1; i < EACH; ++i) most = fmaxf(most, x[i]);
+    const float m = fmaxf(fold_all(most, Most()), -INFINITY), base = m == -INFINITY ? 0.f : m;
     float z = 0.f, t = 0.f;
 #pragma unroll
     for (uint32_t i = 0; i < EACH; ++i) {
-        const float d = x[i] * a.scale - base, p = __builtin_amdgcn_exp2f(d * LOG2E);
+        const float d = x[i] - base, p = __builtin_amdgcn_exp2f(d * scale2);
         z += p;
-        t += p > 0.f ? p * d : p;
+        t = fmaf(p, fmaxf(d, LOWEST), t);  // 0 for -infinity; what a NaN leaves here does not matter, as it is in z
     }
-    z = wave_sum(z);
-    t = wave_sum(t);
+    z = fold_all(z, Sum());
+    t = fold_all(t, Sum());
     if (lane == 0) sh.state[wave] = float4{m, z, t, 0.f};
-    if (a.top) pick([&](uint32_t i) { return key_of(x[i], id_of(i)); }, a.top, sh);
+    if (a.top == 1) {
+        // The first of the largest of each wavefront, then of the block.
+        if (threadIdx.x == 0) sh.top[0] = 0;
+        __syncthreads();
+        if (most == m && m > -INFINITY) {
+            uint32_t id = 0;
+#pragma unroll
+            for (uint32_t i = EACH; i-- > 0;) id = x[i] == m ? id_of(i) : id;
+            __hip_atomic_fetch_max(&sh.top[0], key_of(m, id), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
+        }
+    } else if (a.top)
+        pick<THREADS>(x, most, id_of, a.top, sh);
     __syncthreads();
-    float4 all = sh.state[0];
-#pragma unroll
-    for (uint32_t w = 1; w < WAVES; ++w) all = join(all, sh.state[w]);
+    if (a.slices > 1 && wave > 0) return;
+    float4 all = join_lanes(lane < WAVES ? sh.state[lane] : float4{-INFINITY, 0.f, 0.f, 0.f}, WAVES, scale2);
     if (a.slices > 1) {
-        float* state = (float*)(a.state + (uint64_t)r * a.slices);
-        uint64_t* best = a.best + (uint64_t)r * a.slices * a.top;
-        if (threadIdx.x == 0) {
-            __hip_atomic_store(state + 4 * slice, all.x, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-            __hip_atomic_store(state + 4 * slice + 1, all.y, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-            __hip_atomic_store(state + 4 * slice + 2, all.z, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-        }
-        if (threadIdx.x < a.top)
-            __hip_atomic_store(best + (uint64_t)slice * a.top + threadIdx.x, sh.top[threadIdx.x], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-        // The stores acknowledged, then the count: the block that completes it joins the slices.
-        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-        __syncthreads();
-        if (threadIdx.x == 0)
-            sh.last = __hip_atomic_fetch_add(a.counter + r, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == a.slices - 1;
-        __syncthreads();
-        if (!sh.last) return;
-        if (threadIdx.x == 0) __hip_atomic_store(a.counter + r, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);  // for the next call
-        all = float4{-INFINITY, 0.f, 0.f, 0.f};
-        for (uint32_t s = threadIdx.x; s < a.slices; s += THREADS) {
-            float v[3];
-#pragma unroll
-            for (int i = 0; i < 3; ++i) v[i] = __hip_atomic_load(state + 4 * s + i, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-            all = join(all, float4{v[0], v[1], v[2], 0.f});
-        }
-#pragma unroll
-        for (int o = 1; o < 64; o <<= 1)
-            all = join(all, float4{__shfl_xor(all.x, o, 64), __shfl_xor(all.y, o, 64), __shfl_xor(all.z, o, 64), 0.f});
-        if (lane == 0) sh.state[wave] = all;
-        if (a.top) {
-            // SLICE keys at a time, the best so far among them.
-            const uint32_t keys = a.slices * a.top;
-            uint32_t done = 0, kept = 0;
-            while (done < keys) {
-                const uint32_t some = min(keys - done, SLICE - kept);
-                uint64_t k[EACH];
-#pragma unroll
-                for (uint32_t i = 0; i < EACH; ++i) {
-                    const uint32_t at = i * THREADS + threadIdx.x;
-                    k[i] = 0;
-                    if (at < kept)
-                        k[i] = sh.top[at];
-                    else if (at - kept < some)
-                        k[i] = __hip_atomic_load(best + done + at - kept, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-                }
-                __syncthreads();
-                pick([&](uint32_t i) { return k[i]; }, a.top, sh);
-                done += some;
-                kept = a.top;
-            }
-        }
-        __syncthreads();
-        all = sh.state[0];
-#pragma unroll
-        for (uint32_t w = 1; w < WAVES; ++w) all = join(all, sh.state[w]);
+        if (lane == 0) a.state[(uint64_t)r * a.slices + slice] = all;
+        if (lane < a.top) a.best[((uint64_t)r * a.top + lane) * a.slices + slice] = sh.top[lane];
+        return;
     }
-    // z is NaN with a NaN or an infinity among the logits, 0 where all are -infinity: no distribution.
-    const bool none = !(all.y > 0.f);
-    const float log_z = none ? NAN : logf(all.y);
-    if (a.entropy && threadIdx.x == 0) a.entropy[r] = log_z - all.z / all.y;
-    for (uint32_t i = threadIdx.x; i < a.per_row; i += THREADS) {
-        const uint64_t at = (uint64_t)r * a.per_row + i;
-        const uint32_t id = a.tokens[at];
-        a.token_lp[at] = id < a.vocab ? logit_at<BF16>(row, id) * a.scale - all.x - log_z : NAN;
+    all = float4{__shfl(all.x, 0, 64), __shfl(all.y, 0, 64), __shfl(all.z, 0, 64), 0.f};
+    const uint32_t token = threadIdx.x < a.per_row ? a.tokens[(uint64_t)r * a.per_row + threadIdx.x] : NONE;
+    answer<BF16, THREADS>(a, row, r, all, token, token < a.vocab ? logit_at<BF16>(row, token) : 0.f, sh);
+}
+
+// A block joins the slices of a row.
+template <bool BF16>
+__global__ void __launch_bounds__(256) logprobs_join_kernel(Args a) {
+    constexpr uint32_t THREADS = 256, WAVES = THREADS / 64, SLICE = THREADS * EACH;
+    __shared__ Shared<THREADS> sh;
+    __shared__ uint64_t kept[MOST_TOP];
+    const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r = blockIdx.x;
+    const void* row = row_of<BF16>(a, r);
+    const float4* state = a.state + (uint64_t)r * a.slices;
+    const uint64_t* best = a.best + (uint64_t)r * a.slices * a.top;
+    const uint32_t keys = a.slices * a.top, token = threadIdx.x < a.per_row ? a.tokens[(uint64_t)r * a.per_row + threadIdx.x] : NONE;
+    const float scale2 = a.scale * LOG2E;
+    float4 all = {-INFINITY, 0.f, 0.f, 0.f};
+    for (uint32_t s = threadIdx.x; s < a.slices; s += THREADS) all = join(all, state[s], scale2);
+    const float given = token < a.vocab ? logit_at<BF16>(row, token) : 0.f;
+    if (keys <= RANKED) {
+        if (threadIdx.x < keys) sh.key[threadIdx.x] = best[threadIdx.x];
+        if (threadIdx.x < MOST_TOP) sh.top[threadIdx.x] = 0;
+        if (keys) rank<THREADS>(keys, a.top, sh);
     }
-    if (threadIdx.x < a.top) {
-        const uint64_t k = sh.top[threadIdx.x], at = (uint64_t)r * a.top + threadIdx.x;
-        a.top_ids[at] = none || !k ? NONE : ~(uint32_t)k;
-        a.top_lp[at] = none ? NAN : k ? logit_of(k) * a.scale - all.x - log_z : -INFINITY;
+    // SLICE keys at a time, the best so far among them. They lie by their place among a slice's, so that the groups of lanes that
+    // give a floor have high ones.
+    for (uint32_t done = keys <= RANKED ? keys : 0, held = 0; done < keys; held = a.top) {
+        const uint32_t some = min(keys - done, SLICE - held);
+        float x[EACH], most = -INFINITY;
+        uint32_t ids[EACH];
+#pragma unroll
+        for (uint32_t i = 0; i < EACH; ++i) {
+            const uint32_t at = i * THREADS + threadIdx.x;
+            uint64_t k = 0;
+            if (at < held)
+                k = kept[at];
+            else if (at - held < some)
+                k = best[done + at - held];
+            x[i] = k ? logit_of(k) : -INFINITY;
+            ids[i] = ~(uint32_t)k;
+        }
+#pragma unroll
+        for (uint32_t i = 0; i < EACH; ++i) most = fmaxf(most, x[i]);
+        pick<THREADS>(x, most, [&](uint32_t i) { return ids[i]; }, a.top, sh);
+        if (threadIdx.x < a.top) kept[threadIdx.x] = sh.top[threadIdx.x];
+        done += some;
+        if (done < keys) __syncthreads();
     }
+    all = join_lanes(all, 64, scale2);
+    if (lane == 0) sh.state[wave] = all;
+    __syncthreads();
+    all = join_lanes(lane < WAVES ? sh.state[lane] : float4{-INFINITY, 0.f, 0.f, 0.f}, WAVES, scale2);
+    all = float4{__shfl(all.x, 0, 64), __shfl(all.y, 0, 64), __shfl(all.z, 0, 64), 0.f};
+    answer<BF16, THREADS>(a, row, r, all, token, given, sh);
 }
 
 // ---- host ----
@@ -245,22 +385,25 @@ x0ne_status check_shape(const x0ne_logprobs* d) {
     return X0NE_OK;
 }
 
-uint32_t slices_of(const x0ne_logprobs* d) { return (d->vocab + SLICE - 1) / SLICE; }
-
-// The workspace: a counter per row, then the slices' states and top keys. The counters are as many for every call, as in
-// the 8-bit cache's workspace, so that calls of all shapes may share one. More rows are further launches.
-constexpr uint64_t COUNTERS = 65536, COUNTER_BYTES = 4 * COUNTERS;
-uint64_t rows_at_once(const x0ne_logprobs* d) {
-    // A launch has fewer than 2^32 threads.
-    return std::min<uint64_t>(COUNTERS, ((1ull << 32) / THREADS - 1) / slices_of(d));
+// Blocks of 1024 threads spend the least on a slice's selection and join; those of 256 are over sooner where they are so few
+// that each has a place on the card from the start.
+constexpr uint32_t FEW = 256, MANY = 512;
+uint32_t threads_of(const x0ne_logprobs* d) {
+    return (uint64_t)d->rows * ((d->vocab + FEW * EACH - 1) / (FEW * EACH)) > 1024 ? MANY : FEW;
 }
+uint32_t slices_of(const x0ne_logprobs* d) { return (d->vocab + threads_of(d) * EACH - 1) / (threads_of(d) * EACH); }
+
+// The workspace's first part is left alone: there the calls of the 8-bit cache count, which may share it. Behind it the slices'
+// states, then their top keys.
+constexpr uint64_t COUNTER_BYTES = 4 * 65536;
+// A launch has fewer than 2^32 threads, and the workspace is that of at most so many rows' slices: more rows are further launches.
+uint64_t rows_at_once(const x0ne_logprobs* d) { return std::min<uint64_t>(65536, ((1ull << 32) / threads_of(d) - 1) / slices_of(d)); }
 
 }  // namespace
 
 extern "C" uint64_t x0ne_logprobs_work_bytes(const x0ne_logprobs* d) {
     if (check_shape(d) != X0NE_OK) return 0;
-    const uint64_t slices = slices_of(d);
-    return COUNTER_BYTES + (slices > 1 ? std::min<uint64_t>(d->rows, rows_at_once(d)) * slices * (sizeof(float4) + 8ull * d->top) : 0);
+    return COUNTER_BYTES + std::min<uint64_t>(d->rows, rows_at_once(d)) * slices_of(d) * (sizeof(float4) + 8ull * d->top);
 }
 
 extern "C" x0ne_status x0ne_gpu_logprobs(x0ne_gpu* g, const x0ne_logprobs* d) {
@@ -268,7 +411,7 @@ extern "C" x0ne_status x0ne_gpu_logprobs(x0ne_gpu* g, const x0ne_logprobs* d) {
     const uint64_t each = d->bf16 ? 2 : 4;
     if (!d->logits || d->logits % each || d->stride < d->vocab || d->stride >= (1ull << 32))
         return bad("logits (aligned to one), and a stride of at least a row's logits and below 2^32, are required");
-    if (!(d->scale > 0.f) || !std::isfinite(d->scale)) return bad("a scale that is positive and finite is required");
+    if (!(d->scale >= 0x1p-100f && d->scale <= 0x1p100f)) return bad("a scale from 2^-100 to 2^100 is required");
     if (d->per_row && (!d->tokens || !d->token_lp || d->tokens % 4 || d->token_lp % 4))
         return bad("given tokens need tokens and token_lp (4-byte aligned)");
     if (d->top && (!d->top_ids || !d->top_lp || d->top_ids % 4 || d->top_lp % 4)) return bad("top alternatives need top_ids and top_lp (4-byte aligned)");
@@ -278,10 +421,10 @@ extern "C" x0ne_status x0ne_gpu_logprobs(x0ne_gpu* g, const x0ne_logprobs* d) {
     if (!g) return fail(X0NE_ERR_GPU, "no device");
     if (d->rows == 0) return X0NE_OK;
     const OnDevice on(g->device);
-    const uint32_t slices = slices_of(d);
+    const uint32_t slices = slices_of(d), threads = threads_of(d);
     for (uint64_t first = 0; first < d->rows; first += rows_at_once(d)) {
+        const uint32_t rows = (uint32_t)std::min<uint64_t>(d->rows - first, rows_at_once(d));
         Args a = {};
-        a.rows = (uint32_t)std::min<uint64_t>(d->rows - first, rows_at_once(d));
         a.logits = (const uint8_t*)d->logits + first * d->stride * each;
         a.stride = d->stride;
         a.tokens = (const uint32_t*)d->tokens + first * d->per_row;
@@ -289,16 +432,22 @@ extern "C" x0ne_status x0ne_gpu_logprobs(x0ne_gpu* g, const x0ne_logprobs* d) {
         a.entropy = d->entropy ? (float*)d->entropy + first : nullptr;
         a.top_ids = (uint32_t*)d->top_ids + first * d->top;
         a.top_lp = (float*)d->top_lp + first * d->top;
-        a.counter = (uint32_t*)d->work;
         a.state = (float4*)(d->work + COUNTER_BYTES);
-        a.best = (uint64_t*)(a.state + (uint64_t)a.rows * slices);
+        a.best = (uint64_t*)(a.state + (uint64_t)rows * slices);
         a.vocab = d->vocab;
         a.slices = slices;
+        a.length = ((d->vocab + slices - 1) / slices + 15) / 16 * 16;  // even slices, whose ends would leave groups of lanes empty
         a.per_row = d->per_row;
         a.top = d->top;
         a.scale = d->scale;
         g->counts.launches++;
-        hipLaunchKernelGGL(d->bf16 ? logprobs_kernel<true> : logprobs_kernel<false>, dim3(a.rows * slices), dim3(THREADS), 0, g->stream, a);
+        const auto kernel = threads == FEW ? d->bf16 ? logprobs_slices_kernel<true, FEW> : logprobs_slices_kernel<false, FEW>
+                                           : d->bf16 ? logprobs_slices_kernel<true, MANY> : logprobs_slices_kernel<false, MANY>;
+        hipLaunchKernelGGL(kernel, dim3(rows * slices), dim3(threads), 0, g->stream, a);
+        if (slices > 1) {
+            g->counts.launches++;
+            hipLaunchKernelGGL(d->bf16 ? logprobs_join_kernel<true> : logprobs_join_kernel<false>, dim3(rows), dim3(256), 0, g->stream, a);
+        }
         X0NE_HIP(hipGetLastError(), "logprobs");
     }
     return X0NE_OK;
