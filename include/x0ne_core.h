@@ -275,8 +275,8 @@ x0ne_status x0ne_gpu_kv8_select(x0ne_gpu* g, const x0ne_kv8* c, uint64_t bounds,
    [4 s][4 b], byte b the columns 32 s + 8 q + 2 b (low 4 bits) and the next of a tile; scales
    [ceil(rows / 16)][ceil(cols / 128)][16 rows][128 / group] bf16. Rows and columns past the matrix are
    held as weights of 0. 4 + 16 / group bits for a weight instead of 16. (OCP MXFP4 is such a form:
-   groups of 32 whose scales are powers of two.) rows and cols 1 to 2^24, cols a multiple of 8, else
-   X0NE_ERR_FORMAT, as for a required address that is 0 or not aligned as stated. The calls run on the
+   groups of 32 whose scales are powers of two.) rows and cols 1 to 2^24, up to 2^40 weights, cols a multiple of
+   8, else X0NE_ERR_FORMAT, as for a required address that is 0 or not aligned as stated. The calls run on the
    Gpu's stream, allocate nothing, and may be captured into a graph. */
 typedef struct {
     uint64_t codes, scales;

@@ -69,11 +69,11 @@ def w4(**change):
 
 
 BAD_SHAPES = [dict(rows=0), dict(rows=(1 << 24) + 1), dict(cols=0), dict(cols=12), dict(cols=(1 << 24) + 8), dict(group=0),
-              dict(group=16), dict(group=48), dict(group=256)]
+              dict(group=16), dict(group=48), dict(group=256), dict(rows=1 << 24, cols=(1 << 16) + 8)]
 BAD_MATRICES = BAD_SHAPES + [dict(codes=0), dict(codes=4104), dict(scales=0), dict(scales=4104)]
 
 
-@pytest.mark.parametrize("rows,cols,group", [(1, 8, 128), (16, 128, 64), (17, 136, 32), (151936, 4096, 128), (1 << 24, 1 << 24, 32)])
+@pytest.mark.parametrize("rows,cols,group", [(1, 8, 128), (16, 128, 64), (17, 136, 32), (151936, 4096, 128), (1 << 24, 1 << 16, 32), (1 << 16, 1 << 24, 64)])
 def test_the_sizes_of_a_matrix(rows, cols, group):
     from x0ne_core import W4
     w = W4(0, 0, rows, cols, group)
