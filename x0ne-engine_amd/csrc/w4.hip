@@ -9,6 +9,7 @@
 
 #include "device.h"
 #include "internal.h"
+#include "w4.h"
 
 using namespace x0ne;
 
@@ -39,18 +40,39 @@ __device__ __forceinline__ bf16x8 decode8(uint32_t codes) {
     return __builtin_bit_cast(bf16x8, u32x4{decode2<0>(codes), decode2<1>(codes), decode2<2>(codes), decode2<3>(codes)});
 }
 
+// A wavefront's tile of bf16 values between memory, where it is 16 rows of 256 bytes, and the lanes of a matrix instruction: of
+// a load or store four neighbouring lanes on the 64 bytes of four rows became 16 on the 256 of one, through the wavefront's own
+// LDS, 16-byte pieces placed by an XOR of the row. Piece p of row r is at tile_at(r, p); the instruction's lane l takes piece
+// 4 s + l / 16 of row l % 16 as its word s.
+__device__ __forceinline__ uint32_t tile_at(uint32_t r, uint32_t p) { return r * 16 + ((p ^ r) & 15); }
+// What a wavefront's lanes exchange through LDS: its LDS operations go in order, so that only the compiler has to keep them.
+__device__ __forceinline__ void wave_lds() {
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+}
+
 // A wavefront takes a tile. The four lanes of a row hold 8 columns of each 32: a group's largest magnitude is theirs.
-template <int G>
+template <int G, bool STREAM>
 __global__ void __launch_bounds__(256) w4_quantise_kernel(const bf16_t* __restrict__ from, Form f) {
     const uint32_t lane = threadIdx.x & 63, t = blockIdx.x * 4 + (threadIdx.x >> 6);
     if (t >= f.tiles) return;
-    const uint32_t row = blockIdx.y * TILE_ROWS + (lane & 15), col = t * TILE_COLS + 8 * (lane >> 4);
-    u32x4 w[4];
+    __shared__ u32x4 lds[4][256];
+    u32x4* mine = lds[threadIdx.x >> 6];
+    u32x4 in[4], w[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        const uint32_t row = blockIdx.y * TILE_ROWS + 4 * j + (lane >> 4), col = t * TILE_COLS + 8 * (lane & 15);
+        const u32x4* p = reinterpret_cast<const u32x4*>(from + (size_t)row * f.cols + col);
+        in[j] = u32x4{0, 0, 0, 0};
+        if (row < f.rows && col < f.cols) in[j] = STREAM ? __builtin_nontemporal_load(p) : *p;
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j) mine[tile_at(4 * j + (lane >> 4), lane)] = in[j];
+    wave_lds();
     uint32_t top[4];  // magnitudes as bits: infinities and NaN are above all others
 #pragma unroll
     for (int s = 0; s < 4; ++s) {
-        w[s] = u32x4{0, 0, 0, 0};
-        if (row < f.rows && col + 32 * s < f.cols) w[s] = *reinterpret_cast<const u32x4*>(from + (size_t)row * f.cols + col + 32 * s);
+        w[s] = mine[tile_at(lane & 15, 4 * s + (lane >> 4))];
         uint32_t m = 0;
 #pragma unroll
         for (int i = 0; i < 4; ++i) m = max(m, max(w[s][i] & 0x7FFFu, w[s][i] >> 16 & 0x7FFFu));
@@ -103,24 +125,35 @@ __device__ __forceinline__ float scale_of(const bf16_t* scales, size_t tile, uin
     return bf2f(scales[(tile * TILE_ROWS + row) * (TILE_COLS / G) + s * 32 / G]);
 }
 
-template <int G>
+template <int G, bool STREAM>
 __global__ void __launch_bounds__(256) w4_read_kernel(Form f, bf16_t* __restrict__ to) {
     const uint32_t lane = threadIdx.x & 63, t = blockIdx.x * 4 + (threadIdx.x >> 6);
     if (t >= f.tiles) return;
-    const uint32_t row = blockIdx.y * TILE_ROWS + (lane & 15), col = t * TILE_COLS + 8 * (lane >> 4);
-    if (row >= f.rows) return;
+    __shared__ u32x4 lds[4][256];
+    u32x4* mine = lds[threadIdx.x >> 6];
     const size_t tile = (size_t)blockIdx.y * f.tiles + t;
-    const u32x4 c = *reinterpret_cast<const u32x4*>(f.codes + tile * TILE_BYTES + 16 * lane);
+    const u32x4 c = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(f.codes + tile * TILE_BYTES + 16 * lane));
 #pragma unroll
     for (int s = 0; s < 4; ++s) {
-        if (col + 32 * s >= f.cols) break;
         const float scale = scale_of<G>(f.scales, tile, lane & 15, s);
         const u32x4 v = __builtin_bit_cast(u32x4, decode8(c[s]));
         u32x4 out;
 #pragma unroll
         for (int i = 0; i < 4; ++i)
             out[i] = __builtin_bit_cast(uint32_t, bf16x2{(__bf16)(bf_lo(v[i]) * scale), (__bf16)(bf_hi(v[i]) * scale)});
-        *reinterpret_cast<u32x4*>(to + (size_t)row * f.cols + col + 32 * s) = out;
+        mine[tile_at(lane & 15, 4 * s + (lane >> 4))] = out;
+    }
+    wave_lds();
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        const u32x4 v = mine[tile_at(4 * j + (lane >> 4), lane)];
+        const uint32_t row = blockIdx.y * TILE_ROWS + 4 * j + (lane >> 4), col = t * TILE_COLS + 8 * (lane & 15);
+        u32x4* p = reinterpret_cast<u32x4*>(to + (size_t)row * f.cols + col);
+        if (row >= f.rows || col >= f.cols) continue;
+        if (STREAM)
+            __builtin_nontemporal_store(v, p);
+        else
+            *p = v;
     }
 }
 
@@ -157,9 +190,9 @@ struct Cut {
 // lane's four sums are four tokens of one row of W, whose scale of a group is one value.
 // A load of X takes 4 rows of a tile's 256 bytes, neighbouring lanes on one row, and passes through the wavefront's own
 // LDS, 16-byte chunks placed by an XOR of the row, into the operand's order.
-template <int G, int OUT, int XL, int P, int V, int U, int POLICY, bool EVEN>
-__global__ void __launch_bounds__(64 * V) w4_gemv_kernel(Form f, const bf16_t* __restrict__ x, uint32_t n, void* __restrict__ y, Cut cut) {
-    constexpr int PAIR = OUT == X0NE_W4_SWIGLU ? 2 : 1, PER = 128 / G, TT = (XL + 3) / 4, TOKENS = XL < 4 ? 4 * XL : 16 * TT;
+template <int G, bool SWIGLU, int XL, int P, int V, int U, bool EVEN>
+__global__ void __launch_bounds__(64 * V) w4_gemv_kernel(Form f, const bf16_t* __restrict__ x, uint32_t n, void* __restrict__ y, uint32_t out_f32, Cut cut) {
+    constexpr int PAIR = SWIGLU ? 2 : 1, POLICY = NT, PER = 128 / G, TT = (XL + 3) / 4, TOKENS = XL < 4 ? 4 * XL : 16 * TT;
     // A wavefront's X tile, then its sums of a unit.
     constexpr int OWN = XL * 64 > P * TT * 64 ? XL * 64 : P * TT * 64;
     __shared__ u32x4 lds[V][OWN];
@@ -208,17 +241,18 @@ __global__ void __launch_bounds__(64 * V) w4_gemv_kernel(Form f, const bf16_t* _
     auto multiply = [&](int slot) {
 #pragma unroll
         for (int i = 0; i < XL; ++i) {
-            const uint32_t r = 4 * i + (lane >> 4);
-            mine[r * 16 + ((lane ^ r) & 15)] = a[slot][i];
+            mine[tile_at(4 * i + (lane >> 4), lane)] = a[slot][i];
         }
+        wave_lds();
         bf16x8 frag[TT][4];
 #pragma unroll
         for (int i = 0; i < TT; ++i)
 #pragma unroll
             for (int s = 0; s < 4; ++s) {
                 const uint32_t r = (16 * i + (lane & 15)) & (4 * XL - 1);
-                frag[i][s] = __builtin_bit_cast(bf16x8, mine[r * 16 + ((4 * s + (lane >> 4)) ^ (r & 15))]);
+                frag[i][s] = __builtin_bit_cast(bf16x8, mine[tile_at(r, 4 * s + (lane >> 4))]);
             }
+        wave_lds();
 #pragma unroll
         for (int p = 0; p < P; ++p) {
             f32x4 acc[TT] = {};
@@ -250,12 +284,12 @@ __global__ void __launch_bounds__(64 * V) w4_gemv_kernel(Form f, const bf16_t* _
             const uint32_t to = token0 + 16 * i + 4 * (lane >> 4) + j;
             if (row >= out_rows || to >= min(n, token0 + TOKENS)) continue;
             const size_t at = (size_t)to * out_rows + row;
-            if (OUT == X0NE_W4_F32)
-                static_cast<float*>(y)[at] = r[0][j];
-            else if (OUT == X0NE_W4_BF16)
-                static_cast<bf16_t*>(y)[at] = f2bf(r[0][j]);
-            else
+            if (SWIGLU)
                 static_cast<bf16_t*>(y)[at] = f2bf(r[0][j] / (1.0f + expf(-r[0][j])) * r[PAIR - 1][j]);
+            else if (out_f32)
+                static_cast<float*>(y)[at] = r[0][j];
+            else
+                static_cast<bf16_t*>(y)[at] = f2bf(r[0][j]);
         }
     };
     // The wavefronts' sums of a unit, and those of the other blocks that have tiles of it: each leaves its part, and the
@@ -350,6 +384,8 @@ __global__ void __launch_bounds__(64 * V) w4_gemv_kernel(Form f, const bf16_t* _
 
 x0ne_status bad(const char* what, const std::string& why) { return fail(X0NE_ERR_FORMAT, std::string(what) + ": " + why); }
 
+static_assert(W4_COUNTERS <= GPU_COUNTERS && W4_PARTS_BYTES <= TILE_PARTS_BYTES, "the Gpu's workspaces");
+
 constexpr uint32_t MOST = 1u << 24;
 constexpr uint64_t MOST_WEIGHTS = 1ull << 40;  // more than memory holds; tiles are counted in 32 bits
 
@@ -373,6 +409,10 @@ uint64_t tiles_of(const x0ne_w4* w) { return (uint64_t)((w->rows + 15) / 16) * (
 Form form_of(const x0ne_w4* w) {
     return Form{(uint8_t*)w->codes, (bf16_t*)w->scales, w->rows, w->cols, (w->cols + TILE_COLS - 1) / TILE_COLS};
 }
+
+constexpr uint64_t INFINITY_CACHE = 256ull << 20;
+// Whether a matrix's bf16 form bypasses the Infinity Cache.
+bool streams(const x0ne_w4* w) { return (uint64_t)w->rows * w->cols * 2 > INFINITY_CACHE / 2; }
 
 // grid y holds at most 65535 panels: a taller matrix is several launches.
 template <class Launch>
@@ -406,7 +446,8 @@ extern "C" x0ne_status x0ne_gpu_w4_quantise(x0ne_gpu* g, const x0ne_w4* w, uint6
     if (!from || from % 16) return bad(what, "a bf16 matrix (16-byte aligned) is required");
     if (!g) return fail(X0NE_ERR_GPU, "no device");
     const OnDevice on(g->device);
-    const auto kernel = w->group == 32 ? w4_quantise_kernel<32> : w->group == 64 ? w4_quantise_kernel<64> : w4_quantise_kernel<128>;
+    const auto kernel = streams(w) ? w->group == 32 ? w4_quantise_kernel<32, true> : w->group == 64 ? w4_quantise_kernel<64, true> : w4_quantise_kernel<128, true>
+                                   : w->group == 32 ? w4_quantise_kernel<32, false> : w->group == 64 ? w4_quantise_kernel<64, false> : w4_quantise_kernel<128, false>;
     return by_panels(g, what, w, [&](dim3 grid, const Form& f, size_t at) {
         hipLaunchKernelGGL(kernel, grid, dim3(256), 0, g->stream, (const bf16_t*)from + at, f);
     });
@@ -418,39 +459,51 @@ extern "C" x0ne_status x0ne_gpu_w4_read(x0ne_gpu* g, const x0ne_w4* w, uint64_t 
     if (!to || to % 16) return bad(what, "a bf16 matrix (16-byte aligned) is required");
     if (!g) return fail(X0NE_ERR_GPU, "no device");
     const OnDevice on(g->device);
-    const auto kernel = w->group == 32 ? w4_read_kernel<32> : w->group == 64 ? w4_read_kernel<64> : w4_read_kernel<128>;
+    const auto kernel = streams(w) ? w->group == 32 ? w4_read_kernel<32, true> : w->group == 64 ? w4_read_kernel<64, true> : w4_read_kernel<128, true>
+                                   : w->group == 32 ? w4_read_kernel<32, false> : w->group == 64 ? w4_read_kernel<64, false> : w4_read_kernel<128, false>;
     return by_panels(g, what, w, [&](dim3 grid, const Form& f, size_t at) {
         hipLaunchKernelGGL(kernel, grid, dim3(256), 0, g->stream, f, (bf16_t*)to + at);
     });
 }
 
-static Cut cut_of(const Form& f, uint32_t P, uint32_t V, uint32_t groups, uint32_t slots, bool even, x0ne_gpu* g) {
-    const uint32_t units = ((f.rows + 15) / 16 + P - 1) / P, rounds = (f.tiles + V - 1) / V, each = std::max(1u, slots / groups);
-    Cut c = {units * rounds, rounds, even ? (units * rounds + each - 1) / each : (units + each - 1) / each * rounds, 0, groups, nullptr, nullptr};
-    c.blocks = (c.all + c.run - 1) / c.run;
-    if (even) c.parts = own_parts(g), c.counters = g->counters;
-    return c;
+template <bool SWIGLU, int XL, int P, int V, int U, bool EVEN>
+static void launch_as(const x0ne_gpu* g, const x0ne_w4* w, const W4Plan& p, const bf16_t* x, uint32_t n, void* y, uint32_t out_f32, float* parts) {
+    const auto kernel = w->group == 32   ? w4_gemv_kernel<32, SWIGLU, XL, P, V, U, EVEN>
+                        : w->group == 64 ? w4_gemv_kernel<64, SWIGLU, XL, P, V, U, EVEN>
+                                         : w4_gemv_kernel<128, SWIGLU, XL, P, V, U, EVEN>;
+    const Cut cut = {p.units * p.rounds, p.rounds, p.run, p.blocks, p.groups, parts, g->counters};
+    hipLaunchKernelGGL(kernel, dim3((p.blocks + 7) / 8 * 8 * p.groups), dim3(64 * V), 0, g->stream, form_of(w), x, n, y, out_f32, cut);
 }
 
-template <int OUT, int XL, int P, int V, int U, int POLICY, bool EVEN>
-static void launch_gemv(x0ne_gpu* g, const x0ne_w4* w, const bf16_t* x, uint32_t n, void* y, uint32_t per_cu) {
-    const auto kernel = w->group == 32   ? w4_gemv_kernel<32, OUT, XL, P, V, U, POLICY, EVEN>
-                        : w->group == 64 ? w4_gemv_kernel<64, OUT, XL, P, V, U, POLICY, EVEN>
-                                         : w4_gemv_kernel<128, OUT, XL, P, V, U, POLICY, EVEN>;
-    const Form f = form_of(w);
-    const Cut cut = cut_of(f, P, V, (n + 4 * XL - 1) / (4 * XL), per_cu * g->cus, EVEN, g);
-    hipLaunchKernelGGL(kernel, dim3((cut.blocks + 7) / 8 * 8 * cut.groups), dim3(64 * V), 0, g->stream, f, x, n, y, cut);
-}
-
-template <int OUT>
-static void launch_gemv(x0ne_gpu* g, const x0ne_w4* w, const bf16_t* x, uint32_t n, void* y) {
-    constexpr int PAIR = OUT == X0NE_W4_SWIGLU ? 2 : 1;
-    if (n <= 4)
-        launch_gemv<OUT, 1, PAIR, 8, 2, NT, false>(g, w, x, n, y, 3);
-    else if (n <= 16 && (w->rows + 63) / 64 <= GPU_COUNTERS && own_parts(g))
-        launch_gemv<OUT, 4, 4, 8, 1, NT, true>(g, w, x, n, y, 1);
-    else
-        launch_gemv<OUT, 4, 4, 8, 1, 0, false>(g, w, x, n, y, 2);
+// The kernel of a plan; false for one that has none.
+template <bool SWIGLU>
+static bool launch_plan(const x0ne_gpu* g, const x0ne_w4* w, const W4Plan& p, const bf16_t* x, uint32_t n, void* y, uint32_t out_f32, float* parts) {
+    constexpr uint32_t PAIR = SWIGLU ? 2 : 1;
+    const auto go = [&](auto launch) {
+        launch(g, w, p, x, n, y, out_f32, parts);
+        return true;
+    };
+    if (p.xl == 1 && p.panels == PAIR && !p.even) {
+        if (p.waves == 4) return go(launch_as<SWIGLU, 1, PAIR, 4, 2, false>);
+        if (p.waves == 8) return go(launch_as<SWIGLU, 1, PAIR, 8, 2, false>);
+        if (p.waves == 16) return go(launch_as<SWIGLU, 1, PAIR, 16, 2, false>);
+    }
+    if (p.waves != 8) return false;
+    if (p.panels == 1 && !SWIGLU && !p.even) {
+        if (p.xl == 2) return go(launch_as<false, 2, 1, 8, 1, false>);
+        if (p.xl == 4) return go(launch_as<false, 4, 1, 8, 1, false>);
+    }
+    if (p.panels == 2 && !p.even) {
+        if (p.xl == 2) return go(launch_as<SWIGLU, 2, 2, 8, 1, false>);
+        if (p.xl == 4) return go(launch_as<SWIGLU, 4, 2, 8, 1, false>);
+        if (p.xl == 8) return go(launch_as<SWIGLU, 8, 2, 8, 1, false>);
+    }
+    if (p.panels == 4) {
+        if (p.xl == 2) return go(p.even ? launch_as<SWIGLU, 2, 4, 8, 1, true> : launch_as<SWIGLU, 2, 4, 8, 1, false>);
+        if (p.xl == 4) return go(p.even ? launch_as<SWIGLU, 4, 4, 8, 1, true> : launch_as<SWIGLU, 4, 4, 8, 1, false>);
+        if (p.xl == 8) return go(p.even ? launch_as<SWIGLU, 8, 4, 8, 1, true> : launch_as<SWIGLU, 8, 4, 8, 1, false>);
+    }
+    return false;
 }
 
 extern "C" x0ne_status x0ne_gpu_w4_gemv(x0ne_gpu* g, const x0ne_w4* w, uint64_t x, uint64_t n, uint64_t y, uint32_t out) {
@@ -464,9 +517,13 @@ extern "C" x0ne_status x0ne_gpu_w4_gemv(x0ne_gpu* g, const x0ne_w4* w, uint64_t 
     if (!g) return fail(X0NE_ERR_GPU, "no device");
     if (n == 0) return X0NE_OK;
     const OnDevice on(g->device);
+    const bool swiglu = out == X0NE_W4_SWIGLU;
+    W4Plan p = w4_plan(w->rows, w->cols, (uint32_t)n, swiglu, g->cus, true);
+    float* parts = p.even ? own_parts(g) : nullptr;
+    if (p.even && !parts) p = w4_plan(w->rows, w->cols, (uint32_t)n, swiglu, g->cus, false);
+    if (!(swiglu ? launch_plan<true> : launch_plan<false>)(g, w, p, (const bf16_t*)x, (uint32_t)n, (void*)y, out == X0NE_W4_F32, parts))
+        return fail(X0NE_ERR_GPU, std::string(what) + ": no kernel for its plan");
     g->counts.launches++;
-    const auto launch = out == X0NE_W4_BF16 ? launch_gemv<X0NE_W4_BF16> : out == X0NE_W4_F32 ? launch_gemv<X0NE_W4_F32> : launch_gemv<X0NE_W4_SWIGLU>;
-    launch(g, w, (const bf16_t*)x, (uint32_t)n, (void*)y);
     X0NE_HIP(hipGetLastError(), what);
     return X0NE_OK;
 }
