@@ -277,7 +277,7 @@ x0ne_status x0ne_gpu_kv8_select(x0ne_gpu* g, const x0ne_kv8* c, uint64_t bounds,
    held as weights of 0. 4 + 16 / group bits for a weight instead of 16. (OCP MXFP4 is such a form:
    groups of 32 whose scales are powers of two.) rows and cols 1 to 2^24, up to 2^40 weights, cols a multiple of
    8, else X0NE_ERR_FORMAT, as for a required address that is 0 or not aligned as stated. The calls run on the
-   Gpu's stream, allocate nothing, and may be captured into a graph. */
+   Gpu's stream and may be captured into a graph. */
 typedef struct {
     uint64_t codes, scales;
     uint32_t rows, cols, group;
@@ -295,7 +295,10 @@ x0ne_status x0ne_gpu_w4_read(x0ne_gpu* g, const x0ne_w4* w, uint64_t to);
 /* Y = X W^T, X [n][cols] bf16 row-major (16-byte aligned): products and sums in f32, a group's sum
    times its scale, rounded once. out X0NE_W4_BF16, X0NE_W4_F32: Y [n][rows]; X0NE_W4_SWIGLU: W is
    [gate; up] (rows a multiple of 32) and Y [n][rows / 2] bf16 = silu(gate) up of the f32 sums. Y is
-   4-byte aligned and not in X. n up to 65535 x 16; X below 4 GiB. The same call gives the same bits. */
+   4-byte aligned and not in X. n up to 2^24; for one token to a few dozen (past 256 rows the read-back
+   and x0ne_gpu_gemv are faster). Some shapes' sums go in parts through the Gpu's workspace of
+   x0ne_gpu_gemv (allocated at the first call that needs it or when a capture begins; without it their
+   sums stay whole). The same call gives the same bits. */
 enum { X0NE_W4_BF16 = 0, X0NE_W4_F32 = 1, X0NE_W4_SWIGLU = 2 };
 x0ne_status x0ne_gpu_w4_gemv(x0ne_gpu* g, const x0ne_w4* w, uint64_t x, uint64_t n, uint64_t y, uint32_t out);
 

@@ -8,7 +8,7 @@ import numpy as np
 import pytest
 
 import w4_reference as R
-from common import ROOT
+from common import ROOT, run_cpp
 
 
 # -- the plain forms --
@@ -91,8 +91,8 @@ def test_w4_refusals_come_before_any_device():
              "read": lambda w, x=256, **k: L.x0ne_gpu_w4_read(None, w, x),
              "gemv": lambda w, x=256, n=3, y=256, out=0: L.x0ne_gpu_w4_gemv(None, w, x, n, y, out)}
     more = {"quantise": [dict(x=0), dict(x=264)], "read": [dict(x=0), dict(x=264)],
-            "gemv": [dict(x=0), dict(x=264), dict(y=0), dict(y=258), dict(out=3), dict(n=65535 * 16 + 1), dict(n=1 << 63),
-                     dict(rows=16, out=2), dict(rows=40, out=2), dict(n=1 << 12, cols=1 << 20)]}
+            "gemv": [dict(x=0), dict(x=264), dict(y=0), dict(y=258), dict(out=3), dict(n=(1 << 24) + 1), dict(n=1 << 63),
+                     dict(rows=16, out=2), dict(rows=40, out=2)]}
     for name, call in calls.items():
         for change in BAD_MATRICES + more[name]:
             of_call = {k: v for k, v in change.items() if k in ("x", "n", "y", "out")}
@@ -156,3 +156,55 @@ def test_the_rust_and_python_structs_are_the_headers(name):
     assert mirror._fields_ == [(n, {"uint64_t": C.c_uint64, "uint32_t": C.c_uint32, "float": C.c_float}[k]) for n, k in fields]
     for call in re.findall(r"\b(x0ne_\w*(?:w4|logprobs)\w*)\s*\(", header):
         assert f"pub fn {call}(" in rust, call
+
+
+# -- how a launch is cut --
+
+def plans(tmp_path, shapes):
+    """(xl, panels, waves, even, units, rounds, groups, run, blocks, rows at once) of (rows, cols, n, swiglu, parts)."""
+    out = run_cpp(tmp_path, "w4_plan.cpp", "".join(" ".join(str(int(v)) for v in s) + "\n" for s in shapes))
+    return [tuple(int(v) for v in line.split()) for line in out.splitlines()]
+
+
+def test_a_plan_covers_its_matrix(tmp_path):
+    """Over sizes to the largest: every panel, tile and row of X is some block's, the blocks' runs are all the rounds, a unit
+    a block unless they are even, and grids, counters and parts are within what there is."""
+    sizes = [1, 15, 16, 17, 100, 1000, 4096, 4104, 6144, 12288, 24576, 51200, 151936, 1 << 20, 1 << 24]
+    shapes = [(r, max(8, c // 8 * 8), n, s, p) for r in sizes for c in sizes for n in (1, 4, 5, 8, 9, 16, 17, 32, 33, 64, 65, 96, 200, 512)
+              for s in (0, 1) for p in (0, 1) if r * c <= 1 << 40 and not (s and r % 32)]
+    for (rows, cols, n, swiglu, parts), (xl, panels, waves, even, units, rounds, groups, run, blocks, most) in zip(shapes, plans(tmp_path, shapes)):
+        at = (rows, cols, n, swiglu, parts)
+        assert 1 <= most <= 512 and most * cols * 2 < 1 << 32 and (most == 512 or most % 32 == 0), at
+        if n > most:
+            continue
+        tiles = -(-cols // 128)
+        assert units * panels >= -(-rows // 16) > (units - 1) * panels and rounds * waves >= tiles > (rounds - 1) * waves, at
+        assert groups * 4 * xl >= n > (groups - 1) * 4 * xl and not (swiglu and panels % 2), at
+        assert blocks * run >= units * rounds > (blocks - 1) * run and units * rounds < 1 << 32, at
+        assert -(-blocks // 8) * 8 * groups * 64 * waves < 1 << 32, at
+        if even:
+            tokens = -(-xl // 4)
+            assert parts and units * groups <= 65536 and blocks * groups * 2 * panels * tokens * 1024 <= 64 << 20, at
+            assert blocks * groups <= 256 or blocks == 1, at
+        else:
+            assert run == rounds and blocks == units, at
+
+
+def kernels_of(tmp_path, shapes):
+    return {(bool(s[3]),) + p[:4] for s, p in zip(shapes, plans(tmp_path, shapes))}
+
+
+def test_the_gpu_tests_reach_every_kernel_that_a_plan_uses(tmp_path):
+    """Those of the projections of the Qwen3 shapes and of a grid of others, for one row to 128, are among those of the exact
+    sums' test, for which there is a kernel each."""
+    from bench import QWEN3_0_6B, QWEN3_8B, QWEN3_32B
+    from test_gpu_w4 import EXACT
+    sizes = [16, 64, 256, 1000, 2048, 4096, 8192, 16384, 32768, 65536]
+    shapes = [(r, c, n) for r in sizes for c in sizes for n in (1, 4, 5, 8, 9, 16, 17, 32, 33, 64, 65, 128)]
+    for m in (QWEN3_0_6B, QWEN3_8B, QWEN3_32B):
+        h, i, d = m["hidden_size"], m["intermediate_size"], m["head_dim"]
+        q, kv = m["num_attention_heads"] * d, m["num_key_value_heads"] * d
+        shapes += [(r, c, n) for r, c in ((q + 2 * kv, h), (h, q), (2 * i, h), (h, i), (m["vocab_size"], h)) for n in range(1, 129)]
+    used = kernels_of(tmp_path, [(*s, swiglu, 1) for s in shapes for swiglu in (0, 1) if not (swiglu and s[0] % 32)])
+    tested = kernels_of(tmp_path, [(rows, cols, n, swiglu, 1) for rows, cols, n, _ in EXACT for swiglu in (0, 1) if not (swiglu and rows % 32)])
+    assert used <= tested, used - tested

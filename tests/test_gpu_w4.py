@@ -134,11 +134,20 @@ def test_products_of_large_matrices(kernels, rows, cols, n):
     check_product(w, vals(x), y, "f32", 128)
 
 
-@pytest.mark.parametrize("rows,cols,n,group", [(32, 8, 1, 32), (64, 1160, 1, 32), (64, 4096, 2, 64), (2080, 640, 16, 128), (48, 2000, 23, 32),
-                                               (8256, 384, 37, 64), (16, 25600, 5, 32), (6144, 1024, 64, 128), (70000, 256, 3, 32)])
+# Rows, columns, rows of x, group: every kernel that a plan uses, at sizes of its own (test_cpu_w4.py).
+EXACT = [(32, 8, 1, 32), (2080, 640, 3, 128), (16416, 136, 2, 32), (70000, 256, 3, 32),  # 4 wavefronts
+         (64, 4104, 2, 64), (6176, 2056, 4, 32),  # 8
+         (96, 8200, 1, 32), (1024, 8264, 3, 64), (16, 25600, 1, 128),  # 16
+         (96, 1160, 5, 32), (6176, 136, 8, 64), (8224, 392, 7, 128), (64, 6152, 8, 32), (16416, 640, 6, 64), (16, 25600, 5, 32),
+         (96, 648, 16, 32), (6176, 200, 12, 32), (8224, 264, 16, 64), (160, 6280, 11, 128), (16448, 1032, 9, 32),
+         (544, 2000, 23, 32), (96, 264, 64, 64), (8224, 328, 20, 128), (64, 6152, 45, 32), (16416, 520, 33, 64), (128, 8200, 70, 64),
+         (4128, 6152, 96, 128), (96, 136, 600, 64), (33, 6152, 130, 32)]
+
+
+@pytest.mark.parametrize("rows,cols,n,group", EXACT)
 def test_products_whose_sums_are_exact(kernels, rows, cols, n, group):
     """Whole x up to 7, codes whole multiples of .5 and scales 1, 2 and 4: every sum is exact in f32 (below 2^24 halves),
-    so that each weight, scale and x shows in its place."""
+    so that each weight, scale and x shows in its place. SwiGLU of them: one rounding to bf16, and 8 of f32."""
     rng = np.random.default_rng(rows + cols + n)
     code = np.zeros((-(-rows // 16) * 16, -(-cols // 128) * 128), np.int64)
     code[:rows, :cols] = rng.integers(0, 16, (rows, cols))
@@ -146,8 +155,17 @@ def test_products_whose_sums_are_exact(kernels, rows, cols, n, group):
     x = rng.integers(-7, 8, (n, cols)).astype(np.float64)
     assert 7 * 6 * 4 * 2 * cols < 1 << 24
     codes, scales = R.lay(code, s)
-    y = kernels.w4_gemv(codes, scales, rows, cols, group, bits(x), "f32")
-    assert (y == x @ R.values(code, s)[:rows, :cols].T).all()
+    want = x @ R.values(code, s)[:rows, :cols].T
+    y = kernels.w4_gemv(codes, scales, rows, cols, group, bits(x), "f32", calls=2)
+    assert (y == want).all()
+    assert (kernels.w4_gemv(codes, scales, rows, cols, group, bits(x), "bf16") == bits(want)).all()
+    if rows % 32 == 0:
+        gate, up = want[:, :rows // 2], want[:, rows // 2:]
+        y = vals(kernels.w4_gemv(codes, scales, rows, cols, group, bits(x), "swiglu"))
+        with np.errstate(over="ignore"):
+            want = silu(gate) * up
+        # An exponential below 2^-126 is off by half of f32's least step, 2^-149.
+        assert (np.abs(y - want) <= (2.0 ** -8 + 8 * 2.0 ** -24) * np.abs(want) + 2.0 ** -149 * np.abs(gate * up) + 2.0 ** -134).all()
 
 
 @pytest.mark.parametrize("n", [1, 6, 20, 64])
@@ -184,7 +202,7 @@ def test_swiglu_of_far_gates(kernels):
     y = vals(kernels.w4_gemv(codes, scales, 32, 128, 32, bits(x), "swiglu"))
     with np.errstate(over="ignore"):
         want = silu(x[:, 0]) * 1.5
-    assert (np.abs(y - want[:, None]) <= 2.0 ** -7 * np.abs(want)[:, None] + 1e-37).all()
+    assert (np.abs(y - want[:, None]) <= (2.0 ** -8 + 8 * 2.0 ** -24) * np.abs(want)[:, None] + 2.0 ** -149 * 1.5 * np.abs(x[:, :1]) + 2.0 ** -134).all()
 
 
 @pytest.mark.parametrize("rows,cols,n,out", [(4096, 1024, 1, "bf16"), (2048, 2048, 33, "swiglu")])
@@ -194,3 +212,89 @@ def test_the_same_call_gives_the_same_bits(kernels, rows, cols, n, out):
     x = bits(rng.standard_normal((n, cols)))
     first = kernels.w4_gemv(codes, scales, rows, cols, 64, x, out)
     assert (kernels.w4_gemv(codes, scales, rows, cols, 64, x, out, calls=5) == first).all()
+
+
+def test_graphs_that_share_the_workspace_of_parts(kernels):
+    """Two graphs whose products leave their sums in parts, one with a bf16 product in K slices over the same workspace,
+    replayed in turn with eager calls of a third shape between."""
+    from x0ne_core import Arena, W4
+    from x0ne_core.arena import Class
+    rng = np.random.default_rng(12)
+    g, shapes = kernels.gpu, [(160, 6280, 11, "f32"), (96, 8200, 45, "swiglu"), (16416, 640, 6, "bf16")]
+    arrays = {}
+    for i, (rows, cols, n, out) in enumerate(shapes):
+        codes, scales, _ = held(rng, rows, cols, 64)
+        arrays |= {f"c{i}": codes, f"s{i}": scales, f"x{i}": bits(rng.standard_normal((n, cols))), f"y{i}": np.zeros(n * rows, np.float32)}
+    arrays |= {"w": bits(rng.standard_normal((512, 4096))), "x": bits(rng.standard_normal((40, 4096))), "y": np.zeros(40 * 512, np.float32)}
+    a = Arena()
+    sl = {k: a.alloc(k, v.nbytes, Class.CLIENT_DATA) for k, v in arrays.items()}
+    a.freeze(g)
+    for k, v in arrays.items():
+        a.write(sl[k], 0, v)
+    at = {k: a.ptr(v) for k, v in sl.items()}
+
+    def call(i):
+        rows, cols, n, out = shapes[i]
+        g.w4_gemv(W4(at[f"c{i}"], at[f"s{i}"], rows, cols, 64), at[f"x{i}"], n, at[f"y{i}"], out)
+
+    def sliced():
+        g.gemv(at["w"], 512, 4096, at["x"], 40, at["y"], True)
+
+    def result(k):
+        g.sync()
+        got = a.read_array(sl[k], 0, arrays[k].size, np.float32).copy()
+        a.write(sl[k], 0, np.zeros(arrays[k].size, np.float32))
+        return got
+
+    want = {}
+    for i in range(3):
+        call(i)
+        want[f"y{i}"] = result(f"y{i}")
+    sliced()
+    want["y"] = result("y")
+    one, two = g.capture(lambda: (call(0), sliced())), g.capture(lambda: (call(1), call(0)))
+    for _ in range(4):
+        g.launch_graph(one)
+        g.launch_graph(two)
+        call(2)
+        g.launch_graph(one)
+        for k, v in want.items():
+            assert (result(k).view(np.uint32) == v.view(np.uint32)).all(), k
+    one.close()
+    two.close()
+
+
+def test_matrices_in_one_buffer_keep_to_their_own(kernels):
+    """Two matrices whose codes and scales lie one behind the other, quantised and multiplied: nothing of the one shows in the
+    other, and what lies behind the last stays."""
+    from x0ne_core import Arena, W4
+    from x0ne_core.arena import Class
+    rng = np.random.default_rng(13)
+    g, shapes, group = kernels.gpu, [(33, 200), (17, 136)], 32
+    ws = [trained(rng, *s) for s in shapes]
+    x = bits(rng.standard_normal((3, 200)))
+    ds = [W4(0, 0, *s, group) for s in shapes]
+    code_at, scale_at = np.cumsum([0] + [d.code_bytes() for d in ds]), np.cumsum([0] + [d.scale_bytes() for d in ds])
+    a = Arena()
+    need = {"codes": int(code_at[-1]) + 1024, "scales": int(scale_at[-1]) + 256, "w0": ws[0].nbytes, "w1": ws[1].nbytes, "x": x.nbytes, "y0": 3 * 33 * 4,
+            "y1": 3 * 17 * 4}
+    sl = {k: a.alloc(k, v, Class.CLIENT_DATA) for k, v in need.items()}
+    a.freeze(g)
+    at = {k: a.ptr(v) for k, v in sl.items()}
+    for k in ("codes", "scales"):
+        a.write(sl[k], 0, np.full(need[k], 0xA5, np.uint8))
+    for i, w in enumerate(ws):
+        a.write(sl[f"w{i}"], 0, w)
+    a.write(sl["x"], 0, x)
+    for i, s in enumerate(shapes):
+        ds[i] = W4(at["codes"] + int(code_at[i]), at["scales"] + int(scale_at[i]), *s, group)
+        g.w4_quantise(ds[i], at[f"w{i}"])
+    g.w4_gemv(ds[0], at["x"], 3, at["y0"], "f32")
+    g.w4_gemv(ds[1], at["x"], 3, at["y1"], "f32")  # its rows of x are 136 long: x as [3][136]
+    g.sync()
+    for i, (rows, cols) in enumerate(shapes):
+        code, s = R.quantise(vals(ws[i]), group)
+        xs = vals(x).ravel()[:3 * cols].reshape(3, cols)
+        check_product(R.values(code, s)[:rows, :cols], xs, a.read_array(sl[f"y{i}"], 0, 3 * rows, np.float32).reshape(3, rows), "f32", group)
+    for k, end in (("codes", code_at[-1]), ("scales", scale_at[-1])):
+        assert (a.read_array(sl[k], 0, need[k], np.uint8)[int(end):] == 0xA5).all()

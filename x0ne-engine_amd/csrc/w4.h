@@ -6,6 +6,9 @@
 // Counters that a launch whose units are cut may use, and bytes of their sums.
 constexpr uint64_t W4_COUNTERS = 65536, W4_PARTS_BYTES = 64ull << 20;
 
+// Rows of X that a launch takes.
+inline uint32_t w4_rows_at_once(uint32_t cols) { return std::min<uint32_t>(512, (uint32_t)(0xFFFFFFF0ull / (2 * (uint64_t)cols)) / 32 * 32); }
+
 struct W4Plan {
     uint32_t xl;      // loads of 4 rows of X to a wavefront's tile: 1, 2, 4 or 8
     uint32_t panels;  // panels of 16 rows of W to a unit
@@ -52,7 +55,9 @@ inline W4Plan w4_plan(uint32_t rows, uint32_t cols, uint32_t n, bool swiglu, uin
     p.units = units(p.panels);
     p.rounds = (tiles + p.waves - 1) / p.waves;
     p.run = p.rounds;
-    const uint64_t each = std::max<uint64_t>(1, cus / p.groups);  // blocks to a group
+    // Blocks to a group: whole rounds of the 8 XCDs, so that none gets a block more than it has CUs (96 rows of 24576 x 4096:
+    // 65 us with 85 blocks to each of three groups, 39 with 80).
+    const uint64_t each = std::max<uint64_t>(1, cus / p.groups >= 8 ? cus / 8 / p.groups * 8 : cus / p.groups);
     p.even = p.even && parts && (uint64_t)p.units * p.groups <= W4_COUNTERS &&
              each * p.groups * 2 * p.panels * ((p.xl + 3) / 4) * 1024 <= W4_PARTS_BYTES;
     if (p.even) p.run = (uint32_t)(((uint64_t)p.units * p.rounds + each - 1) / each);

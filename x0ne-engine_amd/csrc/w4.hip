@@ -177,6 +177,12 @@ struct Piece {
     uint32_t scales[G == 32 ? 2 : 1];
 };
 
+// x / (1 + e^-x), by an exponential that does not overflow for far gates.
+__device__ __forceinline__ float silu(float x) {
+    const float e = expf(-fabsf(x));
+    return x * ((x < 0.f ? e : 1.f) / (1.f + e));
+}
+
 // How a launch's blocks share the work: a unit is `rounds` rounds of a tile to each wavefront, and block b takes the rounds
 // from b run to (b + 1) run - 1 of all units' one behind the other.
 struct Cut {
@@ -285,7 +291,7 @@ __global__ void __launch_bounds__(64 * V) w4_gemv_kernel(Form f, const bf16_t* _
             if (row >= out_rows || to >= min(n, token0 + TOKENS)) continue;
             const size_t at = (size_t)to * out_rows + row;
             if (SWIGLU)
-                static_cast<bf16_t*>(y)[at] = f2bf(r[0][j] / (1.0f + expf(-r[0][j])) * r[PAIR - 1][j]);
+                static_cast<bf16_t*>(y)[at] = f2bf(silu(r[0][j]) * r[PAIR - 1][j]);
             else if (out_f32)
                 static_cast<float*>(y)[at] = r[0][j];
             else
@@ -511,19 +517,24 @@ extern "C" x0ne_status x0ne_gpu_w4_gemv(x0ne_gpu* g, const x0ne_w4* w, uint64_t 
     X0NE_TRY(check_matrix(what, w));
     if (out > X0NE_W4_SWIGLU) return bad(what, "no output " + std::to_string(out));
     if (out == X0NE_W4_SWIGLU && w->rows % 32) return bad(what, std::to_string(w->rows) + " rows of gate and up (a multiple of 32)");
-    if (n > 65535 * 16) return bad(what, std::to_string(n) + " rows of x (up to 65535 x 16)");
-    if (n * w->cols * 2 >= (1ull << 32) - 16) return bad(what, std::to_string(n) + " rows of " + std::to_string(w->cols) + " columns of x (below 4 GiB)");
+    if (n > MOST) return bad(what, std::to_string(n) + " rows of x (up to 2^24)");
     if (!x || !y || x % 16 || y % 4) return bad(what, "x (16-byte aligned) and y (4-byte aligned) are required");
     if (!g) return fail(X0NE_ERR_GPU, "no device");
     if (n == 0) return X0NE_OK;
     const OnDevice on(g->device);
     const bool swiglu = out == X0NE_W4_SWIGLU;
-    W4Plan p = w4_plan(w->rows, w->cols, (uint32_t)n, swiglu, g->cus, true);
-    float* parts = p.even ? own_parts(g) : nullptr;
-    if (p.even && !parts) p = w4_plan(w->rows, w->cols, (uint32_t)n, swiglu, g->cus, false);
-    if (!(swiglu ? launch_plan<true> : launch_plan<false>)(g, w, p, (const bf16_t*)x, (uint32_t)n, (void*)y, out == X0NE_W4_F32, parts))
-        return fail(X0NE_ERR_GPU, std::string(what) + ": no kernel for its plan");
-    g->counts.launches++;
-    X0NE_HIP(hipGetLastError(), what);
+    const uint64_t out_row = (swiglu ? w->rows / 2 : w->rows) * (out == X0NE_W4_F32 ? 4ull : 2ull);
+    // X in pieces of which a launch's offsets are below 4 GiB and its threads below 2^32.
+    for (uint64_t first = 0, some; first < n; first += some) {
+        some = std::min<uint64_t>(n - first, w4_rows_at_once(w->cols));
+        W4Plan p = w4_plan(w->rows, w->cols, (uint32_t)some, swiglu, g->cus, true);
+        float* parts = p.even ? own_parts(g) : nullptr;
+        if (p.even && !parts) p = w4_plan(w->rows, w->cols, (uint32_t)some, swiglu, g->cus, false);
+        if (!(swiglu ? launch_plan<true> : launch_plan<false>)(g, w, p, (const bf16_t*)x + first * w->cols, (uint32_t)some, (uint8_t*)y + first * out_row,
+                                                               out == X0NE_W4_F32, parts))
+            return fail(X0NE_ERR_GPU, std::string(what) + ": no kernel for its plan");
+        g->counts.launches++;
+        X0NE_HIP(hipGetLastError(), what);
+    }
     return X0NE_OK;
 }
