@@ -416,8 +416,10 @@ Form form_of(const x0ne_w4* w) {
     return Form{(uint8_t*)w->codes, (bf16_t*)w->scales, w->rows, w->cols, (w->cols + TILE_COLS - 1) / TILE_COLS};
 }
 
+// Whether a matrix's bf16 form bypasses the Infinity Cache: one of more than half of it, which is seldom there alone (24576 x
+// 4096, 201 MB, quantised and read back into another 201 MB: 101 us through it, 81 past it; alone and quantised again and again
+// 43 through it, 48 past it; 51200 x 5120 read back 116 and 108).
 constexpr uint64_t INFINITY_CACHE = 256ull << 20;
-// Whether a matrix's bf16 form bypasses the Infinity Cache.
 bool streams(const x0ne_w4* w) { return (uint64_t)w->rows * w->cols * 2 > INFINITY_CACHE / 2; }
 
 // grid y holds at most 65535 panels: a taller matrix is several launches.
@@ -465,7 +467,8 @@ extern "C" x0ne_status x0ne_gpu_w4_read(x0ne_gpu* g, const x0ne_w4* w, uint64_t 
     if (!to || to % 16) return bad(what, "a bf16 matrix (16-byte aligned) is required");
     if (!g) return fail(X0NE_ERR_GPU, "no device");
     const OnDevice on(g->device);
-    const auto kernel = streams(w) ? w->group == 32 ? w4_read_kernel<32, true> : w->group == 64 ? w4_read_kernel<64, true> : w4_read_kernel<128, true>
+    // Stores past the cache want whole pieces of 64 bytes (24576 x 4104: 74 us with them, 45 without).
+    const auto kernel = streams(w) && w->cols % 32 == 0 ? w->group == 32 ? w4_read_kernel<32, true> : w->group == 64 ? w4_read_kernel<64, true> : w4_read_kernel<128, true>
                                    : w->group == 32 ? w4_read_kernel<32, false> : w->group == 64 ? w4_read_kernel<64, false> : w4_read_kernel<128, false>;
     return by_panels(g, what, w, [&](dim3 grid, const Form& f, size_t at) {
         hipLaunchKernelGGL(kernel, grid, dim3(256), 0, g->stream, f, (bf16_t*)to + at);
