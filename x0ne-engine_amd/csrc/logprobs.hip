@@ -79,44 +79,55 @@ struct Shared {
     uint64_t key[CANDIDATES + 16];
     uint64_t top[MOST_TOP];
     float4 state[THREADS / 64];
-    float group[128];
-    float floor;
+    float all[THREADS / 64], some[THREADS / 64];
     uint32_t count;
 };
 
-// A floor that at least `top` of the block's logits reach, by the largest of each thread's: its lanes are taken in 64 groups,
-// for more than 32 in 128, and the floor is the top-th largest of the groups' largest. On ordinary rows few more reach it.
-// -infinity is no alternative: the floor is above it.
+// The value of lane l ^ X.
+template <int X>
+__device__ __forceinline__ float other(float x) {
+    if (X == 1) return moved<0xB1>(x);
+    if (X == 2) return moved<0x4E>(x);
+    if (X == 3) return moved<0x1B>(x);
+    if (X == 4) return moved<0x1B>(moved<0x141>(x));
+    if (X == 7) return moved<0x141>(x);
+    if (X == 8) return moved<0x128>(x);
+    if (X == 15) return moved<0x140>(x);
+    if (X == 31) return other<16>(moved<0x140>(x));
+    if (X == 63) return other<32>(other<16>(moved<0x140>(x)));
+    const auto a = X == 16 ? __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false)
+                           : __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return __uint_as_float(threadIdx.x & X ? a[0] : a[1]);
+}
+// A step of a bitonic sort of the wavefront's lanes, falling: the larger of lanes l and l ^ X to the one without BIT.
+template <int X, int BIT>
+__device__ __forceinline__ float sorted(float x) {
+    const float o = other<X>(x);
+    return threadIdx.x & BIT ? fminf(x, o) : fmaxf(x, o);
+}
+
+// A floor that at least `top` of the block's logits reach, by the largest of each thread's, which a wavefront sorts: the
+// highest of the wavefronts' top-th ones, or the lowest of the p-th ones, p top over the wavefronts rounded up. On ordinary
+// rows few more reach it (of 4096 logits about 10 for 5, 30 for 20, 80 for 64). -infinity is no alternative: the floor is above it.
 template <uint32_t THREADS>
 __device__ __forceinline__ float floor_of(float most, uint32_t top, Shared<THREADS>& sh) {
-    constexpr int STEPS = THREADS == 256 ? 1 : THREADS == 512 ? 2 : 3;  // to a 128th of the block
-    const uint32_t groups = top > 32 ? 128 : 64;
-    float g = fold<0>(most, Most());
-    if (STEPS > 1) g = fold<1>(g, Most());
-    if (STEPS > 2) g = fold<2>(g, Most());
-    if (groups == 64) g = fold<STEPS>(g, Most());
-    sh.group[threadIdx.x / (THREADS / groups)] = g;
+    constexpr uint32_t WAVES = THREADS / 64;
+    float x = sorted<1, 1>(most);
+    x = sorted<1, 1>(sorted<3, 2>(x));
+    x = sorted<1, 1>(sorted<2, 2>(sorted<7, 4>(x)));
+    x = sorted<1, 1>(sorted<2, 2>(sorted<4, 4>(sorted<15, 8>(x))));
+    x = sorted<1, 1>(sorted<2, 2>(sorted<4, 4>(sorted<8, 8>(sorted<31, 16>(x)))));
+    x = sorted<1, 1>(sorted<2, 2>(sorted<4, 4>(sorted<8, 8>(sorted<16, 16>(sorted<63, 32>(x))))));
+    auto nth = [&](uint32_t l) { return __uint_as_float((uint32_t)__builtin_amdgcn_readlane((int)__float_as_uint(x), (int)l)); };
+    sh.all[threadIdx.x >> 6] = nth(top - 1);
+    sh.some[threadIdx.x >> 6] = nth((top - 1) / WAVES);
     __syncthreads();
-    if (threadIdx.x < 64) {
-        float h = groups == 128 ? sh.group[64 + threadIdx.x] : -INFINITY;
-        g = sh.group[threadIdx.x];
-        if (top > 1) {
-            uint32_t over_g = 0, over_h = 0;
-#pragma unroll 1
-            for (uint32_t o = 0; o < groups; o += 16) {
-#pragma unroll
-                for (uint32_t i = 0; i < 16; ++i) {
-                    over_g += sh.group[o + i] > g;
-                    over_h += sh.group[o + i] > h;
-                }
-            }
-            g = fold_all(fminf(over_g < top ? g : INFINITY, over_h < top ? h : INFINITY), Least());
-        } else
-            g = fold_all(g, Most());
-        if (threadIdx.x == 0) sh.floor = fmaxf(g, LOWEST);
-    }
-    __syncthreads();
-    return sh.floor;
+    const uint32_t w = threadIdx.x & (WAVES - 1);
+    float one = sh.all[w], each = sh.some[w];
+    one = fold<1>(fold<0>(one, Most()), Most());
+    each = fold<1>(fold<0>(each, Least()), Least());
+    if (WAVES == 8) one = fold<2>(one, Most()), each = fold<2>(each, Least());
+    return fmaxf(fmaxf(one, each), LOWEST);
 }
 
 // Room for a thread's `own` keys among the block's candidates: where they go. All threads take part.
@@ -149,18 +160,18 @@ __device__ __forceinline__ void rank(uint32_t found, uint32_t top, Shared<THREAD
 // The `top` largest of the block's logits x[i] of ids id(i), in order, as keys into sh.top, 0 behind the last; `most` is the
 // largest of x. What reaches the floor is ranked by counting. Where that is too much (equal logits, parts that are masked
 // throughout), the floor is raised by bisection over the keys: all differ, so some floor leaves from top to CANDIDATES.
-template <uint32_t THREADS, class Id>
-__device__ __forceinline__ void pick(const float (&x)[EACH], float most, Id id, uint32_t top, Shared<THREADS>& sh) {
+template <uint32_t THREADS, uint32_t N, class Id>
+__device__ __forceinline__ void pick(const float (&x)[N], float most, Id id, uint32_t top, Shared<THREADS>& sh) {
     if (threadIdx.x == 0) sh.count = 0;
     if (threadIdx.x < MOST_TOP) sh.top[threadIdx.x] = 0;
     const float floor = floor_of<THREADS>(most, top, sh);
     uint32_t own = 0;
 #pragma unroll
-    for (uint32_t i = 0; i < EACH; ++i) own += x[i] >= floor;
+    for (uint32_t i = 0; i < N; ++i) own += x[i] >= floor;
     uint32_t at = room(own, sh);
     if (own) {
 #pragma unroll
-        for (uint32_t i = 0; i < EACH; ++i)
+        for (uint32_t i = 0; i < N; ++i)
             if (x[i] >= floor && at < CANDIDATES) sh.key[at++] = key_of(x[i], id(i));
     }
     __syncthreads();
@@ -175,7 +186,7 @@ __device__ __forceinline__ void pick(const float (&x)[EACH], float most, Id id, 
             uint32_t zero = 0;
             asm volatile("" : "+v"(zero));  // the keys are formed here and not kept from turn to turn
 #pragma unroll
-            for (uint32_t i = 0; i < EACH; ++i) own += x[i] >= floor && key_of(x[i], id(i) + zero) >= mid;
+            for (uint32_t i = 0; i < N; ++i) own += x[i] >= floor && key_of(x[i], id(i) + zero) >= mid;
             at = room(own, sh);
             __syncthreads();
             const uint32_t count = sh.count;
@@ -186,7 +197,7 @@ __device__ __forceinline__ void pick(const float (&x)[EACH], float most, Id id, 
             found = (count >= top && count <= CANDIDATES) || high - low < 2;
             if (found && own) {
 #pragma unroll
-                for (uint32_t i = 0; i < EACH; ++i) {
+                for (uint32_t i = 0; i < N; ++i) {
                     const uint64_t k = key_of(x[i], id(i) + zero);
                     if (x[i] >= floor && k >= mid && at < CANDIDATES) sh.key[at++] = k;
                 }
@@ -320,10 +331,10 @@ __global__ void __launch_bounds__(THREADS, 8) logprobs_slices_kernel(Args a) {
     answer<BF16, THREADS>(a, row, r, all, token, token < a.vocab ? logit_at<BF16>(row, token) : 0.f, sh);
 }
 
-// A block joins the slices of a row.
-template <bool BF16>
+// A block joins the slices of a row, N keys to a thread at a time.
+template <bool BF16, uint32_t N>
 __global__ void __launch_bounds__(256) logprobs_join_kernel(Args a) {
-    constexpr uint32_t THREADS = 256, WAVES = THREADS / 64, SLICE = THREADS * EACH;
+    constexpr uint32_t THREADS = 256, WAVES = THREADS / 64;
     __shared__ Shared<THREADS> sh;
     __shared__ uint64_t kept[MOST_TOP];
     const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r = blockIdx.x;
@@ -340,14 +351,14 @@ __global__ void __launch_bounds__(256) logprobs_join_kernel(Args a) {
         if (threadIdx.x < MOST_TOP) sh.top[threadIdx.x] = 0;
         if (keys) rank<THREADS>(keys, a.top, sh);
     }
-    // SLICE keys at a time, the best so far among them. They lie by their place among a slice's, so that the groups of lanes that
+    // N keys to a thread at a time, the best so far among them. They lie by their place among a slice's, so that the groups of lanes that
     // give a floor have high ones.
     for (uint32_t done = keys <= RANKED ? keys : 0, held = 0; done < keys; held = a.top) {
-        const uint32_t some = min(keys - done, SLICE - held);
-        float x[EACH], most = -INFINITY;
-        uint32_t ids[EACH];
+        const uint32_t some = min(keys - done, THREADS * N - held);
+        float x[N], most = -INFINITY;
+        uint32_t ids[N];
 #pragma unroll
-        for (uint32_t i = 0; i < EACH; ++i) {
+        for (uint32_t i = 0; i < N; ++i) {
             const uint32_t at = i * THREADS + threadIdx.x;
             uint64_t k = 0;
             if (at < held)
@@ -358,7 +369,7 @@ __global__ void __launch_bounds__(256) logprobs_join_kernel(Args a) {
             ids[i] = ~(uint32_t)k;
         }
 #pragma unroll
-        for (uint32_t i = 0; i < EACH; ++i) most = fmaxf(most, x[i]);
+        for (uint32_t i = 0; i < N; ++i) most = fmaxf(most, x[i]);
         pick<THREADS>(x, most, [&](uint32_t i) { return ids[i]; }, a.top, sh);
         if (threadIdx.x < a.top) kept[threadIdx.x] = sh.top[threadIdx.x];
         done += some;
@@ -446,7 +457,11 @@ extern "C" x0ne_status x0ne_gpu_logprobs(x0ne_gpu* g, const x0ne_logprobs* d) {
         hipLaunchKernelGGL(kernel, dim3(rows * slices), dim3(threads), 0, g->stream, a);
         if (slices > 1) {
             g->counts.launches++;
-            hipLaunchKernelGGL(d->bf16 ? logprobs_join_kernel<true> : logprobs_join_kernel<false>, dim3(rows), dim3(256), 0, g->stream, a);
+            // Shorter code is over sooner: 760 keys at 4 to a thread 12.2 us for one row, at 16 13.2; more than 1024 in one go.
+            const bool many_keys = (uint64_t)slices * d->top > 1024;
+            const auto joins = many_keys ? d->bf16 ? logprobs_join_kernel<true, EACH> : logprobs_join_kernel<false, EACH>
+                                         : d->bf16 ? logprobs_join_kernel<true, 4> : logprobs_join_kernel<false, 4>;
+            hipLaunchKernelGGL(joins, dim3(rows), dim3(256), 0, g->stream, a);
         }
         X0NE_HIP(hipGetLastError(), "logprobs");
     }
