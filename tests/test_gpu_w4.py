@@ -298,3 +298,42 @@ def test_matrices_in_one_buffer_keep_to_their_own(kernels):
         check_product(R.values(code, s)[:rows, :cols], xs, a.read_array(sl[f"y{i}"], 0, 3 * rows, np.float32).reshape(3, rows), "f32", group)
     for k, end in (("codes", code_at[-1]), ("scales", scale_at[-1])):
         assert (a.read_array(sl[k], 0, need[k], np.uint8)[int(end):] == 0xA5).all()
+
+
+def test_two_gpus_at_once_and_one_made_in_the_others_capture(kernels):
+    """Products in parts on two streams that overlap, each Gpu's counters and parts its own; the second Gpu is made while the
+    first has a capture open."""
+    from x0ne_core import Arena, Gpu, W4
+    from x0ne_core.arena import Class
+    rng = np.random.default_rng(14)
+    rows, cols, n = 16416, 640, 33
+    codes, scales, w = held(rng, rows, cols, 64)
+    xs = [bits(rng.standard_normal((n, cols))) for _ in range(2)]
+    g, made = kernels.gpu, []
+    a = Arena()
+    need = {"codes": codes.nbytes, "scales": scales.nbytes, "x0": xs[0].nbytes, "x1": xs[1].nbytes, "y0": n * rows * 4, "y1": n * rows * 4}
+    sl = {k: a.alloc(k, v, Class.CLIENT_DATA) for k, v in need.items()}
+    a.freeze(g)
+    for k, v in (("codes", codes), ("scales", scales), ("x0", xs[0]), ("x1", xs[1])):
+        a.write(sl[k], 0, v)
+    at = {k: a.ptr(v) for k, v in sl.items()}
+    d = W4(at["codes"], at["scales"], rows, cols, 64)
+
+    def launches():
+        g.w4_gemv(d, at["x0"], n, at["y0"], "f32")
+        made.append(Gpu())
+        g.w4_gemv(d, at["x0"], n, at["y0"], "f32")
+
+    graph, other = g.capture(launches), made[0]
+    assert graph.nodes() == 2
+    for _ in range(20):
+        g.launch_graph(graph)
+        for _ in range(3):
+            other.w4_gemv(d, at["x1"], n, at["y1"], "f32")
+        g.w4_gemv(d, at["x0"], n, at["y0"], "f32")
+    g.sync()
+    other.sync()
+    for i in range(2):
+        check_product(w, vals(xs[i]), a.read_array(sl[f"y{i}"], 0, n * rows, np.float32).reshape(n, rows), "f32", 64)
+    graph.close()
+    other.close()

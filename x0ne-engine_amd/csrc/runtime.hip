@@ -100,9 +100,12 @@ extern "C" x0ne_status x0ne_gpu_new(x0ne_gpu** out) {
         delete g;
         return gpu_fail(e, "hipStreamCreateWithFlags");
     }
+    // In relaxed mode and by a kernel: another thread may have a capture of its own Gpu open.
+    hipStreamCaptureMode mode = hipStreamCaptureModeRelaxed;
+    const bool relaxed = hipThreadExchangeStreamCaptureMode(&mode) == hipSuccess;
     e = hipMalloc((void**)&g->counters, GPU_COUNTERS * 4);
-    if (e == hipSuccess) e = hipMemset(g->counters, 0, GPU_COUNTERS * 4);
-    if (e == hipSuccess) e = hipDeviceSynchronize();
+    if (relaxed) (void)hipThreadExchangeStreamCaptureMode(&mode);
+    if (e == hipSuccess) e = x0ne_launch_fill_u16((uint16_t*)g->counters, GPU_COUNTERS * 2, 0, g->stream);
     if (e != hipSuccess) {
         x0ne_gpu_free(g);
         return gpu_fail(e, "the counters");
