@@ -141,7 +141,8 @@ EXACT = [(32, 8, 1, 32), (2080, 640, 3, 128), (16416, 136, 2, 32), (70000, 256, 
          (96, 1160, 5, 32), (6176, 136, 8, 64), (8224, 392, 7, 128), (64, 6152, 8, 32), (16416, 640, 6, 64), (16, 25600, 5, 32),
          (96, 648, 16, 32), (6176, 200, 12, 32), (8224, 264, 16, 64), (160, 6280, 11, 128), (16448, 1032, 9, 32),
          (544, 2000, 23, 32), (96, 264, 64, 64), (8224, 328, 20, 128), (64, 6152, 45, 32), (16416, 520, 33, 64), (128, 8200, 70, 64),
-         (4128, 6152, 96, 128), (96, 136, 600, 64), (33, 6152, 130, 32)]
+         (4128, 6152, 96, 128), (96, 136, 600, 64), (33, 6152, 130, 32),
+         (33056, 264, 12, 64), (16416, 264, 20, 128), (33030, 136, 40, 32)]
 
 
 @pytest.mark.parametrize("rows,cols,n,group", EXACT)

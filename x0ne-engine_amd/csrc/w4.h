@@ -25,9 +25,12 @@ struct W4Plan {
 //    a panel to a CU at most (4096 x 12288: 7.1 with 16, 8.2 with 8; 1024 x 8192: 5.4 and 5.9).
 //  - More rows: X passes the L2 once for every unit, at about 20 bytes a clock and CU, so the more panels share it the better,
 //    while each CU has a block: 4096 x 4096, 16 rows: 5.7 with 1 panel (256 blocks), 6.4 with 2, 8.0 with 4; 6144 x 4096: 6.6
-//    with 2 (192 blocks), 8.3 with 1; 6150 x 4104, 61 rows: 12.5 with 4 (194), 15.9 with 2. Where that is more than a block to a
-//    CU, or long, even runs, whose cut units cost 3 us to join: 24576 x 4096 SwiGLU, 16 rows: 14.3 even, 15.0 with 4; 64 rows:
-//    28.1 and 29.9; 4096 x 12288: 9.9 even, 11.9 with 1; 5120 x 25600: 20.0 even, 29.1 with 2.
+//    with 2 (192 blocks), 8.3 with 1; 6150 x 4104, 61 rows: 12.5 with 4 (194), 15.9 with 2; 24576 x 4096 SwiGLU, 32 rows: 16.8
+//    with 8 (192), 20.2 with 4.
+//  - Where that is more than a block to a CU, or long, even runs, whose cut units cost 3 us to join, of 8 panels or, where those
+//    were fewer than the CUs, 4: 51200 x 5120 SwiGLU, 32 rows: 37.2 with 8, 42.5 with 4, 48.7 a unit to a block; 151936 x 4096, 16
+//    rows: 59.3, 61.3, 62.7; 5120 x 25600, 16 rows: 20.7 with 8, 19.9 with 4, 29.1 a unit of 2 to a block; 4096 x 12288: 9.9 with
+//    4, 11.9 a unit of 1 to a block.
 inline W4Plan w4_plan(uint32_t rows, uint32_t cols, uint32_t n, bool swiglu, uint32_t cus, bool parts) {
     W4Plan p = {};
     const uint32_t all = (rows + 15) / 16, tiles = (cols + 127) / 128, pair = swiglu ? 2 : 1;
@@ -42,15 +45,11 @@ inline W4Plan w4_plan(uint32_t rows, uint32_t cols, uint32_t n, bool swiglu, uin
         else if (tiles >= 64 && units(pair) <= cus)
             p.waves = 16;
     } else {
-        const uint32_t least = p.xl == 8 ? 2 : pair;
-        p.panels = 4;
-        for (uint32_t panels = least; panels < 4; panels *= 2)
-            if (units(panels) * (uint64_t)p.groups <= cus) {
-                p.panels = panels;
-                break;
-            }
-        p.even = tiles > 48 || units(4) * (uint64_t)p.groups > cus;
-        if (p.even) p.panels = 4;
+        const uint32_t most = p.xl == 2 ? 4 : 8;
+        p.panels = p.xl == 8 ? 2 : pair;
+        while (p.panels < most && units(p.panels) * (uint64_t)p.groups > cus) p.panels *= 2;
+        p.even = tiles > 48 || units(p.panels) * (uint64_t)p.groups > cus;
+        if (p.even) p.panels = units(8) * (uint64_t)p.groups >= cus ? most : 4;
     }
     p.units = units(p.panels);
     p.rounds = (tiles + p.waves - 1) / p.waves;

@@ -512,6 +512,10 @@ static bool launch_plan(const x0ne_gpu* g, const x0ne_w4* w, const W4Plan& p, co
         if (p.xl == 4) return go(p.even ? launch_as<SWIGLU, 4, 4, 8, 1, true> : launch_as<SWIGLU, 4, 4, 8, 1, false>);
         if (p.xl == 8) return go(p.even ? launch_as<SWIGLU, 8, 4, 8, 1, true> : launch_as<SWIGLU, 8, 4, 8, 1, false>);
     }
+    if (p.panels == 8) {
+        if (p.xl == 4) return go(p.even ? launch_as<SWIGLU, 4, 8, 8, 1, true> : launch_as<SWIGLU, 4, 8, 8, 1, false>);
+        if (p.xl == 8) return go(p.even ? launch_as<SWIGLU, 8, 8, 8, 1, true> : launch_as<SWIGLU, 8, 8, 8, 1, false>);
+    }
     return false;
 }
 
