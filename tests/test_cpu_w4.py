@@ -127,7 +127,7 @@ def test_logprobs_refusals_come_before_any_device():
 
 
 def test_the_workspace_of_logprobs():
-    """The same counters in front for every call, at least as long as those of the 8-bit cache; and enough behind them."""
+    """Room in front that is left to the counters of the 8-bit cache, as long as theirs; and enough behind it."""
     from x0ne_core import LogProbs, _lib
     size = lambda **k: _lib.lib().x0ne_logprobs_work_bytes(LogProbs(**k))
     for change in BAD_NUMBERS:

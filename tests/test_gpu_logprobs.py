@@ -135,8 +135,8 @@ def test_more_tokens_than_a_block_and_repeated_ones(kernels):
     check(kernels, logits(rng, 3, 5000), tokens, 3)
 
 
-def test_more_rows_than_counters(kernels):
-    """70000 rows: two launches over one workspace; the second comes upon the counters as the first left them."""
+def test_more_rows_than_a_launch(kernels):
+    """70000 rows: two pairs of launches over one workspace, twice."""
     rng = np.random.default_rng(9)
     x = np.tile(logits(rng, 7, 4100), (10000, 1))
     got = kernels.logprobs(x, np.tile(np.arange(7)[:, None] * 500, (10000, 1)), 2, calls=2)
@@ -160,6 +160,32 @@ def test_the_same_call_gives_the_same_bits(kernels):
     first = check(kernels, x, tokens, 20)
     for a, b in zip(first, check(kernels, x, tokens, 20, calls=6)):
         assert (a == b).all()
+
+
+@pytest.mark.parametrize("kind", ["f32", "bf16"])
+def test_rows_past_32_bits(kernels, kind):
+    """Rows 2^31 and some logits apart: the last begins behind 8 or 16 GiB."""
+    from x0ne_core import Arena, LogProbs
+    from x0ne_core.arena import Class
+    rng = np.random.default_rng(12)
+    g, vocab, stride, top = kernels.gpu, 9000, (1 << 31) + 17, 4
+    x = logits(rng, 3, vocab, kind)
+    a, size = Arena(), g.logprobs_work_bytes(LogProbs(rows=3, vocab=vocab, top=top))
+    need = {"x": (2 * stride + vocab) * x.itemsize, "work": size, "ids": 3 * top * 4, "lp": 3 * top * 4, "tokens": 12, "token_lp": 12}
+    sl = {k: a.alloc(k, v, Class.CLIENT_DATA) for k, v in need.items()}
+    a.freeze(g)
+    at = {k: a.ptr(v) for k, v in sl.items()}
+    for r in range(3):
+        a.write(sl["x"], r * stride * x.itemsize, x[r])
+    tokens = np.array([0, 4500, 8999], np.uint32)
+    a.write(sl["tokens"], 0, tokens)
+    g.logprobs(LogProbs(logits=at["x"], stride=stride, tokens=at["tokens"], token_lp=at["token_lp"], top_ids=at["ids"], top_lp=at["lp"],
+                        work=at["work"], work_bytes=size, rows=3, vocab=vocab, per_row=1, top=top, bf16=int(kind == "bf16")))
+    g.sync()
+    same = kernels.logprobs(x, tokens[:, None], top)
+    assert (a.read_array(sl["token_lp"], 0, 3, np.float32) == same[0][:, 0]).all()
+    assert (a.read_array(sl["ids"], 0, 3 * top, np.uint32).reshape(3, top) == same[2]).all()
+    assert (a.read_array(sl["lp"], 0, 3 * top, np.float32).reshape(3, top) == same[3]).all()
 
 
 # -- as they are used together --

@@ -338,3 +338,57 @@ def test_two_gpus_at_once_and_one_made_in_the_others_capture(kernels):
         check_product(w, vals(xs[i]), a.read_array(sl[f"y{i}"], 0, n * rows, np.float32).reshape(n, rows), "f32", 64)
     graph.close()
     other.close()
+
+
+def whole(rng, rows, cols):
+    """Weights that 4 bits hold as they are: codes of scale 1, a 6 in each group of 32 or more."""
+    w = R.VALUES[rng.integers(0, 16, (rows, cols))]
+    w[:, ::32] = 6.0
+    return w
+
+
+def test_a_matrix_past_32_bits(kernels):
+    """Codes of more than 4 GiB and a bf16 matrix of 18: quantised, read back and multiplied, its first and last rows exactly."""
+    from x0ne_core import Arena, W4
+    from x0ne_core.arena import Class
+    rng = np.random.default_rng(15)
+    g, rows, cols, group, some = kernels.gpu, 140009, 65536, 32, 25
+    d = W4(0, 0, rows, cols, group)
+    assert d.code_bytes() > 1 << 32
+    ends = [whole(rng, some, cols) for _ in range(2)]
+    need = {"w": rows * cols * 2, "codes": d.code_bytes(), "scales": d.scale_bytes(), "x": 20 * cols * 2, "y": 20 * rows * 4}
+    a = Arena()
+    sl = {k: a.alloc(k, v, Class.CLIENT_DATA) for k, v in need.items()}
+    a.freeze(g)
+    at = {k: a.ptr(v) for k, v in sl.items()}
+    d = W4(at["codes"], at["scales"], rows, cols, group)
+    places = [0, (rows - some) * cols * 2]
+    for w, place in zip(ends, places):
+        a.write(sl["w"], place, bits(w))
+    g.w4_quantise(d, at["w"])
+    g.sync()
+    for place in places:
+        a.write(sl["w"], place, np.zeros((some, cols), np.uint16))
+    g.w4_read(d, at["w"])
+    g.sync()
+    for w, place in zip(ends, places):
+        assert (vals(a.read_array(sl["w"], place, some * cols, np.uint16).reshape(some, cols)) == w).all()
+    for n in (1, 5, 20):
+        x = rng.integers(-7, 8, (n, cols)).astype(np.float64)
+        a.write(sl["x"], 0, bits(x))
+        g.w4_gemv(d, at["x"], n, at["y"], "f32")
+        g.sync()
+        y = a.read_array(sl["y"], 0, n * rows, np.float32).reshape(n, rows)
+        assert (y[:, :some] == x @ ends[0].T).all() and (y[:, -some:] == x @ ends[1].T).all(), n
+
+
+def test_more_panels_than_a_grid(kernels):
+    """65538 panels: quantised and read back in two launches, multiplied in one; every row exactly."""
+    rng = np.random.default_rng(16)
+    rows, cols = 65535 * 16 + 41, 8
+    w = whole(rng, rows, cols)
+    codes, scales = kernels.w4_quantise(bits(w), 64)
+    assert (vals(kernels.w4_read(codes, scales, rows, cols, 64)) == w).all()
+    for n in (1, 6, 20):
+        x = rng.integers(-7, 8, (n, cols)).astype(np.float64)
+        assert (kernels.w4_gemv(codes, scales, rows, cols, 64, bits(x), "f32") == x @ w.T).all(), n

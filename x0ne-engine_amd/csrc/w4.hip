@@ -51,7 +51,10 @@ __device__ __forceinline__ void wave_lds() {
     __builtin_amdgcn_wave_barrier();
 }
 
-// A wavefront takes a tile. The four lanes of a row hold 8 columns of each 32: a group's largest magnitude is theirs.
+// s = max |w| / 6 of each group, codes of w / s. A wavefront takes a tile. The four lanes of a row hold 8 columns of each 32: a
+// group's largest magnitude is theirs, found with two shuffles, and each lane's codes are 16 bytes as they lie in memory.
+// Measured on MI355X: 47.9 us for 24576 x 4096 (201 MB read and 52 written: 5.3 TB/s, what a copy of 1 GiB reaches); 4.1 for
+// 1000 x 1096, which is a launch and one trip to memory.
 template <int G, bool STREAM>
 __global__ void __launch_bounds__(256) w4_quantise_kernel(const bf16_t* __restrict__ from, Form f) {
     const uint32_t lane = threadIdx.x & 63, t = blockIdx.x * 4 + (threadIdx.x >> 6);
@@ -125,6 +128,8 @@ __device__ __forceinline__ float scale_of(const bf16_t* scales, size_t tile, uin
     return bf2f(scales[(tile * TILE_ROWS + row) * (TILE_COLS / G) + s * 32 / G]);
 }
 
+// Codes times scales, rounded once to bf16. A wavefront takes a tile and stores whole rows of its 256 bytes. Measured on MI355X:
+// 108.8 us for 51200 x 5120 (147 MB read, 524 written: 6.2 TB/s), 37.2 for 24576 x 4096, 3.8 for 4096 x 1024.
 template <int G, bool STREAM>
 __global__ void __launch_bounds__(256) w4_read_kernel(Form f, bf16_t* __restrict__ to) {
     const uint32_t lane = threadIdx.x & 63, t = blockIdx.x * 4 + (threadIdx.x >> 6);
@@ -191,13 +196,21 @@ struct Cut {
     uint32_t* counters;  // one per unit: zero, left at zero
 };
 
-// Y = X W^T. A block of V wavefronts takes a run of the tiles of units of P panels (SwiGLU: half of them gate, the others up)
-// and 4 XL rows of X; its wavefronts take the run's tiles in turn, so that it reads V KiB in a row. X is the A operand, W the B operand: a
-// lane's four sums are four tokens of one row of W, whose scale of a group is one value.
-// A load of X takes 4 rows of a tile's 256 bytes, neighbouring lanes on one row, and passes through the wavefront's own
-// LDS, 16-byte chunks placed by an XOR of the row, into the operand's order.
+// Y = X W^T: y[t][r] is the sum over the groups g of s[r][g] times the sum over g's columns c of x[t][c] code[r][c]. Codes are
+// exact as bf16, so a group's sum is formed on them as they are and scaled once.
+// A block of V wavefronts takes a run of the tiles of units of P panels (SwiGLU: half of them gate, the others up) and 4 XL
+// rows of X; its wavefronts take the run's tiles in turn, so that it reads V KiB in a row. X is the A operand, W the B operand:
+// a lane's four sums are four tokens of one row of W, whose scale of a group is one value. A load of X takes 4 rows of a tile's
+// 256 bytes, neighbouring lanes on one row, and passes through the wavefront's own LDS into the operand's order (loaded in
+// that order, four lanes to each of 16 rows, 54 us for the 16 rows below): there is no barrier until a unit's end.
+// Measured on MI355X: one row is bound by the weights: 48.5 us for 151936 x 4096 (322 MB, 6.6 TB/s); 9.8 to 11.3 for 24576 x
+// 4096 SwiGLU (54 MB), of which 2 pass before the first product; 3.4 for 4096 x 1024, which is that and one trip to memory.
+// More rows by X's way through the L2, once to a unit, and by the joins of cut units: 16 rows of 5120 x 25600 (82 MB) 20.6,
+// first products after 2.1, 8 rounds of 1.5 at 6.2 TB/s, the cut units' parts joined by 18.6; 61 rows of 6150 x 4104 12.9 in
+// 208 blocks of 5 rounds.
 template <int G, bool SWIGLU, int XL, int P, int V, int U, bool EVEN>
-__global__ void __launch_bounds__(64 * V) w4_gemv_kernel(Form f, const bf16_t* __restrict__ x, uint32_t n, void* __restrict__ y, uint32_t out_f32, Cut cut) {
+__global__ void __launch_bounds__(64 * V) w4_gemv_kernel(Form f, const bf16_t* __restrict__ x, uint32_t n, void* __restrict__ y,
+                                                         uint32_t out_f32, Cut cut) {
     constexpr int PAIR = SWIGLU ? 2 : 1, POLICY = NT, PER = 128 / G, TT = (XL + 3) / 4, TOKENS = XL < 4 ? 4 * XL : 16 * TT;
     // A wavefront's X tile, then its sums of a unit.
     constexpr int OWN = XL * 64 > P * TT * 64 ? XL * 64 : P * TT * 64;
@@ -454,8 +467,10 @@ extern "C" x0ne_status x0ne_gpu_w4_quantise(x0ne_gpu* g, const x0ne_w4* w, uint6
     if (!from || from % 16) return bad(what, "a bf16 matrix (16-byte aligned) is required");
     if (!g) return fail(X0NE_ERR_GPU, "no device");
     const OnDevice on(g->device);
-    const auto kernel = streams(w) ? w->group == 32 ? w4_quantise_kernel<32, true> : w->group == 64 ? w4_quantise_kernel<64, true> : w4_quantise_kernel<128, true>
-                                   : w->group == 32 ? w4_quantise_kernel<32, false> : w->group == 64 ? w4_quantise_kernel<64, false> : w4_quantise_kernel<128, false>;
+    const bool past = streams(w);
+    const auto kernel = w->group == 32   ? past ? w4_quantise_kernel<32, true> : w4_quantise_kernel<32, false>
+                        : w->group == 64 ? past ? w4_quantise_kernel<64, true> : w4_quantise_kernel<64, false>
+                                         : past ? w4_quantise_kernel<128, true> : w4_quantise_kernel<128, false>;
     return by_panels(g, what, w, [&](dim3 grid, const Form& f, size_t at) {
         hipLaunchKernelGGL(kernel, grid, dim3(256), 0, g->stream, (const bf16_t*)from + at, f);
     });
@@ -468,8 +483,10 @@ extern "C" x0ne_status x0ne_gpu_w4_read(x0ne_gpu* g, const x0ne_w4* w, uint64_t 
     if (!g) return fail(X0NE_ERR_GPU, "no device");
     const OnDevice on(g->device);
     // Stores past the cache want whole pieces of 64 bytes (24576 x 4104: 74 us with them, 45 without).
-    const auto kernel = streams(w) && w->cols % 32 == 0 ? w->group == 32 ? w4_read_kernel<32, true> : w->group == 64 ? w4_read_kernel<64, true> : w4_read_kernel<128, true>
-                                   : w->group == 32 ? w4_read_kernel<32, false> : w->group == 64 ? w4_read_kernel<64, false> : w4_read_kernel<128, false>;
+    const bool past = streams(w) && w->cols % 32 == 0;
+    const auto kernel = w->group == 32   ? past ? w4_read_kernel<32, true> : w4_read_kernel<32, false>
+                        : w->group == 64 ? past ? w4_read_kernel<64, true> : w4_read_kernel<64, false>
+                                         : past ? w4_read_kernel<128, true> : w4_read_kernel<128, false>;
     return by_panels(g, what, w, [&](dim3 grid, const Form& f, size_t at) {
         hipLaunchKernelGGL(kernel, grid, dim3(256), 0, g->stream, f, (bf16_t*)to + at);
     });

@@ -499,7 +499,7 @@ impl Gpu {
         check(unsafe { sys::x0ne_gpu_w4_gemv(self.h.0, w, x, n as u64, y, out) })
     }
 
-    /// Bytes of the zeroed workspace of `logprobs`, by the descriptor's numbers; 0 for numbers it refuses.
+    /// Bytes of the workspace of `logprobs`, by the descriptor's numbers; 0 for numbers it refuses.
     pub fn logprobs_work_bytes(d: &sys::x0ne_logprobs) -> u64 {
         // SAFETY: reads the descriptor's numbers only.
         unsafe { sys::x0ne_logprobs_work_bytes(d) }
@@ -510,8 +510,8 @@ impl Gpu {
     ///
     /// # Safety
     ///
-    /// As [`Gpu::w4_quantise`], of the descriptor's addresses; `d.work` was zeroed before its first
-    /// call and no other call uses it meanwhile.
+    /// As [`Gpu::w4_quantise`], of the descriptor's addresses; no other call uses `d.work`
+    /// meanwhile.
     pub unsafe fn logprobs(&self, d: &sys::x0ne_logprobs) -> Result<()> {
         // SAFETY: a live device handle and descriptor; the addresses are the caller's contract.
         check(unsafe { sys::x0ne_gpu_logprobs(self.h.0, d) })

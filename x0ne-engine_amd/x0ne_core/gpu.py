@@ -281,7 +281,7 @@ class Gpu:
         check(lib().x0ne_gpu_w4_gemv(self.h, w, x, n, y, W4_OUT[out]), "w4_gemv")
 
     def logprobs_work_bytes(self, d: LogProbs) -> int:
-        """Bytes of the zeroed workspace of logprobs, by the descriptor's numbers; 0 for numbers it refuses."""
+        """Bytes of the workspace of logprobs, by the descriptor's numbers; 0 for numbers it refuses."""
         return lib().x0ne_logprobs_work_bytes(d)
 
     def logprobs(self, d: LogProbs):
