@@ -321,8 +321,8 @@ typedef struct {
     uint32_t rows, vocab, per_row, top, bf16;
     float scale;
 } x0ne_logprobs;
-/* Bytes of the workspace of a call of these numbers (its addresses are not looked at; 0 where the call
-   refuses the numbers). */
+/* Bytes of the workspace of a call of these numbers, and enough for one of fewer rows, logits or
+   alternatives (its addresses are not looked at; 0 where the call refuses the numbers). */
 uint64_t x0ne_logprobs_work_bytes(const x0ne_logprobs* d);
 x0ne_status x0ne_gpu_logprobs(x0ne_gpu* g, const x0ne_logprobs* d);
 

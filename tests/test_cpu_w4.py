@@ -137,6 +137,21 @@ def test_the_workspace_of_logprobs():
     assert size(rows=1 << 24, vocab=1 << 24, top=64) < 1 << 36
 
 
+def test_a_workspace_of_logprobs_is_enough_for_less():
+    """Fewer rows, logits or alternatives, of either type, need no more, whichever way their rows are cut."""
+    from x0ne_core import LogProbs, _lib
+    size = lambda *n: _lib.lib().x0ne_logprobs_work_bytes(LogProbs(rows=n[0], vocab=n[1], top=n[2], bf16=n[3]))
+    rows = [*range(1, 130), *range(190, 300, 5), 512, 513, 768, 769, 1000, 4096, 65535, 65536, 65537, 1 << 20, 1 << 24]
+    vocabs = [1, 4096, 4097, 8192, 8193, 16384, 16385, 32000, 32768, 32769, 50257, 65536, 151936, 1 << 20, (1 << 24) - 4096, 1 << 24]
+    tops = [0, 1, 2, 20, 64]
+    for bf16 in (0, 1):
+        s = np.array([[[size(r, v, t, bf16) for t in tops] for v in vocabs] for r in rows], np.int64)
+        assert all((np.diff(s, axis=k) >= 0).all() for k in range(3))
+        if bf16:
+            assert (s == other).all()
+        other = s
+
+
 def test_the_python_out_names():
     from x0ne_core import FormatError, Gpu, W4
     with pytest.raises(FormatError):

@@ -128,6 +128,21 @@ def test_strides(kernels, vocab, stride, kind):
     check(kernels, bits(x) if kind == "bf16" else x, rng.integers(0, vocab, (5, 1)), 7, vocab=vocab)
 
 
+@pytest.mark.parametrize("kind", ["f32", "bf16"])
+@pytest.mark.parametrize("rows,vocab", [(1, 8192), (600, 8000), (300, 8192), (2, 16384), (40, 16001), (2, 16385), (256, 17000), (257, 17000),
+                                        (1, 32768), (30, 32768), (1, 32769), (60, 50257), (62, 50001), (3, 262144), (12, 262145)])
+def test_rows_cut_in_every_way(kernels, rows, vocab, kind):
+    """Sizes at both sides of each rule by which rows are cut, with no, one and more alternatives; equal logits in rows that
+    the floor does not part."""
+    rng = np.random.default_rng(rows + vocab)
+    x = logits(rng, rows, vocab, kind)
+    x[0] = bits(np.full(vocab, 0.5)) if kind == "bf16" else 0.5
+    x[rows // 2, :-3] = bits(np.array([-np.inf])) if kind == "bf16" else -np.inf
+    tokens = rng.integers(0, vocab, (rows, 1))
+    for top in (0, 1, 7):
+        check(kernels, x, tokens, top)
+
+
 def test_more_tokens_than_a_block_and_repeated_ones(kernels):
     rng = np.random.default_rng(8)
     tokens = rng.integers(0, 5000, (3, 1111))
@@ -240,7 +255,7 @@ def test_a_step_from_the_head_to_its_log_probabilities_in_a_graph(kernels, n):
     g.w4_quantise(d, at["w"])
     want_other = R.logprobs(other.astype(np.float64), 1.0, None, 64)[2]
     graph = g.capture(step)
-    assert graph.nodes() == 3
+    assert graph.nodes() == 2
     for _ in range(4):
         x = bits(rng.standard_normal((n, hidden)) * 3)
         a.write(sl["x"], 0, x)

@@ -1,9 +1,9 @@
 // Log probabilities of rows of logits: those of given tokens, the entropy, and the top alternatives.
 //
 // With l the logits, m = max l, z = sum e^(scale (l - m)), t = sum (l - m) e^(scale (l - m)): log p = scale (l - m) - log z
-// and the entropy is log z - scale t / z. One pass over the logits: a block holds a slice of a row in registers, 16 logits to a
-// thread, forms (m, z, t) of them and picks its top ones. A second, small kernel joins the slices of a row: joined by the last
-// block of the row to count itself, the code of that came from memory while the card waited (15 to 30 us).
+// and the entropy is log z - scale t / z. One pass over the logits: a block holds a row or a slice of one in registers, 16 or
+// 32 logits to a thread, forms (m, z, t) of them and picks its top ones. A second, small kernel joins a row's slices: joined by
+// the last block of the row to count itself, the code of that came from memory while the card waited (15 to 30 us).
 #include <algorithm>
 #include <string>
 
@@ -14,7 +14,6 @@ using namespace x0ne;
 
 namespace {
 
-constexpr uint32_t EACH = 16;  // logits to a thread
 constexpr uint32_t MOST_TOP = 64;
 constexpr uint32_t CANDIDATES = 512;
 constexpr uint32_t RANKED = 128;  // so many keys are ranked without a floor
@@ -127,7 +126,8 @@ __device__ __forceinline__ float floor_of(float most, uint32_t top, Shared<THREA
     float one = sh.all[w], each = sh.some[w];
     one = fold<1>(fold<0>(one, Most()), Most());
     each = fold<1>(fold<0>(each, Least()), Least());
-    if (WAVES == 8) one = fold<2>(one, Most()), each = fold<2>(each, Least());
+    if (WAVES >= 8) one = fold<2>(one, Most()), each = fold<2>(each, Least());
+    if (WAVES == 16) one = fold<3>(one, Most()), each = fold<3>(each, Least());
     return fmaxf(fmaxf(one, each), LOWEST);
 }
 
@@ -263,11 +263,15 @@ __device__ __forceinline__ const void* row_of(const Args& a, uint32_t r) {
     return static_cast<const uint8_t*>(a.logits) + r * a.stride * (BF16 ? 2 : 4);
 }
 
-// Measured on MI355X: 48.9 us for 512 rows of 151936 f32 logits with one alternative (311 MB, 6.4 TB/s); 5.6 for one row with
+// Measured on MI355X: 47.9 us for 512 rows of 151936 f32 logits with one alternative (311 MB, 6.5 TB/s); 5.6 for one row with
 // 20, a launch, a trip to memory and the selection one after the other. Those 512 rows without alternatives and with 1, 5, 20
-// and 64, both kernels: 52.5, 55, 75, 81 and 93, where the sort, the ranking and their barriers take the place of loads.
-template <bool BF16, uint32_t THREADS>
-__global__ void __launch_bounds__(THREADS, 8) logprobs_slices_kernel(Args a) {
+// and 64, both kernels: 51.4, 55.8, 59.8, 64.1 and 77.4, where the sort, the ranking and their barriers take the place of loads.
+// Wavefronts of a kernel to a SIMD: as many as its registers allow; 512 threads of 32 logits are 6 with a few spills outside the
+// sums (4096 rows of 16000 bf16 logits, 5 alternatives: 50.9 us, with 4 and none 59.9).
+constexpr int waves_of(uint32_t threads, uint32_t each) { return each == 16 ? 8 : threads == 256 ? 5 : threads == 512 ? 6 : 4; }
+
+template <bool BF16, uint32_t THREADS, uint32_t EACH>
+__global__ void __launch_bounds__(THREADS, waves_of(THREADS, EACH)) logprobs_slices_kernel(Args a) {
     constexpr uint32_t WAVES = THREADS / 64;
     constexpr uint32_t PIECE = BF16 ? 8 : 4;  // logits of a 16-byte load
     __shared__ Shared<THREADS> sh;
@@ -401,25 +405,53 @@ x0ne_status check_shape(const x0ne_logprobs* d) {
     return X0NE_OK;
 }
 
-// Blocks of 512 threads spend less on each logit's selection and join; those of 256 are over sooner where they are so few that
-// each has a place on the card from the start.
-constexpr uint32_t FEW = 256, MANY = 512;
-uint32_t threads_of(const x0ne_logprobs* d) {
-    return (uint64_t)d->rows * ((d->vocab + FEW * EACH - 1) / (FEW * EACH)) > 1024 ? MANY : FEW;
+// How a row is cut: threads to a block, logits to a thread.
+struct Slices {
+    uint32_t threads, each, count;
+};
+// Measured on MI355X (us; threads x logits). A row in one slice needs no second kernel: 8000 logits, one row with 20 alternatives
+// 6.0 with 512 x 16, 9.3 in two slices; 16000: 7.9 with 512 x 32, 9.8 in four; 32001: 9.6 with 1024 x 32, 10.7 in eight, while
+// a row has a CU (256 rows with 5: 10.4, 14.8; 1024 rows 41 and 34), and one alternative 6.5 and 7.8. Many short rows: 256 x 32
+// (4096 of 8000 with 5: 27.2; 33.8 with 512 x 16).
+// Longer rows: 256 x 16 while there are up to 3 blocks to a CU (one row of 151936, 20 alternatives: 10.8; 11.8 with 256 x 32),
+// then 256 x 32, which selects once for twice the logits (512 rows, 20: 62; 73 with 256 x 16, 80 with 512 x 16), but f32
+// without selection, which is bound by its loads: 512 x 16 (1024 rows of 151936: 104; 110 with 256 x 32).
+constexpr uint64_t FEW = 768;
+Slices slices_of(const x0ne_logprobs* d) {
+    const auto cut = [&](uint32_t threads, uint32_t each) { return Slices{threads, each, (d->vocab + threads * each - 1) / (threads * each)}; };
+    if (d->vocab <= 4096) return cut(256, 16);
+    if (d->vocab <= 8192) return d->rows > 512 ? cut(256, 32) : cut(512, 16);
+    if (d->vocab <= 16384) return cut(512, 32);
+    if (d->vocab <= 32768 && d->rows <= 256) return cut(1024, 32);
+    const Slices few = cut(256, 16);
+    if ((uint64_t)d->rows * few.count <= FEW) return few;
+    return d->top <= 1 && !d->bf16 ? cut(512, 16) : cut(256, 32);
 }
-uint32_t slices_of(const x0ne_logprobs* d) { return (d->vocab + threads_of(d) * EACH - 1) / (threads_of(d) * EACH); }
 
 // The workspace's first part is left alone: there the calls of the 8-bit cache count, which may share it. Behind it the slices'
 // states, then their top keys.
 constexpr uint64_t COUNTER_BYTES = 4 * 65536;
-// A launch has fewer than 2^32 threads, and the workspace is that of at most so many rows' slices: more rows are further launches.
-uint64_t rows_at_once(const x0ne_logprobs* d) { return std::min<uint64_t>(65536, ((1ull << 32) / threads_of(d) - 1) / slices_of(d)); }
+// A launch has so many rows and slices at most (fewer than 2^32 threads), and the workspace is a launch's: more are further launches.
+constexpr uint64_t MOST_ROWS = 65536, MOST_SLICES = 1u << 22;
+uint64_t rows_at_once(const x0ne_logprobs* d) { return std::min(MOST_ROWS, MOST_SLICES / slices_of(d).count); }
+
+using Kernel = void (*)(Args);
+template <bool BF16>
+Kernel kernel_as(const Slices& s) {
+    if (s.threads == 256) return s.each == 16 ? logprobs_slices_kernel<BF16, 256, 16> : logprobs_slices_kernel<BF16, 256, 32>;
+    if (s.threads == 512) return s.each == 16 ? logprobs_slices_kernel<BF16, 512, 16> : logprobs_slices_kernel<BF16, 512, 32>;
+    return logprobs_slices_kernel<BF16, 1024, 32>;
+}
+Kernel kernel_of(const Slices& s, bool bf16) { return bf16 ? kernel_as<true>(s) : kernel_as<false>(s); }
 
 }  // namespace
 
 extern "C" uint64_t x0ne_logprobs_work_bytes(const x0ne_logprobs* d) {
     if (check_shape(d) != X0NE_OK) return 0;
-    return COUNTER_BYTES + std::min<uint64_t>(d->rows, rows_at_once(d)) * slices_of(d) * (sizeof(float4) + 8ull * d->top);
+    // Enough for fewer rows too, which may be cut into more slices, up to FEW.
+    const uint64_t rows = std::min<uint64_t>(d->rows, MOST_ROWS);
+    const uint64_t slices = std::max(std::min(rows * slices_of(d).count, MOST_SLICES), std::min(rows * ((d->vocab + 4095) / 4096), FEW));
+    return COUNTER_BYTES + slices * (sizeof(float4) + 8ull * d->top);
 }
 
 extern "C" x0ne_status x0ne_gpu_logprobs(x0ne_gpu* g, const x0ne_logprobs* d) {
@@ -437,7 +469,8 @@ extern "C" x0ne_status x0ne_gpu_logprobs(x0ne_gpu* g, const x0ne_logprobs* d) {
     if (!g) return fail(X0NE_ERR_GPU, "no device");
     if (d->rows == 0) return X0NE_OK;
     const OnDevice on(g->device);
-    const uint32_t slices = slices_of(d), threads = threads_of(d);
+    const Slices cut = slices_of(d);
+    const uint32_t slices = cut.count, threads = cut.threads;
     for (uint64_t first = 0; first < d->rows; first += rows_at_once(d)) {
         const uint32_t rows = (uint32_t)std::min<uint64_t>(d->rows - first, rows_at_once(d));
         Args a = {};
@@ -457,14 +490,13 @@ extern "C" x0ne_status x0ne_gpu_logprobs(x0ne_gpu* g, const x0ne_logprobs* d) {
         a.top = d->top;
         a.scale = d->scale;
         g->counts.launches++;
-        const auto kernel = threads == FEW ? d->bf16 ? logprobs_slices_kernel<true, FEW> : logprobs_slices_kernel<false, FEW>
-                                           : d->bf16 ? logprobs_slices_kernel<true, MANY> : logprobs_slices_kernel<false, MANY>;
+        const auto kernel = kernel_of(cut, d->bf16);
         hipLaunchKernelGGL(kernel, dim3(rows * slices), dim3(threads), 0, g->stream, a);
         if (slices > 1) {
             g->counts.launches++;
             // Shorter code is over sooner: 760 keys at 4 to a thread 12.2 us for one row, at 16 13.2; more than 1024 in one go.
             const bool many_keys = (uint64_t)slices * d->top > 1024;
-            const auto joins = many_keys ? d->bf16 ? logprobs_join_kernel<true, EACH> : logprobs_join_kernel<false, EACH>
+            const auto joins = many_keys ? d->bf16 ? logprobs_join_kernel<true, 16> : logprobs_join_kernel<false, 16>
                                          : d->bf16 ? logprobs_join_kernel<true, 4> : logprobs_join_kernel<false, 4>;
             hipLaunchKernelGGL(joins, dim3(rows), dim3(256), 0, g->stream, a);
         }
