@@ -158,6 +158,21 @@ __device__ __forceinline__ void rank(uint32_t found, uint32_t top, Shared<THREAD
     __syncthreads();
 }
 
+// x[i] of an i of the lane's own, by halving (bits, so that the compiler keeps x in registers).
+template <uint32_t N, class T>
+__device__ __forceinline__ T chosen(const T (&x)[N], uint32_t i) {
+    if constexpr (N == 1)
+        return x[0];
+    else {
+        T half[N / 2];
+        const uint32_t odd = 0u - (i & 1);
+#pragma unroll
+        for (uint32_t k = 0; k < N / 2; ++k)
+            half[k] = __builtin_bit_cast(T, (__builtin_bit_cast(uint32_t, x[2 * k + 1]) & odd) | (__builtin_bit_cast(uint32_t, x[2 * k]) & ~odd));
+        return chosen(half, i >> 1);
+    }
+}
+
 // The `top` largest of the block's logits x[i] of ids id(i), in order, as keys into sh.top, 0 behind the last; `most` is the
 // largest of x. What reaches the floor is ranked by counting. Where that is too much (equal logits, parts that are masked
 // throughout), the floor is raised by bisection over the keys: all differ, so some floor leaves from top to CANDIDATES.
@@ -166,43 +181,44 @@ __device__ __forceinline__ void pick(const float (&x)[N], float most, Id id, uin
     if (threadIdx.x == 0) sh.count = 0;
     if (threadIdx.x < MOST_TOP) sh.top[threadIdx.x] = 0;
     const float floor = floor_of<THREADS>(most, top, sh);
-    uint32_t own = 0;
+    uint32_t reach = 0;  // bit i: x[i] does
 #pragma unroll
-    for (uint32_t i = 0; i < N; ++i) own += x[i] >= floor;
-    uint32_t at = room(own, sh);
-    if (own) {
-#pragma unroll
-        for (uint32_t i = 0; i < N; ++i)
-            if (x[i] >= floor && at < CANDIDATES) sh.key[at++] = key_of(x[i], id(i));
-    }
+    for (uint32_t i = N; i-- > 0;) reach += reach + (x[i] >= floor);
+    uint32_t own = __popc(reach), at = room(own, sh);
+    auto leave = [&] {
+        for (; reach && at < CANDIDATES; reach &= reach - 1) {
+            const uint32_t i = __ffs(reach) - 1;
+            sh.key[at++] = key_of(chosen(x, i), id(i));
+        }
+    };
+    leave();
     __syncthreads();
     if (sh.count > CANDIDATES) {
-        uint64_t low = key_of(floor, NONE), high = ~0ull;
+        const uint64_t from = key_of(floor, NONE);
+        uint64_t low = (uint64_t)__builtin_amdgcn_readfirstlane((uint32_t)(from >> 32)) << 32, high = ~0ull;
         for (bool found = false; !found;) {
             const uint64_t mid = low + (high - low) / 2;
             __syncthreads();
             if (threadIdx.x == 0) sh.count = 0;
             __syncthreads();
-            own = 0;
+            // Keys of mid and more, by their logits and ids: none is that of -0, and above infinity's the edge is a NaN.
+            const float edge = logit_of(mid);
+            const uint32_t least = (uint32_t)(mid >> 32) == 0x7FFFFFFFu ? 0u : (uint32_t)mid;
             uint32_t zero = 0;
-            asm volatile("" : "+v"(zero));  // the keys are formed here and not kept from turn to turn
+            asm volatile("" : "+v"(zero));  // the ids are formed here and not kept from turn to turn
+            reach = 0;
 #pragma unroll
-            for (uint32_t i = 0; i < N; ++i) own += x[i] >= floor && key_of(x[i], id(i) + zero) >= mid;
+            for (uint32_t i = N; i-- > 0;) reach += reach + (x[i] > edge || (x[i] == edge && ~(id(i) + zero) >= least));
+            own = __popc(reach);
             at = room(own, sh);
             __syncthreads();
-            const uint32_t count = sh.count;
+            const uint32_t count = __builtin_amdgcn_readfirstlane(sh.count);
             if (count >= top)
                 low = mid;
             else
                 high = mid;
             found = (count >= top && count <= CANDIDATES) || high - low < 2;
-            if (found && own) {
-#pragma unroll
-                for (uint32_t i = 0; i < N; ++i) {
-                    const uint64_t k = key_of(x[i], id(i) + zero);
-                    if (x[i] >= floor && k >= mid && at < CANDIDATES) sh.key[at++] = k;
-                }
-            }
+            if (found) leave();
         }
         __syncthreads();
     }
@@ -265,15 +281,18 @@ __device__ __forceinline__ const void* row_of(const Args& a, uint32_t r) {
 
 // Measured on MI355X: 47.9 us for 512 rows of 151936 f32 logits with one alternative (311 MB, 6.5 TB/s); 5.6 for one row with
 // 20, a launch, a trip to memory and the selection one after the other. Those 512 rows without alternatives and with 1, 5, 20
-// and 64, both kernels: 51.4, 55.8, 59.8, 64.1 and 77.4, where the sort, the ranking and their barriers take the place of loads.
-// Wavefronts of a kernel to a SIMD: as many as its registers allow; 512 threads of 32 logits are 6 with a few spills outside the
-// sums (4096 rows of 16000 bf16 logits, 5 alternatives: 50.9 us, with 4 and none 59.9).
-constexpr int waves_of(uint32_t threads, uint32_t each) { return each == 16 ? 8 : threads == 256 ? 5 : threads == 512 ? 6 : 4; }
+// and 64, both kernels: 50.9, 54.3, 58.9, 61.4 and 74.6, where the sort, the ranking and their barriers take the place of loads.
+// Wavefronts of a kernel to a SIMD: as many as its registers allow without a spill (512 rows of 151936 f32 logits, 20
+// alternatives: 61 us with 6 of 32 logits to a thread, 79 with 7, 92 with 8).
+constexpr int waves_of(uint32_t threads, uint32_t each) { return each == 16 ? 8 : threads == 1024 ? 4 : 6; }
 
 template <bool BF16, uint32_t THREADS, uint32_t EACH>
 __global__ void __launch_bounds__(THREADS, waves_of(THREADS, EACH)) logprobs_slices_kernel(Args a) {
     constexpr uint32_t WAVES = THREADS / 64;
     constexpr uint32_t PIECE = BF16 ? 8 : 4;  // logits of a 16-byte load
+    // 56 registers of the 40 needed: with more wavefronts in flight memory is slower (512 rows of 151936 f32 logits that no cache
+    // has: 57.1 us, 59.0 without).
+    if constexpr (EACH == 16) asm volatile("" ::: "v55");
     __shared__ Shared<THREADS> sh;
     const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const uint32_t r = blockIdx.x / a.slices, slice = blockIdx.x % a.slices;
@@ -379,7 +398,7 @@ __global__ void __launch_bounds__(256) logprobs_join_kernel(Args a) {
         }
 #pragma unroll
         for (uint32_t i = 0; i < N; ++i) most = fmaxf(most, x[i]);
-        pick<THREADS>(x, most, [&](uint32_t i) { return ids[i]; }, a.top, sh);
+        pick<THREADS>(x, most, [&](uint32_t i) { return chosen(ids, i); }, a.top, sh);
         if (threadIdx.x < a.top) kept[threadIdx.x] = sh.top[threadIdx.x];
         done += some;
         if (done < keys) __syncthreads();
@@ -410,11 +429,11 @@ struct Slices {
     uint32_t threads, each, count;
 };
 // Measured on MI355X (us; threads x logits). A row in one slice needs no second kernel: 8000 logits, one row with 20 alternatives
-// 6.0 with 512 x 16, 9.3 in two slices; 16000: 7.9 with 512 x 32, 9.8 in four; 32001: 9.6 with 1024 x 32, 10.7 in eight, while
-// a row has a CU (256 rows with 5: 10.4, 14.8; 1024 rows 41 and 34), and one alternative 6.5 and 7.8. Many short rows: 256 x 32
+// 6.0 with 512 x 16, 9.3 in two slices; 16000: 7.4 with 512 x 32, 9.8 in four; 32001: 9.2 with 1024 x 32, 10.7 in eight, while
+// a row has a CU (256 rows with 5: 10.1, 14.8; 1024 rows 41 and 34), and one alternative 6.5 and 7.8. Many short rows: 256 x 32
 // (4096 of 8000 with 5: 27.2; 33.8 with 512 x 16).
 // Longer rows: 256 x 16 while there are up to 3 blocks to a CU (one row of 151936, 20 alternatives: 10.8; 11.8 with 256 x 32),
-// then 256 x 32, which selects once for twice the logits (512 rows, 20: 62; 73 with 256 x 16, 80 with 512 x 16), but f32
+// then 256 x 32, which selects once for twice the logits (512 rows, 20: 61; 73 with 256 x 16, 80 with 512 x 16), but f32
 // without selection, which is bound by its loads: 512 x 16 (1024 rows of 151936: 104; 110 with 256 x 32).
 constexpr uint64_t FEW = 768;
 Slices slices_of(const x0ne_logprobs* d) {
