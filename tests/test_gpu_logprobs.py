@@ -129,7 +129,7 @@ def test_strides(kernels, vocab, stride, kind):
 
 
 @pytest.mark.parametrize("kind", ["f32", "bf16"])
-@pytest.mark.parametrize("rows,vocab", [(1, 8192), (600, 8000), (300, 8192), (2, 16384), (40, 16001), (2, 16385), (256, 17000), (257, 17000),
+@pytest.mark.parametrize("rows,vocab", [(1, 8192), (600, 8000), (300, 8192), (2, 16384), (40, 16001), (2, 16385), (256, 17000), (257, 17000), (512, 16390), (513, 16390),
                                         (1, 32768), (30, 32768), (1, 32769), (60, 50257), (62, 50001), (3, 262144), (12, 262145)])
 def test_rows_cut_in_every_way(kernels, rows, vocab, kind):
     """Sizes at both sides of each rule by which rows are cut, with no, one and more alternatives; equal logits in rows that

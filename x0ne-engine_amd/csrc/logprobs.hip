@@ -79,7 +79,7 @@ struct Shared {
     uint64_t key[CANDIDATES + 16];
     uint64_t top[MOST_TOP];
     float4 state[THREADS / 64];
-    float all[THREADS / 64], some[THREADS / 64];
+    float all[THREADS / 64], some[THREADS / 64], group[32];
     uint32_t count;
 };
 
@@ -106,21 +106,36 @@ __device__ __forceinline__ float sorted(float x) {
     return threadIdx.x & BIT ? fminf(x, o) : fmaxf(x, o);
 }
 
-// A floor that at least `top` of the block's logits reach, by the largest of each thread's, which a wavefront sorts: the
-// highest of the wavefronts' top-th ones, or the lowest of the p-th ones, p top over the wavefronts rounded up. On ordinary
-// rows few more reach it (of 4096 logits about 10 for 5, 30 for 20, 80 for 64). -infinity is no alternative: the floor is above it.
+// A floor that at least `top` of the block's logits reach, by the largest of each thread's. -infinity is no alternative: the
+// floor is above it. Few alternatives: the top-th of the largest of 16 or 32 groups of neighbouring threads, which few more
+// reach (6 for 5, 31 for 20). More: each wavefront sorts its threads' largest, and the floor is the highest of the wavefronts'
+// top-th ones or the lowest of the p-th ones, p top over the wavefronts rounded up (of 4096 logits 30 for 20, 80 for 64).
+// 32 groups are for blocks of 512 and more, where the sort of 64 is dearer (61 rows of 32001, 20 alternatives: 9.7 us, 11.7
+// by wavefronts; with 256 threads one row of 151936 11.4 and 10.7, as the join's keys lie in order).
 template <uint32_t THREADS>
 __device__ __forceinline__ float floor_of(float most, uint32_t top, Shared<THREADS>& sh) {
     constexpr uint32_t WAVES = THREADS / 64;
-    float x = sorted<1, 1>(most);
-    x = sorted<1, 1>(sorted<3, 2>(x));
-    x = sorted<1, 1>(sorted<2, 2>(sorted<7, 4>(x)));
-    x = sorted<1, 1>(sorted<2, 2>(sorted<4, 4>(sorted<15, 8>(x))));
-    x = sorted<1, 1>(sorted<2, 2>(sorted<4, 4>(sorted<8, 8>(sorted<31, 16>(x)))));
+    const auto sorted16 = [](float x) {
+        x = sorted<1, 1>(x);
+        x = sorted<1, 1>(sorted<3, 2>(x));
+        x = sorted<1, 1>(sorted<2, 2>(sorted<7, 4>(x)));
+        return sorted<1, 1>(sorted<2, 2>(sorted<4, 4>(sorted<15, 8>(x))));
+    };
+    const auto nth = [](float x, uint32_t l) { return __uint_as_float((uint32_t)__builtin_amdgcn_readlane((int)__float_as_uint(x), (int)l)); };
+    const auto sorted32 = [&](float x) { return sorted<1, 1>(sorted<2, 2>(sorted<4, 4>(sorted<8, 8>(sorted<31, 16>(sorted16(x)))))); };
+    if (top <= (THREADS >= 512 ? 24 : 12)) {
+        const uint32_t lanes = THREADS / (top <= 12 ? 16 : 32);  // to a group: 16, 32 or 64
+        float largest = fold<3>(fold<2>(fold<1>(fold<0>(most, Most()), Most()), Most()), Most());
+        if (lanes >= 32) largest = fold<4>(largest, Most());
+        if (lanes == 64) largest = fold<5>(largest, Most());
+        if (threadIdx.x % lanes == 0) sh.group[threadIdx.x / lanes] = largest;
+        __syncthreads();
+        return fmaxf(top <= 12 ? nth(sorted16(sh.group[threadIdx.x & 15]), top - 1) : nth(sorted32(sh.group[threadIdx.x & 31]), top - 1), LOWEST);
+    }
+    float x = sorted32(most);
     x = sorted<1, 1>(sorted<2, 2>(sorted<4, 4>(sorted<8, 8>(sorted<16, 16>(sorted<63, 32>(x))))));
-    auto nth = [&](uint32_t l) { return __uint_as_float((uint32_t)__builtin_amdgcn_readlane((int)__float_as_uint(x), (int)l)); };
-    sh.all[threadIdx.x >> 6] = nth(top - 1);
-    sh.some[threadIdx.x >> 6] = nth((top - 1) / WAVES);
+    sh.all[threadIdx.x >> 6] = nth(x, top - 1);
+    sh.some[threadIdx.x >> 6] = nth(x, (top - 1) / WAVES);
     __syncthreads();
     const uint32_t w = threadIdx.x & (WAVES - 1);
     float one = sh.all[w], each = sh.some[w];
@@ -279,11 +294,11 @@ __device__ __forceinline__ const void* row_of(const Args& a, uint32_t r) {
     return static_cast<const uint8_t*>(a.logits) + r * a.stride * (BF16 ? 2 : 4);
 }
 
-// Measured on MI355X: 47.9 us for 512 rows of 151936 f32 logits with one alternative (311 MB, 6.5 TB/s); 5.6 for one row with
+// Measured on MI355X: 46.9 us for 512 rows of 151936 f32 logits with one alternative (311 MB, 6.6 TB/s); 5.6 for one row with
 // 20, a launch, a trip to memory and the selection one after the other. Those 512 rows without alternatives and with 1, 5, 20
-// and 64, both kernels: 50.9, 54.3, 58.9, 61.4 and 74.6, where the sort, the ranking and their barriers take the place of loads.
+// and 64, both kernels: 51.4, 54.3, 57.0, 62.5 and 74.6, where the sort, the ranking and their barriers take the place of loads.
 // Wavefronts of a kernel to a SIMD: as many as its registers allow without a spill (512 rows of 151936 f32 logits, 20
-// alternatives: 61 us with 6 of 32 logits to a thread, 79 with 7, 92 with 8).
+// alternatives: 62 us with 6 of 32 logits to a thread, 79 with 7, 92 with 8).
 constexpr int waves_of(uint32_t threads, uint32_t each) { return each == 16 ? 8 : threads == 1024 ? 4 : 6; }
 
 template <bool BF16, uint32_t THREADS, uint32_t EACH>
@@ -429,19 +444,19 @@ struct Slices {
     uint32_t threads, each, count;
 };
 // Measured on MI355X (us; threads x logits). A row in one slice needs no second kernel: 8000 logits, one row with 20 alternatives
-// 6.0 with 512 x 16, 9.3 in two slices; 16000: 7.4 with 512 x 32, 9.8 in four; 32001: 9.2 with 1024 x 32, 10.7 in eight, while
-// a row has a CU (256 rows with 5: 10.1, 14.8; 1024 rows 41 and 34), and one alternative 6.5 and 7.8. Many short rows: 256 x 32
-// (4096 of 8000 with 5: 27.2; 33.8 with 512 x 16).
-// Longer rows: 256 x 16 while there are up to 3 blocks to a CU (one row of 151936, 20 alternatives: 10.8; 11.8 with 256 x 32),
-// then 256 x 32, which selects once for twice the logits (512 rows, 20: 61; 73 with 256 x 16, 80 with 512 x 16), but f32
-// without selection, which is bound by its loads: 512 x 16 (1024 rows of 151936: 104; 110 with 256 x 32).
+// 5.5 with 512 x 16, 9.2 in two slices; 16000: 6.9 with 512 x 32, 9.8 in four; 32001: 8.6 with 1024 x 32, 10.6 in eight, while
+// there are up to 2 rows to a CU (512 rows with 5: 17.1, 19.1 in slices; 1024 rows 33.4, 28.8). Many short rows: 256 x 32
+// (4096 of 8000 with 5: 24.7; 31.0 with 512 x 16).
+// Longer rows: 256 x 16 while there are up to 3 blocks to a CU (one row of 151936, 20 alternatives: 10.7; 11.4 with 256 x 32),
+// then 256 x 32, which selects once for twice the logits (512 rows, 20: 63.1; 77.7 with 256 x 16, 74.0 with 512 x 16), but f32
+// without selection, which is bound by its loads: 512 x 16 (1024 rows of 151936: 107.3; 110.7 with 256 x 32, 112.4 with 256 x 16).
 constexpr uint64_t FEW = 768;
 Slices slices_of(const x0ne_logprobs* d) {
     const auto cut = [&](uint32_t threads, uint32_t each) { return Slices{threads, each, (d->vocab + threads * each - 1) / (threads * each)}; };
     if (d->vocab <= 4096) return cut(256, 16);
     if (d->vocab <= 8192) return d->rows > 512 ? cut(256, 32) : cut(512, 16);
     if (d->vocab <= 16384) return cut(512, 32);
-    if (d->vocab <= 32768 && d->rows <= 256) return cut(1024, 32);
+    if (d->vocab <= 32768 && d->rows <= 512) return cut(1024, 32);
     const Slices few = cut(256, 16);
     if ((uint64_t)d->rows * few.count <= FEW) return few;
     return d->top <= 1 && !d->bf16 ? cut(512, 16) : cut(256, 32);
