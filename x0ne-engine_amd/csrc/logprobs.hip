@@ -294,7 +294,7 @@ __device__ __forceinline__ const void* row_of(const Args& a, uint32_t r) {
     return static_cast<const uint8_t*>(a.logits) + r * a.stride * (BF16 ? 2 : 4);
 }
 
-// Measured on MI355X: 46.9 us for 512 rows of 151936 f32 logits with one alternative (311 MB, 6.6 TB/s); 5.6 for one row with
+// Measured on MI355X: 47.2 us for 512 rows of 151936 f32 logits with one alternative (311 MB, 6.6 TB/s); 5.4 for one row with
 // 20, a launch, a trip to memory and the selection one after the other. Those 512 rows without alternatives and with 1, 5, 20
 // and 64, both kernels: 51.4, 54.3, 57.0, 62.5 and 74.6, where the sort, the ranking and their barriers take the place of loads.
 // Wavefronts of a kernel to a SIMD: as many as its registers allow without a spill (512 rows of 151936 f32 logits, 20
