@@ -66,6 +66,16 @@ constexpr uint64_t SCRATCH_COUNTERS = 256;
 constexpr uint64_t SCRATCH_BYTES = SCRATCH_STATE_BYTES + SCRATCH_COUNTERS * 4;
 static __device__ __align__(256) uint8_t scratch[SCRATCH_BYTES];
 
+// The calling thread's capture mode is relaxed meanwhile: another thread may have a capture of its own Gpu open, which an
+// allocation or a free in the default mode ends.
+struct Relaxed {
+    hipStreamCaptureMode mode = hipStreamCaptureModeRelaxed;
+    const bool on = hipThreadExchangeStreamCaptureMode(&mode) == hipSuccess;
+    ~Relaxed() {
+        if (on) (void)hipThreadExchangeStreamCaptureMode(&mode);
+    }
+};
+
 extern "C" x0ne_status x0ne_gpu_new(x0ne_gpu** out) {
     if (!out) return fail(X0NE_ERR_FORMAT, "x0ne_gpu_new: null out");
     *out = nullptr;
@@ -100,11 +110,11 @@ extern "C" x0ne_status x0ne_gpu_new(x0ne_gpu** out) {
         delete g;
         return gpu_fail(e, "hipStreamCreateWithFlags");
     }
-    // In relaxed mode and by a kernel: another thread may have a capture of its own Gpu open.
-    hipStreamCaptureMode mode = hipStreamCaptureModeRelaxed;
-    const bool relaxed = hipThreadExchangeStreamCaptureMode(&mode) == hipSuccess;
-    e = hipMalloc((void**)&g->counters, GPU_COUNTERS * 4);
-    if (relaxed) (void)hipThreadExchangeStreamCaptureMode(&mode);
+    // Filled by a kernel, which another thread's capture allows too.
+    {
+        const Relaxed relaxed;
+        e = hipMalloc((void**)&g->counters, GPU_COUNTERS * 4);
+    }
     if (e == hipSuccess) e = x0ne_launch_fill_u16((uint16_t*)g->counters, GPU_COUNTERS * 2, 0, g->stream);
     if (e != hipSuccess) {
         x0ne_gpu_free(g);
@@ -119,12 +129,19 @@ namespace x0ne {
 
 extern "C" void x0ne_gpu_free(x0ne_gpu* g) {
     if (!g) return;
-    if (g->stream) {
-        (void)hipStreamSynchronize(g->stream);
-        (void)hipStreamDestroy(g->stream);
+    {
+        const Relaxed relaxed;
+        // Nobody is told of an error here: it is not left for this thread's next launch either.
+        const auto done = [](hipError_t e) {
+            if (e != hipSuccess) (void)hipGetLastError();
+        };
+        if (g->stream) {
+            done(hipStreamSynchronize(g->stream));
+            done(hipStreamDestroy(g->stream));
+        }
+        if (g->tile_parts) done(hipFree(g->tile_parts));
+        if (g->counters) done(hipFree(g->counters));
     }
-    if (g->tile_parts) (void)hipFree(g->tile_parts);
-    if (g->counters) (void)hipFree(g->counters);
     delete g;
 }
 
@@ -299,16 +316,12 @@ namespace x0ne {
 // Gpu's GEMMs then stay unsplit.
 float* own_parts(x0ne_gpu* g) {
     if (!g->tile_parts && !g->tile_parts_refused && !g->capturing) {
-        // Another thread may have a capture of its own Gpu open: this thread's mode is relaxed for the
-        // allocation, so that it is neither refused nor ends that capture.
-        hipStreamCaptureMode mode = hipStreamCaptureModeRelaxed;
-        const bool relaxed = hipThreadExchangeStreamCaptureMode(&mode) == hipSuccess;
+        const Relaxed relaxed;
         if (hipMalloc((void**)&g->tile_parts, TILE_PARTS_BYTES) != hipSuccess) {
             (void)hipGetLastError();
             g->tile_parts = nullptr;
             g->tile_parts_refused = true;
         }
-        if (relaxed) (void)hipThreadExchangeStreamCaptureMode(&mode);
     }
     return g->tile_parts;
 }
