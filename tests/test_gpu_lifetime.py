@@ -1,5 +1,6 @@
 """A Gpu is closed while a capture of another is open: its memory comes back, the capture stays whole, and no error is left
 behind for a later launch."""
+import ctypes as C
 import threading
 
 import numpy as np
@@ -83,3 +84,31 @@ def test_a_gpu_is_closed_while_another_captures(kernels, same_thread):
     graph.close()
     third.close()
     a.close()
+
+
+def test_a_gpu_takes_no_device_memory_beside_its_stream(kernels):
+    """64 of them against 64 streams of the runtime: less than 8 MiB apart, 128 KiB to each. The first turn of either makes what
+    the runtime keeps."""
+    from x0ne_core import Gpu, lib
+    streams = []
+
+    def stream():
+        s = C.c_void_p()
+        assert lib().hipStreamCreateWithFlags(C.byref(s), 1) == 0  # non-blocking, of the runtime that the library uses
+        streams.append(s)
+
+    def taken(make):
+        before = kernels.gpu.mem_info()[0]
+        made = [make() for _ in range(64)]
+        took = (before - kernels.gpu.mem_info()[0]) / (1 << 20)
+        for g in made:
+            if g:
+                g.close()
+        while streams:
+            assert lib().hipStreamDestroy(streams.pop()) == 0
+        return took
+
+    for _ in range(2):
+        of_streams, of_gpus = taken(stream), taken(Gpu)
+    print(f"MEASURE MiB taken by 64 streams {of_streams}, by 64 Gpus {of_gpus}")
+    assert of_gpus - of_streams < 8

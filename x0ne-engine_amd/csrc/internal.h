@@ -68,7 +68,7 @@ struct x0ne_gpu {
     // first needed and freed with the Gpu. Its calls run on one stream, one after the other.
     float* tile_parts = nullptr;
     bool tile_parts_refused = false;  // the allocation failed once: its calls stay unsplit
-    // Counters of blocks that finish one another's sums (w4.hip): zero, left at zero by every launch.
+    // Counters of blocks that finish one another's sums (w4.hip), behind tile_parts: zero, left at zero by every launch.
     uint32_t* counters = nullptr;
 };
 
@@ -131,7 +131,8 @@ constexpr uint64_t TILE_PARTS_BYTES = 64ull << 20;
 constexpr TileWork OWN_TILE_WORK = {nullptr, TILE_PARTS_BYTES, true};
 x0ne_status tiled_gemm(x0ne_gpu* g, int tile, uint32_t layout, const void* w, uint64_t rows, uint64_t cols,
                        const void* x, uint64_t n, void* y, bool out_f32, TileWork work = {}, uint32_t slices = 1);
-// The Gpu's workspace of TILE_PARTS_BYTES for sums in parts, taken when first asked for outside a capture; null without.
+// The Gpu's workspace of TILE_PARTS_BYTES for sums in parts and its counters, taken when first asked for outside a capture;
+// null without.
 float* own_parts(x0ne_gpu* g);
 // Words of x0ne_gpu::counters.
 constexpr uint32_t GPU_COUNTERS = 65536;

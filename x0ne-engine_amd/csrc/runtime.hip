@@ -110,16 +110,6 @@ extern "C" x0ne_status x0ne_gpu_new(x0ne_gpu** out) {
         delete g;
         return gpu_fail(e, "hipStreamCreateWithFlags");
     }
-    // Filled by a kernel, which another thread's capture allows too.
-    {
-        const Relaxed relaxed;
-        e = hipMalloc((void**)&g->counters, GPU_COUNTERS * 4);
-    }
-    if (e == hipSuccess) e = x0ne_launch_fill_u16((uint16_t*)g->counters, GPU_COUNTERS * 2, 0, g->stream);
-    if (e != hipSuccess) {
-        x0ne_gpu_free(g);
-        return gpu_fail(e, "the counters");
-    }
     *out = g;
     return X0NE_OK;
 }
@@ -140,7 +130,6 @@ extern "C" void x0ne_gpu_free(x0ne_gpu* g) {
             done(hipStreamDestroy(g->stream));
         }
         if (g->tile_parts) done(hipFree(g->tile_parts));
-        if (g->counters) done(hipFree(g->counters));
     }
     delete g;
 }
@@ -312,14 +301,22 @@ static constexpr uint64_t GEMM_MAX_BYTES = 0xFFFFFFF0ull;
 namespace x0ne {
 
 // The Gpu's own workspace for the tiled GEMM's slices, allocated at the first call whose plan has
-// slices or when a capture begins (a capture must not allocate); null without the memory for it: the
-// Gpu's GEMMs then stay unsplit.
+// slices or when a capture begins (a capture must not allocate), with the counters behind it; null
+// without the memory for it: the Gpu's GEMMs then stay unsplit.
 float* own_parts(x0ne_gpu* g) {
     if (!g->tile_parts && !g->tile_parts_refused && !g->capturing) {
         const Relaxed relaxed;
-        if (hipMalloc((void**)&g->tile_parts, TILE_PARTS_BYTES) != hipSuccess) {
+        const OnDevice on(g->device);
+        void* p = nullptr;
+        hipError_t e = hipMalloc(&p, TILE_PARTS_BYTES + GPU_COUNTERS * 4);
+        uint32_t* counters = (uint32_t*)((uint8_t*)p + TILE_PARTS_BYTES);
+        // Cleared by a kernel, ahead of the call's own on the stream.
+        if (e == hipSuccess && (e = x0ne_launch_fill_u16((uint16_t*)counters, GPU_COUNTERS * 2, 0, g->stream)) != hipSuccess) (void)hipFree(p);
+        if (e == hipSuccess) {
+            g->tile_parts = (float*)p;
+            g->counters = counters;
+        } else {
             (void)hipGetLastError();
-            g->tile_parts = nullptr;
             g->tile_parts_refused = true;
         }
     }
