@@ -136,6 +136,9 @@ x0ne_status tiled_gemm(x0ne_gpu* g, int tile, uint32_t layout, const void* w, ui
 float* own_parts(x0ne_gpu* g);
 // Words of x0ne_gpu::counters.
 constexpr uint32_t GPU_COUNTERS = 65536;
+// Counters in front of the caller's workspaces: zeroed once by the caller, left at zero by every launch that counts there
+// (kv8.hip), left alone by every other (logprobs.hip), so that calls of all kinds and shapes share a workspace.
+constexpr uint64_t WORK_COUNTERS = 65536, WORK_COUNTER_BYTES = 4 * WORK_COUNTERS;
 // x0ne_gpu_gemv with the tiled GEMM's workspace given.
 x0ne_status gemv_rows(x0ne_gpu* g, uint64_t w, uint64_t rows, uint64_t cols, uint64_t x, uint64_t n, uint64_t y,
                       bool out_f32, TileWork work);

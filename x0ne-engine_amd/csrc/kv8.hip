@@ -1216,8 +1216,7 @@ static Kv8Cut cut_of(const x0ne_kv8* c, uint32_t budget = 0) { return kv8_cut(c-
 // The workspace: a counter per (sequence, kv head), then the states of attention or the scores of selection. The counters
 // are as many for every cache, so that no call's states lie where another's counters are: caches of any shapes share a
 // workspace. Sequences beyond 65536 pairs are further launches, which come upon the counters left at zero.
-static constexpr uint64_t COUNTERS = 65536, COUNTER_BYTES = 4 * COUNTERS;
-static uint32_t seqs_at_once(const x0ne_kv8* c) { return (uint32_t)(COUNTERS / c->kv_heads) / 64 * 64; }
+static uint32_t seqs_at_once(const x0ne_kv8* c) { return (uint32_t)(WORK_COUNTERS / c->kv_heads) / 64 * 64; }
 static Table table_of(const x0ne_kv8* c, uint64_t first) {  // of a launch's sequences
     return Table{(const uint32_t*)c->page_table + first * c->seq_pages, (uint32_t)std::min<uint64_t>(c->seqs - first, seqs_at_once(c)),
                  c->seq_pages, c->pool, c->kv_heads};
@@ -1227,7 +1226,7 @@ extern "C" uint64_t x0ne_kv8_work_bytes(const x0ne_kv8* c, uint32_t q_heads) {
     if (check_shape("kv8 workspace", c) != X0NE_OK || check_heads("kv8 workspace", c, q_heads) != X0NE_OK) return 0;
     const uint64_t states = (uint64_t)c->seqs * q_heads * cut_of(c).slices * STATE * 4;
     const uint64_t scores = (uint64_t)c->seqs * c->kv_heads * c->seq_pages * 8;
-    return COUNTER_BYTES + std::max(states, scores);
+    return WORK_COUNTER_BYTES + std::max(states, scores);
 }
 
 extern "C" x0ne_status x0ne_gpu_kv8_attention(x0ne_gpu* g, const x0ne_kv8* c, uint64_t q, uint32_t q_heads, uint64_t lens,
@@ -1256,7 +1255,7 @@ extern "C" x0ne_status x0ne_gpu_kv8_attention(x0ne_gpu* g, const x0ne_kv8* c, ui
         a.list = page_list ? (const uint32_t*)page_list + s * c->kv_heads * budget : nullptr;
         a.out = (bf16_t*)out + s * q_heads * KV8_HEAD;
         a.counter = (uint32_t*)work;
-        a.state = (float*)(work + COUNTER_BYTES);
+        a.state = (float*)(work + WORK_COUNTER_BYTES);
         a.budget = budget;
         a.q_heads = q_heads;
         a.group = q_heads / c->kv_heads;
@@ -1291,7 +1290,7 @@ extern "C" x0ne_status x0ne_gpu_kv8_select(x0ne_gpu* g, const x0ne_kv8* c, uint6
         g->counts.launches++;
         hipLaunchKernelGGL(kv8_select_kernel, dim3(c->kv_heads, blocks, t.seqs), dim3(SELECT_THREADS), 0, g->stream, t,
                            (const bf16_t*)bounds, (const bf16_t*)q + s * q_heads * KV8_HEAD, (const uint32_t*)lens + s, budget,
-                           (uint32_t*)page_list + s * c->kv_heads * budget, (uint64_t*)(work + COUNTER_BYTES), (uint32_t*)work,
+                           (uint32_t*)page_list + s * c->kv_heads * budget, (uint64_t*)(work + WORK_COUNTER_BYTES), (uint32_t*)work,
                            q_heads / c->kv_heads);
         X0NE_HIP(hipGetLastError(), what);
     }

@@ -462,9 +462,7 @@ Slices slices_of(const x0ne_logprobs* d) {
     return d->top <= 1 && !d->bf16 ? cut(512, 16) : cut(256, 32);
 }
 
-// The workspace's first part is left alone: there the calls of the 8-bit cache count, which may share it. Behind it the slices'
-// states, then their top keys.
-constexpr uint64_t COUNTER_BYTES = 4 * 65536;
+// The workspace: the counters' part, which is left alone, the slices' states, then their top keys.
 // A launch has so many rows and slices at most (fewer than 2^32 threads), and the workspace is a launch's: more are further launches.
 constexpr uint64_t MOST_ROWS = 65536, MOST_SLICES = 1u << 22;
 uint64_t rows_at_once(const x0ne_logprobs* d) { return std::min(MOST_ROWS, MOST_SLICES / slices_of(d).count); }
@@ -485,7 +483,7 @@ extern "C" uint64_t x0ne_logprobs_work_bytes(const x0ne_logprobs* d) {
     // Enough for fewer rows too, which may be cut into more slices, up to FEW.
     const uint64_t rows = std::min<uint64_t>(d->rows, MOST_ROWS);
     const uint64_t slices = std::max(std::min(rows * slices_of(d).count, MOST_SLICES), std::min(rows * ((d->vocab + 4095) / 4096), FEW));
-    return COUNTER_BYTES + slices * (sizeof(float4) + 8ull * d->top);
+    return WORK_COUNTER_BYTES + slices * (sizeof(float4) + 8ull * d->top);
 }
 
 extern "C" x0ne_status x0ne_gpu_logprobs(x0ne_gpu* g, const x0ne_logprobs* d) {
@@ -515,7 +513,7 @@ extern "C" x0ne_status x0ne_gpu_logprobs(x0ne_gpu* g, const x0ne_logprobs* d) {
         a.entropy = d->entropy ? (float*)d->entropy + first : nullptr;
         a.top_ids = (uint32_t*)d->top_ids + first * d->top;
         a.top_lp = (float*)d->top_lp + first * d->top;
-        a.state = (float4*)(d->work + COUNTER_BYTES);
+        a.state = (float4*)(d->work + WORK_COUNTER_BYTES);
         a.best = (uint64_t*)(a.state + (uint64_t)rows * slices);
         a.vocab = d->vocab;
         a.slices = slices;
