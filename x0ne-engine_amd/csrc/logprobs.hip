@@ -241,13 +241,14 @@ __device__ __forceinline__ void pick(const float (&x)[N], float most, Id id, uin
 }
 
 // (m, z, t) of two sets: one at the larger m as it is, one so far below it that nothing is left without an infinity times
-// zero. A set of nothing but -infinity has m = -infinity and z = t = 0, or NaN.
+// zero. An exponential times its difference is at most 1 / (e scale) and comes first: a difference times z may be past f32.
+// A set of nothing but -infinity has m = -infinity and z = t = 0, or NaN.
 __device__ __forceinline__ float4 join(float4 a, float4 b, float scale2) {
     const float m = fmaxf(a.x, b.x), da = a.x - m, db = b.x - m;
     float4 r = {m, 0.f, 0.f, 0.f};
     const float pa = __builtin_amdgcn_exp2f(da * scale2), pb = __builtin_amdgcn_exp2f(db * scale2);
     r.y = (a.x == m ? a.y : pa * a.y) + (b.x == m ? b.y : pb * b.y);
-    r.z = (a.x == m ? a.z : pa > 0.f ? pa * (a.z + da * a.y) : 0.f) + (b.x == m ? b.z : pb > 0.f ? pb * (b.z + db * b.y) : 0.f);
+    r.z = (a.x == m ? a.z : pa > 0.f ? pa * a.z + pa * da * a.y : 0.f) + (b.x == m ? b.z : pb > 0.f ? pb * b.z + pb * db * b.y : 0.f);
     return r;
 }
 
