@@ -9,12 +9,13 @@
 
 #include "device.h"
 #include "internal.h"
+#include "logprobs.h"
 
 using namespace x0ne;
 
 namespace {
 
-constexpr uint32_t MOST_TOP = 64;
+constexpr uint32_t MOST_TOP = LOGPROBS_MOST_TOP;
 constexpr uint32_t CANDIDATES = 512;
 constexpr uint32_t RANKED = 128;  // so many keys are ranked without a floor
 constexpr float LOG2E = 1.44269504088896340736f, LOWEST = -3.40282347e38f;
@@ -123,7 +124,7 @@ __device__ __forceinline__ float floor_of(float most, uint32_t top, Shared<THREA
     };
     const auto nth = [](float x, uint32_t l) { return __uint_as_float((uint32_t)__builtin_amdgcn_readlane((int)__float_as_uint(x), (int)l)); };
     const auto sorted32 = [&](float x) { return sorted<1, 1>(sorted<2, 2>(sorted<4, 4>(sorted<8, 8>(sorted<31, 16>(sorted16(x)))))); };
-    if (top <= (THREADS >= 512 ? 24 : 12)) {
+    if (top <= logprobs_in_groups(THREADS)) {
         const uint32_t lanes = THREADS / (top <= 12 ? 16 : 32);  // to a group: 16, 32 or 64
         float largest = fold<3>(fold<2>(fold<1>(fold<0>(most, Most()), Most()), Most()), Most());
         if (lanes >= 32) largest = fold<4>(largest, Most());
@@ -440,50 +441,21 @@ x0ne_status check_shape(const x0ne_logprobs* d) {
     return X0NE_OK;
 }
 
-// How a row is cut: threads to a block, logits to a thread.
-struct Slices {
-    uint32_t threads, each, count;
-};
-// Measured on MI355X (us; threads x logits). A row in one slice needs no second kernel: 8000 logits, one row with 20 alternatives
-// 5.5 with 512 x 16, 9.2 in two slices; 16000: 6.9 with 512 x 32, 9.8 in four; 32001: 8.6 with 1024 x 32, 10.6 in eight, while
-// there are up to 2 rows to a CU (512 rows with 5: 17.1, 19.1 in slices; 1024 rows 33.4, 28.8). Many short rows: 256 x 32
-// (4096 of 8000 with 5: 24.7; 31.0 with 512 x 16).
-// Longer rows: 256 x 16 while there are up to 3 blocks to a CU (one row of 151936, 20 alternatives: 10.7; 11.4 with 256 x 32),
-// then 256 x 32, which selects once for twice the logits (512 rows, 20: 63.1; 77.7 with 256 x 16, 74.0 with 512 x 16), but f32
-// without selection, which is bound by its loads: 512 x 16 (1024 rows of 151936: 107.3; 110.7 with 256 x 32, 112.4 with 256 x 16).
-constexpr uint64_t FEW = 768;
-Slices slices_of(const x0ne_logprobs* d) {
-    const auto cut = [&](uint32_t threads, uint32_t each) { return Slices{threads, each, (d->vocab + threads * each - 1) / (threads * each)}; };
-    if (d->vocab <= 4096) return cut(256, 16);
-    if (d->vocab <= 8192) return d->rows > 512 ? cut(256, 32) : cut(512, 16);
-    if (d->vocab <= 16384) return cut(512, 32);
-    if (d->vocab <= 32768 && d->rows <= 512) return cut(1024, 32);
-    const Slices few = cut(256, 16);
-    if ((uint64_t)d->rows * few.count <= FEW) return few;
-    return d->top <= 1 && !d->bf16 ? cut(512, 16) : cut(256, 32);
-}
-
-// The workspace: the counters' part, which is left alone, the slices' states, then their top keys.
-// A launch has so many rows and slices at most (fewer than 2^32 threads), and the workspace is a launch's: more are further launches.
-constexpr uint64_t MOST_ROWS = 65536, MOST_SLICES = 1u << 22;
-uint64_t rows_at_once(const x0ne_logprobs* d) { return std::min(MOST_ROWS, MOST_SLICES / slices_of(d).count); }
-
 using Kernel = void (*)(Args);
 template <bool BF16>
-Kernel kernel_as(const Slices& s) {
+Kernel kernel_as(const LogprobsCut& s) {
     if (s.threads == 256) return s.each == 16 ? logprobs_slices_kernel<BF16, 256, 16> : logprobs_slices_kernel<BF16, 256, 32>;
     if (s.threads == 512) return s.each == 16 ? logprobs_slices_kernel<BF16, 512, 16> : logprobs_slices_kernel<BF16, 512, 32>;
     return logprobs_slices_kernel<BF16, 1024, 32>;
 }
-Kernel kernel_of(const Slices& s, bool bf16) { return bf16 ? kernel_as<true>(s) : kernel_as<false>(s); }
+Kernel kernel_of(const LogprobsCut& s, bool bf16) { return bf16 ? kernel_as<true>(s) : kernel_as<false>(s); }
 
 }  // namespace
 
+// The workspace: the counters' part, which is left alone, the slices' states, then their top keys.
 extern "C" uint64_t x0ne_logprobs_work_bytes(const x0ne_logprobs* d) {
     if (check_shape(d) != X0NE_OK) return 0;
-    // Enough for fewer rows too, which may be cut into more slices, up to FEW.
-    const uint64_t rows = std::min<uint64_t>(d->rows, MOST_ROWS);
-    const uint64_t slices = std::max(std::min(rows * slices_of(d).count, MOST_SLICES), std::min(rows * ((d->vocab + 4095) / 4096), FEW));
+    const uint64_t slices = logprobs_most_slices(d->rows, d->vocab, d->top, d->bf16);
     return WORK_COUNTER_BYTES + slices * (sizeof(float4) + 8ull * d->top);
 }
 
@@ -502,10 +474,10 @@ extern "C" x0ne_status x0ne_gpu_logprobs(x0ne_gpu* g, const x0ne_logprobs* d) {
     if (!g) return fail(X0NE_ERR_GPU, "no device");
     if (d->rows == 0) return X0NE_OK;
     const OnDevice on(g->device);
-    const Slices cut = slices_of(d);
+    const LogprobsCut cut = logprobs_cut(d->rows, d->vocab, d->top, d->bf16);
     const uint32_t slices = cut.count, threads = cut.threads;
-    for (uint64_t first = 0; first < d->rows; first += rows_at_once(d)) {
-        const uint32_t rows = (uint32_t)std::min<uint64_t>(d->rows - first, rows_at_once(d));
+    for (uint64_t first = 0; first < d->rows; first += cut.at_once) {
+        const uint32_t rows = (uint32_t)std::min<uint64_t>(d->rows - first, cut.at_once);
         Args a = {};
         a.logits = (const uint8_t*)d->logits + first * d->stride * each;
         a.stride = d->stride;
@@ -518,7 +490,7 @@ extern "C" x0ne_status x0ne_gpu_logprobs(x0ne_gpu* g, const x0ne_logprobs* d) {
         a.best = (uint64_t*)(a.state + (uint64_t)rows * slices);
         a.vocab = d->vocab;
         a.slices = slices;
-        a.length = ((d->vocab + slices - 1) / slices + 15) / 16 * 16;  // even slices, whose ends would leave groups of lanes empty
+        a.length = cut.length;
         a.per_row = d->per_row;
         a.top = d->top;
         a.scale = d->scale;
@@ -527,10 +499,8 @@ extern "C" x0ne_status x0ne_gpu_logprobs(x0ne_gpu* g, const x0ne_logprobs* d) {
         hipLaunchKernelGGL(kernel, dim3(rows * slices), dim3(threads), 0, g->stream, a);
         if (slices > 1) {
             g->counts.launches++;
-            // Shorter code is over sooner: 760 keys at 4 to a thread 12.2 us for one row, at 16 13.2; more than 1024 in one go.
-            const bool many_keys = (uint64_t)slices * d->top > 1024;
-            const auto joins = many_keys ? d->bf16 ? logprobs_join_kernel<true, 16> : logprobs_join_kernel<false, 16>
-                                         : d->bf16 ? logprobs_join_kernel<true, 4> : logprobs_join_kernel<false, 4>;
+            const auto joins = cut.join == 16 ? d->bf16 ? logprobs_join_kernel<true, 16> : logprobs_join_kernel<false, 16>
+                                              : d->bf16 ? logprobs_join_kernel<true, 4> : logprobs_join_kernel<false, 4>;
             hipLaunchKernelGGL(joins, dim3(rows), dim3(256), 0, g->stream, a);
         }
         X0NE_HIP(hipGetLastError(), "logprobs");
