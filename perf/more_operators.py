@@ -11,6 +11,9 @@ Ops:
   read      a matrix in 4 bits as bf16
   product   y = x w^T of a few rows x: bf16 or f32 out, or silu(gate) up of a packed [gate; up] matrix
   logprobs  per row of logits: log probabilities of given tokens, entropy, and the top alternatives
+
+Where own is true, run's calls are on the framework's own stream and wait for nothing: prepare's work is done when it returns,
+and outputs are read after torch.cuda.synchronize() or gpu().sync().
 """
 import math
 import os
@@ -209,11 +212,13 @@ def gpu():
 
 
 def call_of(state):
-    """What the program keeps of a matrix in 4 bits, or of a sampler's buffers: their descriptor and workspace."""
+    """What the program keeps of a matrix in 4 bits, or of a sampler's buffers: their descriptor and workspace. torch's own work
+    on the inputs is done behind it, as the calls are on another stream."""
     case, g = state["case"], gpu()
     from x0ne_core import LogProbs, W4
     at = {k: v.data_ptr() if v.numel() else 0 for k, v in state.items() if isinstance(v, torch.Tensor)}
     if case["op"] != "logprobs":
+        torch.cuda.synchronize()
         return W4(codes=at["codes"], scales=at["scales"], rows=case["rows"], cols=case["cols"], group=case["group"])
     d = LogProbs(logits=at["logits"], stride=case["stride"], tokens=at["tokens"], token_lp=at["token_lp"], entropy=at["entropy"],
                  top_ids=at["top_ids"], top_lp=at["top_lp"], rows=case["rows"], vocab=case["vocab"], per_row=case["tokens"],
