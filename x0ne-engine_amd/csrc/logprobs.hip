@@ -249,7 +249,7 @@ __device__ __forceinline__ float4 join(float4 a, float4 b, float scale2) {
     float4 r = {m, 0.f, 0.f, 0.f};
     const float pa = __builtin_amdgcn_exp2f(da * scale2), pb = __builtin_amdgcn_exp2f(db * scale2);
     r.y = (a.x == m ? a.y : pa * a.y) + (b.x == m ? b.y : pb * b.y);
-    r.z = (a.x == m ? a.z : pa > 0.f ? pa * a.z + pa * da * a.y : 0.f) + (b.x == m ? b.z : pb > 0.f ? pb * b.z + pb * db * b.y : 0.f);
+    r.z = (a.x == m ? a.z : pa > 0.f ? fmaf(pa * da, a.y, pa * a.z) : 0.f) + (b.x == m ? b.z : pb > 0.f ? fmaf(pb * db, b.y, pb * b.z) : 0.f);
     return r;
 }
 
