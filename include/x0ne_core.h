@@ -295,8 +295,8 @@ x0ne_status x0ne_gpu_w4_read(x0ne_gpu* g, const x0ne_w4* w, uint64_t to);
 /* Y = X W^T, X [n][cols] bf16 row-major (16-byte aligned): products and sums in f32, a group's sum
    times its scale, rounded once. out X0NE_W4_BF16, X0NE_W4_F32: Y [n][rows]; X0NE_W4_SWIGLU: W is
    [gate; up] (rows a multiple of 32) and Y [n][rows / 2] bf16 = silu(gate) up of the f32 sums. Y is
-   4-byte aligned and not in X. n up to 2^24; for one token to a few dozen (past 256 rows the read-back
-   and x0ne_gpu_gemv are faster). Some shapes' sums go in parts through the Gpu's workspace of
+   4-byte aligned and not in X. n up to 2^24; for one token to a few dozen (past about 500 rows reading back
+   before x0ne_gpu_gemv is faster). A group's sum has to stay in f32 before its scale too: |x| below 2^118. Some shapes' sums go in parts through the Gpu's workspace of
    x0ne_gpu_gemv (allocated at the first call that needs it or when a capture begins; without it their
    sums stay whole). The same call gives the same bits. */
 enum { X0NE_W4_BF16 = 0, X0NE_W4_F32 = 1, X0NE_W4_SWIGLU = 2 };
@@ -304,7 +304,7 @@ x0ne_status x0ne_gpu_w4_gemv(x0ne_gpu* g, const x0ne_w4* w, uint64_t x, uint64_t
 
 /* ---- log probabilities: no counterpart in the reference beside the engine's run ----
    Of rows of logits l, f32 or bf16 (bf16 = 1), row r at logits + r stride elements, vocab of them: with
-   x = scale l, log p = x - log sum e^x. Device addresses; what is 0 is not computed.
+   x = scale l, log p = x - log sum e^x. Device addresses; what is 0 is not written.
    tokens [rows][per_row] u32: token_lp [rows][per_row] f32 their log p, NaN for an id of vocab or more.
    entropy [rows] f32: - sum p log p (a p of 0 adds 0).
    top (0 to 64): top_ids [rows][top] u32 the ids of the largest logits, falling, the lower id first of

@@ -113,6 +113,10 @@ __device__ __forceinline__ float sorted(float x) {
 // top-th ones or the lowest of the p-th ones, p top over the wavefronts rounded up (of 4096 logits 30 for 20, 80 for 64).
 // 32 groups are for blocks of 512 and more, where the sort of 64 is dearer (61 rows of 32001, 20 alternatives: 9.7 us, 11.7
 // by wavefronts; with 256 threads one row of 151936 11.4 and 10.7, as the join's keys lie in order).
+// The floor supposes that the largest logits lie anywhere. Where they crowd into a few threads' pieces (rows that rise or fall
+// with the id), many more reach it, in blocks of 512 and more than fit, so that the bisection takes over: with 5 alternatives
+// one row of 151936 12.8 to 16.7 us instead of 9.6, 64 rows of 32001 in bf16 44 to 46 instead of 9.1, 4096 rows of 50257 in
+// bf16 700 to 922 instead of 145.
 template <uint32_t THREADS>
 __device__ __forceinline__ float floor_of(float most, uint32_t top, Shared<THREADS>& sh) {
     constexpr uint32_t WAVES = THREADS / 64;
@@ -296,9 +300,11 @@ __device__ __forceinline__ const void* row_of(const Args& a, uint32_t r) {
     return static_cast<const uint8_t*>(a.logits) + r * a.stride * (BF16 ? 2 : 4);
 }
 
-// Measured on MI355X: 47.2 us for 512 rows of 151936 f32 logits with one alternative (311 MB, 6.6 TB/s); 5.4 for one row with
-// 20, a launch, a trip to memory and the selection one after the other. Those 512 rows without alternatives and with 1, 5, 20
-// and 64, both kernels: 51.4, 54.3, 57.0, 62.5 and 74.6, where the sort, the ranking and their barriers take the place of loads.
+// Measured on MI355X by a kernel trace: 46.8 us for 512 rows of 151936 f32 logits with one alternative (311 MB, 6.6 TB/s); 5.5
+// for one row with 20, a launch, a trip to memory and the selection one after the other. Those 512 rows without alternatives
+// and with 1, 5, 20 and 64, both kernels back to back in a captured graph, logits in turn past the Infinity Cache: 57, 57.7,
+// 62.7, 66.1 and 73.5: the sort, the ranking and their barriers take the place of loads. So do they for bf16, whose logits come
+// at twice the rate: 4096 rows of 50257 (412 MB) 111.5, 125.1, 144.7 and, with 64, 197.
 // Wavefronts of a kernel to a SIMD: as many as its registers allow without a spill (512 rows of 151936 f32 logits, 20
 // alternatives: 62 us with 6 of 32 logits to a thread, 79 with 7, 92 with 8).
 constexpr int waves_of(uint32_t threads, uint32_t each) { return each == 16 ? 8 : threads == 1024 ? 4 : 6; }
@@ -307,8 +313,10 @@ template <bool BF16, uint32_t THREADS, uint32_t EACH>
 __global__ void __launch_bounds__(THREADS, waves_of(THREADS, EACH)) logprobs_slices_kernel(Args a) {
     constexpr uint32_t WAVES = THREADS / 64;
     constexpr uint32_t PIECE = BF16 ? 8 : 4;  // logits of a 16-byte load
-    // 56 registers of the 40 needed: with more wavefronts in flight memory is slower (512 rows of 151936 f32 logits that no cache
-    // has: 57.1 us, 59.0 without).
+    // 56 registers of the 40 needed. 8 wavefronts to a SIMD are the most with either, but by the counters 24.2 to a CU are there on
+    // average, 24.6 without it, and the fewer are faster (f32 logits that no cache has, one alternative: 512 rows of 151936 57.9
+    // us, 58.7 without; 1024 rows 108.4 and 109.5; 2000 of 40000 62.5 and 63.2). Rows in one slice and few long rows take the
+    // same with either.
     if constexpr (EACH == 16) asm volatile("" ::: "v55");
     __shared__ Shared<THREADS> sh;
     const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6;

@@ -53,8 +53,9 @@ __device__ __forceinline__ void wave_lds() {
 
 // s = max |w| / 6 of each group, codes of w / s. A wavefront takes a tile. The four lanes of a row hold 8 columns of each 32: a
 // group's largest magnitude is theirs, found with two shuffles, and each lane's codes are 16 bytes as they lie in memory.
-// Measured on MI355X: 47.9 us for 24576 x 4096 (201 MB read and 52 written: 5.3 TB/s, what a copy of 1 GiB reaches); 4.1 for
-// 1000 x 1096, which is a launch and one trip to memory.
+// Measured on MI355X (back to back in a captured graph, matrices in turn past the Infinity Cache): 47.2 us for 24576 x 4096
+// (201 MB read and 52 written: 5.4 TB/s; a copy of 1 GiB reaches 5.1); 4.7 for 1000 x 1096, which is a launch and one trip to
+// memory.
 template <int G, bool STREAM>
 __global__ void __launch_bounds__(256) w4_quantise_kernel(const bf16_t* __restrict__ from, Form f) {
     const uint32_t lane = threadIdx.x & 63, t = blockIdx.x * 4 + (threadIdx.x >> 6);
@@ -128,8 +129,9 @@ __device__ __forceinline__ float scale_of(const bf16_t* scales, size_t tile, uin
     return bf2f(scales[(tile * TILE_ROWS + row) * (TILE_COLS / G) + s * 32 / G]);
 }
 
-// Codes times scales, rounded once to bf16. A wavefront takes a tile and stores whole rows of its 256 bytes. Measured on MI355X:
-// 108.8 us for 51200 x 5120 (147 MB read, 524 written: 6.2 TB/s), 37.2 for 24576 x 4096, 3.8 for 4096 x 1024.
+// Codes times scales, rounded once to bf16. A wavefront takes a tile and stores whole rows of its 256 bytes. Measured on
+// MI355X, as above: 109.9 us for 51200 x 5120 (147 MB read, 524 written: 6.1 TB/s), 42.6 for 24576 x 4096 (37.1 behind its
+// quantising, whose codes the cache still has), 4.1 for 4096 x 1024.
 template <int G, bool STREAM>
 __global__ void __launch_bounds__(256) w4_read_kernel(Form f, bf16_t* __restrict__ to) {
     const uint32_t lane = threadIdx.x & 63, t = blockIdx.x * 4 + (threadIdx.x >> 6);
@@ -203,11 +205,12 @@ struct Cut {
 // a lane's four sums are four tokens of one row of W, whose scale of a group is one value. A load of X takes 4 rows of a tile's
 // 256 bytes, neighbouring lanes on one row, and passes through the wavefront's own LDS into the operand's order (loaded in
 // that order, four lanes to each of 16 rows, 54 us for the 16 rows below): there is no barrier until a unit's end.
-// Measured on MI355X: one row is bound by the weights: 48.5 us for 151936 x 4096 (322 MB, 6.6 TB/s); 9.8 to 11.3 for 24576 x
-// 4096 SwiGLU (54 MB), of which 2 pass before the first product; 3.4 for 4096 x 1024, which is that and one trip to memory.
-// More rows by X's way through the L2, once to a unit, and by the joins of cut units: 16 rows of 5120 x 25600 (82 MB) 20.6,
-// first products after 2.1, 8 rounds of 1.5 at 6.2 TB/s, the cut units' parts joined by 18.6; 61 rows of 6150 x 4104 12.9 in
-// 208 blocks of 5 rounds.
+// Measured on MI355X, as above: one row is bound by the weights: 50.6 us for 151936 x 4096 (322 MB, 6.4 TB/s); 11.3 for 24576 x
+// 4096 SwiGLU (54 MB, 4.7 TB/s; 9.7 from the cache), of which 2 pass before the first product; 3.0 for 4096 x 1024 (3.4 by a
+// kernel trace), which is that and one trip to memory. More rows by X's way through the L2, once to a unit, and by the joins of
+// cut units: 16 rows of 5120 x 25600 (82 MB) 20.4 (20.1 from the cache, with first products after 2.1, 8 rounds of 1.5, the cut
+// units' parts joined by 18.6); 61 rows of 6150 x 4104 13.2 (12.2) in 194 blocks of 5 rounds (208 launched, for whole rounds of
+// the XCDs).
 template <int G, bool SWIGLU, int XL, int P, int V, int U, bool EVEN>
 __global__ void __launch_bounds__(64 * V) w4_gemv_kernel(Form f, const bf16_t* __restrict__ x, uint32_t n, void* __restrict__ y,
                                                          uint32_t out_f32, Cut cut) {
